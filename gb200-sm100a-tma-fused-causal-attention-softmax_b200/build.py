@@ -14,6 +14,7 @@ import os
 import shutil
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
@@ -33,7 +34,8 @@ ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-O3", "-std=c++17", "-lineinfo", "--fmad=false", "-Xcompiler",
               "-fPIC,-ffp-contract=off", "--expt-relaxed-constexpr"]
 
-LIB_SOURCES = [os.path.join(CSRC, "api.cu"), os.path.join(CSRC, "host", "host.cpp")]
+LIB_SOURCES = [os.path.join(CSRC, n) for n in ("api.cu", "bias.cu", "attention.cu")] + \
+    [os.path.join(CSRC, "host", "host.cpp")]
 CLI_SOURCES = [os.path.join(CSRC, "host", "cli.cpp")]
 
 
@@ -88,17 +90,28 @@ def build_library(force: bool = False, verbose: bool = False) -> str:
         return _build_library(verbose)
 
 
+def _run(cmd):
+    return subprocess.run(cmd, capture_output=True, text=True)
+
+
 def _build_library(verbose: bool) -> str:
     os.makedirs(LIB_DIR, exist_ok=True)
     tmp = LIB_PATH + ".tmp"
-    cmd = [_nvcc(), *ARCH, *NVCC_FLAGS, "-Xptxas", "-v", "-shared", "-I", INCLUDE, "-I", CSRC,
-           "-o", tmp, *LIB_SOURCES]
-    res = subprocess.run(cmd, capture_output=True, text=True)
-    if res.returncode != 0:
-        sys.stderr.write(res.stdout + res.stderr)
-        raise RuntimeError("nvcc failed building libcausal_softmax.so")
+    objects = [os.path.join(LIB_DIR, os.path.basename(s) + ".o") for s in LIB_SOURCES]
+    compile_ = [[_nvcc(), *ARCH, *NVCC_FLAGS, "-Xptxas", "-v", "-c", "-I", INCLUDE, "-I", CSRC,
+                 "-o", o, s] for s, o in zip(LIB_SOURCES, objects)]
+    link = [_nvcc(), *ARCH, "-shared", "-o", tmp, *objects]
+    report = ""
+    with ThreadPoolExecutor(len(compile_)) as pool:
+        done = list(pool.map(_run, compile_))
+    for cmd, res in [*zip(compile_, done), (link, None)]:
+        res = _run(cmd) if res is None else res
+        if res.returncode != 0:
+            sys.stderr.write(res.stdout + res.stderr)
+            raise RuntimeError("nvcc failed building libcausal_softmax.so")
+        report += " ".join(cmd) + "\n" + res.stderr
     with open(os.path.join(LIB_DIR, "ptxas.txt"), "w") as fh:
-        fh.write(" ".join(cmd) + "\n" + res.stderr)
+        fh.write(report)
     os.replace(tmp, LIB_PATH)
     if verbose:
         print(f"built {LIB_PATH}")

@@ -1,4 +1,5 @@
-"""Python binding of the B200 fused causal softmax C ABI (include/causal_softmax.h).
+"""Python binding of the B200 fused causal softmax C ABI (include/causal_softmax.h)
+and of the operators beside it (include/causal_attention.h, operators.py).
 
 This module is plumbing: it loads lib/libcausal_softmax.so with ctypes and
 passes raw device pointers (from torch tensors) and CUDA stream handles to the
@@ -18,7 +19,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 PKG_DIR = os.path.dirname(_HERE)
 LIB_PATH = os.path.join(PKG_DIR, "lib", "libcausal_softmax.so")
 HEADER_PATHS = [os.path.join(os.path.dirname(PKG_DIR), "include", n)
-                for n in ("causal_softmax.h", "causal_softmax_host.h")]
+                for n in ("causal_softmax.h", "causal_attention.h", "causal_softmax_host.h")]
 
 AUTO, BASELINE, WARP, TMA, PIPELINE, ONLINE = range(6)
 KERNELS = {"auto": AUTO, "baseline": BASELINE, "warp": WARP, "tma": TMA,
@@ -157,6 +158,16 @@ def _declare(L) -> None:
         "cs_host_register": (c_int, [vp, sz]),
         "cs_host_unregister": (c_int, [vp]),
         "cs_device_sm_count": (c_int, [c_int]),
+        # operators beside the softmax (causal_attention.h)
+        "cs_bias_buckets": (c_int, [c_i32, c_i32, vp]),
+        "cs_bias_softmax": (c_int, [vp, vp, vp, vp, vp]),
+        "cs_bias_softmax_backward_workspace": (c_i64, [vp]),
+        "cs_bias_softmax_backward": (c_int, [vp, vp, vp, vp, vp, vp, sz, vp]),
+        "cs_attention_workspace": (c_i64, [vp]),
+        "cs_attention": (c_int, [vp, vp, sz, vp]),
+        "cs_attention_backward_workspace": (c_i64, [vp]),
+        "cs_attention_backward": (c_int, [vp, vp, vp, sz, vp]),
+        "cs_attention_status": (c_int, [vp, vp]),
         # host surface (causal_softmax_host.h)
         "cs_pattern_name": (ctypes.c_char_p, [c_int]),
         "cs_f32_to_half": (ctypes.c_uint16, [c_f32]),
@@ -439,3 +450,7 @@ def parse_config(args: list[str]) -> dict:
     if rc != 0:
         raise ValueError(err.value.decode())
     return {n: getattr(cfg, n) for n, _ in Config._fields_}
+
+
+from .operators import (attention, attention_backward, attention_status, bias_buckets,  # noqa: E402,F401
+                        bias_softmax, bias_softmax_backward)

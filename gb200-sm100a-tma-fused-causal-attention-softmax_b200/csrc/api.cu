@@ -8,6 +8,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <cstdarg>
 #include <cstdint>
 #include <cstdio>
 #include <cstring>
@@ -20,6 +21,7 @@
 #endif
 
 #include "causal_softmax.h"
+#include "internal.hpp"
 #include "kernels/baseline.cuh"
 #include "kernels/cluster.cuh"
 #include "kernels/narrow.cuh"
@@ -986,6 +988,30 @@ void zero_output_tails(uint16_t* h_out, int64_t batch, int32_t rows, int32_t col
 }
 
 }  // namespace
+
+namespace cs_host {
+
+int fail(int code, const char* fmt, ...) {
+  va_list ap;
+  va_start(ap, fmt);
+  std::vsnprintf(t_detail, sizeof t_detail, fmt, ap);
+  va_end(ap);
+  return code;
+}
+
+int fail_cuda(cudaError_t e, const char* what) { return cuda_fail(e, what); }
+
+int current_device(Device* out) {
+  CS_CUDA(cudaGetDevice(&out->id));
+  DeviceInfo* d = nullptr;
+  const int rc = device_info(out->id, &d);
+  if (rc) return rc;
+  out->sms = d->sms;
+  out->max_smem = d->max_smem_optin;
+  return CS_OK;
+}
+
+}  // namespace cs_host
 
 extern "C" {
 

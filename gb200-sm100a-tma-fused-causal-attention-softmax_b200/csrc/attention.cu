@@ -1,0 +1,195 @@
+// C ABI of attention with a sliding window and sinks: argument checks and
+// launches (kernels/attention*.cuh).
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <cstdint>
+#include <mutex>
+
+#include "causal_attention.h"
+#include "causal_softmax.h"
+#include "internal.hpp"
+#include "kernels/attention_rows.cuh"
+
+// Timeout bits of the attention kernels on each device (cs_attention_status).
+static __device__ __align__(256) uint32_t g_attention_status[1];
+
+namespace {
+
+using cs_host::fail;
+using cs_host::fail_cuda;
+
+constexpr int64_t kI32Max = 2147483647;
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+int check_tensor(const char* name, const cs_tensor& t, int32_t batch, int32_t tokens, int32_t heads, int32_t dim) {
+  if (!t.data) return fail(CS_ERR_NULL, "%s is null", name);
+  if (!aligned16(t.data)) return fail(CS_ERR_ALIGNMENT, "%s must be 16-byte aligned", name);
+  const int64_t strides[3] = {t.batch_stride, t.token_stride, t.head_stride};
+  const int32_t sizes[3] = {batch, tokens, heads};
+  for (int i = 0; i < 3; ++i)
+    if (sizes[i] > 1 && (strides[i] < dim || (strides[i] & 7) || strides[i] >= (int64_t)1 << 38))
+      return fail(CS_ERR_PITCH, "%s: stride %lld of dimension %d must be a multiple of 8, at least head_dim (%d) and below 2^38",
+                  name, (long long)strides[i], i, dim);
+  return CS_OK;
+}
+
+int check_args(const cs_attention_args* a) {
+  if (!a) return fail(CS_ERR_NULL, "arguments are null");
+  if (a->type != CS_TYPE_F16 && a->type != CS_TYPE_BF16) return fail(CS_ERR_ARG, "unknown element type %d", a->type);
+  if (a->batch <= 0 || a->heads <= 0 || a->kv_heads <= 0 || a->head_dim <= 0 || a->q_len <= 0 || a->kv_len <= 0)
+    return fail(CS_ERR_EMPTY, "batch %d, heads %d and %d, head_dim %d, q_len %d and kv_len %d must be positive", a->batch,
+                a->heads, a->kv_heads, a->head_dim, a->q_len, a->kv_len);
+  if (a->heads % a->kv_heads) return fail(CS_ERR_ARG, "%d heads over %d kv heads", a->heads, a->kv_heads);
+  if ((a->head_dim & 7) || a->head_dim > CS_MAX_HEAD_DIM)
+    return fail(CS_ERR_UNSUPPORTED, "head_dim %d: a multiple of 8 up to %d", a->head_dim, CS_MAX_HEAD_DIM);
+  if ((int64_t)a->batch * a->heads > 1 << 20 || a->q_len > kI32Max - 1024 || a->kv_len > kI32Max - 1024)
+    return fail(CS_ERR_WRONG_LENGTH, "batch %d x heads %d (at most 2^20), q_len %d, kv_len %d", a->batch, a->heads, a->q_len, a->kv_len);
+  if (a->window < 0 || a->sinks < 0) return fail(CS_ERR_ARG, "window %d and sinks %d must not be negative", a->window, a->sinks);
+  if (!std::isfinite(a->scale) || !(a->scale >= 0.f && a->scale <= CS_MAX_ATTENTION_SCALE))
+    return fail(CS_ERR_BAD_SCALE, "scale %g: at most %g", (double)a->scale, (double)CS_MAX_ATTENTION_SCALE);
+  int rc = check_tensor("q", a->q, a->batch, a->q_len, a->heads, a->head_dim);
+  if (!rc) rc = check_tensor("k", a->k, a->batch, a->kv_len, a->kv_heads, a->head_dim);
+  if (!rc) rc = check_tensor("v", a->v, a->batch, a->kv_len, a->kv_heads, a->head_dim);
+  if (!rc) rc = check_tensor("o", a->o, a->batch, a->q_len, a->heads, a->head_dim);
+  return rc;
+}
+
+int check_grads(const cs_attention_args* a, const cs_attention_grads* g) {
+  if (!g) return fail(CS_ERR_NULL, "gradients are null");
+  if (!a->lse) return fail(CS_ERR_NULL, "lse is null");
+  int rc = check_tensor("d_o", g->d_o, a->batch, a->q_len, a->heads, a->head_dim);
+  if (!rc) rc = check_tensor("dq", g->dq, a->batch, a->q_len, a->heads, a->head_dim);
+  if (!rc) rc = check_tensor("dk", g->dk, a->batch, a->kv_len, a->kv_heads, a->head_dim);
+  if (!rc) rc = check_tensor("dv", g->dv, a->batch, a->kv_len, a->kv_heads, a->head_dim);
+  return rc;
+}
+
+cs::Strided strided(const cs_tensor& t) {
+  return cs::Strided{static_cast<uint16_t*>(t.data), t.batch_stride, t.token_stride, t.head_stride};
+}
+
+// The current device's status word; also the first use of a device.
+int set_up(const cs_host::Device& d, uint32_t** status) {
+  static std::mutex mu;
+  static uint32_t* words[cs_host::kMaxDeviceIds];
+  std::lock_guard<std::mutex> lock(mu);
+  if (!words[d.id]) {
+    uint32_t* w = nullptr;
+    const cudaError_t e = cudaGetSymbolAddress(reinterpret_cast<void**>(&w), g_attention_status);
+    if (e != cudaSuccess) return fail_cuda(e, "attention status word");
+    words[d.id] = w;
+  }
+  *status = words[d.id];
+  return CS_OK;
+}
+
+int params_of(const cs_attention_args* a, cs::AttentionParams* p, cs_host::Device* d) {
+  int rc = cs_host::current_device(d);
+  if (!rc) rc = set_up(*d, &p->status);
+  if (rc) return rc;
+  p->q = strided(a->q);
+  p->k = strided(a->k);
+  p->v = strided(a->v);
+  p->o = strided(a->o);
+  p->lse = a->lse;
+  p->q_lens = a->q_lens;
+  p->kv_lens = a->kv_lens;
+  p->batch = a->batch;
+  p->heads = a->heads;
+  p->kv_heads = a->kv_heads;
+  p->group = a->heads / a->kv_heads;
+  p->head_dim = a->head_dim;
+  p->q_len = a->q_len;
+  p->kv_len = a->kv_len;
+  p->window = a->window;
+  p->sinks = a->sinks;
+  p->scale = a->scale;
+  return CS_OK;
+}
+
+dim3 rows_grid(int32_t tokens, int32_t heads) {
+  return dim3((unsigned)((tokens + 3) / 4), (unsigned)std::min(heads, 65535));
+}
+
+int64_t backward_workspace(const cs_attention_args* a) { return (int64_t)a->batch * a->heads * a->q_len * 4; }
+
+int check_workspace(const void* workspace, size_t bytes, int64_t need) {
+  if (need == 0) return CS_OK;
+  if (!workspace) return fail(CS_ERR_NULL, "workspace is null, %lld bytes needed", (long long)need);
+  if (!aligned16(workspace)) return fail(CS_ERR_ALIGNMENT, "workspace must be 16-byte aligned");
+  if ((int64_t)bytes < need) return fail(CS_ERR_WRONG_LENGTH, "workspace of %zu bytes, %lld needed", bytes, (long long)need);
+  return CS_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t cs_attention_workspace(const cs_attention_args* args) {
+  const int rc = check_args(args);
+  return rc ? rc : 0;
+}
+
+int cs_attention(const cs_attention_args* args, void* workspace, size_t workspace_bytes, void* stream) {
+  int rc = check_args(args);
+  if (!rc) rc = check_workspace(workspace, workspace_bytes, 0);
+  if (rc) return rc;
+  cs::AttentionParams p{};
+  cs_host::Device d;
+  rc = params_of(args, &p, &d);
+  if (rc) return rc;
+  auto* kernel = args->type == CS_TYPE_F16 ? &cs::attention_rows_kernel<cs::F16> : &cs::attention_rows_kernel<cs::BF16>;
+  const cudaError_t e = cs_host::launch(kernel, rows_grid(p.q_len, p.batch * p.heads), 128, 0, stream, p);
+  return e == cudaSuccess ? CS_OK : fail_cuda(e, "attention");
+}
+
+int64_t cs_attention_backward_workspace(const cs_attention_args* args) {
+  const int rc = check_args(args);
+  return rc ? rc : backward_workspace(args);
+}
+
+int cs_attention_backward(const cs_attention_args* args, const cs_attention_grads* grads, void* workspace,
+                          size_t workspace_bytes, void* stream) {
+  int rc = check_args(args);
+  if (!rc) rc = check_grads(args, grads);
+  if (!rc) rc = check_workspace(workspace, workspace_bytes, backward_workspace(args));
+  if (rc) return rc;
+  cs::AttentionParams p{};
+  cs_host::Device d;
+  rc = params_of(args, &p, &d);
+  if (rc) return rc;
+  p.d_o = strided(grads->d_o);
+  p.dq = strided(grads->dq);
+  p.dk = strided(grads->dk);
+  p.dv = strided(grads->dv);
+  p.delta = static_cast<float*>(workspace);
+  const bool half = args->type == CS_TYPE_F16;
+  cudaError_t e = cs_host::launch(half ? &cs::attention_dq_rows_kernel<cs::F16> : &cs::attention_dq_rows_kernel<cs::BF16>,
+                                  rows_grid(p.q_len, p.batch * p.heads), 128, 0, stream, p);
+  if (e != cudaSuccess) return fail_cuda(e, "attention backward, queries");
+  e = cs_host::launch(half ? &cs::attention_dkv_rows_kernel<cs::F16> : &cs::attention_dkv_rows_kernel<cs::BF16>,
+                      rows_grid(p.kv_len, p.batch * p.kv_heads), 128, 0, stream, p);
+  return e == cudaSuccess ? CS_OK : fail_cuda(e, "attention backward, keys");
+}
+
+int cs_attention_status(uint32_t* status, void* stream) {
+  if (!status) return fail(CS_ERR_NULL, "status is null");
+  cs_host::Device d;
+  uint32_t* word = nullptr;
+  int rc = cs_host::current_device(&d);
+  if (!rc) rc = set_up(d, &word);
+  if (rc) return rc;
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  uint32_t bits = 0;
+  cudaError_t e = cudaMemcpyAsync(&bits, word, sizeof bits, cudaMemcpyDeviceToHost, st);
+  if (e == cudaSuccess) e = cudaMemsetAsync(word, 0, sizeof bits, st);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+  if (e != cudaSuccess) return fail_cuda(e, "attention status");
+  *status = bits;
+  return cs_status_error(bits);
+}
+
+}  // extern "C"

@@ -1,0 +1,300 @@
+// C ABI of the biased causal softmax and its gradient: bucket borders,
+// argument checks, launch shapes (kernels/bias.cuh).
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <cstdint>
+#include <mutex>
+
+#include "causal_attention.h"
+#include "causal_softmax.h"
+#include "internal.hpp"
+#include "kernels/bias.cuh"
+
+namespace {
+
+using cs_host::fail;
+using cs_host::fail_cuda;
+
+constexpr int64_t kI32Max = 2147483647;
+
+// Whole numbers of up to 1024 bits: powers of a distance (14 bits) up to the
+// 64th, the most that cs_bias_buckets forms.
+struct Big {
+  uint32_t limb[32] = {1};
+  int n = 1;
+};
+
+void multiply(Big* a, uint32_t by) {
+  uint64_t carry = 0;
+  for (int i = 0; i < a->n; ++i) {
+    carry += (uint64_t)a->limb[i] * by;
+    a->limb[i] = (uint32_t)carry;
+    carry >>= 32;
+  }
+  if (carry) a->limb[a->n++] = (uint32_t)carry;
+}
+
+Big power(uint32_t base, int exp, Big from = Big{}) {
+  for (int i = 0; i < exp; ++i) multiply(&from, base);
+  return from;
+}
+
+bool less(const Big& a, const Big& b) {
+  if (a.n != b.n) return a.n < b.n;
+  for (int i = a.n; i-- > 0;)
+    if (a.limb[i] != b.limb[i]) return a.limb[i] < b.limb[i];
+  return false;
+}
+
+int check_args(const cs_bias_args* a) {
+  if (!a) return fail(CS_ERR_NULL, "arguments are null");
+  if (a->type != CS_TYPE_F16 && a->type != CS_TYPE_BF16) return fail(CS_ERR_ARG, "unknown element type %d", a->type);
+  if (a->batch <= 0 || a->heads <= 0 || a->rows <= 0 || a->cols <= 0)
+    return fail(CS_ERR_EMPTY, "batch %d, heads %d, rows %d and cols %d must be positive", a->batch, a->heads, a->rows, a->cols);
+  if (a->pitch < a->cols || (a->pitch & 7)) return fail(CS_ERR_PITCH, "pitch %d for %d columns", a->pitch, a->cols);
+  if (a->row_offset < 0 || a->row_offset > kI32Max - a->rows || a->pitch > kI32Max - 8)
+    return fail(CS_ERR_WRONG_LENGTH, "row offset %d with %d rows", a->row_offset, a->rows);
+  // The matrices' elements count in 62 bits.
+  const int64_t matrices = (int64_t)a->batch * a->heads, size = (int64_t)a->rows * a->pitch;
+  if (matrices > (INT64_MAX >> 1) / size)
+    return fail(CS_ERR_WRONG_LENGTH, "%lld matrices of %lld elements", (long long)matrices, (long long)size);
+  if (matrices > (int64_t)1 << 30) return fail(CS_ERR_WRONG_LENGTH, "%lld matrices: at most 2^30", (long long)matrices);
+  if (a->window < 0 || a->sinks < 0) return fail(CS_ERR_ARG, "window %d and sinks %d must not be negative", a->window, a->sinks);
+  if (!std::isfinite(a->scale) || !(a->scale >= 0.f && a->scale <= CS_MAX_SCALE))
+    return fail(CS_ERR_BAD_SCALE, "scale %g", (double)a->scale);
+  if (a->buckets < 1 || a->buckets > CS_MAX_BUCKETS) return fail(CS_ERR_ARG, "%d buckets: 1 to %d", a->buckets, CS_MAX_BUCKETS);
+  if (!a->bucket_starts) return fail(CS_ERR_NULL, "bucket_starts is null");
+  for (int j = 0; j < a->buckets; ++j) {
+    const int32_t s = a->bucket_starts[j];
+    if (j == 0 ? s != 0 : s <= a->bucket_starts[j - 1] || s > CS_MAX_BUCKET_START)
+      return fail(CS_ERR_ARG, "bucket %d starts at %d: starts begin at 0 and ascend to at most %d", j, s, CS_MAX_BUCKET_START);
+  }
+  return CS_OK;
+}
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+bool overlap(const void* a, const void* b, int64_t bytes) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return x < y + (uintptr_t)bytes && y < x + (uintptr_t)bytes;
+}
+
+int check_matrices(const cs_bias_args* a, const void* x, const void* y, const void* out) {
+  if (!x || !y || !out) return fail(CS_ERR_NULL, "a matrix pointer is null");
+  if (!aligned16(x) || !aligned16(y) || !aligned16(out)) return fail(CS_ERR_ALIGNMENT, "matrices must be 16-byte aligned");
+  const int64_t bytes = (int64_t)a->batch * a->heads * a->rows * a->pitch * 2;
+  if (overlap(x, out, bytes) || overlap(y, out, bytes)) return fail(CS_ERR_ARG, "the output overlaps an input");
+  return CS_OK;
+}
+
+// Launch shape: a row takes `warps` warps of `vec` vectors a lane; a CTA works
+// on `groups` rows at a time, and each matrix has `ctas` CTAs.
+struct Shape {
+  int vec, warps, block, ctas;
+  size_t smem;
+};
+
+// Most visible 16-byte vectors a row has.
+int64_t max_vectors(const cs_bias_args* a) {
+  const int64_t last = std::min<int64_t>(a->cols, (int64_t)a->row_offset + a->rows);
+  int64_t n = (last + 7) / 8;
+  if (a->window) n = std::min<int64_t>(n, ((int64_t)a->window + 14) / 8 + ((int64_t)a->sinks + 7) / 8);
+  return n;
+}
+
+// CTAs of a matrix: enough that the launch holds about four rounds of resident
+// CTAs (rows differ in length), no more than its rows fill.
+int ctas_per_matrix(const cs_bias_args* a, int sms, int groups) {
+  const int64_t matrices = (int64_t)a->batch * a->heads;
+  const int64_t want = ((int64_t)sms * 8 * 4 + matrices - 1) / matrices;
+  const int64_t most = ((int64_t)a->rows + groups - 1) / groups;
+  return (int)std::max<int64_t>(1, std::min(want, most));
+}
+
+constexpr int kWarps = cs::kBiasThreads / 32, kMaxWarps = cs::kBiasMaxThreads / 32;
+
+Shape forward_shape(const cs_bias_args* a, int sms) {
+  const int64_t nv = max_vectors(a);
+  Shape s{};
+  s.vec = nv <= 64 ? 2 : nv <= 128 ? 4 : nv <= 256 ? 8 : nv <= kWarps * 32 * 16 ? 16 : 8;
+  s.warps = 1;
+  while (s.warps < kMaxWarps && (int64_t)s.warps * 32 * s.vec < nv) s.warps *= 2;
+  s.block = std::max(kWarps, s.warps) * 32;
+  s.ctas = ctas_per_matrix(a, sms, s.block / 32 / s.warps);
+  s.smem = (size_t)(cs::bias_slot(a->bucket_starts[a->buckets - 1]) + 1 + s.block / 32 * 2) * 4;
+  return s;
+}
+
+Shape backward_shape(const cs_bias_args* a, int sms) {
+  const int64_t nv = max_vectors(a);
+  const int slots = cs::bias_slot(a->bucket_starts[a->buckets - 1]) + 1;
+  Shape s{};
+  s.vec = nv <= 64 ? 2 : nv <= 128 ? 4 : 8;
+  s.warps = 1;
+  // Each group has an array by distance: few groups where the arrays are long.
+  while (s.warps < kMaxWarps && ((int64_t)s.warps * 32 * s.vec < nv ||
+                                 (s.warps < kWarps && (int64_t)kWarps / s.warps * slots * 4 > 64 * 1024)))
+    s.warps *= 2;
+  s.block = std::max(kWarps, s.warps) * 32;
+  const int groups = s.block / 32 / s.warps;
+  s.ctas = ctas_per_matrix(a, sms, groups);
+  s.smem = (size_t)((int64_t)groups * slots + s.block / 32 * 3) * 4;
+  return s;
+}
+
+using Kernel = void (*)(cs::BiasParams);
+
+template <typename T>
+Kernel forward_of(int vec) {
+  return vec == 2 ? &cs::bias_softmax_kernel<T, 2> : vec == 4 ? &cs::bias_softmax_kernel<T, 4>
+       : vec == 8 ? &cs::bias_softmax_kernel<T, 8> : &cs::bias_softmax_kernel<T, 16>;
+}
+
+template <typename T>
+Kernel backward_of(int vec) {
+  return vec == 2 ? &cs::bias_backward_kernel<T, 2> : vec == 4 ? &cs::bias_backward_kernel<T, 4>
+                                                               : &cs::bias_backward_kernel<T, 8>;
+}
+
+Kernel forward_kernel(int type, int vec) { return type == CS_TYPE_F16 ? forward_of<cs::F16>(vec) : forward_of<cs::BF16>(vec); }
+Kernel backward_kernel(int type, int vec) { return type == CS_TYPE_F16 ? backward_of<cs::F16>(vec) : backward_of<cs::BF16>(vec); }
+
+// Shared-memory limits of the kernels, once per device.
+int set_up(const cs_host::Device& d) {
+  static std::mutex mu;
+  static bool done[cs_host::kMaxDeviceIds];
+  std::lock_guard<std::mutex> lock(mu);
+  if (done[d.id]) return CS_OK;
+  for (int type : {CS_TYPE_F16, CS_TYPE_BF16})
+    for (int vec : {2, 4, 8, 16}) {
+      cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(forward_kernel(type, vec)),
+                                           cudaFuncAttributeMaxDynamicSharedMemorySize, d.max_smem);
+      if (e == cudaSuccess && vec < 16)
+        e = cudaFuncSetAttribute(reinterpret_cast<const void*>(backward_kernel(type, vec)),
+                                 cudaFuncAttributeMaxDynamicSharedMemorySize, d.max_smem);
+      if (e != cudaSuccess) return fail_cuda(e, "bias kernels");
+    }
+  cudaFuncAttributes fa{};
+  const cudaError_t e = cudaFuncGetAttributes(&fa, reinterpret_cast<const void*>(&cs::bias_table_kernel));
+  if (e != cudaSuccess) return fail_cuda(e, "bias kernels");
+  done[d.id] = true;
+  return CS_OK;
+}
+
+cs::BiasParams params_of(const cs_bias_args* a, const Shape& s) {
+  cs::BiasParams p{};
+  p.heads = a->heads;
+  p.rows = a->rows;
+  p.cols = a->cols;
+  p.pitch = a->pitch;
+  p.row_offset = a->row_offset;
+  p.window = a->window;
+  p.sinks = a->sinks;
+  p.ctas = s.ctas;
+  p.warps = s.warps;
+  p.buckets = a->buckets;
+  p.near = a->bucket_starts[a->buckets - 1];
+  p.scale = a->scale;
+  std::copy(a->bucket_starts, a->bucket_starts + a->buckets, p.starts);
+  return p;
+}
+
+int grid_of(const cs_bias_args* a, const Shape& s, int64_t* grid) {
+  *grid = (int64_t)a->batch * a->heads * s.ctas;
+  return *grid <= kI32Max ? CS_OK : fail(CS_ERR_WRONG_LENGTH, "%lld CTAs", (long long)*grid);
+}
+
+}  // namespace
+
+extern "C" {
+
+int cs_bias_buckets(int32_t buckets, int32_t max_distance, int32_t* starts) {
+  if (!starts) return fail(CS_ERR_NULL, "starts is null");
+  if (buckets < 2 || buckets > CS_MAX_BUCKETS || max_distance <= buckets / 2 || max_distance > CS_MAX_BUCKET_START)
+    return fail(CS_ERR_ARG, "%d buckets up to distance %d: 2 to %d buckets, distance above half of them and at most %d",
+                buckets, max_distance, CS_MAX_BUCKETS, CS_MAX_BUCKET_START);
+  const int e = buckets / 2, m = buckets - e;
+  for (int j = 0; j < e; ++j) starts[j] = j;
+  for (int t = 0; t < m; ++t) {
+    const Big goal = power((uint32_t)e, m - t, power((uint32_t)max_distance, t));
+    int32_t lo = starts[e + t - 1] + 1, hi = std::max(lo, max_distance);  // the least n in [lo, hi]
+    while (lo < hi) {
+      const int32_t mid = lo + (hi - lo) / 2;
+      if (less(power((uint32_t)mid, m), goal)) lo = mid + 1; else hi = mid;
+    }
+    starts[e + t] = lo;
+  }
+  // Buckets pushed up one by one by those before them may pass the limit.
+  if (starts[buckets - 1] > CS_MAX_BUCKET_START) return fail(CS_ERR_ARG, "the last bucket starts at %d", starts[buckets - 1]);
+  return CS_OK;
+}
+
+int cs_bias_softmax(const cs_bias_args* args, const void* x, const float* table, void* p, void* stream) {
+  int rc = check_args(args);
+  if (!rc) rc = check_matrices(args, x, x, p);
+  if (rc) return rc;
+  if (!table) return fail(CS_ERR_NULL, "table is null");
+  cs_host::Device d;
+  rc = cs_host::current_device(&d);
+  if (!rc) rc = set_up(d);
+  if (rc) return rc;
+  const Shape s = forward_shape(args, d.sms);
+  int64_t grid = 0;
+  rc = grid_of(args, s, &grid);
+  if (rc) return rc;
+  cs::BiasParams k = params_of(args, s);
+  k.x = static_cast<const uint16_t*>(x);
+  k.out = static_cast<uint16_t*>(p);
+  k.table = table;
+  const cudaError_t e = cs_host::launch(forward_kernel(args->type, s.vec), dim3((unsigned)grid), s.block, s.smem, stream, k);
+  return e == cudaSuccess ? CS_OK : fail_cuda(e, "biased softmax");
+}
+
+int64_t cs_bias_softmax_backward_workspace(const cs_bias_args* args) {
+  int rc = check_args(args);
+  cs_host::Device d;
+  if (!rc) rc = cs_host::current_device(&d);
+  if (rc) return rc;
+  const Shape s = backward_shape(args, d.sms);
+  return (int64_t)args->batch * args->heads * s.ctas * args->buckets * 4;
+}
+
+int cs_bias_softmax_backward(const cs_bias_args* args, const void* p, const void* dp, void* ds, float* dtable,
+                             void* workspace, size_t workspace_bytes, void* stream) {
+  int rc = check_args(args);
+  if (!rc) rc = check_matrices(args, p, dp, ds);
+  if (rc) return rc;
+  if (!dtable || !workspace) return fail(CS_ERR_NULL, "dtable or workspace is null");
+  if (!aligned16(workspace)) return fail(CS_ERR_ALIGNMENT, "workspace must be 16-byte aligned");
+  cs_host::Device d;
+  rc = cs_host::current_device(&d);
+  if (!rc) rc = set_up(d);
+  if (rc) return rc;
+  const Shape s = backward_shape(args, d.sms);
+  int64_t grid = 0;
+  rc = grid_of(args, s, &grid);
+  if (rc) return rc;
+  const int64_t need = grid * args->buckets * 4;
+  if ((int64_t)workspace_bytes < need)
+    return fail(CS_ERR_WRONG_LENGTH, "workspace of %zu bytes, %lld needed", workspace_bytes, (long long)need);
+  cs::BiasParams k = params_of(args, s);
+  k.x = static_cast<const uint16_t*>(p);
+  k.dp = static_cast<const uint16_t*>(dp);
+  k.out = static_cast<uint16_t*>(ds);
+  k.partial = static_cast<float*>(workspace);
+  cudaError_t e = cs_host::launch(backward_kernel(args->type, s.vec), dim3((unsigned)grid), s.block, s.smem, stream, k);
+  if (e != cudaSuccess) return fail_cuda(e, "biased softmax backward");
+  cs::BiasReduceParams r{};
+  r.partial = k.partial;
+  r.dtable = dtable;
+  r.batch = args->batch;
+  r.heads = args->heads;
+  r.ctas = s.ctas;
+  r.buckets = args->buckets;
+  e = cs_host::launch(&cs::bias_table_kernel, dim3((unsigned)args->heads), 1024, 0, stream, r);
+  return e == cudaSuccess ? CS_OK : fail_cuda(e, "bias table gradient");
+}
+
+}  // extern "C"

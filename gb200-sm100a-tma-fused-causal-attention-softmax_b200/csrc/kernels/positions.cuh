@@ -1,0 +1,58 @@
+// The positional mask shared by the biased softmax and the attention kernels.
+//
+// A query at absolute position p sees key k when
+//     k <= p  and  k < keys  and  (window == 0 or p - k < window or k < sinks).
+// So a row's visible keys are at most two runs: [0, s_end) and [lo, hi) with
+// s_end <= lo. Plain integer code, host-callable: the CPU tests compile it as C++.
+#pragma once
+
+#include <stdint.h>
+
+#ifdef __CUDACC__
+#define CS_HD __host__ __device__ __forceinline__
+#else
+#define CS_HD inline
+#endif
+
+namespace cs {
+
+struct Visible {
+  int32_t s_end;   // sinks: [0, s_end)
+  int32_t lo, hi;  // the window: [lo, hi), empty if lo >= hi
+};
+
+// window > 0, or 0 for none. p may be negative (a query before the first key: sees nothing).
+CS_HD Visible visible_keys(int64_t p, int32_t keys, int32_t window, int32_t sinks) {
+  Visible v;
+  const int64_t hi = p + 1 < keys ? p + 1 : keys;
+  v.hi = (int32_t)(hi > 0 ? hi : 0);
+  const int64_t lo = window > 0 ? p + 1 - window : 0;
+  const int64_t lo0 = lo > 0 ? lo : 0;
+  const int32_t cut = (int32_t)(lo0 < v.hi ? lo0 : v.hi);
+  v.lo = cut;  // lo == hi for an empty window run
+  v.s_end = sinks < cut ? sinks : cut;
+  return v;
+}
+
+CS_HD bool sees(const Visible& v, int32_t k) { return k < v.s_end || (k >= v.lo && k < v.hi); }
+
+// The 8-element vectors that hold a row's visible columns, numbered densely:
+// vector j < n_sink is vector j of the row, the others start at w_beg.
+struct VisibleVectors {
+  int32_t n_sink, w_beg, n;
+};
+
+CS_HD VisibleVectors visible_vectors(const Visible& v) {
+  VisibleVectors m;
+  const int32_t s_vec = (v.s_end + 7) >> 3;
+  const int32_t w_beg = v.lo < v.hi ? v.lo >> 3 : s_vec;
+  const int32_t w_end = v.lo < v.hi ? (v.hi + 7) >> 3 : s_vec;
+  m.n_sink = s_vec < w_beg ? s_vec : w_beg;
+  m.w_beg = w_beg;
+  m.n = m.n_sink + (w_end - w_beg);
+  return m;
+}
+
+CS_HD int32_t vector_at(const VisibleVectors& m, int32_t j) { return j < m.n_sink ? j : j - m.n_sink + m.w_beg; }
+
+}  // namespace cs

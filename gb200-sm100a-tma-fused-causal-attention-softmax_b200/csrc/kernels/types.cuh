@@ -1,0 +1,49 @@
+// The two 16-bit element types of the operators beside the plain softmax.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <stdint.h>
+
+namespace cs {
+
+struct F16 {
+  static constexpr bool kIsHalf = true;
+  static __device__ __forceinline__ float2 unpack(uint32_t bits) {
+    return __half22float2(*reinterpret_cast<const __half2*>(&bits));
+  }
+  static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+};
+
+struct BF16 {
+  static constexpr bool kIsHalf = false;
+  static __device__ __forceinline__ float2 unpack(uint32_t bits) {
+    return make_float2(__uint_as_float(bits << 16), __uint_as_float(bits & 0xFFFF0000u));
+  }
+  static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+};
+
+// The 8 elements of a 16-byte vector, and back.
+template <typename T>
+__device__ __forceinline__ void unpack8(const uint4& r, float* f) {
+  const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const float2 t = T::unpack(w[q]);
+    f[2 * q] = t.x;
+    f[2 * q + 1] = t.y;
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ uint4 pack8(const float* f) {
+  return make_uint4(T::pack(f[0], f[1]), T::pack(f[2], f[3]), T::pack(f[4], f[5]), T::pack(f[6], f[7]));
+}
+
+}  // namespace cs
