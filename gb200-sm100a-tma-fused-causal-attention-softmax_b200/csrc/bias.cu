@@ -89,10 +89,11 @@ int check_matrices(const cs_bias_args* a, const void* x, const void* y, const vo
   return CS_OK;
 }
 
-// Launch shape: a row takes `warps` warps of `vec` vectors a lane; a CTA works
-// on `groups` rows at a time, and each matrix has `ctas` CTAs.
+// Launch shape: a row takes `lanes` lanes; a CTA works on block / lanes rows at
+// a time, and each matrix has `ctas` CTAs. slots: vectors of a staged
+// row's buffer, 0 where rows stay in global memory.
 struct Shape {
-  int vec, warps, block, ctas;
+  int lanes, block, ctas, slots;
   size_t smem;
 };
 
@@ -113,53 +114,58 @@ int ctas_per_matrix(const cs_bias_args* a, int sms, int groups) {
   return (int)std::max<int64_t>(1, std::min(want, most));
 }
 
-constexpr int kWarps = cs::kBiasThreads / 32, kMaxWarps = cs::kBiasMaxThreads / 32;
+// Few lanes a row keep the work that each row costs a warp (its geometry, the
+// reductions, the vectors near the diagonal) shared among several rows, and
+// shared memory for two rows a group limits how few: a CTA takes up to
+// kTargetSmem, three CTAs an SM. Measured on B200 in us, lanes 8 / 16 / 32 / 64
+// (/ 128): forward 64 x 16 matrices of 512^2 223 / 267 / 457 / 859, 16 x 16 of
+// 1024^2 197 / 187 / 287 / 513, 8 x 16 of 2048^2 626 / 318 / 363 / 589,
+// 64 x 4096^2 1096 / 1046 / 609 / 742, 16 x 8192^2 - / 1043 / 1059 / 635 / 722;
+// backward 512^2 x 512 367 / 250 / 312 / 464, 128 x 1024^2 766 / 231 / 205 / 279
+// (each group has its array by distance), 32 x 4096^2 856 / 640 / 854 / 451 / 544.
+constexpr int64_t kTargetSmem = 72 * 1024;
 
-Shape forward_shape(const cs_bias_args* a, int sms) {
+// matrices: 1 (scores) or 2 (probabilities and their gradient); words: fp32
+// words a CTA needs besides, per group and once.
+Shape shape_of(const cs_bias_args* a, const cs_host::Device& d, int matrices, int64_t group_words, int64_t words) {
   const int64_t nv = max_vectors(a);
+  auto bytes = [&](int lanes) {
+    const int64_t block = std::max(cs::kBiasThreads, lanes), groups = block / lanes;
+    return groups * (nv * 32 * matrices + group_words * 4) + (words + block / 32 * 2) * 4;
+  };
   Shape s{};
-  s.vec = nv <= 64 ? 2 : nv <= 128 ? 4 : nv <= 256 ? 8 : nv <= kWarps * 32 * 16 ? 16 : 8;
-  s.warps = 1;
-  while (s.warps < kMaxWarps && (int64_t)s.warps * 32 * s.vec < nv) s.warps *= 2;
-  s.block = std::max(kWarps, s.warps) * 32;
-  s.ctas = ctas_per_matrix(a, sms, s.block / 32 / s.warps);
-  s.smem = (size_t)(cs::bias_slot(a->bucket_starts[a->buckets - 1]) + 1 + s.block / 32 * 2) * 4;
+  s.lanes = (nv <= 64 ? 8 : 16) * matrices;
+  while (s.lanes < cs::kBiasMaxThreads && bytes(s.lanes) > kTargetSmem) s.lanes *= 2;
+  s.block = std::max(cs::kBiasThreads, s.lanes);
+  s.slots = (int)nv;
+  s.smem = (size_t)bytes(s.lanes);
+  if ((int64_t)s.smem > d.max_smem) {
+    s.smem -= (size_t)(s.block / s.lanes * nv * 32 * matrices);
+    s.slots = 0;
+  }
+  s.ctas = ctas_per_matrix(a, d.sms, s.block / s.lanes);
   return s;
 }
 
-Shape backward_shape(const cs_bias_args* a, int sms) {
-  const int64_t nv = max_vectors(a);
-  const int slots = cs::bias_slot(a->bucket_starts[a->buckets - 1]) + 1;
-  Shape s{};
-  s.vec = nv <= 64 ? 2 : nv <= 128 ? 4 : 8;
-  s.warps = 1;
-  // Each group has an array by distance: few groups where the arrays are long.
-  while (s.warps < kMaxWarps && ((int64_t)s.warps * 32 * s.vec < nv ||
-                                 (s.warps < kWarps && (int64_t)kWarps / s.warps * slots * 4 > 64 * 1024)))
-    s.warps *= 2;
-  s.block = std::max(kWarps, s.warps) * 32;
-  const int groups = s.block / 32 / s.warps;
-  s.ctas = ctas_per_matrix(a, sms, groups);
-  s.smem = (size_t)((int64_t)groups * slots + s.block / 32 * 3) * 4;
-  return s;
+Shape forward_shape(const cs_bias_args* a, const cs_host::Device& d) {
+  return shape_of(a, d, 1, 0, cs::bias_slots(a->bucket_starts[a->buckets - 1]));
+}
+
+Shape backward_shape(const cs_bias_args* a, const cs_host::Device& d) {
+  return shape_of(a, d, 2, cs::bias_slots(a->bucket_starts[a->buckets - 1]), 0);
 }
 
 using Kernel = void (*)(cs::BiasParams);
 
-template <typename T>
-Kernel forward_of(int vec) {
-  return vec == 2 ? &cs::bias_softmax_kernel<T, 2> : vec == 4 ? &cs::bias_softmax_kernel<T, 4>
-       : vec == 8 ? &cs::bias_softmax_kernel<T, 8> : &cs::bias_softmax_kernel<T, 16>;
+Kernel forward_kernel(int type, bool staged) {
+  return type == CS_TYPE_F16 ? (staged ? &cs::bias_softmax_kernel<cs::F16, true> : &cs::bias_softmax_kernel<cs::F16, false>)
+                             : (staged ? &cs::bias_softmax_kernel<cs::BF16, true> : &cs::bias_softmax_kernel<cs::BF16, false>);
 }
 
-template <typename T>
-Kernel backward_of(int vec) {
-  return vec == 2 ? &cs::bias_backward_kernel<T, 2> : vec == 4 ? &cs::bias_backward_kernel<T, 4>
-                                                               : &cs::bias_backward_kernel<T, 8>;
+Kernel backward_kernel(int type, bool staged) {
+  return type == CS_TYPE_F16 ? (staged ? &cs::bias_backward_kernel<cs::F16, true> : &cs::bias_backward_kernel<cs::F16, false>)
+                             : (staged ? &cs::bias_backward_kernel<cs::BF16, true> : &cs::bias_backward_kernel<cs::BF16, false>);
 }
-
-Kernel forward_kernel(int type, int vec) { return type == CS_TYPE_F16 ? forward_of<cs::F16>(vec) : forward_of<cs::BF16>(vec); }
-Kernel backward_kernel(int type, int vec) { return type == CS_TYPE_F16 ? backward_of<cs::F16>(vec) : backward_of<cs::BF16>(vec); }
 
 // Shared-memory limits of the kernels, once per device.
 int set_up(const cs_host::Device& d) {
@@ -168,11 +174,11 @@ int set_up(const cs_host::Device& d) {
   std::lock_guard<std::mutex> lock(mu);
   if (done[d.id]) return CS_OK;
   for (int type : {CS_TYPE_F16, CS_TYPE_BF16})
-    for (int vec : {2, 4, 8, 16}) {
-      cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(forward_kernel(type, vec)),
+    for (bool staged : {true, false}) {
+      cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(forward_kernel(type, staged)),
                                            cudaFuncAttributeMaxDynamicSharedMemorySize, d.max_smem);
-      if (e == cudaSuccess && vec < 16)
-        e = cudaFuncSetAttribute(reinterpret_cast<const void*>(backward_kernel(type, vec)),
+      if (e == cudaSuccess)
+        e = cudaFuncSetAttribute(reinterpret_cast<const void*>(backward_kernel(type, staged)),
                                  cudaFuncAttributeMaxDynamicSharedMemorySize, d.max_smem);
       if (e != cudaSuccess) return fail_cuda(e, "bias kernels");
     }
@@ -193,7 +199,8 @@ cs::BiasParams params_of(const cs_bias_args* a, const Shape& s) {
   p.window = a->window;
   p.sinks = a->sinks;
   p.ctas = s.ctas;
-  p.warps = s.warps;
+  p.lanes = s.lanes;
+  p.slots = s.slots;
   p.buckets = a->buckets;
   p.near = a->bucket_starts[a->buckets - 1];
   p.scale = a->scale;
@@ -240,7 +247,7 @@ int cs_bias_softmax(const cs_bias_args* args, const void* x, const float* table,
   rc = cs_host::current_device(&d);
   if (!rc) rc = set_up(d);
   if (rc) return rc;
-  const Shape s = forward_shape(args, d.sms);
+  const Shape s = forward_shape(args, d);
   int64_t grid = 0;
   rc = grid_of(args, s, &grid);
   if (rc) return rc;
@@ -248,7 +255,7 @@ int cs_bias_softmax(const cs_bias_args* args, const void* x, const float* table,
   k.x = static_cast<const uint16_t*>(x);
   k.out = static_cast<uint16_t*>(p);
   k.table = table;
-  const cudaError_t e = cs_host::launch(forward_kernel(args->type, s.vec), dim3((unsigned)grid), s.block, s.smem, stream, k);
+  const cudaError_t e = cs_host::launch(forward_kernel(args->type, s.slots > 0), dim3((unsigned)grid), s.block, s.smem, stream, k);
   return e == cudaSuccess ? CS_OK : fail_cuda(e, "biased softmax");
 }
 
@@ -257,7 +264,7 @@ int64_t cs_bias_softmax_backward_workspace(const cs_bias_args* args) {
   cs_host::Device d;
   if (!rc) rc = cs_host::current_device(&d);
   if (rc) return rc;
-  const Shape s = backward_shape(args, d.sms);
+  const Shape s = backward_shape(args, d);
   return (int64_t)args->batch * args->heads * s.ctas * args->buckets * 4;
 }
 
@@ -272,7 +279,7 @@ int cs_bias_softmax_backward(const cs_bias_args* args, const void* p, const void
   rc = cs_host::current_device(&d);
   if (!rc) rc = set_up(d);
   if (rc) return rc;
-  const Shape s = backward_shape(args, d.sms);
+  const Shape s = backward_shape(args, d);
   int64_t grid = 0;
   rc = grid_of(args, s, &grid);
   if (rc) return rc;
@@ -284,7 +291,7 @@ int cs_bias_softmax_backward(const cs_bias_args* args, const void* p, const void
   k.dp = static_cast<const uint16_t*>(dp);
   k.out = static_cast<uint16_t*>(ds);
   k.partial = static_cast<float*>(workspace);
-  cudaError_t e = cs_host::launch(backward_kernel(args->type, s.vec), dim3((unsigned)grid), s.block, s.smem, stream, k);
+  cudaError_t e = cs_host::launch(backward_kernel(args->type, s.slots > 0), dim3((unsigned)grid), s.block, s.smem, stream, k);
   if (e != cudaSuccess) return fail_cuda(e, "biased softmax backward");
   cs::BiasReduceParams r{};
   r.partial = k.partial;
@@ -293,7 +300,8 @@ int cs_bias_softmax_backward(const cs_bias_args* args, const void* p, const void
   r.heads = args->heads;
   r.ctas = s.ctas;
   r.buckets = args->buckets;
-  e = cs_host::launch(&cs::bias_table_kernel, dim3((unsigned)args->heads), 1024, 0, stream, r);
+  e = cs_host::launch(&cs::bias_table_kernel, dim3((unsigned)args->heads, (unsigned)((args->buckets + 31) / 32)), 1024, 0,
+                      stream, r);
   return e == cudaSuccess ? CS_OK : fail_cuda(e, "bias table gradient");
 }
 

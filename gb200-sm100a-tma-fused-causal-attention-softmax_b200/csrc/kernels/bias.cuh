@@ -1,15 +1,26 @@
 // Causal softmax with a learned relative-position bias, and its gradient.
 //
-// A group of W warps owns one row at a time; each lane keeps V 16-byte vectors
-// of the row's visible columns in registers, so scores (or probabilities and
-// their gradients) are read once. Rows longer than the group's registers are
-// walked in chunks and read again from L2. Bound: HBM (2 bytes in per visible
-// score, 2 out per column; the backward reads two matrices).
+// A group of 8 to 256 lanes works on one row at a time. The row's visible 16-byte
+// vectors are copied to shared memory (cp.async) while the group works on the
+// row before, and the passes (maximum, sum, result; backward: the row's sum of
+// p dp, result) read them there, so HBM sees each score once. Rows too long for
+// the group's two buffers are read from global memory in each pass.
+// Bound: HBM (2 bytes in per visible score, 2 out per column; the backward
+// reads two matrices).
 //
 // Bias: a distance d = position - key lies in the last bucket from its start
-// on, and the other distances (fewer than CS_MAX_BUCKET_START) are looked up in
-// a shared-memory table of the head's bias by distance, already in units of
-// log2. Vectors wholly in the last bucket, most of a long row, take one constant.
+// on; the other distances (at most CS_MAX_BUCKET_START) are looked up in a
+// shared-memory table of the head's bias by distance, in units of log2. Most
+// vectors of a long row lie wholly in the last bucket and are wholly visible:
+// these "plain" vectors take one constant, packed arithmetic and, for the
+// maximum, a packed 16-bit comparison (scale >= 0 keeps the order); only the
+// others pay for masks and look-ups. With both kinds in one unrolled loop over
+// registers the instructions, not HBM, bound the kernel: 64 x 4096^2 took
+// 1.0-2.5 ms at every split tried.
+//
+// Exponents are scale x + bias rounded once, minus the rounded maximum: fusing
+// the subtraction into the multiply-add would leave the rounding error of the
+// maximum, which a large scale blows up.
 //
 // Table gradient: a row holds each distance once, so a group adds its row's dz
 // into its own array by distance without conflicts, row after row: no atomics,
@@ -24,8 +35,8 @@
 namespace cs {
 
 constexpr int kMaxBuckets = 128;
-constexpr int kBiasThreads = 256;     // CTA size while a row takes at most 8 warps
-constexpr int kBiasMaxThreads = 512;  // CTA size of longer rows (16 warps a row)
+constexpr int kBiasThreads = 128;     // CTA size while a row takes at most 4 warps
+constexpr int kBiasMaxThreads = 256;  // rows of 8 warps
 
 struct BiasParams {
   const uint16_t* x;    // scores; backward: probabilities
@@ -35,15 +46,18 @@ struct BiasParams {
   float* partial;       // backward: [matrix, CTA, buckets]
   int32_t heads, rows, cols, pitch, row_offset, window, sinks;
   int32_t ctas;         // per matrix
-  int32_t warps;        // W, per row
+  int32_t lanes;        // of a group: a power of two, 8 to 256
+  int32_t slots;        // vectors of one shared-memory row buffer (0: rows stay in global memory)
   int32_t buckets, near;  // near: first distance of the last bucket
   float scale;
   int32_t starts[kMaxBuckets];
 };
 
-// Distances sit 9 words per 8, so that the lanes of a warp, 8 distances apart,
-// meet different banks.
-__host__ __device__ __forceinline__ int bias_slot(int d) { return d + (d >> 3); }
+// Arrays by distance hold 9 words per 8 distances, so that the lanes of a warp,
+// 8 distances apart, meet different banks. A vector's distances d0, d0 - 1, ...
+// d0 - 7 reach from -7 (masked) to near + 7 (clipped).
+__host__ __device__ __forceinline__ int bias_slot(int d) { return d + 8 + ((d + 8) >> 3); }
+__host__ __device__ __forceinline__ int bias_slots(int near) { return bias_slot(near + 7) + 1; }
 
 __device__ __forceinline__ int bucket_of(const BiasParams& p, int d) {
   int lo = 0, hi = p.buckets;  // starts[lo] <= d < starts[hi]
@@ -54,22 +68,62 @@ __device__ __forceinline__ int bucket_of(const BiasParams& p, int d) {
   return lo;
 }
 
-// Barrier of one group's threads (W warps; one warp needs none).
-__device__ __forceinline__ void group_sync(int id, int threads) {
-  if (threads == 32) __syncwarp();
-  else asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
-}
+// One group: its lanes, and what they do together. Groups of up to 32 lanes
+// share a warp; larger ones take whole warps, a named barrier and a word of
+// shared memory per warp.
+struct Group {
+  int lanes, id, rank;  // rank: this lane's
+  uint32_t mask;        // the group's lanes of this warp
+  __device__ __forceinline__ explicit Group(int n) : lanes(n) {
+    id = threadIdx.x / n;
+    rank = threadIdx.x - id * n;
+    mask = n >= 32 ? 0xffffffffu : ((1u << n) - 1u) << (threadIdx.x & 31 & ~(n - 1));
+  }
+  __device__ __forceinline__ void sync() const {
+    if (lanes <= 32) __syncwarp(mask);
+    else asm volatile("bar.sync %0, %1;" ::"r"(1 + id), "r"(lanes) : "memory");
+  }
+  __device__ __forceinline__ float max(float v, float* words) const {
+    float m;
+    asm volatile("redux.sync.max.f32 %0, %1, %2;" : "=f"(m) : "f"(v), "r"(mask));
+    if (lanes > 32) {
+      if ((rank & 31) == 0) words[rank >> 5] = m;
+      sync();
+      for (int k = 0; k < lanes >> 5; ++k) m = fmaxf(m, words[k]);
+    }
+    return m;
+  }
+  __device__ __forceinline__ float sum(float v, float* words) const {
+    for (int o = (lanes < 32 ? lanes : 32) >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(mask, v, o);
+    if (lanes > 32) {
+      if ((rank & 31) == 0) words[rank >> 5] = v;
+      sync();
+      v = 0.f;
+      for (int k = 0; k < lanes >> 5; ++k) v += words[k];
+    }
+    return v;
+  }
+};
 
+// One row: its visible vectors, numbered densely, and the plain ones among
+// them, [f0, f1): wholly visible and wholly in the last bucket.
 struct RowWalk {
   Visible v;
   VisibleVectors m;
-  int32_t pos;
+  int32_t pos, f0, f1;
   __device__ __forceinline__ RowWalk(const BiasParams& p, int row) {
-    const int64_t at = (int64_t)p.row_offset + row;
-    v = visible_keys(at, p.cols, p.window, p.sinks);
+    pos = p.row_offset + row;  // below 2^31
+    v = visible_columns(pos, p.cols, p.window, p.sinks);
     m = visible_vectors(v);
-    pos = (int32_t)at;
+    f0 = m.n_sink + ((v.lo & 7) ? 1 : 0);
+    // Last element 8 j + 7 of window vector j: below hi and at distance near or more.
+    const int32_t end = min(v.hi, pos - p.near + 1) >> 3;
+    f1 = max(f0, min(m.n, m.n_sink + end - m.w_beg));
+    if (v.lo >= v.hi) f0 = f1 = m.n;
   }
+  // The vectors that are not plain, numbered densely.
+  __device__ __forceinline__ int others() const { return m.n - (f1 - f0); }
+  __device__ __forceinline__ int other(int t) const { return t < f0 ? t : t - f0 + f1; }
 };
 
 __device__ __forceinline__ void zero_masked(const BiasParams& p, const RowWalk& w, uint4* row, int gt, int gn) {
@@ -79,27 +133,87 @@ __device__ __forceinline__ void zero_masked(const BiasParams& p, const RowWalk& 
   for (int j = w_end + gt; j < (p.pitch >> 3); j += gn) __stcs(row + j, z);
 }
 
-// The biased scores of one vector in units of log2; -infinity where masked.
+__device__ __forceinline__ void cp_async16(void* dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_addr(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+__device__ __forceinline__ void fetch_row(const RowWalk& w, const uint4* in, uint4* buffer, int gt, int gn) {
+  for (int j = gt; j < w.m.n; j += gn) cp_async16(buffer + j, in + vector_at(w.m, j));
+}
+
+// Two floats in one 64-bit register (packed arithmetic).
+using F2 = unsigned long long;
+__device__ __forceinline__ F2 f2(float a, float b) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 f2_out(F2 v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ F2 f2_add(F2 a, F2 b) {
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ F2 f2_mul(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ F2 f2_fma(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+
 template <typename T>
-__device__ __forceinline__ void biased8(const BiasParams& p, const RowWalk& w, const float* tab, float far, float sl,
-                                        int c0, const uint4& raw, float* z) {
+__device__ __forceinline__ void unpack_pairs(const uint4& r, F2* f) {
+  const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const float2 t = T::unpack(w[q]);
+    f[q] = f2(t.x, t.y);
+  }
+}
+
+// 2^(scale x + bias - m) of a plain vector.
+template <typename T>
+__device__ __forceinline__ void plain_exp(const uint4& raw, F2 sl, F2 far, F2 minus_m, F2* e) {
+  unpack_pairs<T>(raw, e);
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const float2 t = f2_out(f2_add(f2_fma(e[q], sl, far), minus_m));
+    e[q] = f2(ex2(t.x), ex2(t.y));
+  }
+}
+
+// Slots of a vector's distances: that of element e is first - e - (e > part).
+struct DistanceSlots {
+  int first, part;
+  __device__ __forceinline__ DistanceSlots(int d0, int near) {
+    const int d = min(d0, near + 7);  // all 8 are in the last bucket from there on
+    first = bias_slot(d);
+    part = d & 7;
+  }
+  __device__ __forceinline__ int operator[](int e) const { return first - e - (e > part ? 1 : 0); }
+};
+
+// The biased scores of any vector in units of log2; -infinity where masked.
+template <typename T>
+__device__ __forceinline__ uint32_t biased8(const BiasParams& p, const RowWalk& w, const float* tab, float sl, int c0,
+                                            const uint4& raw, float* z) {
   unpack8<T>(raw, z);
-  const int d0 = w.pos - c0;
-  if (d0 - 7 >= p.near) {
+  const uint32_t bits = visible_bits(w.v, c0);
+  const DistanceSlots at(w.pos - c0, p.near);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) z[e] = __fmaf_rn(z[e], sl, far);
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int d = min(max(d0 - e, 0), p.near);
-      z[e] = __fmaf_rn(z[e], sl, tab[bias_slot(d)]);
-    }
-  }
-  if (!((c0 >= w.v.lo && c0 + 8 <= w.v.hi) || c0 + 8 <= w.v.s_end)) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (!sees(w.v, c0 + e)) z[e] = -INFINITY;
-  }
+  for (int e = 0; e < 8; ++e) z[e] = (bits >> e) & 1 ? __fmaf_rn(z[e], sl, tab[at[e]]) : -INFINITY;
+  return bits;
 }
 
 __device__ __forceinline__ float max8(const float* z) {
@@ -110,229 +224,278 @@ __device__ __forceinline__ float sum8(const float* z) {
   return ((z[0] + z[1]) + (z[2] + z[3])) + ((z[4] + z[5]) + (z[6] + z[7]));
 }
 
-template <typename T, int V>
-__global__ void __launch_bounds__(V == 16 ? kBiasThreads : kBiasMaxThreads, 1) bias_softmax_kernel(const __grid_constant__ BiasParams p) {
-  extern __shared__ float smem[];
-  float* tab = smem;                              // bias by distance, [0, near]
-  float* red = smem + bias_slot(p.near) + 1;      // two words per warp
-  const int gn = p.warps * 32, groups = blockDim.x / gn;
-  const int group = threadIdx.x / gn, gt = threadIdx.x - group * gn;
-  const int lane = threadIdx.x & 31, gw = gt >> 5;
-  float* red_max = red + group * p.warps * 2;
-  float* red_sum = red_max + p.warps;
+// kStaged: rows go through shared memory (p.slots vectors a buffer, two buffers a group).
+template <typename T, bool kStaged>
+__global__ void __launch_bounds__(kBiasMaxThreads) bias_softmax_kernel(const __grid_constant__ BiasParams p) {
+  extern __shared__ __align__(16) uint4 smem[];
+  const Group group(p.lanes);
+  const int gn = p.lanes, groups = blockDim.x / gn, gt = group.rank;
+  uint4* buffers = smem + group.id * 2 * p.slots;
+  float* tab = reinterpret_cast<float*>(smem + groups * 2 * p.slots);  // bias by distance, [0, near]
+  float* words = tab + bias_slots(p.near);  // two per warp, for groups of several warps
+  float* words_max = words + (threadIdx.x / 32 - gt / 32) * 2;
+  float* words_sum = words_max + (gn >> 5);
   const int64_t matrix = blockIdx.x / p.ctas;
   const int cta = blockIdx.x - (int)(matrix * p.ctas);
   const float* table = p.table + (matrix % p.heads) * p.buckets;
+  const int64_t base = matrix * p.rows * (int64_t)p.pitch;
+  const int step = p.ctas * groups;
+  int row = p.rows - 1 - (cta * groups + group.id);  // the longest rows first
 
   pdl_wait();
-  for (int d = threadIdx.x; d <= p.near; d += blockDim.x) tab[bias_slot(d)] = table[bucket_of(p, d)] * kLog2e;
+  auto source = [&](int r) { return reinterpret_cast<const uint4*>(p.x + base + (int64_t)r * p.pitch); };
+  if (kStaged) {
+    if (row >= 0) fetch_row(RowWalk(p, row), source(row), buffers, gt, gn);
+    cp_async_commit();
+  }
+  for (int d = threadIdx.x - 8; d < p.near + 8; d += blockDim.x)
+    tab[bias_slot(d)] = table[bucket_of(p, max(d, 0))] * kLog2e;
   __syncthreads();
-  const float far = tab[bias_slot(p.near)];
-  const float sl = p.scale * kLog2e;
-  const int64_t base = matrix * p.rows * (int64_t)p.pitch;
+  const float far = tab[bias_slot(p.near)], sl = p.scale * kLog2e;
+  const F2 far2 = f2(far, far), sl2 = f2(sl, sl);
 
-  for (int i = cta * groups + group; i < p.rows; i += p.ctas * groups) {
-    const int row = p.rows - 1 - i;  // the longest first
-    const RowWalk w(p, row);
-    const uint4* in = reinterpret_cast<const uint4*>(p.x + base + (int64_t)row * p.pitch);
+  RowWalk w(p, max(row, 0));
+  for (int turn = 0; row >= 0; row -= step, turn ^= 1) {
     uint4* out = reinterpret_cast<uint4*>(p.out + base + (int64_t)row * p.pitch);
-    const int chunks = (w.m.n + V * gn - 1) / (V * gn);
-    uint4 raw[V];
-    auto load = [&](int ch) {
-#pragma unroll
-      for (int q = 0; q < V; ++q) {
-        const int j = (ch * V + q) * gn + gt;
-        if (j < w.m.n) raw[q] = __ldcs(in + vector_at(w.m, j));
-      }
-    };
-    load(0);
-    zero_masked(p, w, out, gt, gn);
-    float z[8];
+    const uint4* in = source(row);
+    const uint4* staged = buffers + turn * p.slots;
+    const RowWalk next(p, max(row - step, 0));
+    if (kStaged) {
+      group.sync();  // the row before, in the other buffer, is done with
+      if (row >= step) fetch_row(next, source(row - step), buffers + (turn ^ 1) * p.slots, gt, gn);
+      cp_async_commit();
+      zero_masked(p, w, out, gt, gn);
+      cp_async_wait<1>();
+      group.sync();
+    } else {
+      zero_masked(p, w, out, gt, gn);
+    }
+    auto vec = [&](int j) { return kStaged ? staged[j] : in[vector_at(w.m, j)]; };
+    // A lane's first vector that is not plain, mostly its only one, stays in registers.
+    const int others = w.others(), at0 = vector_at(w.m, w.other(gt));
+    float z[8], z0[8];
+    F2 e[4];
+    uint32_t bits0 = 0;
     float m = -INFINITY;
-#pragma unroll 1
-    for (int ch = 0; ch < chunks; ++ch) {
-      if (ch) load(ch);
-#pragma unroll
-      for (int q = 0; q < V; ++q) {
-        const int j = (ch * V + q) * gn + gt;
-        if (j < w.m.n) {
-          biased8<T>(p, w, tab, far, sl, vector_at(w.m, j) * 8, raw[q], z);
-          m = fmaxf(m, max8(z));
-        }
-      }
+    if (gt < others) {
+      bits0 = biased8<T>(p, w, tab, sl, at0 * 8, vec(w.other(gt)), z0);
+      m = max8(z0);
     }
-    m = redux_max(m);
-    if (p.warps > 1) {
-      if (lane == 0) red_max[gw] = m;
-      group_sync(1 + group, gn);
-      for (int k = 0; k < p.warps; ++k) m = fmaxf(m, red_max[k]);
+    for (int t = gt + gn; t < others; t += gn) {
+      const int j = w.other(t);
+      biased8<T>(p, w, tab, sl, vector_at(w.m, j) * 8, vec(j), z);
+      m = fmaxf(m, max8(z));
     }
-    m = fmaxf(m, -3.0e38f);  // a row of -infinity only: every exponential is 0
+    if (w.f0 + gt < w.f1) {
+      uint32_t most = vector_max<T>(vec(w.f0 + gt));
+#pragma unroll 4
+      for (int j = w.f0 + gt + gn; j < w.f1; j += gn) most = T::max2(most, vector_max<T>(vec(j)));
+      const float2 t = T::unpack(most);
+      m = fmaxf(m, __fmaf_rn(fmaxf(t.x, t.y), sl, far));
+    }
+    m = fmaxf(group.max(m, words_max), -3.0e38f);  // a row of -infinity only: every exponential is 0
+    const F2 minus_m = f2(-m, -m);
+
     float s = 0.f;
-#pragma unroll 1
-    for (int ch = 0; ch < chunks; ++ch) {
-      if (chunks > 1) load(ch);
+    F2 s2 = f2(0.f, 0.f), s3 = s2;
+    if (gt < others) {
 #pragma unroll
-      for (int q = 0; q < V; ++q) {
-        const int j = (ch * V + q) * gn + gt;
-        if (j < w.m.n) {
-          biased8<T>(p, w, tab, far, sl, vector_at(w.m, j) * 8, raw[q], z);
+      for (int q = 0; q < 8; ++q) z0[q] = ex2(z0[q] - m);
+      s = sum8(z0);
+    }
+    for (int t = gt + gn; t < others; t += gn) {
+      const int j = w.other(t);
+      biased8<T>(p, w, tab, sl, vector_at(w.m, j) * 8, vec(j), z);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) z[e] = ex2(z[e] - m);
-          s += sum8(z);
-        }
-      }
+      for (int q = 0; q < 8; ++q) z[q] = ex2(z[q] - m);
+      s += sum8(z);
     }
-    s = warp_sum(s);
-    if (p.warps > 1) {
-      if (lane == 0) red_sum[gw] = s;
-      group_sync(1 + group, gn);
-      s = 0.f;
-      for (int k = 0; k < p.warps; ++k) s += red_sum[k];
+#pragma unroll 2
+    for (int j = w.f0 + gt; j < w.f1; j += gn) {
+      plain_exp<T>(vec(j), sl2, far2, minus_m, e);
+      s2 = f2_add(s2, f2_add(e[0], e[1]));
+      s3 = f2_add(s3, f2_add(e[2], e[3]));
     }
+    const float2 s4 = f2_out(f2_add(s2, s3));
+    s = group.sum(s + (s4.x + s4.y), words_sum);
     const float inv = s == 0.f ? 0.f : rcp_rn(s);  // a NaN stays one
-#pragma unroll 1
-    for (int ch = 0; ch < chunks; ++ch) {
-      if (chunks > 1) load(ch);
+    const F2 inv2 = f2(inv, inv);
+
+    if (gt < others) {
 #pragma unroll
-      for (int q = 0; q < V; ++q) {
-        const int j = (ch * V + q) * gn + gt;
-        if (j < w.m.n) {
-          const int vec = vector_at(w.m, j);
-          biased8<T>(p, w, tab, far, sl, vec * 8, raw[q], z);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) z[e] = ex2(z[e] - m) * inv;
-          if (!((vec * 8 >= w.v.lo && vec * 8 + 8 <= w.v.hi) || vec * 8 + 8 <= w.v.s_end)) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-              if (!sees(w.v, vec * 8 + e)) z[e] = 0.f;  // +0.0 also where the row is NaN
-          }
-          __stcs(out + vec, pack8<T>(z));
-        }
-      }
+      for (int q = 0; q < 8; ++q) z0[q] = (bits0 >> q) & 1 ? z0[q] * inv : 0.f;  // +0.0 in a NaN row too
+      __stcs(out + at0, pack8<T>(z0));
     }
+    for (int t = gt + gn; t < others; t += gn) {
+      const int j = w.other(t), at = vector_at(w.m, j);
+      const uint32_t bits = biased8<T>(p, w, tab, sl, at * 8, vec(j), z);
+#pragma unroll
+      for (int q = 0; q < 8; ++q) z[q] = (bits >> q) & 1 ? ex2(z[q] - m) * inv : 0.f;
+      __stcs(out + at, pack8<T>(z));
+    }
+    uint4* plain_out = out + (w.m.w_beg - w.m.n_sink);  // plain vectors are the window's
+#pragma unroll 2
+    for (int j = w.f0 + gt; j < w.f1; j += gn) {
+      plain_exp<T>(vec(j), sl2, far2, minus_m, e);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const float2 t = f2_out(f2_mul(e[q], inv2));
+        z[2 * q] = t.x;
+        z[2 * q + 1] = t.y;
+      }
+      __stcs(plain_out + j, pack8<T>(z));
+    }
+    w = next;
   }
   pdl_trigger();
 }
 
-template <typename T, int V>
-__global__ void __launch_bounds__(kBiasMaxThreads, 1) bias_backward_kernel(const __grid_constant__ BiasParams p) {
-  extern __shared__ float smem[];
-  const int gn = p.warps * 32, groups = blockDim.x / gn;
-  const int group = threadIdx.x / gn, gt = threadIdx.x - group * gn;
-  const int lane = threadIdx.x & 31, gw = gt >> 5;
-  const int slots = bias_slot(p.near) + 1;
-  float* acc = smem + group * slots;                      // sums by distance, [0, near)
-  float* red = smem + groups * slots + group * p.warps * 2;  // two sets, used in turn
-  float* far_sums = smem + groups * slots + blockDim.x / 32 * 2;  // one per warp
+template <typename T, bool kStaged>
+__global__ void __launch_bounds__(kBiasMaxThreads) bias_backward_kernel(const __grid_constant__ BiasParams p) {
+  extern __shared__ __align__(16) uint4 smem[];
+  const Group group(p.lanes);
+  const int gn = p.lanes, groups = blockDim.x / gn, gt = group.rank, lane = threadIdx.x & 31;
+  const int slots = bias_slots(p.near);
+  uint4* buffers = smem + group.id * 4 * p.slots;  // two rows of p, two of dp
+  float* sums = reinterpret_cast<float*>(smem + groups * 4 * p.slots);
+  float* acc = sums + group.id * slots;  // sums by distance, [0, near)
+  float* words = sums + groups * slots + (threadIdx.x / 32 - gt / 32);  // one per warp
+  float* far_sums = sums + groups * slots + blockDim.x / 32;  // one per warp
   const int64_t matrix = blockIdx.x / p.ctas;
   const int cta = blockIdx.x - (int)(matrix * p.ctas);
-  for (int d = gt; d < slots; d += gn) acc[d] = 0.f;
-  group_sync(1 + group, gn);
-  pdl_wait();
   const int64_t base = matrix * p.rows * (int64_t)p.pitch;
-  float far = 0.f;
-  int turn = 0;
+  const int step = p.ctas * groups;
+  int row = p.rows - 1 - (cta * groups + group.id);
+  for (int d = gt; d < slots; d += gn) acc[d] = 0.f;
 
-  for (int i = cta * groups + group; i < p.rows; i += p.ctas * groups) {
-    const int row = p.rows - 1 - i;
-    const RowWalk w(p, row);
-    const uint4* in = reinterpret_cast<const uint4*>(p.x + base + (int64_t)row * p.pitch);
-    const uint4* in2 = reinterpret_cast<const uint4*>(p.dp + base + (int64_t)row * p.pitch);
+  pdl_wait();
+  auto source = [&](const uint16_t* x, int r) { return reinterpret_cast<const uint4*>(x + base + (int64_t)r * p.pitch); };
+  auto fetch = [&](const RowWalk& w, int r, uint4* to) {
+    fetch_row(w, source(p.x, r), to, gt, gn);
+    fetch_row(w, source(p.dp, r), to + p.slots, gt, gn);
+  };
+  if (kStaged) {
+    if (row >= 0) fetch(RowWalk(p, row), row, buffers);
+    cp_async_commit();
+  }
+  group.sync();
+  float far = 0.f;
+
+  RowWalk w(p, max(row, 0));
+  for (int turn = 0; row >= 0; row -= step, turn ^= 1) {
     uint4* out = reinterpret_cast<uint4*>(p.out + base + (int64_t)row * p.pitch);
-    const int chunks = (w.m.n + V * gn - 1) / (V * gn);
-    uint4 raw[V], raw2[V];
-    auto load = [&](int ch) {
+    const uint4* in = source(p.x, row);
+    const uint4* in2 = source(p.dp, row);
+    const uint4* staged = buffers + turn * 2 * p.slots;
+    const RowWalk next(p, max(row - step, 0));
+    group.sync();  // the row before is done with: its buffer, and its additions to acc
+    if (kStaged) {
+      if (row >= step) fetch(next, row - step, buffers + (turn ^ 1) * 2 * p.slots);
+      cp_async_commit();
+      zero_masked(p, w, out, gt, gn);
+      cp_async_wait<1>();
+      group.sync();
+    } else {
+      zero_masked(p, w, out, gt, gn);
+    }
+    auto vec = [&](int j) { return kStaged ? staged[j] : in[vector_at(w.m, j)]; };
+    auto vec2 = [&](int j) { return kStaged ? staged[p.slots + j] : in2[vector_at(w.m, j)]; };
+    const int others = w.others(), at0 = vector_at(w.m, w.other(gt));
+    float a[8], g[8], a0[8], g0[8];
+    F2 x[4], y[4];
+    // p and dp of any vector, 0 where masked.
+    auto masked8 = [&](int j, int at, float* a, float* g) {
+      unpack8<T>(vec(j), a);
+      unpack8<T>(vec2(j), g);
+      const uint32_t bits = visible_bits(w.v, at * 8);
 #pragma unroll
-      for (int q = 0; q < V; ++q) {
-        const int j = (ch * V + q) * gn + gt;
-        if (j < w.m.n) {
-          raw[q] = __ldcs(in + vector_at(w.m, j));
-          raw2[q] = __ldcs(in2 + vector_at(w.m, j));
-        }
-      }
+      for (int q = 0; q < 8; ++q)
+        if (!((bits >> q) & 1)) a[q] = g[q] = 0.f;
+      return bits;
     };
-    auto values = [&](int q, int c0, float* a, float* g) {
-      unpack8<T>(raw[q], a);
-      unpack8<T>(raw2[q], g);
-      if (!((c0 >= w.v.lo && c0 + 8 <= w.v.hi) || c0 + 8 <= w.v.s_end)) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (!sees(w.v, c0 + e)) a[e] = g[e] = 0.f;
-      }
-    };
-    load(0);
-    zero_masked(p, w, out, gt, gn);
-    float a[8], g[8];
+    uint32_t bits0 = 0;
     float dot = 0.f;
-#pragma unroll 1
-    for (int ch = 0; ch < chunks; ++ch) {
-      if (ch) load(ch);
+    F2 d2 = f2(0.f, 0.f), d3 = d2;
+    if (gt < others) {
+      bits0 = masked8(w.other(gt), at0, a0, g0);
 #pragma unroll
-      for (int q = 0; q < V; ++q) {
-        const int j = (ch * V + q) * gn + gt;
-        if (j < w.m.n) {
-          values(q, vector_at(w.m, j) * 8, a, g);
+      for (int q = 0; q < 8; ++q) dot = __fmaf_rn(a0[q], g0[q], dot);
+    }
+    for (int t = gt + gn; t < others; t += gn) {
+      const int j = w.other(t);
+      masked8(j, vector_at(w.m, j), a, g);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) dot = __fmaf_rn(a[e], g[e], dot);
-        }
+      for (int q = 0; q < 8; ++q) dot = __fmaf_rn(a[q], g[q], dot);
+    }
+#pragma unroll 2
+    for (int j = w.f0 + gt; j < w.f1; j += gn) {
+      unpack_pairs<T>(vec(j), x);
+      unpack_pairs<T>(vec2(j), y);
+      d2 = f2_fma(x[0], y[0], d2);
+      d3 = f2_fma(x[1], y[1], d3);
+      d2 = f2_fma(x[2], y[2], d2);
+      d3 = f2_fma(x[3], y[3], d3);
+    }
+    const float2 d4 = f2_out(f2_add(d2, d3));
+    dot = group.sum(dot + (d4.x + d4.y), words);
+
+    // Distances below 0 (masked) and from near on have slots of their own that
+    // nothing reads or that count to the last bucket; clipped ones go to a register.
+    auto finish8 = [&](int at, uint32_t bits, float* a, const float* g) {
+      const int d0 = w.pos - at * 8;
+      const DistanceSlots slot(d0, p.near);
+#pragma unroll
+      for (int q = 0; q < 8; ++q) a[q] = (bits >> q) & 1 ? a[q] * (g[q] - dot) : 0.f;  // masked: 0 in a NaN row too
+      if (d0 > p.near + 7) {
+        far += sum8(a);
+      } else {
+#pragma unroll
+        for (int q = 0; q < 8; ++q) acc[slot[q]] += a[q];
       }
+#pragma unroll
+      for (int q = 0; q < 8; ++q) a[q] *= p.scale;
+      __stcs(out + at, pack8<T>(a));
+    };
+    if (gt < others) finish8(at0, bits0, a0, g0);
+    for (int t = gt + gn; t < others; t += gn) {
+      const int j = w.other(t), at = vector_at(w.m, j);
+      const uint32_t bits = masked8(j, at, a, g);
+      finish8(at, bits, a, g);
     }
-    dot = warp_sum(dot);
-    if (p.warps > 1) {
-      // The barrier also puts this row's additions into acc behind the last row's.
-      if (lane == 0) red[turn * p.warps + gw] = dot;
-      group_sync(1 + group, gn);
-      dot = 0.f;
-      for (int k = 0; k < p.warps; ++k) dot += red[turn * p.warps + k];
-      turn ^= 1;
-    }
-#pragma unroll 1
-    for (int ch = 0; ch < chunks; ++ch) {
-      if (chunks > 1) load(ch);
+    uint4* plain_out = out + (w.m.w_beg - w.m.n_sink);
+    const F2 minus_dot = f2(-dot, -dot), scale2 = f2(p.scale, p.scale);
+    F2 far2 = f2(0.f, 0.f);
+#pragma unroll 2
+    for (int j = w.f0 + gt; j < w.f1; j += gn) {
+      unpack_pairs<T>(vec(j), x);
+      unpack_pairs<T>(vec2(j), y);
 #pragma unroll
-      for (int q = 0; q < V; ++q) {
-        const int j = (ch * V + q) * gn + gt;
-        if (j < w.m.n) {
-          const int vec = vector_at(w.m, j);
-          values(q, vec * 8, a, g);
+      for (int q = 0; q < 4; ++q) x[q] = f2_mul(x[q], f2_add(y[q], minus_dot));
+      far2 = f2_add(far2, f2_add(f2_add(x[0], x[1]), f2_add(x[2], x[3])));
 #pragma unroll
-          for (int e = 0; e < 8; ++e) a[e] = a[e] * (g[e] - dot);
-          const int d0 = w.pos - vec * 8;
-          if (!((vec * 8 >= w.v.lo && vec * 8 + 8 <= w.v.hi) || vec * 8 + 8 <= w.v.s_end)) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-              if (!sees(w.v, vec * 8 + e)) a[e] = 0.f;  // also where the row is NaN
-          }
-          if (d0 - 7 >= p.near) {
-            far += sum8(a);
-          } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const int d = d0 - e;
-              if (d >= p.near) far += a[e];
-              else if (d >= 0) acc[bias_slot(d)] += a[e];
-            }
-          }
-#pragma unroll
-          for (int e = 0; e < 8; ++e) a[e] *= p.scale;
-          __stcs(out + vec, pack8<T>(a));
-        }
+      for (int q = 0; q < 4; ++q) {
+        const float2 t = f2_out(f2_mul(x[q], scale2));
+        a[2 * q] = t.x;
+        a[2 * q + 1] = t.y;
       }
+      __stcs(plain_out + j, pack8<T>(a));
     }
-    __syncwarp();  // one warp a row: this row's additions before the next row's
+    const float2 far3 = f2_out(far2);
+    far += far3.x + far3.y;
+    w = next;
   }
   far = warp_sum(far);
   if (lane == 0) far_sums[threadIdx.x >> 5] = far;
   __syncthreads();
   float* partial = p.partial + (int64_t)blockIdx.x * p.buckets;
-  for (int b = threadIdx.x >> 5; b < p.buckets; b += blockDim.x >> 5) {
+  for (int b = threadIdx.x >> 5; b < p.buckets; b += blockDim.x / 32) {
     float s = 0.f;
     if (b == p.buckets - 1) {
-      for (int k = lane; k < (int)(blockDim.x >> 5); k += 32) s += far_sums[k];
+      for (int k = lane; k < groups * 8; k += 32) s += sums[(k >> 3) * slots + bias_slot(p.near + (k & 7))];
+      if (lane < (int)(blockDim.x / 32)) s += far_sums[lane];
     } else {
       for (int k = 0; k < groups; ++k)
-        for (int d = p.starts[b] + lane; d < p.starts[b + 1]; d += 32) s += smem[k * slots + bias_slot(d)];
+        for (int d = p.starts[b] + lane; d < p.starts[b + 1]; d += 32) s += sums[k * slots + bias_slot(d)];
     }
     s = warp_sum(s);
     if (lane == 0) partial[b] = s;
@@ -346,21 +509,29 @@ struct BiasReduceParams {
   int32_t batch, heads, ctas, buckets;
 };
 
-// dtable[h, j]: one CTA per head; a warp sums a bucket's partials in 64 bits.
+// dtable[h, j]: grid.x heads, grid.y tiles of 32 buckets. Lanes are buckets, so
+// that a warp's loads are contiguous; the warps take turns at the partials and
+// their sums are added in a fixed order, in 64 bits.
 __global__ void __launch_bounds__(1024) bias_table_kernel(const __grid_constant__ BiasReduceParams p) {
+  __shared__ double sums[32][33];
   pdl_wait();
-  const int h = blockIdx.x, lane = threadIdx.x & 31;
-  const int64_t n = (int64_t)p.batch * p.ctas;
-  for (int b = threadIdx.x >> 5; b < p.buckets; b += blockDim.x >> 5) {
-    double s = 0.0;
-    for (int64_t k = lane; k < n; k += 32) {
-      const int64_t matrix = k / p.ctas * p.heads + h;
-      s += (double)p.partial[(matrix * p.ctas + k % p.ctas) * p.buckets + b];
+  const int h = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int b = blockIdx.y * 32 + lane;
+  double s = 0.0;
+  if (b < p.buckets) {
+    for (int64_t k = 0; k < p.batch; ++k) {
+      const float* part = p.partial + (k * p.heads + h) * p.ctas * (int64_t)p.buckets + b;
+#pragma unroll 4
+      for (int c = warp; c < p.ctas; c += 32) s += (double)part[(int64_t)c * p.buckets];
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    if (lane == 0) p.dtable[h * p.buckets + b] = (float)s;
   }
+  sums[warp][lane] = s;
+  __syncthreads();
+  double t = sums[lane][warp];  // warp: the bucket, lane: whose sum
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+  const int bucket = blockIdx.y * 32 + warp;
+  if (lane == 0 && bucket < p.buckets) p.dtable[h * p.buckets + bucket] = (float)t;
 }
 
 }  // namespace cs

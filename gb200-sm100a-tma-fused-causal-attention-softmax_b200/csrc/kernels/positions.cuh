@@ -34,6 +34,17 @@ CS_HD Visible visible_keys(int64_t p, int32_t keys, int32_t window, int32_t sink
   return v;
 }
 
+// The same for 0 <= p <= 2^31 - 2 in 32-bit arithmetic.
+CS_HD Visible visible_columns(int32_t p, int32_t keys, int32_t window, int32_t sinks) {
+  Visible v;
+  v.hi = p + 1 < keys ? p + 1 : keys;
+  const int32_t lo = window > 0 ? p + 1 - window : 0;
+  const int32_t lo0 = lo > 0 ? lo : 0;
+  v.lo = lo0 < v.hi ? lo0 : v.hi;
+  v.s_end = sinks < v.lo ? sinks : v.lo;
+  return v;
+}
+
 CS_HD bool sees(const Visible& v, int32_t k) { return k < v.s_end || (k >= v.lo && k < v.hi); }
 
 // The 8-element vectors that hold a row's visible columns, numbered densely:
@@ -51,6 +62,14 @@ CS_HD VisibleVectors visible_vectors(const Visible& v) {
   m.w_beg = w_beg;
   m.n = m.n_sink + (w_end - w_beg);
   return m;
+}
+
+CS_HD int32_t clip8(int32_t n) { return n < 0 ? 0 : n > 8 ? 8 : n; }
+
+// Bit e: the row sees column c0 + e.
+CS_HD uint32_t visible_bits(const Visible& v, int32_t c0) {
+  const uint32_t below_hi = (1u << clip8(v.hi - c0)) - 1u, below_lo = (1u << clip8(v.lo - c0)) - 1u;
+  return (below_hi & ~below_lo) | ((1u << clip8(v.s_end - c0)) - 1u);
 }
 
 CS_HD int32_t vector_at(const VisibleVectors& m, int32_t j) { return j < m.n_sink ? j : j - m.n_sink + m.w_beg; }

@@ -16,6 +16,10 @@ struct F16 {
     const __half2 h = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&h);
   }
+  static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+    const __half2 h = __hmax2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
 };
 
 struct BF16 {
@@ -25,6 +29,11 @@ struct BF16 {
   }
   static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
     const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+    const __nv_bfloat162 h =
+        __hmax2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
     return *reinterpret_cast<const uint32_t*>(&h);
   }
 };
@@ -39,6 +48,12 @@ __device__ __forceinline__ void unpack8(const uint4& r, float* f) {
     f[2 * q] = t.x;
     f[2 * q + 1] = t.y;
   }
+}
+
+// Two maxima whose larger one is the vector's.
+template <typename T>
+__device__ __forceinline__ uint32_t vector_max(const uint4& r) {
+  return T::max2(T::max2(r.x, r.y), T::max2(r.z, r.w));
 }
 
 template <typename T>
