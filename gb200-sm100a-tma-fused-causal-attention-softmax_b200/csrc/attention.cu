@@ -11,6 +11,7 @@
 #include "causal_softmax.h"
 #include "internal.hpp"
 #include "kernels/attention_rows.cuh"
+#include "kernels/attention_tokens.cuh"
 
 // Timeout bits of the attention kernels on each device (cs_attention_status).
 static __device__ __align__(256) uint32_t g_attention_status[1];
@@ -124,23 +125,92 @@ int check_workspace(const void* workspace, size_t bytes, int64_t need) {
   return CS_OK;
 }
 
+// Few queries: the kernel for single tokens. Its launch shape.
+struct TokenShape {
+  int rows, dim, blocks, splits;  // rows: 8 or 16 of a block; blocks: per kv head
+  int64_t ctas;
+  int64_t part_bytes, stats_bytes;
+};
+
+constexpr int kTokenQueries = 16;     // longest q_len that takes it
+constexpr int kTokenCtasPerSm = 12;   // about four rounds of resident CTAs, for an even end
+constexpr int kTokenKeysPerCta = 256; // at least: 4 steps a warp
+
+bool few_queries(const cs_attention_args* a) { return a->q_len <= kTokenQueries; }
+
+TokenShape token_shape(const cs_attention_args* a, int sms) {
+  TokenShape s{};
+  const int64_t rows = (int64_t)a->q_len * (a->heads / a->kv_heads);
+  s.rows = rows <= 8 ? 8 : 16;
+  s.dim = a->head_dim <= 64 ? 64 : 128;
+  s.blocks = (int)((rows + s.rows - 1) / s.rows);
+  const int64_t base = (int64_t)a->batch * a->kv_heads * s.blocks;
+  int64_t keys = a->kv_len;
+  if (a->window) keys = std::min<int64_t>(keys, (int64_t)a->window + a->q_len + a->sinks + 32);
+  const int64_t want = ((int64_t)sms * kTokenCtasPerSm + base - 1) / base;
+  s.splits = (int)std::max<int64_t>(1, std::min(want, keys / kTokenKeysPerCta));
+  s.ctas = base * s.splits;
+  if (s.splits > 1) {
+    s.part_bytes = s.ctas * s.rows * s.dim * 4;
+    s.stats_bytes = s.ctas * s.rows * 8;
+  }
+  return s;
+}
+
+using TokenKernel = void (*)(cs::TokenParams);
+
+template <typename T>
+TokenKernel token_kernel_of(int dim, int rows) {
+  if (dim == 64) return rows == 8 ? &cs::attention_tokens_kernel<T, 64, 1> : &cs::attention_tokens_kernel<T, 64, 2>;
+  return rows == 8 ? &cs::attention_tokens_kernel<T, 128, 1> : &cs::attention_tokens_kernel<T, 128, 2>;
+}
+
+int launch_tokens(const cs_attention_args* a, const cs::AttentionParams& p, const TokenShape& s, void* workspace, void* stream) {
+  cs::TokenParams t{};
+  t.a = p;
+  t.part_o = static_cast<float*>(workspace);
+  t.part_stats = reinterpret_cast<float*>(static_cast<char*>(workspace) + s.part_bytes);
+  t.splits = s.splits;
+  t.blocks = s.blocks;
+  t.block_rows = s.rows;
+  t.dim_pad = s.dim;
+  if (s.ctas * s.rows > kI32Max) return fail(CS_ERR_WRONG_LENGTH, "%lld CTAs", (long long)s.ctas);
+  const bool half = a->type == CS_TYPE_F16;
+  cudaError_t e = cs_host::launch(half ? token_kernel_of<cs::F16>(s.dim, s.rows) : token_kernel_of<cs::BF16>(s.dim, s.rows),
+                                  dim3((unsigned)s.ctas), cs::kTokenWarps * 32, 0, stream, t);
+  if (e != cudaSuccess) return fail_cuda(e, "attention, few queries");
+  if (s.splits == 1) return CS_OK;
+  e = cs_host::launch(half ? &cs::attention_join_kernel<cs::F16> : &cs::attention_join_kernel<cs::BF16>,
+                      dim3((unsigned)(s.ctas / s.splits * s.rows)), 128, 0, stream, t);
+  return e == cudaSuccess ? CS_OK : fail_cuda(e, "attention, joining the splits");
+}
+
 }  // namespace
 
 extern "C" {
 
 int64_t cs_attention_workspace(const cs_attention_args* args) {
-  const int rc = check_args(args);
-  return rc ? rc : 0;
+  int rc = check_args(args);
+  if (rc || !few_queries(args)) return rc;
+  cs_host::Device d;
+  rc = cs_host::current_device(&d);
+  if (rc) return rc;
+  const TokenShape s = token_shape(args, d.sms);
+  return s.part_bytes + s.stats_bytes;
 }
 
 int cs_attention(const cs_attention_args* args, void* workspace, size_t workspace_bytes, void* stream) {
   int rc = check_args(args);
-  if (!rc) rc = check_workspace(workspace, workspace_bytes, 0);
   if (rc) return rc;
   cs::AttentionParams p{};
   cs_host::Device d;
   rc = params_of(args, &p, &d);
   if (rc) return rc;
+  if (few_queries(args)) {
+    const TokenShape s = token_shape(args, d.sms);
+    rc = check_workspace(workspace, workspace_bytes, s.part_bytes + s.stats_bytes);
+    return rc ? rc : launch_tokens(args, p, s, workspace, stream);
+  }
   auto* kernel = args->type == CS_TYPE_F16 ? &cs::attention_rows_kernel<cs::F16> : &cs::attention_rows_kernel<cs::BF16>;
   const cudaError_t e = cs_host::launch(kernel, rows_grid(p.q_len, p.batch * p.heads), 128, 0, stream, p);
   return e == cudaSuccess ? CS_OK : fail_cuda(e, "attention");
