@@ -1,5 +1,6 @@
 // C ABI of attention with a sliding window and sinks: argument checks and
 // launches (kernels/attention*.cuh).
+#include <cuda.h>
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -11,6 +12,7 @@
 #include "causal_softmax.h"
 #include "internal.hpp"
 #include "kernels/attention_rows.cuh"
+#include "kernels/attention_tiles.cuh"
 #include "kernels/attention_tokens.cuh"
 
 // Timeout bits of the attention kernels on each device (cs_attention_status).
@@ -72,14 +74,58 @@ cs::Strided strided(const cs_tensor& t) {
   return cs::Strided{static_cast<uint16_t*>(t.data), t.batch_stride, t.token_stride, t.head_stride};
 }
 
-// The current device's status word; also the first use of a device.
+// The driver's tensor-map encoder, looked up once.
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                 const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                 CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiled g_encode = nullptr;
+
+// Boxes of 64 dims x `rows` tokens of one head, 128-byte swizzle. A dimension of
+// size 1 may have any stride: it gets a valid one.
+int make_map(CUtensorMap* map, const cs_attention_args* a, const cs_tensor& t, int32_t tokens, int32_t heads, int rows) {
+  const cuuint64_t row = (cuuint64_t)a->head_dim * 2;
+  const cuuint64_t dims[4] = {(cuuint64_t)a->head_dim, (cuuint64_t)heads, (cuuint64_t)tokens, (cuuint64_t)a->batch};
+  const cuuint64_t strides[3] = {heads > 1 ? (cuuint64_t)t.head_stride * 2 : row, tokens > 1 ? (cuuint64_t)t.token_stride * 2 : row,
+                                 a->batch > 1 ? (cuuint64_t)t.batch_stride * 2 : row};
+  const cuuint32_t box[4] = {64, 1, (cuuint32_t)rows, 1}, step[4] = {1, 1, 1, 1};
+  const CUresult r = g_encode(map, a->type == CS_TYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+                              4, t.data, dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? CS_OK : fail(CS_ERR_CUDA, "tensor map: driver error %d", (int)r);
+}
+
+using TileKernel = void (*)(cs::TileParams);
+
+TileKernel tile_kernel(int type, int dim) {
+  if (type == CS_TYPE_F16) return dim == 64 ? &cs::attention_tiles_kernel<cs::F16, 64> : &cs::attention_tiles_kernel<cs::F16, 128>;
+  return dim == 64 ? &cs::attention_tiles_kernel<cs::BF16, 64> : &cs::attention_tiles_kernel<cs::BF16, 128>;
+}
+
+int tile_smem(int dim) { return dim == 64 ? cs::TileSmem<64>::kBytes : cs::TileSmem<128>::kBytes; }
+
+// First use of a device: kernel attributes, the status word's address.
 int set_up(const cs_host::Device& d, uint32_t** status) {
   static std::mutex mu;
   static uint32_t* words[cs_host::kMaxDeviceIds];
   std::lock_guard<std::mutex> lock(mu);
   if (!words[d.id]) {
+    cudaError_t e = cudaSuccess;
+    if (!g_encode) {
+      void* f = nullptr;
+      cudaDriverEntryPointQueryResult found{};
+      e = cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &found);
+      if (e != cudaSuccess) return fail_cuda(e, "cuTensorMapEncodeTiled");
+      if (found != cudaDriverEntryPointSuccess || !f) return fail(CS_ERR_DEVICE, "the driver has no cuTensorMapEncodeTiled");
+      g_encode = reinterpret_cast<EncodeTiled>(f);
+    }
+    for (int type : {CS_TYPE_F16, CS_TYPE_BF16})
+      for (int dim : {64, 128}) {
+        e = cudaFuncSetAttribute(reinterpret_cast<const void*>(tile_kernel(type, dim)),
+                                 cudaFuncAttributeMaxDynamicSharedMemorySize, tile_smem(dim));
+        if (e != cudaSuccess) return fail_cuda(e, "attention kernels");
+      }
     uint32_t* w = nullptr;
-    const cudaError_t e = cudaGetSymbolAddress(reinterpret_cast<void**>(&w), g_attention_status);
+    e = cudaGetSymbolAddress(reinterpret_cast<void**>(&w), g_attention_status);
     if (e != cudaSuccess) return fail_cuda(e, "attention status word");
     words[d.id] = w;
   }
@@ -185,6 +231,23 @@ int launch_tokens(const cs_attention_args* a, const cs::AttentionParams& p, cons
   return e == cudaSuccess ? CS_OK : fail_cuda(e, "attention, joining the splits");
 }
 
+int launch_tiles(const cs_attention_args* a, const cs::AttentionParams& p, void* stream) {
+  cs::TileParams t{};
+  t.a = p;
+  int rc = make_map(&t.q, a, a->q, a->q_len, a->heads, cs::kTile);
+  if (!rc) rc = make_map(&t.k, a, a->k, a->kv_len, a->kv_heads, cs::kTile);
+  if (!rc) rc = make_map(&t.v, a, a->v, a->kv_len, a->kv_heads, cs::kTile);
+  if (!rc) rc = make_map(&t.o, a, a->o, a->q_len, a->heads, cs::kTile);
+  if (rc) return rc;
+  t.q_tiles = (a->q_len + cs::kTile - 1) / cs::kTile;
+  const int64_t ctas = (int64_t)a->batch * a->heads * t.q_tiles;
+  if (ctas > kI32Max) return fail(CS_ERR_WRONG_LENGTH, "%lld CTAs", (long long)ctas);
+  const int dim = a->head_dim <= 64 ? 64 : 128;
+  const cudaError_t e = cs_host::launch(tile_kernel(a->type, dim), dim3((unsigned)ctas), cs::kTileThreads,
+                                        (size_t)tile_smem(dim), stream, t);
+  return e == cudaSuccess ? CS_OK : fail_cuda(e, "attention, tiles");
+}
+
 }  // namespace
 
 extern "C" {
@@ -211,9 +274,7 @@ int cs_attention(const cs_attention_args* args, void* workspace, size_t workspac
     rc = check_workspace(workspace, workspace_bytes, s.part_bytes + s.stats_bytes);
     return rc ? rc : launch_tokens(args, p, s, workspace, stream);
   }
-  auto* kernel = args->type == CS_TYPE_F16 ? &cs::attention_rows_kernel<cs::F16> : &cs::attention_rows_kernel<cs::BF16>;
-  const cudaError_t e = cs_host::launch(kernel, rows_grid(p.q_len, p.batch * p.heads), 128, 0, stream, p);
-  return e == cudaSuccess ? CS_OK : fail_cuda(e, "attention");
+  return launch_tiles(args, p, stream);
 }
 
 int64_t cs_attention_backward_workspace(const cs_attention_args* args) {

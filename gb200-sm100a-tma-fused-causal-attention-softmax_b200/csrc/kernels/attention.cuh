@@ -7,6 +7,8 @@
 
 namespace cs {
 
+constexpr uint64_t kWaitNs = 2000000000ull;  // bound on a device-side wait: 2 s of GPU time
+
 struct Strided {  // [batch, token, head, dim], element strides, dim contiguous
   uint16_t* data;
   int64_t batch, token, head;

@@ -1,4 +1,4 @@
-// Attention, one warp per row: the plain form of the formulas.
+// Gradients of attention, one warp per row: the plain form of the formulas.
 //
 // Lane l holds dims 4 l .. 4 l + 3 of a row; a score is a warp sum.
 #pragma once
@@ -33,39 +33,7 @@ __device__ __forceinline__ void add4(float4& a, float s, float4 b) {
 
 __device__ __forceinline__ float4 times4(float4 a, float s) { return make_float4(a.x * s, a.y * s, a.z * s, a.w * s); }
 
-// Warp index -> (batch, head, query); grid.y = batch * heads.
-template <typename T>
-__global__ void __launch_bounds__(128) attention_rows_kernel(const __grid_constant__ AttentionParams p) {
-  pdl_wait();
-  const int lane = threadIdx.x & 31, i = blockIdx.x * 4 + (threadIdx.x >> 5);
-  if (i >= p.q_len) return;
-  for (int bh = blockIdx.y; bh < p.batch * p.heads; bh += gridDim.y) {
-    const int b = bh / p.heads, h = bh - b * p.heads, hk = h / p.group;
-    const Lengths n(p, b);
-    const Visible v = visible_keys(i < n.q ? n.position(i) : -1, n.kv, p.window, p.sinks);
-    const float4 q = load_dims<T>(p.q.at(b, i, h), lane, p.head_dim);
-    const float sl = p.scale * kLog2e;
-    float m = -INFINITY, s = 0.f;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int k = v.s_end > 0 ? 0 : v.lo; k < v.hi; ++k) {
-      if (k == v.s_end && (k = v.lo) >= v.hi) break;
-      const float x = dot4(q, load_dims<T>(p.k.at(b, k, hk), lane, p.head_dim)) * sl;
-      if (x > m) {
-        const float f = ex2(m - x);
-        s *= f;
-        o = times4(o, f);
-        m = x;
-      }
-      const float e = ex2(x - m);
-      s += e;
-      add4(o, e, load_dims<T>(p.v.at(b, k, hk), lane, p.head_dim));
-    }
-    store_dims<T>(p.o.at(b, i, h), lane, p.head_dim, times4(o, s == 0.f ? 0.f : rcp_rn(s)));
-    if (p.lse && lane == 0) p.lse[(int64_t)bh * p.q_len + i] = s == 0.f ? -INFINITY : (m + __log2f(s)) * (1.f / kLog2e);
-  }
-}
-
-// dq and delta, one warp per query.
+// dq and delta, one warp per query; grid.y = batch * heads.
 template <typename T>
 __global__ void __launch_bounds__(128) attention_dq_rows_kernel(const __grid_constant__ AttentionParams p) {
   pdl_wait();

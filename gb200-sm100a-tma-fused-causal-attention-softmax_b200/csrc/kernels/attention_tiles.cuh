@@ -1,0 +1,354 @@
+// Attention of many queries: tiles of 128 queries x 128 keys on the
+// 5th-generation tensor core.
+//
+// A CTA owns one tile of queries of one head and streams key and value tiles
+// through a ring of shared-memory stages; two CTAs share an SM.
+//
+//   warps 0-3: softmax, one thread per query; they hold a row of 128 scores
+//   warp 4:    TMA loads     warp 5: products (one thread)     6, 7: no work
+//
+// The second four give registers to the first: 128 x 176 + 128 x 80 = 256 x 128.
+//
+// Per key tile: S = Q K^T (TMEM, fp32) -> the softmax warps read their rows and
+// write P over S as 16-bit pairs -> O += P V with P from TMEM. S of the next key
+// tile follows P V in the tensor core's queue, so S overwrites P only after its
+// use, and once S is there O is complete and may be rescaled. While one CTA is
+// in its softmax the tensor core works for the other, whose start and end it
+// also covers. Measured against one CTA an SM with two query tiles that share
+// each key tile (half the L2 traffic): 16384 queries x 16 heads, window 4096,
+// dim 128: 468 us against 509; dim 64: 425 against 459; 512 over 8192: 112
+// against 147.
+//
+// Running maximum: it moves only when a row passes it by more than 2^8, so the
+// output in TMEM is rescaled rarely (all sums are relative to the same
+// maximum, so the result does not depend on it). P is rounded to 16 bits for
+// the tensor core, fp16 after a factor of 2^7 that keeps small probabilities
+// out of its subnormals; sums are fp32 over unrounded values.
+//
+// Bound: at dim 128 a tile pair costs 1024 tensor-core cycles (two products of
+// 2 128^3 at 8192 a cycle) and 1024 cycles of the exponential unit (128^2 at
+// 16 a cycle), at dim 64 512 and 1024.
+#pragma once
+
+#include "attention.cuh"
+#include "tcgen05.cuh"
+
+namespace cs {
+
+constexpr int kTile = 128;
+
+struct TileParams {
+  CUtensorMap q, k, v, o;
+  AttentionParams a;
+  int32_t q_tiles;  // per head
+};
+
+// The visible keys of a tile of queries: the union over its rows, and what
+// all of its rows see.
+struct TileKeys {
+  int32_t s_end, lo, hi;             // union: [0, s_end) and [lo, hi)
+  int32_t all_s_end, all_lo, all_hi; // every row sees [0, all_s_end) and [all_lo, all_hi)
+  __device__ __forceinline__ TileKeys(const AttentionParams& p, const Lengths& n, int i0) {
+    s_end = lo = hi = all_s_end = all_lo = all_hi = 0;
+    const int i1 = min(i0 + kTile, n.q) - 1;
+    if (i0 > i1) return;
+    const Visible first = visible_keys(n.position(i0), n.kv, p.window, p.sinks);
+    const Visible last = visible_keys(n.position(i1), n.kv, p.window, p.sinks);
+    lo = first.lo;
+    hi = last.hi;
+    s_end = min(last.s_end, lo);
+    all_lo = last.lo;
+    all_hi = first.hi;
+    all_s_end = first.s_end;
+  }
+  __device__ __forceinline__ bool every(int k0) const {
+    return k0 + kTile <= all_s_end || (k0 >= all_lo && k0 + kTile <= all_hi);
+  }
+};
+
+// A query tile's key tiles, numbered densely.
+struct TileList {
+  int32_t n_sink, w_beg, n;
+  __device__ __forceinline__ explicit TileList(const TileKeys& a) {
+    const int s = (a.s_end + kTile - 1) / kTile;
+    w_beg = a.lo < a.hi ? a.lo / kTile : s;
+    n_sink = min(s, w_beg);
+    n = n_sink + (a.lo < a.hi ? (a.hi + kTile - 1) / kTile - w_beg : s - n_sink);
+  }
+  __device__ __forceinline__ int key(int j) const { return (j < n_sink ? j : j - n_sink + w_beg) * kTile; }
+};
+
+__device__ __forceinline__ uint32_t below_bits(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
+
+// Bit c: the row sees key k0 + c, 32 keys.
+__device__ __forceinline__ uint32_t visible_bits32(const Visible& v, int k0) {
+  return (below_bits(v.hi - k0) & ~below_bits(v.lo - k0)) | below_bits(v.s_end - k0);
+}
+
+// Zero the rows of a staged value (or key) tile that no query of the sequence
+// sees: they may hold NaN, and 0 times NaN is NaN. One warp.
+template <int DP>
+__device__ __forceinline__ void clear_unseen(const Visible& seen, uint8_t* tile, int k0, int lane) {
+  if (k0 + kTile <= seen.s_end || (k0 >= seen.lo && k0 + kTile <= seen.hi)) return;
+  for (int r = 0; r < kTile; ++r) {
+    if (sees(seen, k0 + r)) continue;
+#pragma unroll
+    for (int box = 0; box < DP / 64; ++box)
+      if (lane < 8) *reinterpret_cast<uint4*>(tile + box * (kTile * 128) + r * 128 + lane * 16) = make_uint4(0, 0, 0, 0);
+  }
+  fence_proxy_async_smem();
+  __syncwarp();
+}
+
+// What the queries of a sequence see together.
+__device__ __forceinline__ Visible sequence_keys(const AttentionParams& p, const Lengths& n) {
+  Visible v{0, 0, 0};
+  if (n.q > 0) {
+    const Visible first = visible_keys(n.position(0), n.kv, p.window, p.sinks);
+    v = visible_keys(n.position(n.q - 1), n.kv, p.window, p.sinks);
+    v.lo = min(v.lo, first.lo);
+    v.s_end = min(v.s_end, v.lo);
+  }
+  return v;
+}
+
+template <int DP>
+struct TileSmem {
+  static constexpr int kTileBytes = kTile * DP * 2;
+  static constexpr int kStages = DP == 128 ? 2 : 4;
+  static constexpr int kBytes = (1 + kStages) * kTileBytes + 1024;  // 1024: alignment of the swizzle
+};
+
+struct TileBarriers {
+  uint64_t q_full, s_full, p_full, o_full, kv_full[4], kv_empty[4];
+  uint32_t tmem, gone;
+};
+
+constexpr int kTileThreads = 256;
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kTileThreads, 2) attention_tiles_kernel(const __grid_constant__ TileParams tp) {
+  using Smem = TileSmem<DP>;
+  constexpr int kStages = Smem::kStages, kTileBytes = Smem::kTileBytes, kBox = kTile * 128;
+  constexpr uint32_t kColumns = 256;
+  constexpr float kShift = T::kIsHalf ? 7.f : 0.f, kMaxLag = 8.f;
+  extern __shared__ uint8_t dynamic[];
+  __shared__ TileBarriers bars;
+  uint8_t* q_tile = dynamic + ((1024 - (smem_addr(dynamic) & 1023)) & 1023);
+  uint8_t* stages = q_tile + kTileBytes;
+  const AttentionParams& p = tp.a;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (warp == 4 && lane == 0) {
+    mbar_init(&bars.q_full, 1);
+    mbar_init(&bars.s_full, 1);
+    mbar_init(&bars.p_full, 4);
+    mbar_init(&bars.o_full, 1);
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(&bars.kv_full[i], 1);
+      mbar_init(&bars.kv_empty[i], 1);
+    }
+    bars.gone = 0;
+    fence_barrier_init();
+    prefetch_map(&tp.q);
+    prefetch_map(&tp.k);
+    prefetch_map(&tp.v);
+    prefetch_map(&tp.o);
+  }
+  if (warp == 5) tmem_alloc(&bars.tmem, kColumns);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = bars.tmem, s_tmem = tmem, o_tmem = tmem + 128;
+  pdl_wait();
+
+  // Which tile: the longest (latest) queries first.
+  const int bk = blockIdx.x % (p.batch * p.kv_heads), unit = blockIdx.x / (p.batch * p.kv_heads);
+  const int b = bk / p.kv_heads, hk = bk - b * p.kv_heads;
+  const int head = hk * p.group + unit % p.group, first = (tp.q_tiles - 1 - unit / p.group) * kTile;
+  const Lengths len(p, b);
+  const TileKeys keys(p, len, first);
+  const TileList list(keys);
+  const Waiter wait{&bars.gone, p.status, kWaitNs};
+
+  if (warp >= 4) {
+    registers_down<80>();
+    if (warp == 4) {
+      // ---- loads
+      if (lane == 0) {
+        mbar_arrive_expect_tx(&bars.q_full, kTileBytes);
+#pragma unroll
+        for (int box = 0; box < DP / 64; ++box)
+          tma_load(q_tile + box * kBox, &tp.q, box * 64, head, first, b, &bars.q_full);
+        RingPos ring;
+        for (int j = 0; j < 2 * list.n; ++j, ring.next(kStages)) {  // K and V in turn
+          if (!wait(&bars.kv_empty[ring.s], ring.ph ^ 1)) break;
+          mbar_arrive_expect_tx(&bars.kv_full[ring.s], kTileBytes);
+#pragma unroll
+          for (int box = 0; box < DP / 64; ++box)
+            tma_load(stages + ring.s * kTileBytes + box * kBox, j & 1 ? &tp.v : &tp.k, box * 64, hk, list.key(j >> 1), b,
+                     &bars.kv_full[ring.s]);
+        }
+      }
+      __syncwarp();
+    } else if (warp == 5) {
+      // ---- products: S(j), then P(j) V(j) and S(j + 1), ...
+      const Visible seen = sequence_keys(p, len);
+      auto warp_wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)) != 0; };
+      RingPos ring;
+      bool ok = warp_wait(&bars.q_full, 0);
+      for (int j = 0; j <= list.n && ok; ++j) {
+        if (j > 0) {
+          const uint8_t* tile = stages + ring.s * kTileBytes;
+          if (!warp_wait(&bars.kv_full[ring.s], ring.ph)) break;
+          clear_unseen<DP>(seen, stages + ring.s * kTileBytes, list.key(j - 1), lane);
+          if (!warp_wait(&bars.p_full, (j - 1) & 1)) break;
+          tc_fence_after();
+          if (lane == 0) {
+            mma_columns<T, DP, kTile>(o_tmem, s_tmem, tile, kBox, j > 1);
+            mma_commit(&bars.kv_empty[ring.s]);
+          }
+          ring.next(kStages);
+        }
+        if (j < list.n) {
+          if (!warp_wait(&bars.kv_full[ring.s], ring.ph)) break;
+          if (lane == 0) {
+            mma_rows<T, DP, kTile>(s_tmem, q_tile, kBox, stages + ring.s * kTileBytes, kBox);
+            mma_commit(&bars.s_full);
+            mma_commit(&bars.kv_empty[ring.s]);
+          }
+          ring.next(kStages);
+        } else if (lane == 0) {
+          mma_commit(&bars.o_full);
+        }
+        __syncwarp();
+      }
+    }
+  } else {
+    // ---- softmax, one thread per query
+    registers_up<176>();
+    const int i = first + threadIdx.x;
+    const uint32_t lanes = (uint32_t)(warp * 32) << 16;
+    const uint32_t s_at = s_tmem + lanes, o_at = o_tmem + lanes;
+    const bool in = i < len.q;
+    const Visible see = visible_keys(in ? len.position(i) : -1, len.kv, p.window, p.sinks);
+    // Scale 0 would make masked scores 0 * -infinity; the least normal number
+    // gives the same result for scores below 10^30.
+    const float sl = fmaxf(p.scale * kLog2e, 1.1754944e-38f);
+    float m = -INFINITY, l = 0.f;
+    bool ok = true;
+    for (int j = 0; j < list.n; ++j) {
+      const int k0 = list.key(j);
+      ok = __all_sync(0xffffffffu, wait(&bars.s_full, j & 1));
+      if (!ok) break;
+      tc_fence_after();
+      uint32_t raw[128];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tmem_load32(s_at + c * 32, raw + c * 32);
+      tmem_wait_loads();
+      if (!keys.every(k0)) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const uint32_t bits = visible_bits32(see, k0 + c * 32);
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            if (!((bits >> e) & 1)) raw[c * 32 + e] = 0xFF800000u;
+        }
+      }
+      float top = __uint_as_float(raw[0]);
+#pragma unroll
+      for (int e = 1; e < 128; ++e) top = fmaxf(top, __uint_as_float(raw[e]));
+      top *= sl;
+      if (__any_sync(0xffffffffu, top > m + kMaxLag)) {
+        const float next = fmaxf(m, top), f = next == -INFINITY ? 1.f : ex2(m - next);
+        m = next;
+        l *= f;
+        if (j > 0) {
+#pragma unroll 1
+          for (int c = 0; c < DP; c += 32) {
+            uint32_t o[32];
+            tmem_load32(o_at + c, o);
+            tmem_wait_loads();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+            tmem_store32(o_at + c, o);
+          }
+        }
+      }
+      const float nb = m == -INFINITY ? 0.f : kShift - m;
+      float sum0 = 0.f, sum1 = 0.f;
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        uint32_t packed[32];
+#pragma unroll
+        for (int e = 0; e < 32; ++e) {
+          const float x = ex2(__fmaf_rn(__uint_as_float(raw[c * 64 + 2 * e]), sl, nb));
+          const float y = ex2(__fmaf_rn(__uint_as_float(raw[c * 64 + 2 * e + 1]), sl, nb));
+          sum0 += x;
+          sum1 += y;
+          packed[e] = T::pack(x, y);
+        }
+        tmem_store32(s_at + c * 32, packed);
+      }
+      l += sum0 + sum1;
+      tmem_wait_stores();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars.p_full);
+    }
+    // ---- output, staged where the queries were
+    if (ok) ok = __all_sync(0xffffffffu, wait(&bars.o_full, 0));
+    if (ok) {
+      tc_fence_after();
+      const float inv = !in || l == 0.f ? 0.f : l > 0.f ? rcp_rn(l) : l;  // a NaN stays one
+      const bool some = list.n > 0 && inv != 0.f;
+      uint8_t* row = q_tile + threadIdx.x * 128;
+      const int swizzle = lane & 7;
+#pragma unroll 1
+      for (int c = 0; c < DP; c += 32) {
+        uint32_t o[32];
+        if (list.n > 0) {
+          tmem_load32(o_at + c, o);
+          tmem_wait_loads();
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          uint32_t w[4];
+#pragma unroll
+          for (int h = 0; h < 4; ++h)
+            w[h] = some ? T::pack(__uint_as_float(o[8 * e + 2 * h]) * inv, __uint_as_float(o[8 * e + 2 * h + 1]) * inv) : 0u;
+          const int chunk = (c & 63) / 8 + e;
+          *reinterpret_cast<uint4*>(row + (c >> 6) * kBox + ((chunk ^ swizzle) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+      }
+      if (p.lse && i < p.q_len)
+        p.lse[((int64_t)b * p.heads + head) * p.q_len + i] =
+            !in || l == 0.f ? -INFINITY : (m - kShift + __log2f(l)) * (1.f / kLog2e);
+      fence_proxy_async_smem();
+    }
+    asm volatile("bar.sync 1, 128;" ::: "memory");
+    if (threadIdx.x == 0 && !*(volatile uint32_t*)&bars.gone) {
+#pragma unroll
+      for (int box = 0; box < DP / 64; ++box)
+        if (box * 64 < p.head_dim) tma_store(&tp.o, q_tile + box * kBox, box * 64, head, first, b);
+      bulk_commit();
+      bulk_wait_all();
+    }
+  }
+  // ---- end
+  tc_fence_before();
+  __syncthreads();
+  pdl_trigger();
+  if (bars.gone) {
+    // Given up: let copies and products in flight land before the memory goes.
+    const uint64_t start = global_timer_ns();
+    while (global_timer_ns() - start < 1000000ull) {}
+    __syncthreads();
+  }
+  if (warp == 5) {
+    tc_fence_after();
+    tmem_free(tmem, kColumns);
+  }
+}
+
+}  // namespace cs
