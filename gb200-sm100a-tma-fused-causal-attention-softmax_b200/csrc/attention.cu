@@ -11,7 +11,7 @@
 #include "causal_attention.h"
 #include "causal_softmax.h"
 #include "internal.hpp"
-#include "kernels/attention_rows.cuh"
+#include "kernels/attention_backward.cuh"
 #include "kernels/attention_tiles.cuh"
 #include "kernels/attention_tokens.cuh"
 
@@ -103,6 +103,26 @@ TileKernel tile_kernel(int type, int dim) {
 
 int tile_smem(int dim) { return dim == 64 ? cs::TileSmem<64>::kBytes : cs::TileSmem<128>::kBytes; }
 
+using GradKernel = void (*)(cs::GradParams);
+
+GradKernel dq_kernel(int type, int dim) {
+  if (type == CS_TYPE_F16) return dim == 64 ? &cs::attention_dq_kernel<cs::F16, 64> : &cs::attention_dq_kernel<cs::F16, 128>;
+  return dim == 64 ? &cs::attention_dq_kernel<cs::BF16, 64> : &cs::attention_dq_kernel<cs::BF16, 128>;
+}
+
+GradKernel dkv_kernel(int type, int dim) {
+  if (type == CS_TYPE_F16) return dim == 64 ? &cs::attention_dkv_kernel<cs::F16, 64> : &cs::attention_dkv_kernel<cs::F16, 128>;
+  return dim == 64 ? &cs::attention_dkv_kernel<cs::BF16, 64> : &cs::attention_dkv_kernel<cs::BF16, 128>;
+}
+
+GradKernel dkv_join_kernel(int type, int dim) {
+  if (type == CS_TYPE_F16) return dim == 64 ? &cs::attention_dkv_join_kernel<cs::F16, 64> : &cs::attention_dkv_join_kernel<cs::F16, 128>;
+  return dim == 64 ? &cs::attention_dkv_join_kernel<cs::BF16, 64> : &cs::attention_dkv_join_kernel<cs::BF16, 128>;
+}
+
+int dq_smem(int dim) { return dim == 64 ? cs::QuerySmem<64>::kBytes : cs::QuerySmem<128>::kBytes; }
+int dkv_smem(int dim) { return dim == 64 ? cs::KeySmem<64>::kBytes : cs::KeySmem<128>::kBytes; }
+
 // First use of a device: kernel attributes, the status word's address.
 int set_up(const cs_host::Device& d, uint32_t** status) {
   static std::mutex mu;
@@ -122,6 +142,12 @@ int set_up(const cs_host::Device& d, uint32_t** status) {
       for (int dim : {64, 128}) {
         e = cudaFuncSetAttribute(reinterpret_cast<const void*>(tile_kernel(type, dim)),
                                  cudaFuncAttributeMaxDynamicSharedMemorySize, tile_smem(dim));
+        if (e == cudaSuccess)
+          e = cudaFuncSetAttribute(reinterpret_cast<const void*>(dq_kernel(type, dim)),
+                                   cudaFuncAttributeMaxDynamicSharedMemorySize, dq_smem(dim));
+        if (e == cudaSuccess)
+          e = cudaFuncSetAttribute(reinterpret_cast<const void*>(dkv_kernel(type, dim)),
+                                   cudaFuncAttributeMaxDynamicSharedMemorySize, dkv_smem(dim));
         if (e != cudaSuccess) return fail_cuda(e, "attention kernels");
       }
     uint32_t* w = nullptr;
@@ -156,12 +182,6 @@ int params_of(const cs_attention_args* a, cs::AttentionParams* p, cs_host::Devic
   p->scale = a->scale;
   return CS_OK;
 }
-
-dim3 rows_grid(int32_t tokens, int32_t heads) {
-  return dim3((unsigned)((tokens + 3) / 4), (unsigned)std::min(heads, 65535));
-}
-
-int64_t backward_workspace(const cs_attention_args* a) { return (int64_t)a->batch * a->heads * a->q_len * 4; }
 
 int check_workspace(const void* workspace, size_t bytes, int64_t need) {
   if (need == 0) return CS_OK;
@@ -248,6 +268,111 @@ int launch_tiles(const cs_attention_args* a, const cs::AttentionParams& p, void*
   return e == cudaSuccess ? CS_OK : fail_cuda(e, "attention, tiles");
 }
 
+// The backward's launch shapes and workspace.
+struct GradShape {
+  int dim, q_pad, q_tiles, k_tiles;
+  int share, window_shares, sink_tiles, sink_shares;
+  int64_t dkv_ctas;
+  int64_t rows_bytes, norms_bytes, partial_bytes;  // two arrays of rows
+  int64_t bytes() const { return 2 * rows_bytes + norms_bytes + partial_bytes; }
+};
+
+// A key tile's work is its (head, 64 queries) units. Tiles are cut into shares
+// only where that evens out the SMs: the sinks' tile, which every query sees,
+// and tiles of long rows when there are few of them; each share costs a part of
+// dK and dV in fp32, written and read once more. So: about two shares an SM,
+// and no cut of a window's tiles as long as that makes them at most twice as long.
+GradShape grad_shape(const cs_attention_args* a, int sms) {
+  GradShape s{};
+  s.dim = a->head_dim <= 64 ? 64 : 128;
+  s.q_pad = (a->q_len + cs::kSub - 1) / cs::kSub * cs::kSub;
+  s.q_tiles = (a->q_len + cs::kTile - 1) / cs::kTile;
+  s.k_tiles = (a->kv_len + cs::kTile - 1) / cs::kTile;
+  const int64_t group = a->heads / a->kv_heads, heads = (int64_t)a->batch * a->kv_heads;
+  const int64_t all = s.q_pad / cs::kSub * group;  // units of a tile that every query sees
+  int64_t usual = all;
+  if (a->window) {
+    usual = std::min(all, (((int64_t)a->window + cs::kTile - 1 + cs::kSub - 1) / cs::kSub + 1) * group);
+    s.sink_tiles = (int)std::min<int64_t>(s.k_tiles, ((int64_t)a->sinks + cs::kTile - 1) / cs::kTile);
+  }
+  // Without a window tiles see half of the queries on average.
+  const int64_t total = heads * (s.sink_tiles * all + (s.k_tiles - s.sink_tiles) * (a->window ? usual : (usual + 1) / 2));
+  int64_t share = std::max<int64_t>(32, (total + 2 * sms - 1) / (2 * sms));
+  if (usual <= 2 * share) share = std::max(share, usual);
+  s.share = (int)std::min(share, std::max(all, usual));
+  s.window_shares = (int)((usual + s.share - 1) / s.share);
+  s.sink_shares = (int)((all + s.share - 1) / s.share);
+  s.dkv_ctas = heads * ((int64_t)s.sink_tiles * s.sink_shares + (int64_t)(s.k_tiles - s.sink_tiles) * s.window_shares);
+  s.rows_bytes = (int64_t)a->batch * a->heads * s.q_pad * 4;
+  s.norms_bytes = a->type == CS_TYPE_F16 ? (2 * heads * 4 + 15) / 16 * 16 : 0;
+  if (s.window_shares > 1 || (s.sink_tiles && s.sink_shares > 1)) s.partial_bytes = s.dkv_ctas * 2 * cs::kTile * s.dim * 4;
+  return s;
+}
+
+int launch_backward(const cs_attention_args* a, const cs_attention_grads* g, const cs::AttentionParams& p, const GradShape& s,
+                    void* workspace, void* stream) {
+  if (s.dkv_ctas > kI32Max || (int64_t)a->batch * a->heads * s.q_tiles > kI32Max)
+    return fail(CS_ERR_WRONG_LENGTH, "%lld CTAs", (long long)s.dkv_ctas);
+  char* at = static_cast<char*>(workspace);
+  float* lse2 = reinterpret_cast<float*>(at);
+  float* delta = reinterpret_cast<float*>(at + s.rows_bytes);
+  float* norms = reinterpret_cast<float*>(at + 2 * s.rows_bytes);
+  const bool half = a->type == CS_TYPE_F16;
+
+  cs::RowsParams r{};
+  r.a = p;
+  r.lse2 = lse2;
+  r.delta = delta;
+  r.norms = reinterpret_cast<uint32_t*>(norms);
+  r.q_pad = s.q_pad;
+  cudaError_t e = cudaSuccess;
+  if (half) e = cudaMemsetAsync(norms, 0, (size_t)s.norms_bytes, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return fail_cuda(e, "attention backward, norms");
+  const unsigned rows = (unsigned)(s.q_pad / 16 + (half ? (a->kv_len + 15) / 16 : 0));
+  e = cs_host::launch(half ? &cs::attention_rows_kernel<cs::F16> : &cs::attention_rows_kernel<cs::BF16>,
+                      dim3(rows, (unsigned)std::min(a->batch * a->heads, 65535)), 256, 0, stream, r);
+  if (e != cudaSuccess) return fail_cuda(e, "attention backward, rows");
+
+  cs::GradParams k{};
+  k.a = p;
+  k.lse2 = lse2;
+  k.delta = delta;
+  k.norms = norms;
+  k.partial = reinterpret_cast<float*>(at + 2 * s.rows_bytes + s.norms_bytes);
+  k.q_pad = s.q_pad;
+  k.share = s.share;
+  k.window_shares = s.window_shares;
+  k.sink_tiles = s.sink_tiles;
+  k.sink_shares = s.sink_shares;
+  k.tiles = s.k_tiles;
+  int rc = make_map(&k.q, a, a->q, a->q_len, a->heads, cs::kSub);
+  if (!rc) rc = make_map(&k.d_o, a, g->d_o, a->q_len, a->heads, cs::kSub);
+  if (!rc) rc = make_map(&k.k, a, a->k, a->kv_len, a->kv_heads, cs::kTile);
+  if (!rc) rc = make_map(&k.v, a, a->v, a->kv_len, a->kv_heads, cs::kTile);
+  if (!rc) rc = make_map(&k.out0, a, g->dk, a->kv_len, a->kv_heads, cs::kTile);
+  if (!rc) rc = make_map(&k.out1, a, g->dv, a->kv_len, a->kv_heads, cs::kTile);
+  if (rc) return rc;
+  e = cs_host::launch(dkv_kernel(a->type, s.dim), dim3((unsigned)s.dkv_ctas), 384, (size_t)dkv_smem(s.dim), stream, k);
+  if (e != cudaSuccess) return fail_cuda(e, "attention backward, keys");
+
+  cs::GradParams q = k;
+  q.tiles = s.q_tiles;
+  rc = make_map(&q.q, a, a->q, a->q_len, a->heads, cs::kTile);
+  if (!rc) rc = make_map(&q.d_o, a, g->d_o, a->q_len, a->heads, cs::kTile);
+  if (!rc) rc = make_map(&q.k, a, a->k, a->kv_len, a->kv_heads, cs::kSub);
+  if (!rc) rc = make_map(&q.v, a, a->v, a->kv_len, a->kv_heads, cs::kSub);
+  if (!rc) rc = make_map(&q.out0, a, g->dq, a->q_len, a->heads, cs::kTile);
+  if (rc) return rc;
+  e = cs_host::launch(dq_kernel(a->type, s.dim), dim3((unsigned)(a->batch * a->heads * s.q_tiles)), 256, (size_t)dq_smem(s.dim),
+                      stream, q);
+  if (e != cudaSuccess) return fail_cuda(e, "attention backward, queries");
+  if (s.partial_bytes) {
+    const int64_t tiles = (int64_t)a->batch * a->kv_heads * (s.window_shares > 1 ? s.k_tiles : s.sink_tiles);
+    e = cs_host::launch(dkv_join_kernel(a->type, s.dim), dim3((unsigned)tiles, 4), 256, 0, stream, k);
+  }
+  return e == cudaSuccess ? CS_OK : fail_cuda(e, "attention backward, joining the shares");
+}
+
 }  // namespace
 
 extern "C" {
@@ -278,32 +403,30 @@ int cs_attention(const cs_attention_args* args, void* workspace, size_t workspac
 }
 
 int64_t cs_attention_backward_workspace(const cs_attention_args* args) {
-  const int rc = check_args(args);
-  return rc ? rc : backward_workspace(args);
+  int rc = check_args(args);
+  cs_host::Device d;
+  if (!rc) rc = cs_host::current_device(&d);
+  return rc ? rc : grad_shape(args, d.sms).bytes();
 }
 
 int cs_attention_backward(const cs_attention_args* args, const cs_attention_grads* grads, void* workspace,
                           size_t workspace_bytes, void* stream) {
   int rc = check_args(args);
   if (!rc) rc = check_grads(args, grads);
-  if (!rc) rc = check_workspace(workspace, workspace_bytes, backward_workspace(args));
+  if (!rc) rc = check_workspace(workspace, workspace_bytes, 16);
   if (rc) return rc;
   cs::AttentionParams p{};
   cs_host::Device d;
   rc = params_of(args, &p, &d);
   if (rc) return rc;
+  const GradShape s = grad_shape(args, d.sms);
+  rc = check_workspace(workspace, workspace_bytes, s.bytes());
+  if (rc) return rc;
   p.d_o = strided(grads->d_o);
   p.dq = strided(grads->dq);
   p.dk = strided(grads->dk);
   p.dv = strided(grads->dv);
-  p.delta = static_cast<float*>(workspace);
-  const bool half = args->type == CS_TYPE_F16;
-  cudaError_t e = cs_host::launch(half ? &cs::attention_dq_rows_kernel<cs::F16> : &cs::attention_dq_rows_kernel<cs::BF16>,
-                                  rows_grid(p.q_len, p.batch * p.heads), 128, 0, stream, p);
-  if (e != cudaSuccess) return fail_cuda(e, "attention backward, queries");
-  e = cs_host::launch(half ? &cs::attention_dkv_rows_kernel<cs::F16> : &cs::attention_dkv_rows_kernel<cs::BF16>,
-                      rows_grid(p.kv_len, p.batch * p.kv_heads), 128, 0, stream, p);
-  return e == cudaSuccess ? CS_OK : fail_cuda(e, "attention backward, keys");
+  return launch_backward(args, grads, p, s, workspace, stream);
 }
 
 int cs_attention_status(uint32_t* status, void* stream) {

@@ -21,7 +21,6 @@ struct AttentionParams {
   Strided q, k, v, o;       // o: output; backward: the forward's output
   Strided d_o, dq, dk, dv;  // backward
   float* lse;               // [batch, heads, q_len]
-  float* delta;             // backward: sum over dim of d_o * o, as lse
   const int32_t* q_lens;
   const int32_t* kv_lens;
   uint32_t* status;

@@ -61,21 +61,23 @@ struct TileKeys {
     all_hi = first.hi;
     all_s_end = first.s_end;
   }
+  template <int STEP>
   __device__ __forceinline__ bool every(int k0) const {
-    return k0 + kTile <= all_s_end || (k0 >= all_lo && k0 + kTile <= all_hi);
+    return k0 + STEP <= all_s_end || (k0 >= all_lo && k0 + STEP <= all_hi);
   }
 };
 
-// A query tile's key tiles, numbered densely.
+// A query tile's key tiles of STEP keys, numbered densely.
+template <int STEP>
 struct TileList {
   int32_t n_sink, w_beg, n;
   __device__ __forceinline__ explicit TileList(const TileKeys& a) {
-    const int s = (a.s_end + kTile - 1) / kTile;
-    w_beg = a.lo < a.hi ? a.lo / kTile : s;
+    const int s = (a.s_end + STEP - 1) / STEP;
+    w_beg = a.lo < a.hi ? a.lo / STEP : s;
     n_sink = min(s, w_beg);
-    n = n_sink + (a.lo < a.hi ? (a.hi + kTile - 1) / kTile - w_beg : s - n_sink);
+    n = n_sink + (a.lo < a.hi ? (a.hi + STEP - 1) / STEP - w_beg : s - n_sink);
   }
-  __device__ __forceinline__ int key(int j) const { return (j < n_sink ? j : j - n_sink + w_beg) * kTile; }
+  __device__ __forceinline__ int key(int j) const { return (j < n_sink ? j : j - n_sink + w_beg) * STEP; }
 };
 
 __device__ __forceinline__ uint32_t below_bits(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
@@ -85,19 +87,26 @@ __device__ __forceinline__ uint32_t visible_bits32(const Visible& v, int k0) {
   return (below_bits(v.hi - k0) & ~below_bits(v.lo - k0)) | below_bits(v.s_end - k0);
 }
 
-// Zero the rows of a staged value (or key) tile that no query of the sequence
-// sees: they may hold NaN, and 0 times NaN is NaN. One warp.
-template <int DP>
-__device__ __forceinline__ void clear_unseen(const Visible& seen, uint8_t* tile, int k0, int lane) {
-  if (k0 + kTile <= seen.s_end || (k0 >= seen.lo && k0 + kTile <= seen.hi)) return;
-  for (int r = 0; r < kTile; ++r) {
-    if (sees(seen, k0 + r)) continue;
+// Zero the rows of a staged tile for which keep(row) is false: they may hold
+// NaN, and 0 times NaN is NaN. One warp; boxes of ROWS x 64 elements.
+template <int DP, int ROWS, typename Keep>
+__device__ __forceinline__ void clear_rows(uint8_t* tile, int lane, Keep keep) {
+#pragma unroll 1
+  for (int r = 0; r < ROWS; ++r) {
+    if (keep(r)) continue;
 #pragma unroll
     for (int box = 0; box < DP / 64; ++box)
-      if (lane < 8) *reinterpret_cast<uint4*>(tile + box * (kTile * 128) + r * 128 + lane * 16) = make_uint4(0, 0, 0, 0);
+      if (lane < 8) *reinterpret_cast<uint4*>(tile + box * (ROWS * 128) + r * 128 + lane * 16) = make_uint4(0, 0, 0, 0);
   }
   fence_proxy_async_smem();
   __syncwarp();
+}
+
+// Keys (or values) k0.. of which no query of the sequence sees some.
+template <int DP, int ROWS>
+__device__ __forceinline__ void clear_unseen(const Visible& seen, uint8_t* tile, int k0, int lane) {
+  if (k0 + ROWS <= seen.s_end || (k0 >= seen.lo && k0 + ROWS <= seen.hi)) return;
+  clear_rows<DP, ROWS>(tile, lane, [&](int r) { return sees(seen, k0 + r); });
 }
 
 // What the queries of a sequence see together.
@@ -168,7 +177,7 @@ __global__ void __launch_bounds__(kTileThreads, 2) attention_tiles_kernel(const 
   const int head = hk * p.group + unit % p.group, first = (tp.q_tiles - 1 - unit / p.group) * kTile;
   const Lengths len(p, b);
   const TileKeys keys(p, len, first);
-  const TileList list(keys);
+  const TileList<kTile> list(keys);
   const Waiter wait{&bars.gone, p.status, kWaitNs};
 
   if (warp >= 4) {
@@ -198,23 +207,25 @@ __global__ void __launch_bounds__(kTileThreads, 2) attention_tiles_kernel(const 
       RingPos ring;
       bool ok = warp_wait(&bars.q_full, 0);
       for (int j = 0; j <= list.n && ok; ++j) {
+        const int v_slot = ring.s;
         if (j > 0) {
-          const uint8_t* tile = stages + ring.s * kTileBytes;
-          if (!warp_wait(&bars.kv_full[ring.s], ring.ph)) break;
-          clear_unseen<DP>(seen, stages + ring.s * kTileBytes, list.key(j - 1), lane);
-          if (!warp_wait(&bars.p_full, (j - 1) & 1)) break;
-          tc_fence_after();
-          if (lane == 0) {
-            mma_columns<T, DP, kTile>(o_tmem, s_tmem, tile, kBox, j > 1);
-            mma_commit(&bars.kv_empty[ring.s]);
-          }
+          if (!warp_wait(&bars.kv_full[v_slot], ring.ph)) break;
+          clear_unseen<DP, kTile>(seen, stages + v_slot * kTileBytes, list.key(j - 1), lane);
           ring.next(kStages);
         }
+        if (j < list.n && !warp_wait(&bars.kv_full[ring.s], ring.ph)) break;
+        if (j > 0) {
+          if (!warp_wait(&bars.p_full, (j - 1) & 1)) break;
+          tc_fence_after();
+          if (lane == 0) mma_columns<T, DP, kTile>(o_tmem, s_tmem, stages + v_slot * kTileBytes, kBox, j > 1);
+        }
         if (j < list.n) {
-          if (!warp_wait(&bars.kv_full[ring.s], ring.ph)) break;
+          // One queue of products: commits come behind both (a commit between
+          // them cost 7% at 16384 queries, window 4096, dim 128: 508 us, now 474).
           if (lane == 0) {
             mma_rows<T, DP, kTile>(s_tmem, q_tile, kBox, stages + ring.s * kTileBytes, kBox);
             mma_commit(&bars.s_full);
+            if (j > 0) mma_commit(&bars.kv_empty[v_slot]);
             mma_commit(&bars.kv_empty[ring.s]);
           }
           ring.next(kStages);
@@ -246,7 +257,7 @@ __global__ void __launch_bounds__(kTileThreads, 2) attention_tiles_kernel(const 
 #pragma unroll
       for (int c = 0; c < 4; ++c) tmem_load32(s_at + c * 32, raw + c * 32);
       tmem_wait_loads();
-      if (!keys.every(k0)) {
+      if (!keys.every<kTile>(k0)) {
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           const uint32_t bits = visible_bits32(see, k0 + c * 32);
@@ -335,20 +346,7 @@ __global__ void __launch_bounds__(kTileThreads, 2) attention_tiles_kernel(const 
       bulk_wait_all();
     }
   }
-  // ---- end
-  tc_fence_before();
-  __syncthreads();
-  pdl_trigger();
-  if (bars.gone) {
-    // Given up: let copies and products in flight land before the memory goes.
-    const uint64_t start = global_timer_ns();
-    while (global_timer_ns() - start < 1000000ull) {}
-    __syncthreads();
-  }
-  if (warp == 5) {
-    tc_fence_after();
-    tmem_free(tmem, kColumns);
-  }
+  finish_tmem(bars.gone, warp == 5, tmem, kColumns);
 }
 
 }  // namespace cs

@@ -97,8 +97,34 @@ __device__ __forceinline__ void tmem_store32(uint32_t at, const uint32_t* r) {
       : "memory");
 }
 
+__device__ __forceinline__ void tmem_store16(uint32_t at, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(at),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+
 __device__ __forceinline__ void tmem_wait_loads() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_stores() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// End of a kernel that holds TMEM, all threads: after a wait was given up,
+// time for copies and products in flight before their memory goes.
+__device__ __forceinline__ void finish_tmem(volatile uint32_t& gone, bool owner, uint32_t at, uint32_t columns) {
+  tc_fence_before();
+  __syncthreads();
+  pdl_trigger();
+  if (gone) {
+    const uint64_t start = global_timer_ns();
+    while (global_timer_ns() - start < 1000000ull) {}
+    __syncthreads();
+  }
+  if (owner) {
+    tc_fence_after();
+    tmem_free(at, columns);
+  }
+}
 
 // ---- products
 

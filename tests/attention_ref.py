@@ -8,7 +8,11 @@ head_dim products, so it is off by at most E = (dim + 8) 2^-24 scale max|q|.|k|
 (plus the exponential's 2^-20), and a probability by the relative 2 E. What is
 rounded to 16 bits on the way (probabilities before they meet the values, ds
 before it meets q and k) adds u of each term's magnitude. Exponentials below
-FLUSHED, the least normal fp32, count as zero.
+FLUSHED, the least normal fp32, count as zero. In fp16 the backward's
+probabilities are held times 2^15, so those near zero are off by half a subnormal
+step, 2^-25, over 2^15; ds is held times the power of two that brings its bound
+2 max|d_o| max|v| (row norms over a kv head) to between 2^14 and 2^15, so it is
+off by up to 2^-25 of that bound over 2^14.
 """
 from __future__ import annotations
 
@@ -139,11 +143,14 @@ def attention_backward(dout, q, k, v, *, scale, window=0, sinks=0, q_lens=None, 
             # ds: its own rounding, the probability's error, dp's sum in fp32 and the rounded out in the row's sum.
             off = (u + 4 * e) * ds.abs() + p * (u * (G * O).abs().sum(-1, keepdim=True) +
                                                 (4 * e + (dim + 8) * 2 ** -24) * (G.abs() @ V.abs().T))
+            small_p = 2.0 ** -40 if q.dtype == torch.float16 else 0.0
+            group_g = torch.where(sees[:, None, None], dout[b, :nq, hk * group:(hk + 1) * group].double(), 0.0)
+            off += keep * 2.0 ** 2 * small_p * group_g.norm(dim=-1).max() * V.norm(dim=-1).max()
             off += keep * FLUSHED * (dp.abs() + (G * O).sum(-1, keepdim=True).abs())
             g["dq"][0][b, :nq, h] = scale * ds @ K
             g["dq"][1][b, :nq, h] = scale * off @ K.abs()
             g["dk"][0][b, :nk, hk] += scale * ds.T @ Q
             g["dk"][1][b, :nk, hk] += scale * off.T @ Q.abs()
             g["dv"][0][b, :nk, hk] += p.T @ G
-            g["dv"][1][b, :nk, hk] += (u + 4 * e) * (p.T @ G.abs()) + FLUSHED * G.abs().sum(0)
+            g["dv"][1][b, :nk, hk] += (u + 4 * e) * (p.T @ G.abs()) + (FLUSHED + small_p) * G.abs().sum(0)
     return {n: (t, bound + u * t.abs() + 2 * tiny(q.dtype)) for n, (t, bound) in g.items()}

@@ -244,7 +244,9 @@ def test_ragged_batch_with_garbage_behind_the_sequences(q_len, kv_len, q_lens, k
     want = ref.attention_backward(dout, q, k, v, **how, **dev)
     for n, t in zip(("dq", "dk", "dv"), grads):
         within(t, *want[n], n)
-        assert (t[want[n][0] == 0].abs() <= ref.tiny(dtype)).all(), f"{n}: rows outside the sequences are zero"
+        for b in range(4):  # (a row inside may have the exact gradient 0 and be off by its bound)
+            rows = min(max((q_lens if n == "dq" else kv_lens)[b], 0), t.shape[1])
+            assert (t[b, rows:] == 0).all(), f"{n}: rows outside the sequences are zero"
 
 
 @pytest.mark.parametrize("q_len,kv_len", [(1, 200), (190, 200)])
