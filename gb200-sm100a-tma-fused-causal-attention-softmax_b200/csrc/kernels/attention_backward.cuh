@@ -250,6 +250,7 @@ __global__ void __launch_bounds__(256, 2) attention_dq_kernel(const __grid_const
       __syncwarp();
     } else if (warp == 5) {
       const Visible seen = sequence_keys(p, len);
+      const uint32_t one = elect_one();
       auto warp_wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)) != 0; };
       bool ok = warp_wait(&bars.q_full, 0);
       RingPos ring;
@@ -264,20 +265,17 @@ __global__ void __launch_bounds__(256, 2) attention_dq_kernel(const __grid_const
         if (j > 0) {
           if (!warp_wait(&bars.ds_full, (j - 1) & 1)) break;
           tc_fence_after();
-          if (lane == 0) mma_columns<T, DP, kSub>(dq_tmem, dp_tmem, k_last, kSubBox, j > 1);
+          mma_columns<T, DP, kSub>(one, dq_tmem, dp_tmem, k_last, kSubBox, j > 1);
         }
-        if (lane == 0) {
-          if (j < list.n) {
-            mma_rows<T, DP, kSub>(s_tmem, q_tile, kBox, k_tile, kSubBox);
-            mma_rows<T, DP, kSub>(dp_tmem, do_tile, kBox, v_tile, kSubBox);
-            mma_commit(&bars.s_full);
-            mma_commit(&bars.v_empty);
-            if (j > 0) mma_commit(&bars.k_empty[ring.s ^ 1]);
-          } else {
-            mma_commit(&bars.dq_full);
-          }
+        if (j < list.n) {
+          mma_rows<T, DP, kSub>(one, s_tmem, q_tile, kBox, k_tile, kSubBox);
+          mma_rows<T, DP, kSub>(one, dp_tmem, do_tile, kBox, v_tile, kSubBox);
+          mma_commit(one, &bars.s_full);
+          mma_commit(one, &bars.v_empty);
+          if (j > 0) mma_commit(one, &bars.k_empty[ring.s ^ 1]);
+        } else {
+          mma_commit(one, &bars.dq_full);
         }
-        __syncwarp();
         ring.next(2);
       }
     }
@@ -473,28 +471,28 @@ __global__ void __launch_bounds__(384, 1) attention_dkv_kernel(const __grid_cons
       }
       __syncwarp();
     } else if (warp == 9) {
+      const uint32_t one = elect_one();
       auto warp_wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)) != 0; };
       const int q_lo = max(0, -len.position(0));  // queries before it are at negative positions
       bool ok = n > 0 && warp_wait(&bars.kv_full, 0);
       RingPos next, ring;  // of the scores; of the gradients, one unit behind
+      int sub = n > 0 ? u0 % units.per_head : 0;
       for (int u = 0; u <= n && ok; ++u) {
         if (u < n) {
           uint8_t* stage = stages + next.s * Smem::kStage;
           if (!warp_wait(&bars.q_full[next.s], next.ph)) break;
-          const int i0 = units.q_first + (u0 + u) % units.per_head * kSub;
+          const int i0 = units.q_first + sub * kSub;
+          if (++sub == units.per_head) sub = 0;
           if (i0 < q_lo || i0 + kSub > len.q) {
             auto keep = [&](int r) { return i0 + r >= q_lo && i0 + r < len.q; };
             clear_rows<DP, kSub>(stage, lane, keep);
             clear_rows<DP, kSub>(stage + kSubBytes, lane, keep);
           }
-          if (lane == 0) {
-            // The buffer is free: unit u - 2's gradients are ahead in the queue.
-            const uint32_t s = tmem + (u & 1) * 128;
-            mma_rows<T, DP, kSub>(s, k_tile, kBox, stage, kSubBox);
-            mma_rows<T, DP, kSub>(s + 64, v_tile, kBox, stage + kSubBytes, kSubBox);
-            mma_commit(&bars.s_full[u & 1]);
-          }
-          __syncwarp();
+          // The buffer is free: unit u - 2's gradients are ahead in the queue.
+          const uint32_t s = tmem + (u & 1) * 128;
+          mma_rows<T, DP, kSub>(one, s, k_tile, kBox, stage, kSubBox);
+          mma_rows<T, DP, kSub>(one, s + 64, v_tile, kBox, stage + kSubBytes, kSubBox);
+          mma_commit(one, &bars.s_full[u & 1]);
           next.next(kStages);
         }
         if (u > 0) {
@@ -502,13 +500,10 @@ __global__ void __launch_bounds__(384, 1) attention_dkv_kernel(const __grid_cons
           uint8_t* stage = stages + ring.s * Smem::kStage;
           if (!warp_wait(&bars.ds_full[w & 1], (w >> 1) & 1)) break;
           tc_fence_after();
-          if (lane == 0) {
-            const uint32_t s = tmem + (w & 1) * 128;
-            mma_columns<T, DP, kSub>(dv_tmem, s, stage + kSubBytes, kSubBox, w > 0);
-            mma_columns<T, DP, kSub>(dk_tmem, s + 64, stage, kSubBox, w > 0);
-            mma_commit(w == n - 1 ? &bars.done : &bars.q_empty[ring.s]);
-          }
-          __syncwarp();
+          const uint32_t s = tmem + (w & 1) * 128;
+          mma_columns<T, DP, kSub>(one, dv_tmem, s, stage + kSubBytes, kSubBox, w > 0);
+          mma_columns<T, DP, kSub>(one, dk_tmem, s + 64, stage, kSubBox, w > 0);
+          mma_commit(one, w == n - 1 ? &bars.done : &bars.q_empty[ring.s]);
           ring.next(kStages);
         }
       }
@@ -523,8 +518,11 @@ __global__ void __launch_bounds__(384, 1) attention_dkv_kernel(const __grid_cons
     int q_lo, q_hi;
     queries_of(p, len, k0 + row, q_lo, q_hi);
     bool ok = true;
+    int sub = n > 0 ? (u0 + group) % units.per_head : 0;
     for (int u = group; u < n; u += 2) {
-      const int i0 = units.q_first + (u0 + u) % units.per_head * kSub;
+      const int i0 = units.q_first + sub * kSub;
+      sub += 2;
+      while (sub >= units.per_head) sub -= units.per_head;
       const uint8_t* stage = stages + (u % kStages) * Smem::kStage + 2 * kSubBytes;
       ok = __all_sync(0xffffffffu, wait(&bars.q_full[u % kStages], (u / kStages) & 1) && wait(&bars.s_full[group], (u >> 1) & 1));
       if (!ok) break;

@@ -203,6 +203,7 @@ __global__ void __launch_bounds__(kTileThreads, 2) attention_tiles_kernel(const 
     } else if (warp == 5) {
       // ---- products: S(j), then P(j) V(j) and S(j + 1), ...
       const Visible seen = sequence_keys(p, len);
+      const uint32_t one = elect_one();
       auto warp_wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)) != 0; };
       RingPos ring;
       bool ok = warp_wait(&bars.q_full, 0);
@@ -217,22 +218,19 @@ __global__ void __launch_bounds__(kTileThreads, 2) attention_tiles_kernel(const 
         if (j > 0) {
           if (!warp_wait(&bars.p_full, (j - 1) & 1)) break;
           tc_fence_after();
-          if (lane == 0) mma_columns<T, DP, kTile>(o_tmem, s_tmem, stages + v_slot * kTileBytes, kBox, j > 1);
+          mma_columns<T, DP, kTile>(one, o_tmem, s_tmem, stages + v_slot * kTileBytes, kBox, j > 1);
         }
         if (j < list.n) {
           // One queue of products: commits come behind both (a commit between
           // them cost 7% at 16384 queries, window 4096, dim 128: 508 us, now 474).
-          if (lane == 0) {
-            mma_rows<T, DP, kTile>(s_tmem, q_tile, kBox, stages + ring.s * kTileBytes, kBox);
-            mma_commit(&bars.s_full);
-            if (j > 0) mma_commit(&bars.kv_empty[v_slot]);
-            mma_commit(&bars.kv_empty[ring.s]);
-          }
+          mma_rows<T, DP, kTile>(one, s_tmem, q_tile, kBox, stages + ring.s * kTileBytes, kBox);
+          mma_commit(one, &bars.s_full);
+          if (j > 0) mma_commit(one, &bars.kv_empty[v_slot]);
+          mma_commit(one, &bars.kv_empty[ring.s]);
           ring.next(kStages);
-        } else if (lane == 0) {
-          mma_commit(&bars.o_full);
+        } else {
+          mma_commit(one, &bars.o_full);
         }
-        __syncwarp();
       }
     }
   } else {

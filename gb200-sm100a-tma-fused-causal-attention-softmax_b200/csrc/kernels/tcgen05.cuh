@@ -144,43 +144,58 @@ __host__ __device__ constexpr uint32_t product(int m, int n, bool b_rows) {
   return 1u << 4 | type << 7 | type << 10 | (b_rows ? 1u << 16 : 0u) | (uint32_t)(n >> 3) << 17 | (uint32_t)(m >> 4) << 24;
 }
 
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t what, bool add) {
+// One lane of a converged warp.
+__device__ __forceinline__ uint32_t elect_one() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+  return r;
+}
+
+// Products and commits are called by a whole converged warp, so that their
+// operands are computed once per warp, and issued by the lane with `one` set.
+// (Called under a branch on the lane, a product took 65 to 80 cycles to issue.)
+__device__ __forceinline__ void mma_ss(uint32_t one, uint32_t d, uint64_t a, uint64_t b, uint32_t what, bool add) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(what), "r"((uint32_t)add)
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %4, 0;\n\tsetp.ne.u32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(what),
+      "r"((uint32_t)add), "r"(one)
       : "memory");
 }
 
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t what, bool add) {
+__device__ __forceinline__ void mma_ts(uint32_t one, uint32_t d, uint32_t a, uint64_t b, uint32_t what, bool add) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(what), "r"((uint32_t)add)
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %4, 0;\n\tsetp.ne.u32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(what),
+      "r"((uint32_t)add), "r"(one)
       : "memory");
 }
 
-// Arrive on `bar` once every product issued so far by this thread is done.
-__device__ __forceinline__ void mma_commit(uint64_t* bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar))
-               : "memory");
+// Arrive on `bar` once every product issued so far by that lane is done.
+__device__ __forceinline__ void mma_commit(uint32_t one, uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\tsetp.ne.u32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_addr(bar)), "r"(one)
+      : "memory");
 }
 
 // D[128, N] (+)= A[128, DP] B[N, DP]^T, both K-major tiles of DP / 64 boxes
 // (rows x 64 elements; box strides in bytes).
 template <typename T, int DP, int N>
-__device__ __forceinline__ void mma_rows(uint32_t d, const uint8_t* a, int a_box, const uint8_t* b, int b_box) {
+__device__ __forceinline__ void mma_rows(uint32_t one, uint32_t d, const uint8_t* a, int a_box, const uint8_t* b, int b_box) {
+  const uint64_t a0 = operand(a), b0 = operand(b);
 #pragma unroll
   for (int k = 0; k < DP / 16; ++k)
-    mma_ss(d, operand(a + (k >> 2) * a_box) + (k & 3) * 2, operand(b + (k >> 2) * b_box) + (k & 3) * 2,
+    mma_ss(one, d, a0 + (k >> 2) * (a_box >> 4) + (k & 3) * 2, b0 + (k >> 2) * (b_box >> 4) + (k & 3) * 2,
            product<T>(128, N, false), k > 0);
 }
 
 // D[128, DP] (+)= A[128, K] B[K, DP]: A in TMEM (two elements a column), B a
 // row tile of DP / 64 boxes.
 template <typename T, int DP, int K>
-__device__ __forceinline__ void mma_columns(uint32_t d, uint32_t a, const uint8_t* b, int b_box, bool add) {
+__device__ __forceinline__ void mma_columns(uint32_t one, uint32_t d, uint32_t a, const uint8_t* b, int b_box, bool add) {
+  const uint64_t b0 = operand(b, (uint32_t)b_box);
 #pragma unroll
-  for (int k = 0; k < K / 16; ++k)
-    mma_ts(d, a + k * 8, operand(b, (uint32_t)b_box) + k * (2048 >> 4), product<T>(128, DP, true), add || k > 0);
+  for (int k = 0; k < K / 16; ++k) mma_ts(one, d, a + k * 8, b0 + k * (2048 >> 4), product<T>(128, DP, true), add || k > 0);
 }
 
 }  // namespace cs
