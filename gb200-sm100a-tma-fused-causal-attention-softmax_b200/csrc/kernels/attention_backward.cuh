@@ -34,8 +34,8 @@ struct GradParams {
   CUtensorMap q, k, v, d_o;  // stationary: 128 rows; streamed: 64
   CUtensorMap out0, out1;    // dq; or dk, dv
   AttentionParams a;
-  const float* lse2;   // [batch * heads, q_pad]: lse in units of log2; +infinity for rows without keys
-  const float* delta;  // the same
+  const float* lse2;   // [batch * heads, q_pad]: minus lse in units of log2; -infinity for rows without keys
+  const float* delta;  // the same: minus the sum of d_o * o
   const float* norms;  // fp16: [2, batch * kv_heads], largest |d_o| and |v| of a row
   float* partial;      // dK, dV parts of key tiles cut into several CTAs' shares
   int32_t q_pad;
@@ -91,8 +91,8 @@ __global__ void __launch_bounds__(256) attention_rows_kernel(const __grid_consta
       }
       if (lane == 0 && i < rp.q_pad) {
         const float lse = in ? p.lse[(int64_t)bh * p.q_len + i] : -INFINITY;
-        rp.lse2[(int64_t)bh * rp.q_pad + i] = lse == -INFINITY ? INFINITY : lse * kLog2e;
-        rp.delta[(int64_t)bh * rp.q_pad + i] = in ? dot : 0.f;
+        rp.lse2[(int64_t)bh * rp.q_pad + i] = lse == -INFINITY ? -INFINITY : -lse * kLog2e;
+        rp.delta[(int64_t)bh * rp.q_pad + i] = in ? -dot : 0.f;
       }
       if (T::kIsHalf) raise_max(rp.norms + b * p.kv_heads + hk, norm);
     } else if (T::kIsHalf && h % p.group == 0) {
@@ -122,24 +122,34 @@ __device__ __forceinline__ float ds_factor(const GradParams& g, int bk) {
   return __uint_as_float((uint32_t)(127 + 15 - up) << 23);
 }
 
-// P and dS of 32 columns: scores s and dp in, packed pairs out (over them).
-// minus_lse: - lse2 + shift of column e; minus_delta: - delta * k1.
+// P and dS of 32 columns: scores s and dp in, packed pairs out.
+// minus_lse: shift - lse2 of columns e and e + 1; minus_delta: - delta.
+// P = 2^(sl s + minus_lse), dS = P (dp + minus_delta) k1.
 template <typename T, typename Lse, typename Delta>
-__device__ __forceinline__ void grad32(const uint32_t* s, const uint32_t* dp, uint32_t bits, float sl, float k1, Lse minus_lse,
-                                       Delta minus_delta, uint32_t* p_out, uint32_t* ds_out) {
+__device__ __forceinline__ void grad32(const uint32_t* s, const uint32_t* dp, bool every, uint32_t bits, float sl, float k1,
+                                       Lse minus_lse, Delta minus_delta, uint32_t* p_out, uint32_t* ds_out) {
+  const F2 sl2 = f2(sl, sl), k2 = f2(k1, k1);
+  float p[32], d[32];
 #pragma unroll
   for (int e = 0; e < 32; e += 2) {
-    float p[2], d[2];
+    const float2 x = f2_out(f2_fma(f2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), sl2, minus_lse(e)));
+    p[e] = ex2(x.x);
+    p[e + 1] = ex2(x.y);
+    F2 v = f2_add(f2(__uint_as_float(dp[e]), __uint_as_float(dp[e + 1])), minus_delta(e));
+    if (T::kIsHalf) v = f2_mul(v, k2);
+    const float2 y = f2_out(f2_mul(f2(p[e], p[e + 1]), v));
+    d[e] = y.x;
+    d[e + 1] = y.y;
+  }
+  if (!every) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      p[h] = ex2(__fmaf_rn(__uint_as_float(s[e + h]), sl, minus_lse(e + h)));
-      d[h] = T::kIsHalf ? __fmaf_rn(__uint_as_float(dp[e + h]), k1, minus_delta(e + h))
-                        : __uint_as_float(dp[e + h]) + minus_delta(e + h);
-      d[h] *= p[h];
-      if (!((bits >> (e + h)) & 1)) p[h] = d[h] = 0.f;
-    }
-    p_out[e / 2] = T::pack(p[0], p[1]);
-    ds_out[e / 2] = T::pack(d[0], d[1]);
+    for (int e = 0; e < 32; ++e)
+      if (!((bits >> e) & 1)) p[e] = d[e] = 0.f;
+  }
+#pragma unroll
+  for (int e = 0; e < 16; ++e) {
+    p_out[e] = T::pack(p[2 * e], p[2 * e + 1]);
+    ds_out[e] = T::pack(d[2 * e], d[2 * e + 1]);
   }
 }
 
@@ -265,7 +275,7 @@ __global__ void __launch_bounds__(256, 2) attention_dq_kernel(const __grid_const
         if (j > 0) {
           if (!warp_wait(&bars.ds_full, (j - 1) & 1)) break;
           tc_fence_after();
-          mma_columns<T, DP, kSub>(one, dq_tmem, dp_tmem, k_last, kSubBox, j > 1);
+          mma_columns<T, DP, kSub, 16>(one, dq_tmem, dp_tmem, k_last, kSubBox, j > 1);
         }
         if (j < list.n) {
           mma_rows<T, DP, kSub>(one, s_tmem, q_tile, kBox, k_tile, kSubBox);
@@ -287,8 +297,8 @@ __global__ void __launch_bounds__(256, 2) attention_dq_kernel(const __grid_const
     const float sl = fmaxf(p.scale * kLog2e, 1.1754944e-38f);
     const int64_t row = ((int64_t)b * p.heads + head) * gp.q_pad + i;
     const float c = ds_factor<T>(gp, bk);
-    const float minus_lse = i < gp.q_pad ? -gp.lse2[row] : -INFINITY;
-    const float minus_delta = i < gp.q_pad ? -gp.delta[row] * c : 0.f;
+    const float lse = i < gp.q_pad ? gp.lse2[row] : -INFINITY, delta = i < gp.q_pad ? gp.delta[row] : 0.f;
+    const F2 minus_lse = f2(lse, lse), minus_delta = f2(delta, delta);
     bool ok = true;
     for (int j = 0; j < list.n; ++j) {
       const int k0 = list.key(j);
@@ -302,8 +312,7 @@ __global__ void __launch_bounds__(256, 2) attention_dq_kernel(const __grid_const
         tmem_load32(s_tmem + lanes + h * 32, s);
         tmem_load32(dp_tmem + lanes + h * 32, dp);
         tmem_wait_loads();
-        const uint32_t bits = every ? 0xffffffffu : visible_bits32(see, k0 + h * 32);
-        grad32<T>(s, dp, bits, sl, c, [&](int) { return minus_lse; }, [&](int) { return minus_delta; }, pp, ds);
+        grad32<T>(s, dp, every, every ? 0u : visible_bits32(see, k0 + h * 32), sl, c, [&](int) { return minus_lse; }, [&](int) { return minus_delta; }, pp, ds);
         tmem_store16(dp_tmem + lanes + h * 16, ds);
       }
       tmem_wait_stores();
@@ -339,7 +348,10 @@ __global__ void __launch_bounds__(256, 2) attention_dq_kernel(const __grid_const
   finish_tmem(bars.gone, warp == 5, tmem, kColumns);
 }
 
-// ---- dK and dV: one CTA an SM, two warpgroups take the streamed tiles in turn
+// ---- dK and dV: one CTA an SM. Two warpgroups take half of the columns each, so
+// that P and dS are there by the time the tensor core is through with the last
+// unit's gradients and the next one's scores (two buffers); taking the units in
+// turn instead left it waiting a third of the time.
 
 struct KeyBarriers {
   uint64_t kv_full, s_full[2], ds_full[2], done, q_full[4], q_empty[4];
@@ -408,7 +420,7 @@ __global__ void __launch_bounds__(384, 1) attention_dkv_kernel(const __grid_cons
     mbar_init(&bars.done, 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bars.s_full[i], 1);
-      mbar_init(&bars.ds_full[i], 4);
+      mbar_init(&bars.ds_full[i], 8);
     }
     for (int i = 0; i < kStages; ++i) {
       mbar_init(&bars.q_full[i], 1);
@@ -501,8 +513,8 @@ __global__ void __launch_bounds__(384, 1) attention_dkv_kernel(const __grid_cons
           if (!warp_wait(&bars.ds_full[w & 1], (w >> 1) & 1)) break;
           tc_fence_after();
           const uint32_t s = tmem + (w & 1) * 128;
-          mma_columns<T, DP, kSub>(one, dv_tmem, s, stage + kSubBytes, kSubBox, w > 0);
-          mma_columns<T, DP, kSub>(one, dk_tmem, s + 64, stage, kSubBox, w > 0);
+          mma_columns<T, DP, kSub, 32>(one, dv_tmem, s, stage + kSubBytes, kSubBox, w > 0);
+          mma_columns<T, DP, kSub, 32>(one, dk_tmem, s + 64, stage, kSubBox, w > 0);
           mma_commit(one, w == n - 1 ? &bars.done : &bars.q_empty[ring.s]);
           ring.next(kStages);
         }
@@ -512,40 +524,42 @@ __global__ void __launch_bounds__(384, 1) attention_dkv_kernel(const __grid_cons
     registers_up<176>();
     const int group = warp >> 2, row = threadIdx.x & 127;  // warpgroup; this thread's key
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t s_at = tmem + lanes + group * 128, dp_at = s_at + 64;
+    const uint32_t half = tmem + lanes + group * 32;  // this warpgroup's columns of the first buffer's S
     const float sl = fmaxf(p.scale * kLog2e, 1.1754944e-38f);
     const float c = ds_factor<T>(gp, bk), k1 = T::kIsHalf ? c * (1.f / kHalfTop) : 1.f;
     int q_lo, q_hi;
     queries_of(p, len, k0 + row, q_lo, q_hi);
     bool ok = true;
-    int sub = n > 0 ? (u0 + group) % units.per_head : 0;
-    for (int u = group; u < n; u += 2) {
+    int sub = n > 0 ? u0 % units.per_head : 0;
+    RingPos ring;
+    for (int u = 0; u < n; ++u, ring.next(kStages)) {
       const int i0 = units.q_first + sub * kSub;
-      sub += 2;
-      while (sub >= units.per_head) sub -= units.per_head;
-      const uint8_t* stage = stages + (u % kStages) * Smem::kStage + 2 * kSubBytes;
-      ok = __all_sync(0xffffffffu, wait(&bars.q_full[u % kStages], (u / kStages) & 1) && wait(&bars.s_full[group], (u >> 1) & 1));
+      if (++sub == units.per_head) sub = 0;
+      const float* rows = reinterpret_cast<const float*>(stages + ring.s * Smem::kStage + 2 * kSubBytes) + group * 32;
+      ok = __all_sync(0xffffffffu, wait(&bars.q_full[ring.s], ring.ph) && wait(&bars.s_full[u & 1], (u >> 1) & 1));
       if (!ok) break;
       tc_fence_after();
       const bool every = i0 >= units.every_lo && i0 + kSub <= units.every_hi;
-      const float* lse = reinterpret_cast<const float*>(stage);
-      const float* delta = reinterpret_cast<const float*>(stage + 256);
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        uint32_t s[32], dp[32], pp[16], ds[16];
-        tmem_load32(s_at + h * 32, s);
-        tmem_load32(dp_at + h * 32, dp);
-        tmem_wait_loads();
-        const uint32_t bits = every ? 0xffffffffu : below_bits(q_hi - i0 - h * 32) & ~below_bits(q_lo - i0 - h * 32);
-        grad32<T>(s, dp, bits, sl, k1, [&](int e) { return kShift - lse[h * 32 + e]; },
-                  [&](int e) { return T::kIsHalf ? -delta[h * 32 + e] * k1 : -delta[h * 32 + e]; }, pp, ds);
-        tmem_store16(s_at + h * 16, pp);
-        tmem_store16(dp_at + h * 16, ds);
-      }
+      const uint32_t s_at = half + (u & 1) * 128, dp_at = s_at + 64;
+      uint32_t s[32], dp[32], pp[16], ds[16];
+      tmem_load32(s_at, s);
+      tmem_load32(dp_at, dp);
+      const int at = i0 + group * 32;
+      const uint32_t bits = every ? 0u : below_bits(q_hi - at) & ~below_bits(q_lo - at);
+      tmem_wait_loads();
+      const F2 shift2 = f2(kShift, kShift);
+      auto pair = [&](int e) {  // two rows' numbers
+        const float2 v = *reinterpret_cast<const float2*>(rows + e);
+        return f2(v.x, v.y);
+      };
+      grad32<T>(s, dp, every, bits, sl, k1, [&](int e) { return T::kIsHalf ? f2_add(pair(e), shift2) : pair(e); },
+                [&](int e) { return pair(64 + e); }, pp, ds);
+      tmem_store16(s_at, pp);  // over this warpgroup's own columns
+      tmem_store16(dp_at, ds);
       tmem_wait_stores();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&bars.ds_full[group]);
+      if (lane == 0) mbar_arrive(&bars.ds_full[u & 1]);
     }
     if (ok && n > 0) ok = __all_sync(0xffffffffu, wait(&bars.done, 0));
     if (ok) {

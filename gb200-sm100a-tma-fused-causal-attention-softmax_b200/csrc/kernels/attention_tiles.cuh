@@ -218,7 +218,7 @@ __global__ void __launch_bounds__(kTileThreads, 2) attention_tiles_kernel(const 
         if (j > 0) {
           if (!warp_wait(&bars.p_full, (j - 1) & 1)) break;
           tc_fence_after();
-          mma_columns<T, DP, kTile>(one, o_tmem, s_tmem, stages + v_slot * kTileBytes, kBox, j > 1);
+          mma_columns<T, DP, kTile, 16>(one, o_tmem, s_tmem, stages + v_slot * kTileBytes, kBox, j > 1);
         }
         if (j < list.n) {
           // One queue of products: commits come behind both (a commit between
@@ -285,21 +285,23 @@ __global__ void __launch_bounds__(kTileThreads, 2) attention_tiles_kernel(const 
         }
       }
       const float nb = m == -INFINITY ? 0.f : kShift - m;
-      float sum0 = 0.f, sum1 = 0.f;
+      const F2 sl2 = f2(sl, sl), nb2 = f2(nb, nb);
+      F2 sum0 = f2(0.f, 0.f), sum1 = sum0;
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         uint32_t packed[32];
 #pragma unroll
         for (int e = 0; e < 32; ++e) {
-          const float x = ex2(__fmaf_rn(__uint_as_float(raw[c * 64 + 2 * e]), sl, nb));
-          const float y = ex2(__fmaf_rn(__uint_as_float(raw[c * 64 + 2 * e + 1]), sl, nb));
-          sum0 += x;
-          sum1 += y;
-          packed[e] = T::pack(x, y);
+          const float2 x = f2_out(f2_fma(f2(__uint_as_float(raw[c * 64 + 2 * e]), __uint_as_float(raw[c * 64 + 2 * e + 1])), sl2, nb2));
+          const float x0 = ex2(x.x), x1 = ex2(x.y);
+          if (e & 1) sum1 = f2_add(sum1, f2(x0, x1));
+          else sum0 = f2_add(sum0, f2(x0, x1));
+          packed[e] = T::pack(x0, x1);
         }
         tmem_store32(s_at + c * 32, packed);
       }
-      l += sum0 + sum1;
+      const float2 sum = f2_out(f2_add(sum0, sum1));
+      l += sum.x + sum.y;
       tmem_wait_stores();
       tc_fence_before();
       __syncwarp();

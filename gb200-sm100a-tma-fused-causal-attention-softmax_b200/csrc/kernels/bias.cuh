@@ -144,34 +144,6 @@ __device__ __forceinline__ void fetch_row(const RowWalk& w, const uint4* in, uin
   for (int j = gt; j < w.m.n; j += gn) cp_async16(buffer + j, in + vector_at(w.m, j));
 }
 
-// Two floats in one 64-bit register (packed arithmetic).
-using F2 = unsigned long long;
-__device__ __forceinline__ F2 f2(float a, float b) {
-  F2 r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ float2 f2_out(F2 v) {
-  float2 r;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-  return r;
-}
-__device__ __forceinline__ F2 f2_add(F2 a, F2 b) {
-  F2 r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ F2 f2_mul(F2 a, F2 b) {
-  F2 r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ F2 f2_fma(F2 a, F2 b, F2 c) {
-  F2 r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-
 template <typename T>
 __device__ __forceinline__ void unpack_pairs(const uint4& r, F2* f) {
   const uint32_t w[4] = {r.x, r.y, r.z, r.w};
