@@ -80,14 +80,14 @@ using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, 
                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 EncodeTiled g_encode = nullptr;
 
-// Boxes of 64 dims x `rows` tokens of one head, 128-byte swizzle. A dimension of
+// Boxes of 64 dims x 128 tokens of one head, 128-byte swizzle. A dimension of
 // size 1 may have any stride: it gets a valid one.
-int make_map(CUtensorMap* map, const cs_attention_args* a, const cs_tensor& t, int32_t tokens, int32_t heads, int rows) {
+int make_map(CUtensorMap* map, const cs_attention_args* a, const cs_tensor& t, int32_t tokens, int32_t heads) {
   const cuuint64_t row = (cuuint64_t)a->head_dim * 2;
   const cuuint64_t dims[4] = {(cuuint64_t)a->head_dim, (cuuint64_t)heads, (cuuint64_t)tokens, (cuuint64_t)a->batch};
   const cuuint64_t strides[3] = {heads > 1 ? (cuuint64_t)t.head_stride * 2 : row, tokens > 1 ? (cuuint64_t)t.token_stride * 2 : row,
                                  a->batch > 1 ? (cuuint64_t)t.batch_stride * 2 : row};
-  const cuuint32_t box[4] = {64, 1, (cuuint32_t)rows, 1}, step[4] = {1, 1, 1, 1};
+  const cuuint32_t box[4] = {64, 1, cs::kTile, 1}, step[4] = {1, 1, 1, 1};
   const CUresult r = g_encode(map, a->type == CS_TYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
                               4, t.data, dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
@@ -254,10 +254,10 @@ int launch_tokens(const cs_attention_args* a, const cs::AttentionParams& p, cons
 int launch_tiles(const cs_attention_args* a, const cs::AttentionParams& p, void* stream) {
   cs::TileParams t{};
   t.a = p;
-  int rc = make_map(&t.q, a, a->q, a->q_len, a->heads, cs::kTile);
-  if (!rc) rc = make_map(&t.k, a, a->k, a->kv_len, a->kv_heads, cs::kTile);
-  if (!rc) rc = make_map(&t.v, a, a->v, a->kv_len, a->kv_heads, cs::kTile);
-  if (!rc) rc = make_map(&t.o, a, a->o, a->q_len, a->heads, cs::kTile);
+  int rc = make_map(&t.q, a, a->q, a->q_len, a->heads);
+  if (!rc) rc = make_map(&t.k, a, a->k, a->kv_len, a->kv_heads);
+  if (!rc) rc = make_map(&t.v, a, a->v, a->kv_len, a->kv_heads);
+  if (!rc) rc = make_map(&t.o, a, a->o, a->q_len, a->heads);
   if (rc) return rc;
   t.q_tiles = (a->q_len + cs::kTile - 1) / cs::kTile;
   const int64_t ctas = (int64_t)a->batch * a->heads * t.q_tiles;
@@ -277,7 +277,7 @@ struct GradShape {
   int64_t bytes() const { return 2 * rows_bytes + norms_bytes + partial_bytes; }
 };
 
-// A key tile's work is its (head, 64 queries) units. Tiles are cut into shares
+// A key tile's work is its (head, tile of queries) units. Tiles are cut into shares
 // only where that evens out the SMs: the sinks' tile, which every query sees,
 // and tiles of long rows when there are few of them; each share costs a part of
 // dK and dV in fp32, written and read once more. So: about two shares an SM,
@@ -285,19 +285,19 @@ struct GradShape {
 GradShape grad_shape(const cs_attention_args* a, int sms) {
   GradShape s{};
   s.dim = a->head_dim <= 64 ? 64 : 128;
-  s.q_pad = (a->q_len + cs::kSub - 1) / cs::kSub * cs::kSub;
   s.q_tiles = (a->q_len + cs::kTile - 1) / cs::kTile;
+  s.q_pad = s.q_tiles * cs::kTile;
   s.k_tiles = (a->kv_len + cs::kTile - 1) / cs::kTile;
   const int64_t group = a->heads / a->kv_heads, heads = (int64_t)a->batch * a->kv_heads;
-  const int64_t all = s.q_pad / cs::kSub * group;  // units of a tile that every query sees
+  const int64_t all = s.q_tiles * group;  // units of a tile that every query sees
   int64_t usual = all;
   if (a->window) {
-    usual = std::min(all, (((int64_t)a->window + cs::kTile - 1 + cs::kSub - 1) / cs::kSub + 1) * group);
+    usual = std::min(all, (((int64_t)a->window + 2 * cs::kTile - 2) / cs::kTile + 1) * group);
     s.sink_tiles = (int)std::min<int64_t>(s.k_tiles, ((int64_t)a->sinks + cs::kTile - 1) / cs::kTile);
   }
   // Without a window tiles see half of the queries on average.
   const int64_t total = heads * (s.sink_tiles * all + (s.k_tiles - s.sink_tiles) * (a->window ? usual : (usual + 1) / 2));
-  int64_t share = std::max<int64_t>(32, (total + 2 * sms - 1) / (2 * sms));
+  int64_t share = std::max<int64_t>(16, (total + 2 * sms - 1) / (2 * sms));
   if (usual <= 2 * share) share = std::max(share, usual);
   s.share = (int)std::min(share, std::max(all, usual));
   s.window_shares = (int)((usual + s.share - 1) / s.share);
@@ -345,26 +345,22 @@ int launch_backward(const cs_attention_args* a, const cs_attention_grads* g, con
   k.sink_tiles = s.sink_tiles;
   k.sink_shares = s.sink_shares;
   k.tiles = s.k_tiles;
-  int rc = make_map(&k.q, a, a->q, a->q_len, a->heads, cs::kSub);
-  if (!rc) rc = make_map(&k.d_o, a, g->d_o, a->q_len, a->heads, cs::kSub);
-  if (!rc) rc = make_map(&k.k, a, a->k, a->kv_len, a->kv_heads, cs::kTile);
-  if (!rc) rc = make_map(&k.v, a, a->v, a->kv_len, a->kv_heads, cs::kTile);
-  if (!rc) rc = make_map(&k.out0, a, g->dk, a->kv_len, a->kv_heads, cs::kTile);
-  if (!rc) rc = make_map(&k.out1, a, g->dv, a->kv_len, a->kv_heads, cs::kTile);
+  int rc = make_map(&k.q, a, a->q, a->q_len, a->heads);
+  if (!rc) rc = make_map(&k.d_o, a, g->d_o, a->q_len, a->heads);
+  if (!rc) rc = make_map(&k.k, a, a->k, a->kv_len, a->kv_heads);
+  if (!rc) rc = make_map(&k.v, a, a->v, a->kv_len, a->kv_heads);
+  if (!rc) rc = make_map(&k.out0, a, g->dk, a->kv_len, a->kv_heads);
+  if (!rc) rc = make_map(&k.out1, a, g->dv, a->kv_len, a->kv_heads);
   if (rc) return rc;
-  e = cs_host::launch(dkv_kernel(a->type, s.dim), dim3((unsigned)s.dkv_ctas), 384, (size_t)dkv_smem(s.dim), stream, k);
+  e = cs_host::launch(dkv_kernel(a->type, s.dim), dim3((unsigned)s.dkv_ctas), cs::kGradThreads, (size_t)dkv_smem(s.dim), stream, k);
   if (e != cudaSuccess) return fail_cuda(e, "attention backward, keys");
 
   cs::GradParams q = k;
   q.tiles = s.q_tiles;
-  rc = make_map(&q.q, a, a->q, a->q_len, a->heads, cs::kTile);
-  if (!rc) rc = make_map(&q.d_o, a, g->d_o, a->q_len, a->heads, cs::kTile);
-  if (!rc) rc = make_map(&q.k, a, a->k, a->kv_len, a->kv_heads, cs::kSub);
-  if (!rc) rc = make_map(&q.v, a, a->v, a->kv_len, a->kv_heads, cs::kSub);
-  if (!rc) rc = make_map(&q.out0, a, g->dq, a->q_len, a->heads, cs::kTile);
+  rc = make_map(&q.out0, a, g->dq, a->q_len, a->heads);
   if (rc) return rc;
-  e = cs_host::launch(dq_kernel(a->type, s.dim), dim3((unsigned)(a->batch * a->heads * s.q_tiles)), 256, (size_t)dq_smem(s.dim),
-                      stream, q);
+  e = cs_host::launch(dq_kernel(a->type, s.dim), dim3((unsigned)(a->batch * a->heads * s.q_tiles)), cs::kGradThreads,
+                      (size_t)dq_smem(s.dim), stream, q);
   if (e != cudaSuccess) return fail_cuda(e, "attention backward, queries");
   if (s.partial_bytes) {
     const int64_t tiles = (int64_t)a->batch * a->kv_heads * (s.window_shares > 1 ? s.k_tiles : s.sink_tiles);

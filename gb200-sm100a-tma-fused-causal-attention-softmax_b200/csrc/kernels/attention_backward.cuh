@@ -10,28 +10,31 @@
 // products instead of five, so that no sum crosses CTAs: no atomics, the same
 // bits every time, and no fp32 copy of dQ in memory.
 //
-// The streamed operand comes in tiles of 64 rows: S and dP of 128 x 64, P and
-// dS written over them in 16 bits as the next products' first operands (TMEM).
+// Tiles of 128 x 128, one CTA an SM: two softmax warpgroups that take 64 columns
+// of each tile, a warp of TMA loads, a warp of products. S and dP are
+// fp32 in TMEM; P and dS are written over them in 16 bits and are the next
+// products' first operands from there. The products are ordered so that the
+// tensor core has a tile's other two while the warpgroups make P or dS. (Tiles
+// of 128 x 64 with two buffers were tried first: a product of 64 columns with
+// both operands in shared memory takes as long as one of 128.)
 //
 // 16 bits: P and dS are rounded for the tensor core. In fp16 P is taken times
 // 2^15 and dS times a power of two, from the largest norms of d_o and v rows of
 // the kv head, that brings the largest possible |dS| to 2^15: small gradients
 // keep their bits and none overflows. bf16 needs neither.
 //
-// Bound: at dim 128 a 128 x 64 tile costs 4 x 256 tensor-core cycles in dK/dV
-// and 3 x 256 in dQ; the two S-like products (64 columns, both operands in
-// shared memory) are held back by shared memory, 384 cycles each.
+// Bound: at dim 128 a tile costs 4 x 512 tensor-core cycles in dK/dV, 3 x 512 in
+// dQ, and 1024 cycles of the exponential unit in each.
 #pragma once
 
 #include "attention_tiles.cuh"
 
 namespace cs {
 
-constexpr int kSub = 64;             // rows of a streamed tile
 constexpr float kHalfTop = 32768.f;  // 2^15
 
 struct GradParams {
-  CUtensorMap q, k, v, d_o;  // stationary: 128 rows; streamed: 64
+  CUtensorMap q, k, v, d_o;
   CUtensorMap out0, out1;    // dq; or dk, dv
   AttentionParams a;
   const float* lse2;   // [batch * heads, q_pad]: minus lse in units of log2; -infinity for rows without keys
@@ -122,34 +125,41 @@ __device__ __forceinline__ float ds_factor(const GradParams& g, int bk) {
   return __uint_as_float((uint32_t)(127 + 15 - up) << 23);
 }
 
-// P and dS of 32 columns: scores s and dp in, packed pairs out.
-// minus_lse: shift - lse2 of columns e and e + 1; minus_delta: - delta.
-// P = 2^(sl s + minus_lse), dS = P (dp + minus_delta) k1.
-template <typename T, typename Lse, typename Delta>
-__device__ __forceinline__ void grad32(const uint32_t* s, const uint32_t* dp, bool every, uint32_t bits, float sl, float k1,
-                                       Lse minus_lse, Delta minus_delta, uint32_t* p_out, uint32_t* ds_out) {
-  const F2 sl2 = f2(sl, sl), k2 = f2(k1, k1);
-  float p[32], d[32];
+// P = 2^(sl s + minus_lse) of 64 columns, 0 where masked. minus_lse(e): of columns
+// e and e + 1. (Packed f32x2 arithmetic: 5% off a training step against scalar.)
+template <typename Lse>
+__device__ __forceinline__ void scores_to_p(const uint32_t* s, bool every, uint32_t bits0, uint32_t bits1, float sl, Lse minus_lse,
+                                            float* p) {
+  const F2 sl2 = f2(sl, sl);
 #pragma unroll
-  for (int e = 0; e < 32; e += 2) {
+  for (int e = 0; e < 64; e += 2) {
     const float2 x = f2_out(f2_fma(f2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), sl2, minus_lse(e)));
     p[e] = ex2(x.x);
     p[e + 1] = ex2(x.y);
-    F2 v = f2_add(f2(__uint_as_float(dp[e]), __uint_as_float(dp[e + 1])), minus_delta(e));
-    if (T::kIsHalf) v = f2_mul(v, k2);
-    const float2 y = f2_out(f2_mul(f2(p[e], p[e + 1]), v));
-    d[e] = y.x;
-    d[e + 1] = y.y;
   }
   if (!every) {
 #pragma unroll
-    for (int e = 0; e < 32; ++e)
-      if (!((bits >> e) & 1)) p[e] = d[e] = 0.f;
+    for (int e = 0; e < 64; ++e)
+      if (!(((e < 32 ? bits0 : bits1) >> (e & 31)) & 1)) p[e] = 0.f;
   }
+}
+
+// dS = P (dP + minus_delta(e)) k1 of 32 columns in 16-bit pairs; 0 where masked,
+// whatever dP holds there.
+template <typename T, typename Delta>
+__device__ __forceinline__ void p_to_ds(const float* p, const uint32_t* dp, bool every, uint32_t bits, float k1, Delta minus_delta,
+                                        uint32_t* out) {
+  const F2 k2 = f2(k1, k1);
 #pragma unroll
-  for (int e = 0; e < 16; ++e) {
-    p_out[e] = T::pack(p[2 * e], p[2 * e + 1]);
-    ds_out[e] = T::pack(d[2 * e], d[2 * e + 1]);
+  for (int e = 0; e < 32; e += 2) {
+    F2 v = f2_add(f2(__uint_as_float(dp[e]), __uint_as_float(dp[e + 1])), minus_delta(e));
+    if (T::kIsHalf) v = f2_mul(v, k2);
+    float2 d = f2_out(f2_mul(f2(p[e], p[e + 1]), v));
+    if (!every) {
+      if (!((bits >> e) & 1)) d.x = 0.f;
+      if (!((bits >> (e + 1)) & 1)) d.y = 0.f;
+    }
+    out[e / 2] = T::pack(d.x, d.y);
   }
 }
 
@@ -168,42 +178,51 @@ __device__ __forceinline__ void stage32(uint8_t* tile, int row, int c, const uin
   }
 }
 
-// ---- dQ: like the forward kernel, two CTAs an SM
+constexpr int kGradThreads = 384;  // registers: 2 x 128 x 208 + 128 x 88 = 384 x 168
+
+// ---- dQ
 
 struct QueryBarriers {
-  uint64_t q_full, s_full, ds_full, dq_full, k_full[2], k_empty[2], v_full, v_empty;
+  uint64_t q_full, s_full[2], dp_full, ds_full, done, k_full[3], k_empty[3], v_full, v_empty;
   uint32_t tmem, gone;
 };
 
 template <int DP>
 struct QuerySmem {
-  static constexpr int kFixed = kTile * DP * 2, kSubBytes = kSub * DP * 2;
-  // Exactly what two CTAs an SM allow at dim 128: the base is 1024-aligned by itself.
-  static constexpr int kBytes = 2 * kFixed + 3 * kSubBytes + 256;
+  static constexpr int kTileBytes = kTile * DP * 2;
+  static constexpr int kKeys = 3;  // key tiles: held until dQ has used them
+  static constexpr int kBytes = (2 + kKeys + 1) * kTileBytes + 256;
 };
 
+// Products in this order (S in two buffers):
+//   S(0) dP(0) S(1) | dQ(0) dP(1) S(2) | dQ(1) dP(2) S(3) | ...
+// While the warpgroups turn S(j + 1) into P(j + 1), the tensor core has dQ(j) and
+// dP(j + 1); while they make dS(j + 1), S(j + 2).
 template <typename T, int DP>
-__global__ void __launch_bounds__(256, 2) attention_dq_kernel(const __grid_constant__ GradParams gp) {
-  constexpr int kBox = kTile * 128, kSubBox = kSub * 128, kFixed = QuerySmem<DP>::kFixed, kSubBytes = QuerySmem<DP>::kSubBytes;
-  constexpr uint32_t kColumns = 256;
+__global__ void __launch_bounds__(kGradThreads, 1) attention_dq_kernel(const __grid_constant__ GradParams gp) {
+  using Smem = QuerySmem<DP>;
+  constexpr int kBox = kTile * 128, kTileBytes = Smem::kTileBytes, kKeys = Smem::kKeys;
+  constexpr uint32_t kColumns = 512;
   extern __shared__ __align__(1024) uint8_t aligned_smem[];
   uint8_t* q_tile = aligned_smem;
-  uint8_t* do_tile = q_tile + kFixed;
-  uint8_t* k_tiles = do_tile + kFixed;
-  uint8_t* v_tile = k_tiles + 2 * kSubBytes;
-  QueryBarriers& bars = *reinterpret_cast<QueryBarriers*>(v_tile + kSubBytes);
+  uint8_t* do_tile = q_tile + kTileBytes;
+  uint8_t* k_tiles = do_tile + kTileBytes;
+  uint8_t* v_tile = k_tiles + kKeys * kTileBytes;
+  QueryBarriers& bars = *reinterpret_cast<QueryBarriers*>(v_tile + kTileBytes);
   const AttentionParams& p = gp.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (smem_addr(aligned_smem) & 1023) {  // the swizzle needs it
     if (threadIdx.x == 0) atomicOr(p.status, kStatusTimeout);
     return;
   }
-  if (warp == 4 && lane == 0) {
+  if (warp == 8 && lane == 0) {
     mbar_init(&bars.q_full, 1);
-    mbar_init(&bars.s_full, 1);
-    mbar_init(&bars.ds_full, 4);
-    mbar_init(&bars.dq_full, 1);
-    for (int i = 0; i < 2; ++i) {
+    mbar_init(&bars.s_full[0], 1);
+    mbar_init(&bars.s_full[1], 1);
+    mbar_init(&bars.dp_full, 1);
+    mbar_init(&bars.ds_full, 8);
+    mbar_init(&bars.done, 1);
+    for (int i = 0; i < kKeys; ++i) {
       mbar_init(&bars.k_full[i], 1);
       mbar_init(&bars.k_empty[i], 1);
     }
@@ -216,11 +235,11 @@ __global__ void __launch_bounds__(256, 2) attention_dq_kernel(const __grid_const
     prefetch_map(&gp.k);
     prefetch_map(&gp.v);
   }
-  if (warp == 5) tmem_alloc(&bars.tmem, kColumns);
+  if (warp == 9) tmem_alloc(&bars.tmem, kColumns);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = bars.tmem, s_tmem = tmem, dp_tmem = tmem + 64, dq_tmem = tmem + 128;
+  const uint32_t tmem = bars.tmem, dp_tmem = tmem + 256, dq_tmem = tmem + 384;
   // Only the rows kernel's results are needed, and it was done before the dK/dV
   // kernel let this one start; the wait for that one is at the end.
 
@@ -229,113 +248,138 @@ __global__ void __launch_bounds__(256, 2) attention_dq_kernel(const __grid_const
   const int head = hk * p.group + unit % p.group, first = (gp.tiles - 1 - unit / p.group) * kTile;
   const Lengths len(p, b);
   const TileKeys keys(p, len, first);
-  const TileList<kSub> list(keys);
+  const TileList list(keys);
   const Waiter wait{&bars.gone, p.status, kWaitNs};
 
-  if (warp >= 4) {
-    registers_down<96>();
-    if (warp == 4) {
-      if (lane == 0) {
-        mbar_arrive_expect_tx(&bars.q_full, 2 * kFixed);
+  if (warp >= 8) {
+    registers_down<88>();
+    if (warp == 8) {
+      if (lane == 0 && list.n > 0) {
+        mbar_arrive_expect_tx(&bars.q_full, 2 * kTileBytes);
 #pragma unroll
         for (int box = 0; box < DP / 64; ++box) {
           tma_load(q_tile + box * kBox, &gp.q, box * 64, head, first, b, &bars.q_full);
           tma_load(do_tile + box * kBox, &gp.d_o, box * 64, head, first, b, &bars.q_full);
         }
         RingPos ring;
-        for (int j = 0; j < list.n; ++j, ring.next(2)) {
-          const int k0 = list.key(j);
-          if (!wait(&bars.k_empty[ring.s], ring.ph ^ 1)) break;
-          mbar_arrive_expect_tx(&bars.k_full[ring.s], kSubBytes);
+        auto load_key = [&](int j) {
+          if (!wait(&bars.k_empty[ring.s], ring.ph ^ 1)) return false;
+          mbar_arrive_expect_tx(&bars.k_full[ring.s], kTileBytes);
 #pragma unroll
           for (int box = 0; box < DP / 64; ++box)
-            tma_load(k_tiles + ring.s * kSubBytes + box * kSubBox, &gp.k, box * 64, hk, k0, b, &bars.k_full[ring.s]);
-          if (!wait(&bars.v_empty, (j & 1) ^ 1)) break;
-          mbar_arrive_expect_tx(&bars.v_full, kSubBytes);
+            tma_load(k_tiles + ring.s * kTileBytes + box * kBox, &gp.k, box * 64, hk, list.key(j), b, &bars.k_full[ring.s]);
+          ring.next(kKeys);
+          return true;
+        };
+        // The order in which the products need them: K(0) V(0) K(1) | V(1) K(2) | ...
+        bool ok = load_key(0);
+        for (int j = 0; j < list.n && ok; ++j) {
+          ok = wait(&bars.v_empty, (j & 1) ^ 1);
+          if (!ok) break;
+          mbar_arrive_expect_tx(&bars.v_full, kTileBytes);
 #pragma unroll
           for (int box = 0; box < DP / 64; ++box)
-            tma_load(v_tile + box * kSubBox, &gp.v, box * 64, hk, k0, b, &bars.v_full);
+            tma_load(v_tile + box * kBox, &gp.v, box * 64, hk, list.key(j), b, &bars.v_full);
+          if (j + 1 < list.n) ok = load_key(j + 1);
         }
       }
       __syncwarp();
-    } else if (warp == 5) {
+    } else if (warp == 9 && list.n > 0) {
       const Visible seen = sequence_keys(p, len);
       const uint32_t one = elect_one();
       auto warp_wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)) != 0; };
-      bool ok = warp_wait(&bars.q_full, 0);
-      RingPos ring;
-      for (int j = 0; j <= list.n && ok; ++j) {
-        uint8_t* k_tile = k_tiles + ring.s * kSubBytes;
-        uint8_t* k_last = k_tiles + (ring.s ^ 1) * kSubBytes;
-        if (j < list.n) {
-          if (!warp_wait(&bars.k_full[ring.s], ring.ph)) break;
-          clear_unseen<DP, kSub>(seen, k_tile, list.key(j), lane);
-          if (!warp_wait(&bars.v_full, j & 1)) break;
-        }
-        if (j > 0) {
-          if (!warp_wait(&bars.ds_full, (j - 1) & 1)) break;
-          tc_fence_after();
-          mma_columns<T, DP, kSub, 16>(one, dq_tmem, dp_tmem, k_last, kSubBox, j > 1);
-        }
-        if (j < list.n) {
-          mma_rows<T, DP, kSub>(one, s_tmem, q_tile, kBox, k_tile, kSubBox);
-          mma_rows<T, DP, kSub>(one, dp_tmem, do_tile, kBox, v_tile, kSubBox);
-          mma_commit(one, &bars.s_full);
-          mma_commit(one, &bars.v_empty);
-          if (j > 0) mma_commit(one, &bars.k_empty[ring.s ^ 1]);
+      RingPos ring, used;  // key tiles: of S; of dQ
+      auto scores = [&](int j) {  // S(j)
+        uint8_t* k_tile = k_tiles + ring.s * kTileBytes;
+        if (!warp_wait(&bars.k_full[ring.s], ring.ph)) return false;
+        clear_unseen<DP>(seen, k_tile, list.key(j), lane);
+        mma_rows<T, DP, kTile>(one, tmem + (j & 1) * 128, q_tile, kBox, k_tile, kBox);
+        mma_commit(one, &bars.s_full[j & 1]);
+        ring.next(kKeys);
+        return true;
+      };
+      auto products = [&](int j) {  // dP(j)
+        if (!warp_wait(&bars.v_full, j & 1)) return false;
+        mma_rows<T, DP, kTile>(one, dp_tmem, do_tile, kBox, v_tile, kBox);
+        mma_commit(one, &bars.dp_full);
+        mma_commit(one, &bars.v_empty);
+        return true;
+      };
+      bool ok = warp_wait(&bars.q_full, 0) && scores(0) && products(0);
+      if (ok && list.n > 1) ok = scores(1);
+      for (int j = 0; j < list.n && ok; ++j) {
+        if (!warp_wait(&bars.ds_full, j & 1)) break;
+        tc_fence_after();
+        mma_columns<T, DP, kTile, 64>(one, dq_tmem, dp_tmem, k_tiles + used.s * kTileBytes, kBox, j > 0);
+        if (j + 1 < list.n) {
+          ok = products(j + 1);
+          mma_commit(one, &bars.k_empty[used.s]);
+          if (ok && j + 2 < list.n) ok = scores(j + 2);
         } else {
-          mma_commit(one, &bars.dq_full);
+          mma_commit(one, &bars.done);
         }
-        ring.next(2);
+        used.next(kKeys);
       }
     }
   } else {
-    registers_up<160>();
-    const int i = first + threadIdx.x;
-    const uint32_t lanes = (uint32_t)(warp * 32) << 16;
+    registers_up<208>();
+    const int group = warp >> 2, in_tile = threadIdx.x & 127, i = first + in_tile;  // this thread's query
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, columns = group * 64;  // and its warpgroup's columns
     const Visible see = visible_keys(i < len.q ? len.position(i) : -1, len.kv, p.window, p.sinks);
     const float sl = fmaxf(p.scale * kLog2e, 1.1754944e-38f);
     const int64_t row = ((int64_t)b * p.heads + head) * gp.q_pad + i;
     const float c = ds_factor<T>(gp, bk);
-    const float lse = i < gp.q_pad ? gp.lse2[row] : -INFINITY, delta = i < gp.q_pad ? gp.delta[row] : 0.f;
-    const F2 minus_lse = f2(lse, lse), minus_delta = f2(delta, delta);
+    const F2 minus_lse = f2(gp.lse2[row], gp.lse2[row]), minus_delta = f2(gp.delta[row], gp.delta[row]);
     bool ok = true;
     for (int j = 0; j < list.n; ++j) {
-      const int k0 = list.key(j);
-      ok = __all_sync(0xffffffffu, wait(&bars.s_full, j & 1));
+      const int k0 = list.key(j) + columns;
+      const bool every = keys.every(list.key(j));
+      const uint32_t bits0 = every ? 0u : visible_bits32(see, k0), bits1 = every ? 0u : visible_bits32(see, k0 + 32);
+      ok = __all_sync(0xffffffffu, wait(&bars.s_full[j & 1], (j >> 1) & 1));
       if (!ok) break;
       tc_fence_after();
-      const bool every = keys.template every<kSub>(k0);
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        uint32_t s[32], dp[32], pp[16], ds[16];
-        tmem_load32(s_tmem + lanes + h * 32, s);
-        tmem_load32(dp_tmem + lanes + h * 32, dp);
+      float pr[64];
+      {
+        uint32_t s[64];
+        const uint32_t s_at = tmem + lanes + (j & 1) * 128 + columns;
+        tmem_load32(s_at, s);
+        tmem_load32(s_at + 32, s + 32);
         tmem_wait_loads();
-        grad32<T>(s, dp, every, every ? 0u : visible_bits32(see, k0 + h * 32), sl, c, [&](int) { return minus_lse; }, [&](int) { return minus_delta; }, pp, ds);
-        tmem_store16(dp_tmem + lanes + h * 16, ds);
+        scores_to_p(s, every, bits0, bits1, sl, [&](int) { return minus_lse; }, pr);
       }
+      ok = __all_sync(0xffffffffu, wait(&bars.dp_full, j & 1));
+      if (!ok) break;
+      tc_fence_after();
+      const uint32_t dp_at = dp_tmem + lanes + columns;
+      uint32_t dp[64], ds[32];
+      tmem_load32(dp_at, dp);
+      tmem_load32(dp_at + 32, dp + 32);
+      tmem_wait_loads();
+      p_to_ds<T>(pr, dp, every, bits0, c, [&](int) { return minus_delta; }, ds);
+      p_to_ds<T>(pr + 32, dp + 32, every, bits1, c, [&](int) { return minus_delta; }, ds + 16);
+      tmem_store32(dp_at, ds);  // over this warpgroup's own columns
       tmem_wait_stores();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars.ds_full);
     }
-    if (ok) ok = __all_sync(0xffffffffu, wait(&bars.dq_full, 0));
+    if (ok && list.n > 0) ok = __all_sync(0xffffffffu, wait(&bars.done, 0));
     if (ok) {
+      // Each warpgroup brings out half of the dims.
       tc_fence_after();
       const bool some = list.n > 0 && see.hi > 0;
 #pragma unroll 1
-      for (int cc = 0; cc < DP; cc += 32) {
+      for (int cc = group * (DP / 2); cc < (group + 1) * (DP / 2); cc += 32) {
         uint32_t o[32];
         if (list.n > 0) {
           tmem_load32(dq_tmem + lanes + cc, o);
           tmem_wait_loads();
         }
-        stage32<T>(q_tile, threadIdx.x, cc, o, p.scale / c, some);
+        stage32<T>(q_tile, in_tile, cc, o, p.scale / c, some);
       }
       fence_proxy_async_smem();
     }
-    asm volatile("bar.sync 1, 128;" ::: "memory");
+    asm volatile("bar.sync 1, 256;" ::: "memory");
     if (threadIdx.x == 0 && !*(volatile uint32_t*)&bars.gone) {
 #pragma unroll
       for (int box = 0; box < DP / 64; ++box)
@@ -345,28 +389,26 @@ __global__ void __launch_bounds__(256, 2) attention_dq_kernel(const __grid_const
     }
   }
   pdl_wait();
-  finish_tmem(bars.gone, warp == 5, tmem, kColumns);
+  finish_tmem(bars.gone, warp == 9, tmem, kColumns);
 }
 
-// ---- dK and dV: one CTA an SM. Two warpgroups take half of the columns each, so
-// that P and dS are there by the time the tensor core is through with the last
-// unit's gradients and the next one's scores (two buffers); taking the units in
-// turn instead left it waiting a third of the time.
+// ---- dK and dV
 
 struct KeyBarriers {
-  uint64_t kv_full, s_full[2], ds_full[2], done, q_full[4], q_empty[4];
+  uint64_t kv_full, s_full[2], s_free, dp_full, ds_full, done, q_full[3], q_empty[3], o_full[2], o_empty[2];
   uint32_t tmem, gone;
 };
 
 template <int DP>
 struct KeySmem {
-  static constexpr int kFixed = kTile * DP * 2, kSubBytes = kSub * DP * 2;
-  static constexpr int kStage = 2 * kSubBytes + 1024;  // Q, d_o, 64 lse2, 64 delta
-  static constexpr int kStages = 4;
-  static constexpr int kBytes = 2 * kFixed + kStages * kStage + 256;
+  static constexpr int kTileBytes = kTile * DP * 2;
+  // Q is read by S, early, and by dK, late; d_o by dP and dV. With a d_o tile
+  // come 128 numbers each of lse2 and delta.
+  static constexpr int kQueries = 3, kGrads = 2, kGrad = kTileBytes + 1024;
+  static constexpr int kBytes = (2 + kQueries) * kTileBytes + kGrads * kGrad + 256;
 };
 
-// The (head, 64 queries) units that see a tile of keys, heads first.
+// The (head, tile of queries) units that see a tile of keys, heads first.
 struct KeyUnits {
   int32_t q_first, per_head, n;  // q_first: of a head's first unit
   int32_t every_lo, every_hi;    // queries [every_lo, every_hi) see all 128 keys
@@ -381,8 +423,8 @@ struct KeyUnits {
       if (k0 + kTile > p.sinks) all = min(all, max((int64_t)k0, (int64_t)p.sinks) + p.window - pos0);
     }
     if (lo >= hi) return;
-    q_first = (int)(lo / kSub) * kSub;
-    per_head = (int)((hi + kSub - 1) / kSub - lo / kSub);
+    q_first = (int)(lo / kTile) * kTile;
+    per_head = (int)((hi + kTile - 1) / kTile - lo / kTile);
     n = per_head * p.group;
     every_lo = (int)max((int64_t)0, k0 + kTile - 1 - pos0);
     every_hi = k0 + kTile <= len.kv ? (int)max(all, (int64_t)0) : 0;
@@ -398,17 +440,26 @@ __device__ __forceinline__ void queries_of(const AttentionParams& p, const Lengt
   if (k >= len.kv) hi = lo;
 }
 
+// S(u), then dP(u), then P(u) and dS(u) live in the half (u & 1) of 256 columns,
+// each written once the warpgroups have read the one before. Products in this
+// order:
+//   S(0) S(1) dP(0) | dV(0) dP(1) dK(0) S(2) | dV(1) dP(2) dK(1) S(3) | ...
+// While the warpgroups turn S(u + 1) into P(u + 1) (kept in registers) the tensor
+// core has dV(u), dP(u + 1) and dK(u); while they make dS(u + 1), S(u + 2).
+// Measured in cycles a tile: P over S, so that S(u + 1) waits for dV(u), 3400; P
+// and dS over dP, so that dP(u + 1) waits for dK(u), 3290; this one TODO.
 template <typename T, int DP>
-__global__ void __launch_bounds__(384, 1) attention_dkv_kernel(const __grid_constant__ GradParams gp) {
+__global__ void __launch_bounds__(kGradThreads, 1) attention_dkv_kernel(const __grid_constant__ GradParams gp) {
   using Smem = KeySmem<DP>;
-  constexpr int kBox = kTile * 128, kSubBox = kSub * 128, kFixed = Smem::kFixed, kSubBytes = Smem::kSubBytes, kStages = Smem::kStages;
+  constexpr int kBox = kTile * 128, kTileBytes = Smem::kTileBytes, kQueries = Smem::kQueries, kGrads = Smem::kGrads, kGrad = Smem::kGrad;
   constexpr uint32_t kColumns = 512;
   constexpr float kShift = T::kIsHalf ? 15.f : 0.f;
   extern __shared__ __align__(1024) uint8_t aligned_smem[];
   uint8_t* k_tile = aligned_smem;
-  uint8_t* v_tile = k_tile + kFixed;
-  uint8_t* stages = v_tile + kFixed;
-  KeyBarriers& bars = *reinterpret_cast<KeyBarriers*>(stages + kStages * Smem::kStage);
+  uint8_t* v_tile = k_tile + kTileBytes;
+  uint8_t* q_tiles = v_tile + kTileBytes;
+  uint8_t* grads = q_tiles + kQueries * kTileBytes;
+  KeyBarriers& bars = *reinterpret_cast<KeyBarriers*>(grads + kGrads * kGrad);
   const AttentionParams& p = gp.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (smem_addr(aligned_smem) & 1023) {
@@ -417,14 +468,19 @@ __global__ void __launch_bounds__(384, 1) attention_dkv_kernel(const __grid_cons
   }
   if (warp == 8 && lane == 0) {
     mbar_init(&bars.kv_full, 1);
+    mbar_init(&bars.s_full[0], 1);
+    mbar_init(&bars.s_full[1], 1);
+    mbar_init(&bars.s_free, 8);
+    mbar_init(&bars.dp_full, 1);
+    mbar_init(&bars.ds_full, 8);
     mbar_init(&bars.done, 1);
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&bars.s_full[i], 1);
-      mbar_init(&bars.ds_full[i], 8);
-    }
-    for (int i = 0; i < kStages; ++i) {
+    for (int i = 0; i < kQueries; ++i) {
       mbar_init(&bars.q_full[i], 1);
       mbar_init(&bars.q_empty[i], 1);
+    }
+    for (int i = 0; i < kGrads; ++i) {
+      mbar_init(&bars.o_full[i], 1);
+      mbar_init(&bars.o_empty[i], 1);
     }
     bars.gone = 0;
     fence_barrier_init();
@@ -443,11 +499,11 @@ __global__ void __launch_bounds__(384, 1) attention_dkv_kernel(const __grid_cons
 
   // Which key tile and which share of its units; a kv head's CTAs are apart, so
   // that neighbours in time read the same queries.
-  const int bk = blockIdx.x % (p.batch * p.kv_heads), at = blockIdx.x / (p.batch * p.kv_heads);
+  const int bk = blockIdx.x % (p.batch * p.kv_heads), which = blockIdx.x / (p.batch * p.kv_heads);
   const int b = bk / p.kv_heads, hk = bk - b * p.kv_heads;
   const int in_sinks = gp.sink_tiles * gp.sink_shares;
-  const int tile = at < in_sinks ? at / gp.sink_shares : gp.sink_tiles + (at - in_sinks) / gp.window_shares;
-  const int share = at < in_sinks ? at % gp.sink_shares : (at - in_sinks) % gp.window_shares;
+  const int tile = which < in_sinks ? which / gp.sink_shares : gp.sink_tiles + (which - in_sinks) / gp.window_shares;
+  const int share = which < in_sinks ? which % gp.sink_shares : (which - in_sinks) % gp.window_shares;
   const int k0 = tile * kTile;
   const Lengths len(p, b);
   const KeyUnits units(p, len, k0);
@@ -455,150 +511,196 @@ __global__ void __launch_bounds__(384, 1) attention_dkv_kernel(const __grid_cons
   const Waiter wait{&bars.gone, p.status, kWaitNs};
 
   if (n > 0 || share == 0) {
-  if (warp >= 8) {
-    registers_down<152>();
-    if (warp == 8) {
-      if (lane == 0 && n > 0) {
-        mbar_arrive_expect_tx(&bars.kv_full, 2 * kFixed);
-#pragma unroll
-        for (int box = 0; box < DP / 64; ++box) {
-          tma_load(k_tile + box * kBox, &gp.k, box * 64, hk, k0, b, &bars.kv_full);
-          tma_load(v_tile + box * kBox, &gp.v, box * 64, hk, k0, b, &bars.kv_full);
-        }
-        RingPos ring;
-        for (int u = u0; u < u0 + n; ++u, ring.next(kStages)) {
-          const int h = u / units.per_head, i0 = units.q_first + (u - h * units.per_head) * kSub, head = hk * p.group + h;
-          uint8_t* stage = stages + ring.s * Smem::kStage;
-          if (!wait(&bars.q_empty[ring.s], ring.ph ^ 1)) break;
-          mbar_arrive_expect_tx(&bars.q_full[ring.s], 2 * kSubBytes + 512);
+    if (warp >= 8) {
+      registers_down<88>();
+      if (warp == 8) {
+        if (lane == 0 && n > 0) {
+          mbar_arrive_expect_tx(&bars.kv_full, 2 * kTileBytes);
 #pragma unroll
           for (int box = 0; box < DP / 64; ++box) {
-            tma_load(stage + box * kSubBox, &gp.q, box * 64, head, i0, b, &bars.q_full[ring.s]);
-            tma_load(stage + kSubBytes + box * kSubBox, &gp.d_o, box * 64, head, i0, b, &bars.q_full[ring.s]);
+            tma_load(k_tile + box * kBox, &gp.k, box * 64, hk, k0, b, &bars.kv_full);
+            tma_load(v_tile + box * kBox, &gp.v, box * 64, hk, k0, b, &bars.kv_full);
           }
-          const int64_t row = ((int64_t)b * p.heads + head) * gp.q_pad + i0;
-          bulk_g2s(stage + 2 * kSubBytes, gp.lse2 + row, 256, &bars.q_full[ring.s]);
-          bulk_g2s(stage + 2 * kSubBytes + 256, gp.delta + row, 256, &bars.q_full[ring.s]);
+          RingPos q_at, o_at;
+          auto load_query = [&](int u) {
+            const int h = u / units.per_head, i0 = units.q_first + (u - h * units.per_head) * kTile, head = hk * p.group + h;
+            if (!wait(&bars.q_empty[q_at.s], q_at.ph ^ 1)) return false;
+            mbar_arrive_expect_tx(&bars.q_full[q_at.s], kTileBytes);
+#pragma unroll
+            for (int box = 0; box < DP / 64; ++box)
+              tma_load(q_tiles + q_at.s * kTileBytes + box * kBox, &gp.q, box * 64, head, i0, b, &bars.q_full[q_at.s]);
+            q_at.next(kQueries);
+            return true;
+          };
+          auto load_grad = [&](int u) {
+            const int h = u / units.per_head, i0 = units.q_first + (u - h * units.per_head) * kTile, head = hk * p.group + h;
+            if (!wait(&bars.o_empty[o_at.s], o_at.ph ^ 1)) return false;
+            uint8_t* to = grads + o_at.s * kGrad;
+            mbar_arrive_expect_tx(&bars.o_full[o_at.s], kGrad);
+#pragma unroll
+            for (int box = 0; box < DP / 64; ++box)
+              tma_load(to + box * kBox, &gp.d_o, box * 64, head, i0, b, &bars.o_full[o_at.s]);
+            const int64_t row = ((int64_t)b * p.heads + head) * gp.q_pad + i0;
+            bulk_g2s(to + kTileBytes, gp.lse2 + row, 512, &bars.o_full[o_at.s]);
+            bulk_g2s(to + kTileBytes + 512, gp.delta + row, 512, &bars.o_full[o_at.s]);
+            o_at.next(kGrads);
+            return true;
+          };
+          // In the order in which the products need them.
+          bool ok = load_query(u0);
+          for (int u = u0; u < u0 + n && ok; ++u) {
+            ok = load_grad(u);
+            if (ok && u + 1 < u0 + n) ok = load_query(u + 1);
+          }
         }
-      }
-      __syncwarp();
-    } else if (warp == 9) {
-      const uint32_t one = elect_one();
-      auto warp_wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)) != 0; };
-      const int q_lo = max(0, -len.position(0));  // queries before it are at negative positions
-      bool ok = n > 0 && warp_wait(&bars.kv_full, 0);
-      RingPos next, ring;  // of the scores; of the gradients, one unit behind
-      int sub = n > 0 ? u0 % units.per_head : 0;
-      for (int u = 0; u <= n && ok; ++u) {
-        if (u < n) {
-          uint8_t* stage = stages + next.s * Smem::kStage;
-          if (!warp_wait(&bars.q_full[next.s], next.ph)) break;
-          const int i0 = units.q_first + sub * kSub;
+        __syncwarp();
+      } else if (warp == 9 && n > 0) {
+        const uint32_t one = elect_one();
+        auto warp_wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)) != 0; };
+        const int q_lo = max(0, -len.position(0));  // queries before it are at negative positions
+        RingPos q_next, q_used, o_next, o_used;  // of S and of dK; of dP and of dV
+        int q_sub = u0 % units.per_head, o_sub = q_sub;
+        // Zero the rows of a tile that are no queries of the sequence.
+        auto clean = [&](uint8_t* tile, int& sub) {
+          const int i0 = units.q_first + sub * kTile;
           if (++sub == units.per_head) sub = 0;
-          if (i0 < q_lo || i0 + kSub > len.q) {
-            auto keep = [&](int r) { return i0 + r >= q_lo && i0 + r < len.q; };
-            clear_rows<DP, kSub>(stage, lane, keep);
-            clear_rows<DP, kSub>(stage + kSubBytes, lane, keep);
-          }
-          // The buffer is free: unit u - 2's gradients are ahead in the queue.
-          const uint32_t s = tmem + (u & 1) * 128;
-          mma_rows<T, DP, kSub>(one, s, k_tile, kBox, stage, kSubBox);
-          mma_rows<T, DP, kSub>(one, s + 64, v_tile, kBox, stage + kSubBytes, kSubBox);
+          if (i0 < q_lo || i0 + kTile > len.q) clear_rows<DP>(tile, lane, [&](int r) { return i0 + r >= q_lo && i0 + r < len.q; });
+        };
+        auto scores = [&](int u) {  // S(u)
+          uint8_t* q_tile = q_tiles + q_next.s * kTileBytes;
+          if (!warp_wait(&bars.q_full[q_next.s], q_next.ph)) return false;
+          clean(q_tile, q_sub);
+          mma_rows<T, DP, kTile>(one, tmem + (u & 1) * 128, k_tile, kBox, q_tile, kBox);
           mma_commit(one, &bars.s_full[u & 1]);
-          next.next(kStages);
-        }
-        if (u > 0) {
-          const int w = u - 1;
-          uint8_t* stage = stages + ring.s * Smem::kStage;
-          if (!warp_wait(&bars.ds_full[w & 1], (w >> 1) & 1)) break;
+          q_next.next(kQueries);
+          return true;
+        };
+        auto products = [&](int u) {  // dP(u)
+          uint8_t* o_tile = grads + o_next.s * kGrad;
+          if (!warp_wait(&bars.o_full[o_next.s], o_next.ph)) return false;
+          clean(o_tile, o_sub);
+          if (!warp_wait(&bars.s_free, u & 1)) return false;
           tc_fence_after();
-          const uint32_t s = tmem + (w & 1) * 128;
-          mma_columns<T, DP, kSub, 32>(one, dv_tmem, s, stage + kSubBytes, kSubBox, w > 0);
-          mma_columns<T, DP, kSub, 32>(one, dk_tmem, s + 64, stage, kSubBox, w > 0);
-          mma_commit(one, w == n - 1 ? &bars.done : &bars.q_empty[ring.s]);
-          ring.next(kStages);
+          mma_rows<T, DP, kTile>(one, tmem + (u & 1) * 128, v_tile, kBox, o_tile, kBox);
+          mma_commit(one, &bars.dp_full);
+          o_next.next(kGrads);
+          return true;
+        };
+        bool ok = warp_wait(&bars.kv_full, 0) && scores(0);
+        if (ok && n > 1) ok = scores(1);
+        if (ok) ok = products(0);
+        for (int u = 0; u < n && ok; ++u) {
+          const uint32_t at = tmem + (u & 1) * 128;
+          if (!warp_wait(&bars.ds_full, u & 1)) break;
+          tc_fence_after();
+          // Each stage is given back as soon as its last product is in the queue:
+          // loads take most of a tile's time.
+          mma_columns<T, DP, kTile, 64>(one, dv_tmem, at, grads + o_used.s * kGrad, kBox, u > 0);
+          mma_commit(one, &bars.o_empty[o_used.s]);
+          if (u + 1 < n && !products(u + 1)) break;
+          mma_columns<T, DP, kTile, 64>(one, dk_tmem, at + 32, q_tiles + q_used.s * kTileBytes, kBox, u > 0);
+          mma_commit(one, u + 1 < n ? &bars.q_empty[q_used.s] : &bars.done);
+          if (u + 2 < n) ok = scores(u + 2);
+          o_used.next(kGrads);
+          q_used.next(kQueries);
         }
       }
-    }
-  } else {
-    registers_up<176>();
-    const int group = warp >> 2, row = threadIdx.x & 127;  // warpgroup; this thread's key
-    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t half = tmem + lanes + group * 32;  // this warpgroup's columns of the first buffer's S
-    const float sl = fmaxf(p.scale * kLog2e, 1.1754944e-38f);
-    const float c = ds_factor<T>(gp, bk), k1 = T::kIsHalf ? c * (1.f / kHalfTop) : 1.f;
-    int q_lo, q_hi;
-    queries_of(p, len, k0 + row, q_lo, q_hi);
-    bool ok = true;
-    int sub = n > 0 ? u0 % units.per_head : 0;
-    RingPos ring;
-    for (int u = 0; u < n; ++u, ring.next(kStages)) {
-      const int i0 = units.q_first + sub * kSub;
-      if (++sub == units.per_head) sub = 0;
-      const float* rows = reinterpret_cast<const float*>(stages + ring.s * Smem::kStage + 2 * kSubBytes) + group * 32;
-      ok = __all_sync(0xffffffffu, wait(&bars.q_full[ring.s], ring.ph) && wait(&bars.s_full[u & 1], (u >> 1) & 1));
-      if (!ok) break;
-      tc_fence_after();
-      const bool every = i0 >= units.every_lo && i0 + kSub <= units.every_hi;
-      const uint32_t s_at = half + (u & 1) * 128, dp_at = s_at + 64;
-      uint32_t s[32], dp[32], pp[16], ds[16];
-      tmem_load32(s_at, s);
-      tmem_load32(dp_at, dp);
-      const int at = i0 + group * 32;
-      const uint32_t bits = every ? 0u : below_bits(q_hi - at) & ~below_bits(q_lo - at);
-      tmem_wait_loads();
-      const F2 shift2 = f2(kShift, kShift);
-      auto pair = [&](int e) {  // two rows' numbers
-        const float2 v = *reinterpret_cast<const float2*>(rows + e);
-        return f2(v.x, v.y);
-      };
-      grad32<T>(s, dp, every, bits, sl, k1, [&](int e) { return T::kIsHalf ? f2_add(pair(e), shift2) : pair(e); },
-                [&](int e) { return pair(64 + e); }, pp, ds);
-      tmem_store16(s_at, pp);  // over this warpgroup's own columns
-      tmem_store16(dp_at, ds);
-      tmem_wait_stores();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bars.ds_full[u & 1]);
-    }
-    if (ok && n > 0) ok = __all_sync(0xffffffffu, wait(&bars.done, 0));
-    if (ok) {
-      // Warpgroup 0 brings out dV, warpgroup 1 dK.
-      tc_fence_after();
-      const uint32_t from = (group ? dk_tmem : dv_tmem) + lanes;
-      const float factor = group ? p.scale / c : T::kIsHalf ? 1.f / kHalfTop : 1.f;
-      uint8_t* tile_smem = group ? k_tile : v_tile;
-      const bool whole = units.n <= gp.share;
-      float4* part = reinterpret_cast<float4*>(gp.partial) + ((int64_t)blockIdx.x * 2 + group) * (kTile * DP / 4) + row;
-#pragma unroll 1
-      for (int cc = 0; cc < DP; cc += 32) {
-        uint32_t o[32];
-        if (n > 0) {
-          tmem_load32(from + cc, o);
+    } else {
+      registers_up<208>();
+      const int group = warp >> 2, row = threadIdx.x & 127;  // this thread's key
+      const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+      const int columns = group * 64;  // this warpgroup's queries of a tile
+      const float sl = fmaxf(p.scale * kLog2e, 1.1754944e-38f);
+      const float c = ds_factor<T>(gp, bk), k1 = T::kIsHalf ? c * (1.f / kHalfTop) : 1.f;
+      int q_lo, q_hi;
+      queries_of(p, len, k0 + row, q_lo, q_hi);
+      bool ok = true;
+      int sub = n > 0 ? u0 % units.per_head : 0;
+      RingPos ring;
+      for (int u = 0; u < n; ++u, ring.next(kGrads)) {
+        const int i0 = units.q_first + sub * kTile, first = i0 + columns;
+        if (++sub == units.per_head) sub = 0;
+        const float* rows = reinterpret_cast<const float*>(grads + ring.s * kGrad + kTileBytes) + columns;
+        const bool every = i0 >= units.every_lo && i0 + kTile <= units.every_hi;
+        const uint32_t bits0 = every ? 0u : below_bits(q_hi - first) & ~below_bits(q_lo - first);
+        const uint32_t bits1 = every ? 0u : below_bits(q_hi - first - 32) & ~below_bits(q_lo - first - 32);
+        float4 quad;
+        auto pair = [&](int e) {  // two queries' numbers, read four at a time
+          if (!(e & 2)) quad = *reinterpret_cast<const float4*>(rows + e);
+          return e & 2 ? f2(quad.z, quad.w) : f2(quad.x, quad.y);
+        };
+        ok = __all_sync(0xffffffffu, wait(&bars.o_full[ring.s], ring.ph) && wait(&bars.s_full[u & 1], (u >> 1) & 1));
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t at = tmem + lanes + (u & 1) * 128 + columns;
+        float pr[64];
+        uint32_t out[32];
+        {
+          uint32_t s[64];
+          tmem_load32(at, s);
+          tmem_load32(at + 32, s + 32);
           tmem_wait_loads();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bars.s_free);
+          scores_to_p(s, every, bits0, bits1, sl, [&](int e) { return T::kIsHalf ? f2_add(pair(e), f2(kShift, kShift)) : pair(e); }, pr);
         }
-        if (whole) {
-          stage32<T>(tile_smem, row, cc, o, factor, n > 0 && q_lo < q_hi);
-        } else {
+        ok = __all_sync(0xffffffffu, wait(&bars.dp_full, u & 1));
+        if (!ok) break;
+        tc_fence_after();
+        uint32_t dp[32], ds[32];
 #pragma unroll
-          for (int e = 0; e < 8; ++e)
-            part[(cc / 4 + e) * kTile] =
-                make_float4(__uint_as_float(o[4 * e]) * factor, __uint_as_float(o[4 * e + 1]) * factor,
-                            __uint_as_float(o[4 * e + 2]) * factor, __uint_as_float(o[4 * e + 3]) * factor);
+        for (int h = 0; h < 2; ++h) {
+          tmem_load32(at + h * 32, dp);
+          tmem_wait_loads();
+          p_to_ds<T>(pr + h * 32, dp, every, h ? bits1 : bits0, k1, [&](int e) { return pair(128 + h * 32 + e); }, ds + h * 16);
+#pragma unroll
+          for (int e = 0; e < 16; ++e) out[h * 16 + e] = T::pack(pr[h * 32 + 2 * e], pr[h * 32 + 2 * e + 1]);
         }
+        tmem_store32(at, out);  // over this warpgroup's own columns: P, then dS
+        tmem_store32(at + 32, ds);
+        tmem_wait_stores();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars.ds_full);
       }
-      fence_proxy_async_smem();
-    }
-    asm volatile("bar.sync %0, 128;" ::"r"(1 + group) : "memory");
-    if (row == 0 && units.n <= gp.share && !*(volatile uint32_t*)&bars.gone) {
+      if (ok && n > 0) ok = __all_sync(0xffffffffu, wait(&bars.done, 0));
+      if (ok) {
+        // Warpgroup 0 brings out dV, warpgroup 1 dK.
+        tc_fence_after();
+        const uint32_t from = (group ? dk_tmem : dv_tmem) + lanes;
+        const float factor = group ? p.scale / c : T::kIsHalf ? 1.f / kHalfTop : 1.f;
+        const bool whole = units.n <= gp.share;
+        float4* part = reinterpret_cast<float4*>(gp.partial) + ((int64_t)blockIdx.x * 2 + group) * (kTile * DP / 4) + row;
+#pragma unroll 1
+        for (int cc = 0; cc < DP; cc += 32) {
+          uint32_t o[32];
+          if (n > 0) {
+            tmem_load32(from + cc, o);
+            tmem_wait_loads();
+          }
+          if (whole) {
+            stage32<T>(group ? k_tile : v_tile, row, cc, o, factor, n > 0 && q_lo < q_hi);
+          } else {
 #pragma unroll
-      for (int box = 0; box < DP / 64; ++box)
-        if (box * 64 < p.head_dim)
-          tma_store(group ? &gp.out0 : &gp.out1, (group ? k_tile : v_tile) + box * kBox, box * 64, hk, k0, b);
-      bulk_commit();
-      bulk_wait_all();
+            for (int e = 0; e < 8; ++e)
+              part[(cc / 4 + e) * kTile] =
+                  make_float4(__uint_as_float(o[4 * e]) * factor, __uint_as_float(o[4 * e + 1]) * factor,
+                              __uint_as_float(o[4 * e + 2]) * factor, __uint_as_float(o[4 * e + 3]) * factor);
+          }
+        }
+        fence_proxy_async_smem();
+      }
+      asm volatile("bar.sync %0, 128;" ::"r"(1 + group) : "memory");
+      if (row == 0 && units.n <= gp.share && !*(volatile uint32_t*)&bars.gone) {
+#pragma unroll
+        for (int box = 0; box < DP / 64; ++box)
+          if (box * 64 < p.head_dim)
+            tma_store(group ? &gp.out0 : &gp.out1, (group ? k_tile : v_tile) + box * kBox, box * 64, hk, k0, b);
+        bulk_commit();
+        bulk_wait_all();
+      }
     }
-  }
   }
   finish_tmem(bars.gone, warp == 9, tmem, kColumns);
 }

@@ -61,23 +61,21 @@ struct TileKeys {
     all_hi = first.hi;
     all_s_end = first.s_end;
   }
-  template <int STEP>
   __device__ __forceinline__ bool every(int k0) const {
-    return k0 + STEP <= all_s_end || (k0 >= all_lo && k0 + STEP <= all_hi);
+    return k0 + kTile <= all_s_end || (k0 >= all_lo && k0 + kTile <= all_hi);
   }
 };
 
-// A query tile's key tiles of STEP keys, numbered densely.
-template <int STEP>
+// A query tile's key tiles, numbered densely.
 struct TileList {
   int32_t n_sink, w_beg, n;
   __device__ __forceinline__ explicit TileList(const TileKeys& a) {
-    const int s = (a.s_end + STEP - 1) / STEP;
-    w_beg = a.lo < a.hi ? a.lo / STEP : s;
+    const int s = (a.s_end + kTile - 1) / kTile;
+    w_beg = a.lo < a.hi ? a.lo / kTile : s;
     n_sink = min(s, w_beg);
-    n = n_sink + (a.lo < a.hi ? (a.hi + STEP - 1) / STEP - w_beg : s - n_sink);
+    n = n_sink + (a.lo < a.hi ? (a.hi + kTile - 1) / kTile - w_beg : s - n_sink);
   }
-  __device__ __forceinline__ int key(int j) const { return (j < n_sink ? j : j - n_sink + w_beg) * STEP; }
+  __device__ __forceinline__ int key(int j) const { return (j < n_sink ? j : j - n_sink + w_beg) * kTile; }
 };
 
 __device__ __forceinline__ uint32_t below_bits(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
@@ -88,25 +86,25 @@ __device__ __forceinline__ uint32_t visible_bits32(const Visible& v, int k0) {
 }
 
 // Zero the rows of a staged tile for which keep(row) is false: they may hold
-// NaN, and 0 times NaN is NaN. One warp; boxes of ROWS x 64 elements.
-template <int DP, int ROWS, typename Keep>
+// NaN, and 0 times NaN is NaN. One warp.
+template <int DP, typename Keep>
 __device__ __forceinline__ void clear_rows(uint8_t* tile, int lane, Keep keep) {
 #pragma unroll 1
-  for (int r = 0; r < ROWS; ++r) {
+  for (int r = 0; r < kTile; ++r) {
     if (keep(r)) continue;
 #pragma unroll
     for (int box = 0; box < DP / 64; ++box)
-      if (lane < 8) *reinterpret_cast<uint4*>(tile + box * (ROWS * 128) + r * 128 + lane * 16) = make_uint4(0, 0, 0, 0);
+      if (lane < 8) *reinterpret_cast<uint4*>(tile + box * (kTile * 128) + r * 128 + lane * 16) = make_uint4(0, 0, 0, 0);
   }
   fence_proxy_async_smem();
   __syncwarp();
 }
 
 // Keys (or values) k0.. of which no query of the sequence sees some.
-template <int DP, int ROWS>
+template <int DP>
 __device__ __forceinline__ void clear_unseen(const Visible& seen, uint8_t* tile, int k0, int lane) {
-  if (k0 + ROWS <= seen.s_end || (k0 >= seen.lo && k0 + ROWS <= seen.hi)) return;
-  clear_rows<DP, ROWS>(tile, lane, [&](int r) { return sees(seen, k0 + r); });
+  if (k0 + kTile <= seen.s_end || (k0 >= seen.lo && k0 + kTile <= seen.hi)) return;
+  clear_rows<DP>(tile, lane, [&](int r) { return sees(seen, k0 + r); });
 }
 
 // What the queries of a sequence see together.
@@ -119,6 +117,43 @@ __device__ __forceinline__ Visible sequence_keys(const AttentionParams& p, const
     v.s_end = min(v.s_end, v.lo);
   }
   return v;
+}
+
+// Maximum of 128 scores: eight chains, so that no long one holds a row up.
+__device__ __forceinline__ float max128(const uint32_t* s) {
+  float m[8];
+#pragma unroll
+  for (int q = 0; q < 8; ++q) m[q] = __uint_as_float(s[q]);
+#pragma unroll
+  for (int e = 8; e < 120; e += 16)
+#pragma unroll
+    for (int q = 0; q < 8; ++q) m[q] = fmaxf(fmaxf(m[q], __uint_as_float(s[e + q])), __uint_as_float(s[e + q + 8]));
+#pragma unroll
+  for (int q = 0; q < 8; ++q) m[q] = fmaxf(m[q], __uint_as_float(s[120 + q]));
+  return fmaxf(fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])), fmaxf(fmaxf(m[4], m[5]), fmaxf(m[6], m[7])));
+}
+
+// A row's P = 2^(sl s + nb) in 16-bit pairs to TMEM; its sum. (Taking some of the
+// exponentials by a polynomial, to spare the exponential unit, was slower at
+// every share from 1 to 4 in 8: 438 us at 0, 445 at 1, 468 at 2 for 16384
+// queries, window 4096, dim 128. Packed f32x2 arithmetic: 438, scalar 434.)
+template <typename T>
+__device__ __forceinline__ float write_p(const uint32_t* s, float sl, float nb, uint32_t at) {
+  float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    uint32_t packed[16];
+#pragma unroll
+    for (int e = 0; e < 32; e += 2) {
+      const float x = ex2(__fmaf_rn(__uint_as_float(s[c * 32 + e]), sl, nb));
+      const float y = ex2(__fmaf_rn(__uint_as_float(s[c * 32 + e + 1]), sl, nb));
+      sum[e & 2] += x;
+      sum[(e & 2) + 1] += y;
+      packed[e / 2] = T::pack(x, y);
+    }
+    tmem_store16(at + c * 16, packed);
+  }
+  return (sum[0] + sum[1]) + (sum[2] + sum[3]);
 }
 
 template <int DP>
@@ -177,7 +212,7 @@ __global__ void __launch_bounds__(kTileThreads, 2) attention_tiles_kernel(const 
   const int head = hk * p.group + unit % p.group, first = (tp.q_tiles - 1 - unit / p.group) * kTile;
   const Lengths len(p, b);
   const TileKeys keys(p, len, first);
-  const TileList<kTile> list(keys);
+  const TileList list(keys);
   const Waiter wait{&bars.gone, p.status, kWaitNs};
 
   if (warp >= 4) {
@@ -211,14 +246,14 @@ __global__ void __launch_bounds__(kTileThreads, 2) attention_tiles_kernel(const 
         const int v_slot = ring.s;
         if (j > 0) {
           if (!warp_wait(&bars.kv_full[v_slot], ring.ph)) break;
-          clear_unseen<DP, kTile>(seen, stages + v_slot * kTileBytes, list.key(j - 1), lane);
+          clear_unseen<DP>(seen, stages + v_slot * kTileBytes, list.key(j - 1), lane);
           ring.next(kStages);
         }
         if (j < list.n && !warp_wait(&bars.kv_full[ring.s], ring.ph)) break;
         if (j > 0) {
           if (!warp_wait(&bars.p_full, (j - 1) & 1)) break;
           tc_fence_after();
-          mma_columns<T, DP, kTile, 16>(one, o_tmem, s_tmem, stages + v_slot * kTileBytes, kBox, j > 1);
+          mma_columns<T, DP, kTile, 32>(one, o_tmem, s_tmem, stages + v_slot * kTileBytes, kBox, j > 1);
         }
         if (j < list.n) {
           // One queue of products: commits come behind both (a commit between
@@ -255,7 +290,7 @@ __global__ void __launch_bounds__(kTileThreads, 2) attention_tiles_kernel(const 
 #pragma unroll
       for (int c = 0; c < 4; ++c) tmem_load32(s_at + c * 32, raw + c * 32);
       tmem_wait_loads();
-      if (!keys.every<kTile>(k0)) {
+      if (!keys.every(k0)) {
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           const uint32_t bits = visible_bits32(see, k0 + c * 32);
@@ -264,10 +299,7 @@ __global__ void __launch_bounds__(kTileThreads, 2) attention_tiles_kernel(const 
             if (!((bits >> e) & 1)) raw[c * 32 + e] = 0xFF800000u;
         }
       }
-      float top = __uint_as_float(raw[0]);
-#pragma unroll
-      for (int e = 1; e < 128; ++e) top = fmaxf(top, __uint_as_float(raw[e]));
-      top *= sl;
+      const float top = max128(raw) * sl;
       if (__any_sync(0xffffffffu, top > m + kMaxLag)) {
         const float next = fmaxf(m, top), f = next == -INFINITY ? 1.f : ex2(m - next);
         m = next;
@@ -285,23 +317,7 @@ __global__ void __launch_bounds__(kTileThreads, 2) attention_tiles_kernel(const 
         }
       }
       const float nb = m == -INFINITY ? 0.f : kShift - m;
-      const F2 sl2 = f2(sl, sl), nb2 = f2(nb, nb);
-      F2 sum0 = f2(0.f, 0.f), sum1 = sum0;
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        uint32_t packed[32];
-#pragma unroll
-        for (int e = 0; e < 32; ++e) {
-          const float2 x = f2_out(f2_fma(f2(__uint_as_float(raw[c * 64 + 2 * e]), __uint_as_float(raw[c * 64 + 2 * e + 1])), sl2, nb2));
-          const float x0 = ex2(x.x), x1 = ex2(x.y);
-          if (e & 1) sum1 = f2_add(sum1, f2(x0, x1));
-          else sum0 = f2_add(sum0, f2(x0, x1));
-          packed[e] = T::pack(x0, x1);
-        }
-        tmem_store32(s_at + c * 32, packed);
-      }
-      const float2 sum = f2_out(f2_add(sum0, sum1));
-      l += sum.x + sum.y;
+      l += write_p<T>(raw, sl, nb, s_at);
       tmem_wait_stores();
       tc_fence_before();
       __syncwarp();

@@ -190,14 +190,14 @@ __device__ __forceinline__ void mma_rows(uint32_t one, uint32_t d, const uint8_t
 }
 
 // D[128, DP] (+)= A[128, K] B[K, DP]: A in TMEM, two elements a column, its
-// 32-element parts PART columns apart (16: contiguous); B a row tile of DP / 64
+// 64-element parts PART columns apart (32: contiguous); B a row tile of DP / 64
 // boxes.
 template <typename T, int DP, int K, int PART>
 __device__ __forceinline__ void mma_columns(uint32_t one, uint32_t d, uint32_t a, const uint8_t* b, int b_box, bool add) {
   const uint64_t b0 = operand(b, (uint32_t)b_box);
 #pragma unroll
   for (int k = 0; k < K / 16; ++k)
-    mma_ts(one, d, a + (k >> 1) * PART + (k & 1) * 8, b0 + k * (2048 >> 4), product<T>(128, DP, true), add || k > 0);
+    mma_ts(one, d, a + (k >> 2) * PART + (k & 3) * 8, b0 + k * (2048 >> 4), product<T>(128, DP, true), add || k > 0);
 }
 
 }  // namespace cs
