@@ -163,22 +163,7 @@ __device__ __forceinline__ void p_to_ds(const float* p, const uint32_t* dp, bool
   }
 }
 
-// Stage 32 columns of this thread's row (128-byte swizzle, box of 128 rows).
-template <typename T>
-__device__ __forceinline__ void stage32(uint8_t* tile, int row, int c, const uint32_t* v, float factor, bool some) {
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    uint32_t w[4];
-#pragma unroll
-    for (int h = 0; h < 4; ++h)
-      w[h] = some ? T::pack(__uint_as_float(v[8 * e + 2 * h]) * factor, __uint_as_float(v[8 * e + 2 * h + 1]) * factor) : 0u;
-    const int chunk = (c & 63) / 8 + e;
-    *reinterpret_cast<uint4*>(tile + (c >> 6) * (kTile * 128) + row * 128 + ((chunk ^ (row & 7)) << 4)) =
-        make_uint4(w[0], w[1], w[2], w[3]);
-  }
-}
-
-constexpr int kGradThreads = 384;  // registers: 2 x 128 x 208 + 128 x 88 = 384 x 168
+constexpr int kGradThreads = 384;  // registers: 384 x 168 = 256 x 192 + 128 x 120 (dQ) = 256 x 232 + 128 x 40 (dK, dV)
 
 // ---- dQ
 
@@ -252,7 +237,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) attention_dq_kernel(const __g
   const Waiter wait{&bars.gone, p.status, kWaitNs};
 
   if (warp >= 8) {
-    registers_down<88>();
+    registers_down<120>();
     if (warp == 8) {
       if (lane == 0 && list.n > 0) {
         mbar_arrive_expect_tx(&bars.q_full, 2 * kTileBytes);
@@ -322,7 +307,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) attention_dq_kernel(const __g
       }
     }
   } else {
-    registers_up<208>();
+    registers_up<192>();
     const int group = warp >> 2, in_tile = threadIdx.x & 127, i = first + in_tile;  // this thread's query
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, columns = group * 64;  // and its warpgroup's columns
     const Visible see = visible_keys(i < len.q ? len.position(i) : -1, len.kv, p.window, p.sinks);
@@ -512,7 +497,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) attention_dkv_kernel(const __
 
   if (n > 0 || share == 0) {
     if (warp >= 8) {
-      registers_down<88>();
+      registers_down<40>();
       if (warp == 8) {
         if (lane == 0 && n > 0) {
           mbar_arrive_expect_tx(&bars.kv_full, 2 * kTileBytes);
@@ -606,7 +591,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) attention_dkv_kernel(const __
         }
       }
     } else {
-      registers_up<208>();
+      registers_up<232>();
       const int group = warp >> 2, row = threadIdx.x & 127;  // this thread's key
       const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
       const int columns = group * 64;  // this warpgroup's queries of a tile

@@ -17,7 +17,9 @@
 // also covers. Measured against one CTA an SM with two query tiles that share
 // each key tile (half the L2 traffic): 16384 queries x 16 heads, window 4096,
 // dim 128: 468 us against 509; dim 64: 425 against 459; 512 over 8192: 112
-// against 147.
+// against 147. (A query in two threads, 64 keys of a tile each: 440, 374 and 104
+// against 435, 362 and 105 of one thread. At dim 128 the power limit holds the
+// clock down: 1.62 GHz under this kernel alone, 1.95 at dim 64.)
 //
 // Running maximum: it moves only when a row passes it by more than 2^8, so the
 // output in TMEM is rescaled rarely (all sums are relative to the same
@@ -117,6 +119,21 @@ __device__ __forceinline__ Visible sequence_keys(const AttentionParams& p, const
     v.s_end = min(v.s_end, v.lo);
   }
   return v;
+}
+
+// Stage 32 columns of this thread's row (128-byte swizzle, box of 128 rows).
+template <typename T>
+__device__ __forceinline__ void stage32(uint8_t* tile, int row, int c, const uint32_t* v, float factor, bool some) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    uint32_t w[4];
+#pragma unroll
+    for (int h = 0; h < 4; ++h)
+      w[h] = some ? T::pack(__uint_as_float(v[8 * e + 2 * h]) * factor, __uint_as_float(v[8 * e + 2 * h + 1]) * factor) : 0u;
+    const int chunk = (c & 63) / 8 + e;
+    *reinterpret_cast<uint4*>(tile + (c >> 6) * (kTile * 128) + row * 128 + ((chunk ^ (row & 7)) << 4)) =
+        make_uint4(w[0], w[1], w[2], w[3]);
+  }
 }
 
 // Maximum of 128 scores: eight chains, so that no long one holds a row up.
@@ -328,9 +345,6 @@ __global__ void __launch_bounds__(kTileThreads, 2) attention_tiles_kernel(const 
     if (ok) {
       tc_fence_after();
       const float inv = !in || l == 0.f ? 0.f : l > 0.f ? rcp_rn(l) : l;  // a NaN stays one
-      const bool some = list.n > 0 && inv != 0.f;
-      uint8_t* row = q_tile + threadIdx.x * 128;
-      const int swizzle = lane & 7;
 #pragma unroll 1
       for (int c = 0; c < DP; c += 32) {
         uint32_t o[32];
@@ -338,15 +352,7 @@ __global__ void __launch_bounds__(kTileThreads, 2) attention_tiles_kernel(const 
           tmem_load32(o_at + c, o);
           tmem_wait_loads();
         }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          uint32_t w[4];
-#pragma unroll
-          for (int h = 0; h < 4; ++h)
-            w[h] = some ? T::pack(__uint_as_float(o[8 * e + 2 * h]) * inv, __uint_as_float(o[8 * e + 2 * h + 1]) * inv) : 0u;
-          const int chunk = (c & 63) / 8 + e;
-          *reinterpret_cast<uint4*>(row + (c >> 6) * kBox + ((chunk ^ swizzle) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
-        }
+        stage32<T>(q_tile, threadIdx.x, c, o, inv, list.n > 0 && inv != 0.f);
       }
       if (p.lse && i < p.q_len)
         p.lse[((int64_t)b * p.heads + head) * p.q_len + i] =
