@@ -4,6 +4,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+
 #include <cmath>
 #include <cstdint>
 #include <mutex>
@@ -80,14 +81,15 @@ using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, 
                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 EncodeTiled g_encode = nullptr;
 
-// Boxes of 64 dims x 128 tokens of one head, 128-byte swizzle. A dimension of
+// Boxes of 64 dims x 128 (token, head) rows, 128-byte swizzle. A dimension of
 // size 1 may have any stride: it gets a valid one.
-int make_map(CUtensorMap* map, const cs_attention_args* a, const cs_tensor& t, int32_t tokens, int32_t heads) {
+int make_map(CUtensorMap* map, const cs_attention_args* a, const cs_tensor& t, int32_t tokens, int32_t heads,
+             int pack_log2) {
   const cuuint64_t row = (cuuint64_t)a->head_dim * 2;
   const cuuint64_t dims[4] = {(cuuint64_t)a->head_dim, (cuuint64_t)heads, (cuuint64_t)tokens, (cuuint64_t)a->batch};
   const cuuint64_t strides[3] = {heads > 1 ? (cuuint64_t)t.head_stride * 2 : row, tokens > 1 ? (cuuint64_t)t.token_stride * 2 : row,
                                  a->batch > 1 ? (cuuint64_t)t.batch_stride * 2 : row};
-  const cuuint32_t box[4] = {64, 1, cs::kTile, 1}, step[4] = {1, 1, 1, 1};
+  const cuuint32_t box[4] = {64, 1u << pack_log2, (cuuint32_t)cs::kTile >> pack_log2, 1}, step[4] = {1, 1, 1, 1};
   const CUresult r = g_encode(map, a->type == CS_TYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
                               4, t.data, dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
@@ -99,6 +101,12 @@ using TileKernel = void (*)(cs::TileParams);
 TileKernel tile_kernel(int type, int dim) {
   if (type == CS_TYPE_F16) return dim == 64 ? &cs::attention_tiles_kernel<cs::F16, 64> : &cs::attention_tiles_kernel<cs::F16, 128>;
   return dim == 64 ? &cs::attention_tiles_kernel<cs::BF16, 64> : &cs::attention_tiles_kernel<cs::BF16, 128>;
+}
+
+TileKernel tile_join_kernel(int type, int dim) {
+  if (type == CS_TYPE_F16)
+    return dim == 64 ? &cs::attention_tiles_join_kernel<cs::F16, 64> : &cs::attention_tiles_join_kernel<cs::F16, 128>;
+  return dim == 64 ? &cs::attention_tiles_join_kernel<cs::BF16, 64> : &cs::attention_tiles_join_kernel<cs::BF16, 128>;
 }
 
 int tile_smem(int dim) { return dim == 64 ? cs::TileSmem<64>::kBytes : cs::TileSmem<128>::kBytes; }
@@ -159,6 +167,15 @@ int set_up(const cs_host::Device& d, uint32_t** status) {
   return CS_OK;
 }
 
+// Heads of a group in one query tile: the largest power of two that divides the
+// group, up to a tile's rows (its logarithm).
+int pack_of(const cs_attention_args* a) {
+  const int group = a->heads / a->kv_heads;
+  int log2 = 0;
+  while (log2 < 7 && group % (2 << log2) == 0) ++log2;
+  return log2;
+}
+
 int params_of(const cs_attention_args* a, cs::AttentionParams* p, cs_host::Device* d) {
   int rc = cs_host::current_device(d);
   if (!rc) rc = set_up(*d, &p->status);
@@ -180,6 +197,10 @@ int params_of(const cs_attention_args* a, cs::AttentionParams* p, cs_host::Devic
   p->window = a->window;
   p->sinks = a->sinks;
   p->scale = a->scale;
+  p->pack_log2 = pack_of(a);
+  p->by_heads = cs::Divider::of((uint32_t)(a->batch * a->kv_heads));
+  p->by_kv_heads = cs::Divider::of((uint32_t)a->kv_heads);
+  p->by_packs = cs::Divider::of((uint32_t)(p->group >> p->pack_log2));
   return CS_OK;
 }
 
@@ -198,11 +219,11 @@ struct TokenShape {
   int64_t part_bytes, stats_bytes;
 };
 
-constexpr int kTokenQueries = 16;     // longest q_len that takes it
-constexpr int kTokenCtasPerSm = 12;   // about four rounds of resident CTAs, for an even end
-constexpr int kTokenKeysPerCta = 256; // at least: 4 steps a warp
+constexpr int kTokenRows = 16;         // most rows of a kv head, (query, head) pairs, that take it
+constexpr int64_t kTokenKeys = 128;    // of a CTA, at least: 2 steps a warp
+constexpr int kTokenResident[2][2] = {{4, 3}, {3, 2}};  // CTAs an SM: dim 64, 128; 8, 16 rows
 
-bool few_queries(const cs_attention_args* a) { return a->q_len <= kTokenQueries; }
+bool few_queries(const cs_attention_args* a) { return (int64_t)a->q_len * (a->heads / a->kv_heads) <= kTokenRows; }
 
 TokenShape token_shape(const cs_attention_args* a, int sms) {
   TokenShape s{};
@@ -213,8 +234,12 @@ TokenShape token_shape(const cs_attention_args* a, int sms) {
   const int64_t base = (int64_t)a->batch * a->kv_heads * s.blocks;
   int64_t keys = a->kv_len;
   if (a->window) keys = std::min<int64_t>(keys, (int64_t)a->window + a->q_len + a->sinks + 32);
-  const int64_t want = ((int64_t)sms * kTokenCtasPerSm + base - 1) / base;
-  s.splits = (int)std::max<int64_t>(1, std::min(want, keys / kTokenKeysPerCta));
+  // Four rounds of resident CTAs or more for an even end, else one.
+  const int64_t wave = (int64_t)sms * kTokenResident[s.dim == 128][s.rows == 16];
+  const int64_t most = std::min<int64_t>(keys / kTokenKeys, cs::kMaxSplits);
+  int64_t splits = (4 * wave + base - 1) / base;
+  if (splits > most) splits = std::min(most, wave / base);
+  s.splits = (int)std::max<int64_t>(1, splits);
   s.ctas = base * s.splits;
   if (s.splits > 1) {
     s.part_bytes = s.ctas * s.rows * s.dim * 4;
@@ -246,38 +271,75 @@ int launch_tokens(const cs_attention_args* a, const cs::AttentionParams& p, cons
                                   dim3((unsigned)s.ctas), cs::kTokenWarps * 32, 0, stream, t);
   if (e != cudaSuccess) return fail_cuda(e, "attention, few queries");
   if (s.splits == 1) return CS_OK;
-  e = cs_host::launch(half ? &cs::attention_join_kernel<cs::F16> : &cs::attention_join_kernel<cs::BF16>,
-                      dim3((unsigned)(s.ctas / s.splits * s.rows)), 128, 0, stream, t);
+  const dim3 rows((unsigned)((int64_t)a->batch * a->heads * a->q_len));
+  if (s.splits > 16)
+    e = cs_host::launch(half ? &cs::attention_join_kernel<cs::F16, 16> : &cs::attention_join_kernel<cs::BF16, 16>, rows, 512, 0, stream, t);
+  else
+    e = cs_host::launch(half ? &cs::attention_join_kernel<cs::F16, 4> : &cs::attention_join_kernel<cs::BF16, 4>, rows, 128, 0, stream, t);
   return e == cudaSuccess ? CS_OK : fail_cuda(e, "attention, joining the splits");
 }
 
-int launch_tiles(const cs_attention_args* a, const cs::AttentionParams& p, void* stream) {
+// Query tiles and, where they are too few for two CTAs an SM, the CTAs that share
+// one's keys: at least kTileKeys key tiles each, and only from four times as many
+// on (joining takes about 3 us, a key tile 1.5).
+struct TileShape {
+  int dim, q_tiles, splits;
+  int64_t ctas, part_bytes, stats_bytes;
+};
+
+constexpr int64_t kTileKeys = 4;
+
+TileShape tile_shape(const cs_attention_args* a, int sms) {
+  TileShape s{};
+  s.dim = a->head_dim <= 64 ? 64 : 128;
+  const int pack = pack_of(a), tokens = cs::kTile >> pack;
+  s.q_tiles = (a->q_len + tokens - 1) / tokens;
+  const int64_t base = (int64_t)a->batch * (a->heads >> pack) * s.q_tiles;
+  int64_t keys = ((int64_t)a->kv_len + cs::kTile - 1) / cs::kTile;
+  if (a->window)
+    keys = std::min(keys, ((int64_t)a->window + tokens + cs::kTile - 1) / cs::kTile + ((int64_t)a->sinks + cs::kTile - 1) / cs::kTile);
+  s.splits = keys < 4 * kTileKeys ? 1 : (int)std::max<int64_t>(1, std::min(2 * (int64_t)sms / base, keys / kTileKeys));
+  s.ctas = base * s.splits;
+  if (s.splits > 1) {
+    s.part_bytes = s.ctas * cs::kTile * s.dim * 4;
+    s.stats_bytes = s.ctas * cs::kTile * 8;
+  }
+  return s;
+}
+
+int launch_tiles(const cs_attention_args* a, const cs::AttentionParams& p, const TileShape& s, void* workspace, void* stream) {
   cs::TileParams t{};
   t.a = p;
-  int rc = make_map(&t.q, a, a->q, a->q_len, a->heads);
-  if (!rc) rc = make_map(&t.k, a, a->k, a->kv_len, a->kv_heads);
-  if (!rc) rc = make_map(&t.v, a, a->v, a->kv_len, a->kv_heads);
-  if (!rc) rc = make_map(&t.o, a, a->o, a->q_len, a->heads);
+  t.q_tiles = s.q_tiles;
+  t.splits = s.splits;
+  t.part_o = static_cast<float*>(workspace);
+  t.part_stats = reinterpret_cast<float*>(static_cast<char*>(workspace) + s.part_bytes);
+  int rc = make_map(&t.q, a, a->q, a->q_len, a->heads, p.pack_log2);
+  if (!rc) rc = make_map(&t.k, a, a->k, a->kv_len, a->kv_heads, 0);
+  if (!rc) rc = make_map(&t.v, a, a->v, a->kv_len, a->kv_heads, 0);
+  if (!rc) rc = make_map(&t.o, a, a->o, a->q_len, a->heads, p.pack_log2);
   if (rc) return rc;
-  t.q_tiles = (a->q_len + cs::kTile - 1) / cs::kTile;
-  const int64_t ctas = (int64_t)a->batch * a->heads * t.q_tiles;
-  if (ctas > kI32Max) return fail(CS_ERR_WRONG_LENGTH, "%lld CTAs", (long long)ctas);
-  const int dim = a->head_dim <= 64 ? 64 : 128;
-  const cudaError_t e = cs_host::launch(tile_kernel(a->type, dim), dim3((unsigned)ctas), cs::kTileThreads,
-                                        (size_t)tile_smem(dim), stream, t);
-  return e == cudaSuccess ? CS_OK : fail_cuda(e, "attention, tiles");
+  if (s.ctas > kI32Max) return fail(CS_ERR_WRONG_LENGTH, "%lld CTAs", (long long)s.ctas);
+  cudaError_t e = cs_host::launch(tile_kernel(a->type, s.dim), dim3((unsigned)s.ctas), cs::kTileThreads, (size_t)tile_smem(s.dim),
+                                  stream, t);
+  if (e != cudaSuccess) return fail_cuda(e, "attention, tiles");
+  if (s.splits == 1) return CS_OK;
+  e = cs_host::launch(tile_join_kernel(a->type, s.dim), dim3((unsigned)(s.ctas / s.splits), (unsigned)s.dim / 8), 256, 0,
+                      stream, t);
+  return e == cudaSuccess ? CS_OK : fail_cuda(e, "attention, joining the splits");
 }
 
 // The backward's launch shapes and workspace.
 struct GradShape {
-  int dim, q_pad, q_tiles, k_tiles;
+  int dim, q_tiles, k_tiles;
+  int64_t q_pad;  // rows of a pack of heads
   int share, window_shares, sink_tiles, sink_shares;
   int64_t dkv_ctas;
   int64_t rows_bytes, norms_bytes, partial_bytes;  // two arrays of rows
   int64_t bytes() const { return 2 * rows_bytes + norms_bytes + partial_bytes; }
 };
 
-// A key tile's work is its (head, tile of queries) units. Tiles are cut into shares
+// A key tile's work is its units, the query tiles that see it. Tiles are cut into shares
 // only where that evens out the SMs: the sinks' tile, which every query sees,
 // and tiles of long rows when there are few of them; each share costs a part of
 // dK and dV in fp32, written and read once more. So: about two shares an SM,
@@ -285,14 +347,15 @@ struct GradShape {
 GradShape grad_shape(const cs_attention_args* a, int sms) {
   GradShape s{};
   s.dim = a->head_dim <= 64 ? 64 : 128;
-  s.q_tiles = (a->q_len + cs::kTile - 1) / cs::kTile;
-  s.q_pad = s.q_tiles * cs::kTile;
+  const int pack = pack_of(a), tokens = cs::kTile >> pack;
+  s.q_tiles = (a->q_len + tokens - 1) / tokens;
+  s.q_pad = (int64_t)s.q_tiles * cs::kTile;
   s.k_tiles = (a->kv_len + cs::kTile - 1) / cs::kTile;
-  const int64_t group = a->heads / a->kv_heads, heads = (int64_t)a->batch * a->kv_heads;
-  const int64_t all = s.q_tiles * group;  // units of a tile that every query sees
+  const int64_t packs = (a->heads / a->kv_heads) >> pack, heads = (int64_t)a->batch * a->kv_heads;
+  const int64_t all = s.q_tiles * packs;  // units of a tile that every query sees
   int64_t usual = all;
   if (a->window) {
-    usual = std::min(all, (((int64_t)a->window + 2 * cs::kTile - 2) / cs::kTile + 1) * group);
+    usual = std::min(all, (((int64_t)a->window + cs::kTile + tokens - 2) / tokens + 1) * packs);
     s.sink_tiles = (int)std::min<int64_t>(s.k_tiles, ((int64_t)a->sinks + cs::kTile - 1) / cs::kTile);
   }
   // Without a window tiles see half of the queries on average.
@@ -303,16 +366,20 @@ GradShape grad_shape(const cs_attention_args* a, int sms) {
   s.window_shares = (int)((usual + s.share - 1) / s.share);
   s.sink_shares = (int)((all + s.share - 1) / s.share);
   s.dkv_ctas = heads * ((int64_t)s.sink_tiles * s.sink_shares + (int64_t)(s.k_tiles - s.sink_tiles) * s.window_shares);
-  s.rows_bytes = (int64_t)a->batch * a->heads * s.q_pad * 4;
+  s.rows_bytes = (int64_t)a->batch * (a->heads >> pack) * s.q_pad * 4;
   s.norms_bytes = a->type == CS_TYPE_F16 ? (2 * heads * 4 + 15) / 16 * 16 : 0;
   if (s.window_shares > 1 || (s.sink_tiles && s.sink_shares > 1)) s.partial_bytes = s.dkv_ctas * 2 * cs::kTile * s.dim * 4;
   return s;
 }
 
+int check_shape(const cs_attention_args* a, const GradShape& s) {
+  if (s.q_pad > kI32Max || s.dkv_ctas > kI32Max || (int64_t)a->batch * a->heads * s.q_tiles > kI32Max)
+    return fail(CS_ERR_WRONG_LENGTH, "backward of q_len %d, kv_len %d: too many tiles", a->q_len, a->kv_len);
+  return CS_OK;
+}
+
 int launch_backward(const cs_attention_args* a, const cs_attention_grads* g, const cs::AttentionParams& p, const GradShape& s,
                     void* workspace, void* stream) {
-  if (s.dkv_ctas > kI32Max || (int64_t)a->batch * a->heads * s.q_tiles > kI32Max)
-    return fail(CS_ERR_WRONG_LENGTH, "%lld CTAs", (long long)s.dkv_ctas);
   char* at = static_cast<char*>(workspace);
   float* lse2 = reinterpret_cast<float*>(at);
   float* delta = reinterpret_cast<float*>(at + s.rows_bytes);
@@ -324,11 +391,11 @@ int launch_backward(const cs_attention_args* a, const cs_attention_grads* g, con
   r.lse2 = lse2;
   r.delta = delta;
   r.norms = reinterpret_cast<uint32_t*>(norms);
-  r.q_pad = s.q_pad;
+  r.q_pad = (int32_t)s.q_pad;
   cudaError_t e = cudaSuccess;
   if (half) e = cudaMemsetAsync(norms, 0, (size_t)s.norms_bytes, static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return fail_cuda(e, "attention backward, norms");
-  const unsigned rows = (unsigned)(s.q_pad / 16 + (half ? (a->kv_len + 15) / 16 : 0));
+  const unsigned rows = (unsigned)(((s.q_pad >> p.pack_log2) + 15) / 16 + (half ? (a->kv_len + 15) / 16 : 0));
   e = cs_host::launch(half ? &cs::attention_rows_kernel<cs::F16> : &cs::attention_rows_kernel<cs::BF16>,
                       dim3(rows, (unsigned)std::min(a->batch * a->heads, 65535)), 256, 0, stream, r);
   if (e != cudaSuccess) return fail_cuda(e, "attention backward, rows");
@@ -339,27 +406,27 @@ int launch_backward(const cs_attention_args* a, const cs_attention_grads* g, con
   k.delta = delta;
   k.norms = norms;
   k.partial = reinterpret_cast<float*>(at + 2 * s.rows_bytes + s.norms_bytes);
-  k.q_pad = s.q_pad;
+  k.q_pad = (int32_t)s.q_pad;
   k.share = s.share;
   k.window_shares = s.window_shares;
   k.sink_tiles = s.sink_tiles;
   k.sink_shares = s.sink_shares;
   k.tiles = s.k_tiles;
-  int rc = make_map(&k.q, a, a->q, a->q_len, a->heads);
-  if (!rc) rc = make_map(&k.d_o, a, g->d_o, a->q_len, a->heads);
-  if (!rc) rc = make_map(&k.k, a, a->k, a->kv_len, a->kv_heads);
-  if (!rc) rc = make_map(&k.v, a, a->v, a->kv_len, a->kv_heads);
-  if (!rc) rc = make_map(&k.out0, a, g->dk, a->kv_len, a->kv_heads);
-  if (!rc) rc = make_map(&k.out1, a, g->dv, a->kv_len, a->kv_heads);
+  int rc = make_map(&k.q, a, a->q, a->q_len, a->heads, p.pack_log2);
+  if (!rc) rc = make_map(&k.d_o, a, g->d_o, a->q_len, a->heads, p.pack_log2);
+  if (!rc) rc = make_map(&k.k, a, a->k, a->kv_len, a->kv_heads, 0);
+  if (!rc) rc = make_map(&k.v, a, a->v, a->kv_len, a->kv_heads, 0);
+  if (!rc) rc = make_map(&k.out0, a, g->dk, a->kv_len, a->kv_heads, 0);
+  if (!rc) rc = make_map(&k.out1, a, g->dv, a->kv_len, a->kv_heads, 0);
   if (rc) return rc;
   e = cs_host::launch(dkv_kernel(a->type, s.dim), dim3((unsigned)s.dkv_ctas), cs::kGradThreads, (size_t)dkv_smem(s.dim), stream, k);
   if (e != cudaSuccess) return fail_cuda(e, "attention backward, keys");
 
   cs::GradParams q = k;
   q.tiles = s.q_tiles;
-  rc = make_map(&q.out0, a, g->dq, a->q_len, a->heads);
+  rc = make_map(&q.out0, a, g->dq, a->q_len, a->heads, p.pack_log2);
   if (rc) return rc;
-  e = cs_host::launch(dq_kernel(a->type, s.dim), dim3((unsigned)(a->batch * a->heads * s.q_tiles)), cs::kGradThreads,
+  e = cs_host::launch(dq_kernel(a->type, s.dim), dim3((unsigned)(a->batch * (a->heads >> p.pack_log2) * s.q_tiles)), cs::kGradThreads,
                       (size_t)dq_smem(s.dim), stream, q);
   if (e != cudaSuccess) return fail_cuda(e, "attention backward, queries");
   if (s.partial_bytes) {
@@ -375,11 +442,14 @@ extern "C" {
 
 int64_t cs_attention_workspace(const cs_attention_args* args) {
   int rc = check_args(args);
-  if (rc || !few_queries(args)) return rc;
   cs_host::Device d;
-  rc = cs_host::current_device(&d);
+  if (!rc) rc = cs_host::current_device(&d);
   if (rc) return rc;
-  const TokenShape s = token_shape(args, d.sms);
+  if (few_queries(args)) {
+    const TokenShape s = token_shape(args, d.sms);
+    return s.part_bytes + s.stats_bytes;
+  }
+  const TileShape s = tile_shape(args, d.sms);
   return s.part_bytes + s.stats_bytes;
 }
 
@@ -395,14 +465,19 @@ int cs_attention(const cs_attention_args* args, void* workspace, size_t workspac
     rc = check_workspace(workspace, workspace_bytes, s.part_bytes + s.stats_bytes);
     return rc ? rc : launch_tokens(args, p, s, workspace, stream);
   }
-  return launch_tiles(args, p, stream);
+  const TileShape s = tile_shape(args, d.sms);
+  rc = check_workspace(workspace, workspace_bytes, s.part_bytes + s.stats_bytes);
+  return rc ? rc : launch_tiles(args, p, s, workspace, stream);
 }
 
 int64_t cs_attention_backward_workspace(const cs_attention_args* args) {
   int rc = check_args(args);
   cs_host::Device d;
   if (!rc) rc = cs_host::current_device(&d);
-  return rc ? rc : grad_shape(args, d.sms).bytes();
+  if (rc) return rc;
+  const GradShape s = grad_shape(args, d.sms);
+  rc = check_shape(args, s);
+  return rc ? rc : s.bytes();
 }
 
 int cs_attention_backward(const cs_attention_args* args, const cs_attention_grads* grads, void* workspace,
@@ -416,7 +491,8 @@ int cs_attention_backward(const cs_attention_args* args, const cs_attention_grad
   rc = params_of(args, &p, &d);
   if (rc) return rc;
   const GradShape s = grad_shape(args, d.sms);
-  rc = check_workspace(workspace, workspace_bytes, s.bytes());
+  rc = check_shape(args, s);
+  if (!rc) rc = check_workspace(workspace, workspace_bytes, s.bytes());
   if (rc) return rc;
   p.d_o = strided(grads->d_o);
   p.dq = strided(grads->dq);

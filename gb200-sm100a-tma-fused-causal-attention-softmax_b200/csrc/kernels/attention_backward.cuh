@@ -37,7 +37,7 @@ struct GradParams {
   CUtensorMap q, k, v, d_o;
   CUtensorMap out0, out1;    // dq; or dk, dv
   AttentionParams a;
-  const float* lse2;   // [batch * heads, q_pad]: minus lse in units of log2; -infinity for rows without keys
+  const float* lse2;   // [pack of heads, q_pad rows]: minus lse in units of log2; -infinity for rows without keys
   const float* delta;  // the same: minus the sum of d_o * o
   const float* norms;  // fp16: [2, batch * kv_heads], largest |d_o| and |v| of a row
   float* partial;      // dK, dV parts of key tiles cut into several CTAs' shares
@@ -62,14 +62,14 @@ __device__ __forceinline__ void raise_max(uint32_t* at, float v) {
   if ((threadIdx.x & 31) == 0 && m > 0.f) atomicMax(at, __float_as_uint(m));
 }
 
-// 16 lanes a row. grid.x covers q_pad rows of a head, then (fp16) the rows of a
-// kv head; grid.y = batch * heads.
+// 16 lanes a row. grid.x covers a head's tokens up to the end of its last tile,
+// then (fp16) the keys of a kv head; grid.y = batch * heads.
 template <typename T>
 __global__ void __launch_bounds__(256) attention_rows_kernel(const __grid_constant__ RowsParams rp) {
   const AttentionParams& p = rp.a;
   pdl_wait();
   const int lane = threadIdx.x & 15, d = lane * 8, per_cta = 16;
-  const int q_ctas = (rp.q_pad + per_cta - 1) / per_cta;
+  const int tokens = rp.q_pad >> p.pack_log2, q_ctas = (tokens + per_cta - 1) / per_cta;
   for (int bh = blockIdx.y; bh < p.batch * p.heads; bh += gridDim.y) {
     const int b = bh / p.heads, h = bh - b * p.heads, hk = h / p.group;
     const Lengths len(p, b);
@@ -92,10 +92,11 @@ __global__ void __launch_bounds__(256) attention_rows_kernel(const __grid_consta
         dot += __shfl_xor_sync(0xffffffffu, dot, x);
         norm += __shfl_xor_sync(0xffffffffu, norm, x);
       }
-      if (lane == 0 && i < rp.q_pad) {
+      if (lane == 0 && i < tokens) {
+        const int64_t row = (int64_t)(bh >> p.pack_log2) * rp.q_pad + (i << p.pack_log2) + (h & ((1 << p.pack_log2) - 1));
         const float lse = in ? p.lse[(int64_t)bh * p.q_len + i] : -INFINITY;
-        rp.lse2[(int64_t)bh * rp.q_pad + i] = lse == -INFINITY ? -INFINITY : -lse * kLog2e;
-        rp.delta[(int64_t)bh * rp.q_pad + i] = in ? -dot : 0.f;
+        rp.lse2[row] = lse == -INFINITY ? -INFINITY : -lse * kLog2e;
+        rp.delta[row] = in ? -dot : 0.f;
       }
       if (T::kIsHalf) raise_max(rp.norms + b * p.kv_heads + hk, norm);
     } else if (T::kIsHalf && h % p.group == 0) {
@@ -163,7 +164,7 @@ __device__ __forceinline__ void p_to_ds(const float* p, const uint32_t* dp, bool
   }
 }
 
-constexpr int kGradThreads = 384;  // registers: 384 x 168 = 256 x 192 + 128 x 120 (dQ) = 256 x 232 + 128 x 40 (dK, dV)
+constexpr int kGradThreads = 384;  // registers: 384 x 168 = 256 x 192 + 128 x 120 (dQ) = 256 x 224 + 128 x 56 (dK, dV)
 
 // ---- dQ
 
@@ -228,11 +229,10 @@ __global__ void __launch_bounds__(kGradThreads, 1) attention_dq_kernel(const __g
   // Only the rows kernel's results are needed, and it was done before the dK/dV
   // kernel let this one start; the wait for that one is at the end.
 
-  const int bk = blockIdx.x % (p.batch * p.kv_heads), unit = blockIdx.x / (p.batch * p.kv_heads);
-  const int b = bk / p.kv_heads, hk = bk - b * p.kv_heads;
-  const int head = hk * p.group + unit % p.group, first = (gp.tiles - 1 - unit / p.group) * kTile;
+  const int unit = p.by_heads.div(blockIdx.x), bk = blockIdx.x - unit * p.by_heads.by, b = p.by_kv_heads.div(bk), hk = bk - b * p.kv_heads;
+  const QueryTile tile(p, hk, unit, gp.tiles);
   const Lengths len(p, b);
-  const TileKeys keys(p, len, first);
+  const TileKeys keys(p, len, tile.first);
   const TileList list(keys);
   const Waiter wait{&bars.gone, p.status, kWaitNs};
 
@@ -243,8 +243,8 @@ __global__ void __launch_bounds__(kGradThreads, 1) attention_dq_kernel(const __g
         mbar_arrive_expect_tx(&bars.q_full, 2 * kTileBytes);
 #pragma unroll
         for (int box = 0; box < DP / 64; ++box) {
-          tma_load(q_tile + box * kBox, &gp.q, box * 64, head, first, b, &bars.q_full);
-          tma_load(do_tile + box * kBox, &gp.d_o, box * 64, head, first, b, &bars.q_full);
+          tma_load(q_tile + box * kBox, &gp.q, box * 64, tile.head, tile.first, b, &bars.q_full);
+          tma_load(do_tile + box * kBox, &gp.d_o, box * 64, tile.head, tile.first, b, &bars.q_full);
         }
         RingPos ring;
         auto load_key = [&](int j) {
@@ -308,11 +308,11 @@ __global__ void __launch_bounds__(kGradThreads, 1) attention_dq_kernel(const __g
     }
   } else {
     registers_up<192>();
-    const int group = warp >> 2, in_tile = threadIdx.x & 127, i = first + in_tile;  // this thread's query
+    const int group = warp >> 2, in_tile = threadIdx.x & 127, i = tile.token(in_tile);  // this thread's query
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, columns = group * 64;  // and its warpgroup's columns
     const Visible see = visible_keys(i < len.q ? len.position(i) : -1, len.kv, p.window, p.sinks);
     const float sl = fmaxf(p.scale * kLog2e, 1.1754944e-38f);
-    const int64_t row = ((int64_t)b * p.heads + head) * gp.q_pad + i;
+    const int64_t row = (int64_t)((b * p.heads + tile.head) >> p.pack_log2) * gp.q_pad + (tile.first << p.pack_log2) + in_tile;
     const float c = ds_factor<T>(gp, bk);
     const F2 minus_lse = f2(gp.lse2[row], gp.lse2[row]), minus_delta = f2(gp.delta[row], gp.delta[row]);
     bool ok = true;
@@ -368,7 +368,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) attention_dq_kernel(const __g
     if (threadIdx.x == 0 && !*(volatile uint32_t*)&bars.gone) {
 #pragma unroll
       for (int box = 0; box < DP / 64; ++box)
-        if (box * 64 < p.head_dim) tma_store(&gp.out0, q_tile + box * kBox, box * 64, head, first, b);
+        if (box * 64 < p.head_dim) tma_store(&gp.out0, q_tile + box * kBox, box * 64, tile.head, tile.first, b);
       bulk_commit();
       bulk_wait_all();
     }
@@ -393,12 +393,14 @@ struct KeySmem {
   static constexpr int kBytes = (2 + kQueries) * kTileBytes + kGrads * kGrad + 256;
 };
 
-// The (head, tile of queries) units that see a tile of keys, heads first.
+// The query tiles (units) that see a tile of keys: of one pack of heads after
+// the other, `per_pack` each, from token q_first on.
 struct KeyUnits {
-  int32_t q_first, per_head, n;  // q_first: of a head's first unit
-  int32_t every_lo, every_hi;    // queries [every_lo, every_hi) see all 128 keys
+  int32_t q_first, per_pack, n, step;  // step: tokens of a query tile
+  int32_t every_lo, every_hi;          // tokens [every_lo, every_hi) see all 128 keys
   __device__ __forceinline__ KeyUnits(const AttentionParams& p, const Lengths& len, int k0) {
-    q_first = per_head = n = every_lo = every_hi = 0;
+    step = kTile >> p.pack_log2;
+    q_first = per_pack = n = every_lo = every_hi = 0;
     if (k0 >= len.kv || len.q <= 0) return;
     const int64_t pos0 = len.position(0), k1 = min(k0 + kTile, len.kv) - 1;
     const int64_t lo = max((int64_t)0, k0 - pos0);
@@ -408,13 +410,16 @@ struct KeyUnits {
       if (k0 + kTile > p.sinks) all = min(all, max((int64_t)k0, (int64_t)p.sinks) + p.window - pos0);
     }
     if (lo >= hi) return;
-    q_first = (int)(lo / kTile) * kTile;
-    per_head = (int)((hi + kTile - 1) / kTile - lo / kTile);
-    n = per_head * p.group;
+    q_first = (int)lo / step * step;
+    per_pack = ((int)hi + step - 1) / step - (int)lo / step;
+    n = per_pack * (p.group >> p.pack_log2);
     every_lo = (int)max((int64_t)0, k0 + kTile - 1 - pos0);
     every_hi = k0 + kTile <= len.kv ? (int)max(all, (int64_t)0) : 0;
   }
 };
+
+// Columns of a query tile, first token i0, that token t is at or behind.
+__device__ __forceinline__ int column_of(int t, int i0, int pack_log2) { return min(max(t - i0, 0), kTile) << pack_log2; }
 
 // Queries [lo, hi) of a sequence see key k.
 __device__ __forceinline__ void queries_of(const AttentionParams& p, const Lengths& len, int k, int& lo, int& hi) {
@@ -497,7 +502,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) attention_dkv_kernel(const __
 
   if (n > 0 || share == 0) {
     if (warp >= 8) {
-      registers_down<40>();
+      registers_down<56>();
       if (warp == 8) {
         if (lane == 0 && n > 0) {
           mbar_arrive_expect_tx(&bars.kv_full, 2 * kTileBytes);
@@ -508,7 +513,8 @@ __global__ void __launch_bounds__(kGradThreads, 1) attention_dkv_kernel(const __
           }
           RingPos q_at, o_at;
           auto load_query = [&](int u) {
-            const int h = u / units.per_head, i0 = units.q_first + (u - h * units.per_head) * kTile, head = hk * p.group + h;
+            const int pack = u / units.per_pack, i0 = units.q_first + (u - pack * units.per_pack) * units.step;
+            const int head = hk * p.group + (pack << p.pack_log2);
             if (!wait(&bars.q_empty[q_at.s], q_at.ph ^ 1)) return false;
             mbar_arrive_expect_tx(&bars.q_full[q_at.s], kTileBytes);
 #pragma unroll
@@ -518,14 +524,15 @@ __global__ void __launch_bounds__(kGradThreads, 1) attention_dkv_kernel(const __
             return true;
           };
           auto load_grad = [&](int u) {
-            const int h = u / units.per_head, i0 = units.q_first + (u - h * units.per_head) * kTile, head = hk * p.group + h;
+            const int pack = u / units.per_pack, i0 = units.q_first + (u - pack * units.per_pack) * units.step;
+            const int head = hk * p.group + (pack << p.pack_log2);
             if (!wait(&bars.o_empty[o_at.s], o_at.ph ^ 1)) return false;
             uint8_t* to = grads + o_at.s * kGrad;
             mbar_arrive_expect_tx(&bars.o_full[o_at.s], kGrad);
 #pragma unroll
             for (int box = 0; box < DP / 64; ++box)
               tma_load(to + box * kBox, &gp.d_o, box * 64, head, i0, b, &bars.o_full[o_at.s]);
-            const int64_t row = ((int64_t)b * p.heads + head) * gp.q_pad + i0;
+            const int64_t row = (int64_t)((b * p.heads + head) >> p.pack_log2) * gp.q_pad + (i0 << p.pack_log2);
             bulk_g2s(to + kTileBytes, gp.lse2 + row, 512, &bars.o_full[o_at.s]);
             bulk_g2s(to + kTileBytes + 512, gp.delta + row, 512, &bars.o_full[o_at.s]);
             o_at.next(kGrads);
@@ -544,12 +551,16 @@ __global__ void __launch_bounds__(kGradThreads, 1) attention_dkv_kernel(const __
         auto warp_wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)) != 0; };
         const int q_lo = max(0, -len.position(0));  // queries before it are at negative positions
         RingPos q_next, q_used, o_next, o_used;  // of S and of dK; of dP and of dV
-        int q_sub = u0 % units.per_head, o_sub = q_sub;
+        int q_sub = u0 % units.per_pack, o_sub = q_sub;
         // Zero the rows of a tile that are no queries of the sequence.
         auto clean = [&](uint8_t* tile, int& sub) {
-          const int i0 = units.q_first + sub * kTile;
-          if (++sub == units.per_head) sub = 0;
-          if (i0 < q_lo || i0 + kTile > len.q) clear_rows<DP>(tile, lane, [&](int r) { return i0 + r >= q_lo && i0 + r < len.q; });
+          const int i0 = units.q_first + sub * units.step;
+          if (++sub == units.per_pack) sub = 0;
+          if (i0 < q_lo || i0 + units.step > len.q)
+            clear_rows<DP>(tile, lane, [&](int r) {
+              const int i = i0 + (r >> p.pack_log2);
+              return i >= q_lo && i < len.q;
+            });
         };
         auto scores = [&](int u) {  // S(u)
           uint8_t* q_tile = q_tiles + q_next.s * kTileBytes;
@@ -591,7 +602,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) attention_dkv_kernel(const __
         }
       }
     } else {
-      registers_up<232>();
+      registers_up<224>();
       const int group = warp >> 2, row = threadIdx.x & 127;  // this thread's key
       const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
       const int columns = group * 64;  // this warpgroup's queries of a tile
@@ -600,26 +611,28 @@ __global__ void __launch_bounds__(kGradThreads, 1) attention_dkv_kernel(const __
       int q_lo, q_hi;
       queries_of(p, len, k0 + row, q_lo, q_hi);
       bool ok = true;
-      int sub = n > 0 ? u0 % units.per_head : 0;
-      RingPos ring;
-      for (int u = 0; u < n; ++u, ring.next(kGrads)) {
-        const int i0 = units.q_first + sub * kTile, first = i0 + columns;
-        if (++sub == units.per_head) sub = 0;
-        const float* rows = reinterpret_cast<const float*>(grads + ring.s * kGrad + kTileBytes) + columns;
-        const bool every = i0 >= units.every_lo && i0 + kTile <= units.every_hi;
-        const uint32_t bits0 = every ? 0u : below_bits(q_hi - first) & ~below_bits(q_lo - first);
-        const uint32_t bits1 = every ? 0u : below_bits(q_hi - first - 32) & ~below_bits(q_lo - first - 32);
+      static_assert(kGrads == 2, "a unit's d_o stage is u & 1");
+      const int i_end = units.q_first + units.per_pack * units.step;
+      int i0 = n > 0 ? units.q_first + u0 % units.per_pack * units.step : 0;
+      for (int u = 0; u < n; ++u, i0 = i0 + units.step == i_end ? units.q_first : i0 + units.step) {
+        const float* rows = reinterpret_cast<const float*>(grads + (u & 1) * kGrad + kTileBytes) + columns;
+        const bool every = i0 >= units.every_lo && i0 + units.step <= units.every_hi;
+        const int c_lo = column_of(q_lo, i0, p.pack_log2) - columns, c_hi = column_of(q_hi, i0, p.pack_log2) - columns;
+        uint32_t bits0 = 0, bits1 = 0;
+        if (!every) {
+          bits0 = below_bits(c_hi) & ~below_bits(c_lo);
+          bits1 = below_bits(c_hi - 32) & ~below_bits(c_lo - 32);
+        }
         float4 quad;
         auto pair = [&](int e) {  // two queries' numbers, read four at a time
           if (!(e & 2)) quad = *reinterpret_cast<const float4*>(rows + e);
           return e & 2 ? f2(quad.z, quad.w) : f2(quad.x, quad.y);
         };
-        ok = __all_sync(0xffffffffu, wait(&bars.o_full[ring.s], ring.ph) && wait(&bars.s_full[u & 1], (u >> 1) & 1));
+        ok = __all_sync(0xffffffffu, wait(&bars.o_full[u & 1], (u >> 1) & 1) && wait(&bars.s_full[u & 1], (u >> 1) & 1));
         if (!ok) break;
         tc_fence_after();
         const uint32_t at = tmem + lanes + (u & 1) * 128 + columns;
         float pr[64];
-        uint32_t out[32];
         {
           uint32_t s[64];
           tmem_load32(at, s);
@@ -633,17 +646,22 @@ __global__ void __launch_bounds__(kGradThreads, 1) attention_dkv_kernel(const __
         ok = __all_sync(0xffffffffu, wait(&bars.dp_full, u & 1));
         if (!ok) break;
         tc_fence_after();
-        uint32_t dp[32], ds[32];
+        // P goes over the first half of this warpgroup's dP columns, dS over the second.
+        uint32_t dp[32], ds[16], out[16];
+        tmem_load32(at, dp);
+        tmem_wait_loads();
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          tmem_load32(at + h * 32, dp);
-          tmem_wait_loads();
-          p_to_ds<T>(pr + h * 32, dp, every, h ? bits1 : bits0, k1, [&](int e) { return pair(128 + h * 32 + e); }, ds + h * 16);
 #pragma unroll
-          for (int e = 0; e < 16; ++e) out[h * 16 + e] = T::pack(pr[h * 32 + 2 * e], pr[h * 32 + 2 * e + 1]);
+          for (int e = 0; e < 16; ++e) out[e] = T::pack(pr[h * 32 + 2 * e], pr[h * 32 + 2 * e + 1]);
+          tmem_store16(at + h * 16, out);
         }
-        tmem_store32(at, out);  // over this warpgroup's own columns: P, then dS
-        tmem_store32(at + 32, ds);
+        p_to_ds<T>(pr, dp, every, bits0, k1, [&](int e) { return pair(128 + e); }, ds);
+        tmem_load32(at + 32, dp);
+        tmem_wait_loads();
+        tmem_store16(at + 32, ds);
+        p_to_ds<T>(pr + 32, dp, every, bits1, k1, [&](int e) { return pair(160 + e); }, out);
+        tmem_store16(at + 48, out);
         tmem_wait_stores();
         tc_fence_before();
         __syncwarp();

@@ -1,8 +1,12 @@
 // Attention of many queries: tiles of 128 queries x 128 keys on the
 // 5th-generation tensor core.
 //
-// A CTA owns one tile of queries of one head and streams key and value tiles
-// through a ring of shared-memory stages; two CTAs share an SM.
+// A tile's 128 rows are (token, head) pairs: 128 / pack tokens of `pack` heads
+// that read the same keys, the largest power of two in the group. Few tokens
+// fill a tile that way, and the keys of a window that only some rows see are
+// fewer. A CTA owns one such tile and streams key and value tiles through a ring
+// of shared-memory stages; two CTAs share an SM. Where tiles are few and their
+// keys many, several CTAs share a tile's keys and a second kernel joins them.
 //
 //   warps 0-3: softmax, one thread per query; they hold a row of 128 scores
 //   warp 4:    TMA loads     warp 5: products (one thread)     6, 7: no work
@@ -42,7 +46,23 @@ constexpr int kTile = 128;
 struct TileParams {
   CUtensorMap q, k, v, o;
   AttentionParams a;
-  int32_t q_tiles;  // per head
+  int32_t q_tiles;      // per pack of heads
+  int32_t splits;       // CTAs per query tile
+  float* part_o;        // splits > 1: [CTA, DP / 4, 128 rows, 4]
+  float* part_stats;    // [CTA, 128 rows, 2]: maximum (log2 units), sum
+};
+
+// A tile of queries: its first token and head.
+struct QueryTile {
+  int32_t first, head, pack_log2;
+  __device__ __forceinline__ QueryTile(const AttentionParams& p, int hk, int unit, int tiles) {
+    pack_log2 = p.pack_log2;
+    const int tile = p.by_packs.div(unit);
+    first = (tiles - 1 - tile) * (kTile >> pack_log2);  // the latest first: they see most
+    head = hk * p.group + ((unit - tile * (int)p.by_packs.by) << pack_log2);
+  }
+  __device__ __forceinline__ int token(int row) const { return first + (row >> pack_log2); }
+  __device__ __forceinline__ int head_of(int row) const { return head + (row & ((1 << pack_log2) - 1)); }
 };
 
 // The visible keys of a tile of queries: the union over its rows, and what
@@ -52,7 +72,7 @@ struct TileKeys {
   int32_t all_s_end, all_lo, all_hi; // every row sees [0, all_s_end) and [all_lo, all_hi)
   __device__ __forceinline__ TileKeys(const AttentionParams& p, const Lengths& n, int i0) {
     s_end = lo = hi = all_s_end = all_lo = all_hi = 0;
-    const int i1 = min(i0 + kTile, n.q) - 1;
+    const int i1 = min(i0 + (kTile >> p.pack_log2), n.q) - 1;
     if (i0 > i1) return;
     const Visible first = visible_keys(n.position(i0), n.kv, p.window, p.sinks);
     const Visible last = visible_keys(n.position(i1), n.kv, p.window, p.sinks);
@@ -223,13 +243,18 @@ __global__ void __launch_bounds__(kTileThreads, 2) attention_tiles_kernel(const 
   const uint32_t tmem = bars.tmem, s_tmem = tmem, o_tmem = tmem + 128;
   pdl_wait();
 
-  // Which tile: the longest (latest) queries first.
-  const int bk = blockIdx.x % (p.batch * p.kv_heads), unit = blockIdx.x / (p.batch * p.kv_heads);
-  const int b = bk / p.kv_heads, hk = bk - b * p.kv_heads;
-  const int head = hk * p.group + unit % p.group, first = (tp.q_tiles - 1 - unit / p.group) * kTile;
+  const int which = p.by_heads.div(blockIdx.x), bk = blockIdx.x - which * p.by_heads.by, b = p.by_kv_heads.div(bk), hk = bk - b * p.kv_heads;
+  const int unit = tp.splits == 1 ? which : which / tp.splits, split = which - unit * tp.splits;
+  const QueryTile tile(p, hk, unit, tp.q_tiles);
   const Lengths len(p, b);
-  const TileKeys keys(p, len, first);
+  const TileKeys keys(p, len, tile.first);
   const TileList list(keys);
+  // This CTA's key tiles.
+  int j0 = 0, n = list.n;
+  if (tp.splits > 1) {
+    j0 = (int)((int64_t)list.n * split / tp.splits);
+    n = (int)((int64_t)list.n * (split + 1) / tp.splits) - j0;
+  }
   const Waiter wait{&bars.gone, p.status, kWaitNs};
 
   if (warp >= 4) {
@@ -240,14 +265,14 @@ __global__ void __launch_bounds__(kTileThreads, 2) attention_tiles_kernel(const 
         mbar_arrive_expect_tx(&bars.q_full, kTileBytes);
 #pragma unroll
         for (int box = 0; box < DP / 64; ++box)
-          tma_load(q_tile + box * kBox, &tp.q, box * 64, head, first, b, &bars.q_full);
+          tma_load(q_tile + box * kBox, &tp.q, box * 64, tile.head, tile.first, b, &bars.q_full);
         RingPos ring;
-        for (int j = 0; j < 2 * list.n; ++j, ring.next(kStages)) {  // K and V in turn
+        for (int j = 0; j < 2 * n; ++j, ring.next(kStages)) {  // K and V in turn
           if (!wait(&bars.kv_empty[ring.s], ring.ph ^ 1)) break;
           mbar_arrive_expect_tx(&bars.kv_full[ring.s], kTileBytes);
 #pragma unroll
           for (int box = 0; box < DP / 64; ++box)
-            tma_load(stages + ring.s * kTileBytes + box * kBox, j & 1 ? &tp.v : &tp.k, box * 64, hk, list.key(j >> 1), b,
+            tma_load(stages + ring.s * kTileBytes + box * kBox, j & 1 ? &tp.v : &tp.k, box * 64, hk, list.key(j0 + (j >> 1)), b,
                      &bars.kv_full[ring.s]);
         }
       }
@@ -259,20 +284,20 @@ __global__ void __launch_bounds__(kTileThreads, 2) attention_tiles_kernel(const 
       auto warp_wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)) != 0; };
       RingPos ring;
       bool ok = warp_wait(&bars.q_full, 0);
-      for (int j = 0; j <= list.n && ok; ++j) {
+      for (int j = 0; j <= n && ok; ++j) {
         const int v_slot = ring.s;
         if (j > 0) {
           if (!warp_wait(&bars.kv_full[v_slot], ring.ph)) break;
-          clear_unseen<DP>(seen, stages + v_slot * kTileBytes, list.key(j - 1), lane);
+          clear_unseen<DP>(seen, stages + v_slot * kTileBytes, list.key(j0 + j - 1), lane);
           ring.next(kStages);
         }
-        if (j < list.n && !warp_wait(&bars.kv_full[ring.s], ring.ph)) break;
+        if (j < n && !warp_wait(&bars.kv_full[ring.s], ring.ph)) break;
         if (j > 0) {
           if (!warp_wait(&bars.p_full, (j - 1) & 1)) break;
           tc_fence_after();
           mma_columns<T, DP, kTile, 32>(one, o_tmem, s_tmem, stages + v_slot * kTileBytes, kBox, j > 1);
         }
-        if (j < list.n) {
+        if (j < n) {
           // One queue of products: commits come behind both (a commit between
           // them cost 7% at 16384 queries, window 4096, dim 128: 508 us, now 474).
           mma_rows<T, DP, kTile>(one, s_tmem, q_tile, kBox, stages + ring.s * kTileBytes, kBox);
@@ -288,7 +313,7 @@ __global__ void __launch_bounds__(kTileThreads, 2) attention_tiles_kernel(const 
   } else {
     // ---- softmax, one thread per query
     registers_up<176>();
-    const int i = first + threadIdx.x;
+    const int i = tile.token(threadIdx.x);
     const uint32_t lanes = (uint32_t)(warp * 32) << 16;
     const uint32_t s_at = s_tmem + lanes, o_at = o_tmem + lanes;
     const bool in = i < len.q;
@@ -298,8 +323,8 @@ __global__ void __launch_bounds__(kTileThreads, 2) attention_tiles_kernel(const 
     const float sl = fmaxf(p.scale * kLog2e, 1.1754944e-38f);
     float m = -INFINITY, l = 0.f;
     bool ok = true;
-    for (int j = 0; j < list.n; ++j) {
-      const int k0 = list.key(j);
+    for (int j = 0; j < n; ++j) {
+      const int k0 = list.key(j0 + j);
       ok = __all_sync(0xffffffffu, wait(&bars.s_full, j & 1));
       if (!ok) break;
       tc_fence_after();
@@ -340,35 +365,86 @@ __global__ void __launch_bounds__(kTileThreads, 2) attention_tiles_kernel(const 
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars.p_full);
     }
-    // ---- output, staged where the queries were
+    // ---- output, staged where the queries were; a part of it straight to memory
     if (ok) ok = __all_sync(0xffffffffu, wait(&bars.o_full, 0));
+    const bool whole = tp.splits == 1;
     if (ok) {
       tc_fence_after();
       const float inv = !in || l == 0.f ? 0.f : l > 0.f ? rcp_rn(l) : l;  // a NaN stays one
+      float4* part = reinterpret_cast<float4*>(tp.part_o) + (int64_t)blockIdx.x * (kTile * DP / 4) + threadIdx.x;
 #pragma unroll 1
       for (int c = 0; c < DP; c += 32) {
         uint32_t o[32];
-        if (list.n > 0) {
+        if (n > 0) {
           tmem_load32(o_at + c, o);
           tmem_wait_loads();
         }
-        stage32<T>(q_tile, threadIdx.x, c, o, inv, list.n > 0 && inv != 0.f);
+        if (whole) {
+          stage32<T>(q_tile, threadIdx.x, c, o, inv, n > 0 && inv != 0.f);
+        } else if (n > 0) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            part[(c / 4 + e) * kTile] = make_float4(__uint_as_float(o[4 * e]), __uint_as_float(o[4 * e + 1]),
+                                                    __uint_as_float(o[4 * e + 2]), __uint_as_float(o[4 * e + 3]));
+        }
       }
-      if (p.lse && i < p.q_len)
-        p.lse[((int64_t)b * p.heads + head) * p.q_len + i] =
+      if (!whole)  // -infinity: no key seen; a NaN among the scores goes on in the sum
+        reinterpret_cast<float2*>(tp.part_stats)[(int64_t)blockIdx.x * kTile + threadIdx.x] =
+            make_float2(!in || l == 0.f ? -INFINITY : m == -INFINITY ? 0.f : m, l);
+      else if (p.lse && i < p.q_len)
+        p.lse[((int64_t)b * p.heads + tile.head_of(threadIdx.x)) * p.q_len + i] =
             !in || l == 0.f ? -INFINITY : (m - kShift + __log2f(l)) * (1.f / kLog2e);
       fence_proxy_async_smem();
     }
     asm volatile("bar.sync 1, 128;" ::: "memory");
-    if (threadIdx.x == 0 && !*(volatile uint32_t*)&bars.gone) {
+    if (threadIdx.x == 0 && whole && !*(volatile uint32_t*)&bars.gone) {
 #pragma unroll
       for (int box = 0; box < DP / 64; ++box)
-        if (box * 64 < p.head_dim) tma_store(&tp.o, q_tile + box * kBox, box * 64, head, first, b);
+        if (box * 64 < p.head_dim) tma_store(&tp.o, q_tile + box * kBox, box * 64, tile.head, tile.first, b);
       bulk_commit();
       bulk_wait_all();
     }
   }
   finish_tmem(bars.gone, warp == 5, tmem, kColumns);
+}
+
+// Joins the CTAs of a query tile: grid.x tiles as in the kernel above, grid.y 8
+// dims each, a thread 4 dims of a row.
+template <typename T, int DP>
+__global__ void __launch_bounds__(256) attention_tiles_join_kernel(const __grid_constant__ TileParams tp) {
+  constexpr float kShift = T::kIsHalf ? 7.f : 0.f;
+  const AttentionParams& p = tp.a;
+  const int unit = p.by_heads.div(blockIdx.x), bk = blockIdx.x - unit * p.by_heads.by, b = p.by_kv_heads.div(bk), hk = bk - b * p.kv_heads;
+  const int row = threadIdx.x & 127, quad = blockIdx.y * 2 + (threadIdx.x >> 7);
+  const QueryTile tile(p, hk, unit, tp.q_tiles);
+  const int i = tile.token(row), h = tile.head_of(row);
+  pdl_wait();
+  if (i >= p.q_len) return;
+  const int64_t first = (int64_t)unit * tp.splits * p.by_heads.by + bk;  // CTA of split 0; the next is by_heads.by further
+  const float2* stats = reinterpret_cast<const float2*>(tp.part_stats) + first * kTile + row;
+  const float4* part = reinterpret_cast<const float4*>(tp.part_o) + first * (kTile * DP / 4) + quad * kTile + row;
+  const int64_t step = (int64_t)p.by_heads.by * kTile;
+  float top = -INFINITY, sum = 0.f;
+#pragma unroll 4
+  for (int s = 0; s < tp.splits; ++s) top = fmaxf(top, stats[s * step].x);
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int s = 0; s < tp.splits; ++s) {
+    const float2 st = stats[s * step];
+    const float4 v = part[s * step * (DP / 4)];
+    if (st.x == -INFINITY) continue;  // saw no key
+    const float f = ex2(st.x - top);
+    sum = __fmaf_rn(f, st.y, sum);
+    o.x = __fmaf_rn(f, v.x, o.x);
+    o.y = __fmaf_rn(f, v.y, o.y);
+    o.z = __fmaf_rn(f, v.z, o.z);
+    o.w = __fmaf_rn(f, v.w, o.w);
+  }
+  const float inv = sum == 0.f ? 0.f : rcp_rn(sum);
+  if (quad * 4 < p.head_dim)
+    *reinterpret_cast<uint2*>(p.o.at(b, i, h) + quad * 4) = make_uint2(T::pack(o.x * inv, o.y * inv), T::pack(o.z * inv, o.w * inv));
+  if (quad == 0 && p.lse)
+    p.lse[((int64_t)b * p.heads + h) * p.q_len + i] = sum == 0.f ? -INFINITY : (top - kShift + __log2f(sum)) * (1.f / kLog2e);
 }
 
 }  // namespace cs

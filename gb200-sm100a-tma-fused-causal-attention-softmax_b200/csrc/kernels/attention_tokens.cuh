@@ -252,7 +252,7 @@ __global__ void __launch_bounds__(kTokenWarps * 32, NT == 1 ? 3 : 2) attention_t
     }
   __syncthreads();
   constexpr int kLanes = DP / 4;  // 4 dims a thread
-  for (int r = threadIdx.x / kLanes; r < kRows; r += kTokenWarps * 32 / kLanes) {
+  for (int r = threadIdx.x / kLanes; r < kRows && row0 + r < rows; r += kTokenWarps * 32 / kLanes) {
     const int d = (threadIdx.x % kLanes) * 4;
     float top = -INFINITY;
 #pragma unroll
@@ -272,8 +272,9 @@ __global__ void __launch_bounds__(kTokenWarps * 32, NT == 1 ? 3 : 2) attention_t
     if (tp.splits > 1) {
       const int64_t at = (int64_t)blockIdx.x * kRows + r;
       *reinterpret_cast<float4*>(tp.part_o + at * DP + d) = v;
-      if (d == 0) *reinterpret_cast<float2*>(tp.part_stats + at * 2) = make_float2(top, sum);
-    } else if (row0 + r < rows) {
+      // -infinity: no key seen; a NaN among the scores goes on in the sum.
+      if (d == 0) *reinterpret_cast<float2*>(tp.part_stats + at * 2) = make_float2(top == -INFINITY && sum != 0.f ? 0.f : top, sum);
+    } else {
       const int i = (row0 + r) / p.group, h = hk * p.group + (row0 + r) - i * p.group;
       const float inv = sum == 0.f ? 0.f : rcp_rn(sum);
       if (d < p.head_dim)
@@ -285,60 +286,74 @@ __global__ void __launch_bounds__(kTokenWarps * 32, NT == 1 ? 3 : 2) attention_t
   pdl_trigger();
 }
 
-// Joins a row block's splits: one CTA per (row block, row), a warp takes every
-// fourth split, lanes hold 4 dims each.
-template <typename T>
-__global__ void __launch_bounds__(128) attention_join_kernel(const __grid_constant__ TokenParams tp) {
+// Joins the splits: one CTA per row. Weights first, then the warps take splits in
+// turn, lanes hold 4 dims each: all loads are independent.
+constexpr int kMaxSplits = 2048;
+
+template <typename T, int kWarps>
+__global__ void __launch_bounds__(kWarps * 32) attention_join_kernel(const __grid_constant__ TokenParams tp) {
   constexpr float kShift = T::kIsHalf ? 7.f : 0.f;
-  __shared__ float sm_v[4][128 + 4], sm_m[4], sm_l[4];
+  constexpr int kJoinThreads = kWarps * 32;
+  __shared__ float weight[kMaxSplits], sm_v[kWarps][128 + 4], words[kWarps];
   const AttentionParams& p = tp.a;
-  const int block = blockIdx.x / tp.block_rows, r = blockIdx.x - block * tp.block_rows;
-  const int bk = block / tp.blocks, rb = block - bk * tp.blocks;
-  const int b = bk / p.kv_heads, hk = bk - b * p.kv_heads, row = rb * tp.block_rows + r;
+  const int rows = p.q_len * p.group, bk = blockIdx.x / rows, row = blockIdx.x - bk * rows;
+  const int rb = row / tp.block_rows, r = row - rb * tp.block_rows, block = bk * tp.blocks + rb;
+  const int b = bk / p.kv_heads, hk = bk - b * p.kv_heads;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, d = lane * 4;
-  if (row >= p.q_len * p.group) return;
+  const int64_t first = (int64_t)block * tp.splits * tp.block_rows + r;  // of the splits' rows
   pdl_wait();
-  float top = -INFINITY, sum = 0.f;
+  // The maximum, the weights, the sum.
+  float top = -INFINITY;
+  for (int s = threadIdx.x; s < tp.splits; s += kJoinThreads) {
+    weight[s] = tp.part_stats[(first + (int64_t)s * tp.block_rows) * 2];
+    top = fmaxf(top, weight[s]);
+  }
+  top = redux_max(top);
+  if (lane == 0) words[warp] = top;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) top = fmaxf(top, words[w]);
+  __syncthreads();
+  float sum = 0.f;
+  for (int s = threadIdx.x; s < tp.splits; s += kJoinThreads) {
+    const float f = weight[s] == -INFINITY ? 0.f : ex2(weight[s] - top);
+    weight[s] = f;
+    if (f != 0.f) sum = __fmaf_rn(f, tp.part_stats[(first + (int64_t)s * tp.block_rows) * 2 + 1], sum);
+  }
+  sum = warp_sum(sum);
+  if (lane == 0) words[warp] = sum;
+  __syncthreads();
+  sum = 0.f;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) sum += words[w];
   float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-  for (int s = warp; s < tp.splits; s += 4) {
-    const int64_t at = ((int64_t)block * tp.splits + s) * tp.block_rows + r;
-    const float2 st = *reinterpret_cast<const float2*>(tp.part_stats + at * 2);
-    const float4 x = d < tp.dim_pad ? *reinterpret_cast<const float4*>(tp.part_o + at * tp.dim_pad + d) : v;
-    if (st.x == -INFINITY) continue;
-    const float both = fmaxf(top, st.x), f0 = top == -INFINITY ? 0.f : ex2(top - both), f1 = ex2(st.x - both);
-    top = both;
-    sum = __fmaf_rn(f1, st.y, sum * f0);
-    v.x = __fmaf_rn(f1, x.x, v.x * f0);
-    v.y = __fmaf_rn(f1, x.y, v.y * f0);
-    v.z = __fmaf_rn(f1, x.z, v.z * f0);
-    v.w = __fmaf_rn(f1, x.w, v.w * f0);
+  if (d < tp.dim_pad) {
+#pragma unroll 8
+    for (int s = warp; s < tp.splits; s += kWarps) {
+      const float4 x = *reinterpret_cast<const float4*>(tp.part_o + (first + (int64_t)s * tp.block_rows) * tp.dim_pad + d);
+      const float f = weight[s];
+      if (f != 0.f) {  // a split without keys holds nothing
+        v.x = __fmaf_rn(f, x.x, v.x);
+        v.y = __fmaf_rn(f, x.y, v.y);
+        v.z = __fmaf_rn(f, x.z, v.z);
+        v.w = __fmaf_rn(f, x.w, v.w);
+      }
+    }
   }
   *reinterpret_cast<float4*>(&sm_v[warp][d]) = v;
-  if (lane == 0) {
-    sm_m[warp] = top;
-    sm_l[warp] = sum;
-  }
   __syncthreads();
-  if (warp) return;
-  top = fmaxf(fmaxf(sm_m[0], sm_m[1]), fmaxf(sm_m[2], sm_m[3]));
-  sum = 0.f;
-  v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    const float f = sm_m[w] == -INFINITY ? 0.f : ex2(sm_m[w] - top);
-    const float4 x = *reinterpret_cast<const float4*>(&sm_v[w][d]);
-    sum = __fmaf_rn(f, sm_l[w], sum);
-    v.x = __fmaf_rn(f, x.x, v.x);
-    v.y = __fmaf_rn(f, x.y, v.y);
-    v.z = __fmaf_rn(f, x.z, v.z);
-    v.w = __fmaf_rn(f, x.w, v.w);
-  }
   const int i = row / p.group, h = hk * p.group + row - i * p.group;
   const float inv = sum == 0.f ? 0.f : rcp_rn(sum);
-  if (d < p.head_dim)
-    *reinterpret_cast<uint2*>(p.o.at(b, i, h) + d) = make_uint2(T::pack(v.x * inv, v.y * inv), T::pack(v.z * inv, v.w * inv));
-  if (lane == 0 && p.lse)
+  if (threadIdx.x < p.head_dim / 2) {
+    float2 o = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      o.x += sm_v[w][threadIdx.x * 2];
+      o.y += sm_v[w][threadIdx.x * 2 + 1];
+    }
+    *reinterpret_cast<uint32_t*>(p.o.at(b, i, h) + threadIdx.x * 2) = T::pack(o.x * inv, o.y * inv);
+  }
+  if (threadIdx.x == 0 && p.lse)
     p.lse[((int64_t)b * p.heads + h) * p.q_len + i] = sum == 0.f ? -INFINITY : (top - kShift + __log2f(sum)) * (1.f / kLog2e);
 }
 

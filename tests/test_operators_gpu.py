@@ -166,6 +166,10 @@ ATTENTION = [
     (1, 513, 513, 2, 1, 8, 200, 300),          # more sinks than window
     (1, 1025, 1025, 2, 2, 120, 0, 0),
     (1, 640, 640, 2, 1, 128, 256, 1),
+    (1, 18, 3000, 16, 2, 128, 0, 0),           # few queries of many heads: shared tiles, split keys
+    (2, 40, 2500, 12, 1, 64, 1500, 5),
+    (1, 33, 700, 64, 1, 16, 0, 0),
+    (2, 150, 150, 24, 2, 64, 60, 2),           # groups of 12: packs of 4
 ]
 
 
