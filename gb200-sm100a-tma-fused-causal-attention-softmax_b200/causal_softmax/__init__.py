@@ -452,5 +452,18 @@ def parse_config(args: list[str]) -> dict:
     return {n: getattr(cfg, n) for n, _ in Config._fields_}
 
 
-from .operators import (attention, attention_backward, attention_status, bias_buckets,  # noqa: E402,F401
-                        bias_softmax, bias_softmax_backward)
+_OPERATORS = ("attention", "attention_backward", "attention_status", "bias_buckets", "bias_softmax",
+              "bias_softmax_backward")
+
+
+def __getattr__(name):
+    """The operators beside the softmax, on first use: they need torch, the rest of the binding does not."""
+    if name in _OPERATORS:
+        from . import operators
+
+        return getattr(operators, name)
+    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
+
+
+def __dir__():
+    return sorted([*globals(), *_OPERATORS])

@@ -13,9 +13,12 @@ of them) or k < sinks.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import functools
-import math
+import struct
+
+import torch
 
 from . import check, lib
 
@@ -44,39 +47,45 @@ class _AttentionGrads(ctypes.Structure):
     _fields_ = [(n, _Tensor) for n in ("d_o", "dq", "dk", "dv")]
 
 
-@functools.lru_cache(maxsize=None)
-def _types():
-    import torch
+# The same layouts for struct: filling a ctypes structure field by field would
+# take most of a small call's time.
+_PACK_BIAS = struct.Struct("@10iPf4x").pack
+_PACK_ATTENTION = struct.Struct("@9if2P" + "P3q" * 4 + "P").pack
+_PACK_GRADS = struct.Struct("@" + "P3q" * 4).pack
 
-    return {torch.float16: 0, torch.bfloat16: 1}
+_TYPES = {torch.float16: 0, torch.bfloat16: 1}
 
 
 class _On:
-    """The tensors' device and the launch stream, current while the call allocates and launches."""
+    """A launch stream other than the current one of the current device, made current
+    (with its device) while a call allocates and launches."""
 
     def __init__(self, device, stream):
-        import torch
-
         if isinstance(stream, int):
             stream = torch.cuda.ExternalStream(stream, device=device) if stream else torch.cuda.default_stream(device)
         if stream is None:  # the device's current stream
-            self._ctx = None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+            self._ctx = torch.cuda.device(device)
+        elif stream.device != device:
+            raise ValueError(f"stream of {stream.device} for tensors of {device}")
         else:
-            if stream.device != device:
-                raise ValueError(f"stream of {stream.device} for tensors of {device}")
             self._ctx = torch.cuda.stream(stream)
-        self._device = device
 
     def __enter__(self):
-        import torch
-
-        if self._ctx is not None:
-            self._ctx.__enter__()
-        return torch.cuda.current_stream(self._device).cuda_stream
+        self._ctx.__enter__()
 
     def __exit__(self, *exc):
-        if self._ctx is not None:
-            self._ctx.__exit__(*exc)
+        self._ctx.__exit__(*exc)
+
+
+_HERE = contextlib.nullcontext()
+
+
+def _on(device, stream):
+    return _HERE if stream is None and device.index == torch.cuda.current_device() else _On(device, stream)
+
+
+def _current(device) -> int:
+    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
 def _int(name: str, v) -> int:
@@ -91,7 +100,7 @@ def _same(name: str, t, dtype, device) -> None:
 
 
 def _sixteen_bit(name: str, t) -> int:
-    kind = _types().get(t.dtype)
+    kind = _TYPES.get(t.dtype)
     if kind is None or not t.is_cuda:
         raise TypeError(f"{name} must be a CUDA float16 or bfloat16 tensor, not {t.dtype} on {t.device}")
     return kind
@@ -113,25 +122,26 @@ def _starts_array(starts: tuple):
     return (ctypes.c_int32 * max(1, len(starts)))(*starts)
 
 
-def _bias_args(x, starts, cols, scale, row_offset, window, sinks) -> _BiasArgs:
+def _bias_args(x, starts, cols, scale, row_offset, window, sinks):
+    """The packed cs_bias_args, and (batch, heads, buckets). The starts' array outlives the call in the cache
+    of its values, or in the frame that holds the result's last item."""
     kind = _sixteen_bit("the matrices", x)
-    if x.dim() not in (3, 4):
+    shape = x.shape
+    if len(shape) not in (3, 4):
         raise ValueError("matrices are [batch,] heads, rows, pitch")
     if not x.is_contiguous():
         raise ValueError("matrices must be contiguous")
-    batch = x.shape[0] if x.dim() == 4 else 1
+    batch = shape[0] if len(shape) == 4 else 1
+    heads, rows, pitch = shape[-3:]
     starts = tuple(starts)
     array = _starts_array(starts)
-    args = _BiasArgs(kind, batch, x.shape[-3], x.shape[-2], _int("cols", cols), x.shape[-1],
-                     _int("row_offset", row_offset), _int("window", window), _int("sinks", sinks), len(starts),
-                     ctypes.addressof(array), scale)
-    args.keep = array  # the structure holds only its address
-    return args
+    args = _PACK_BIAS(kind, _int("batch", batch), _int("heads", heads), _int("rows", rows), _int("cols", cols),
+                      _int("pitch", pitch), _int("row_offset", row_offset), _int("window", window),
+                      _int("sinks", sinks), len(starts), ctypes.addressof(array), scale)
+    return args, heads, len(starts), array
 
 
 def _like(name, out, x):
-    import torch
-
     if out is None:
         return torch.empty_like(x)
     _same(name, out, x.dtype, x.device)
@@ -148,15 +158,14 @@ def bias_softmax(x, table, bucket_starts, *, cols: int, scale: float, row_offset
     position row_offset + i. table: float32 heads, buckets. bucket_starts: the
     buckets' first distances (bias_buckets, or any ascending ones from 0).
     Every other column of the result, padding included, is +0.0."""
-    import torch
-
-    args = _bias_args(x, bucket_starts, cols, scale, row_offset, window, sinks)
-    _same("table", table, torch.float32, x.device)
-    if table.shape != (args.heads, args.buckets) or not table.is_contiguous():
-        raise ValueError(f"table must be contiguous, [{args.heads}, {args.buckets}]")
-    with _On(x.device, stream) as s:
+    args, heads, buckets, _keep = _bias_args(x, bucket_starts, cols, scale, row_offset, window, sinks)
+    device = x.device
+    _same("table", table, torch.float32, device)
+    if table.shape != (heads, buckets) or not table.is_contiguous():
+        raise ValueError(f"table must be contiguous, [{heads}, {buckets}]")
+    with _on(device, stream):
         out = _like("out", out, x)
-        check(lib().cs_bias_softmax(ctypes.byref(args), x.data_ptr(), table.data_ptr(), out.data_ptr(), s),
+        check(lib().cs_bias_softmax(args, x.data_ptr(), table.data_ptr(), out.data_ptr(), _current(device)),
               "cs_bias_softmax")
     return out
 
@@ -167,59 +176,62 @@ def bias_softmax_backward(p, dp, bucket_starts, *, cols: int, scale: float, row_
 
     ds: of the scores x, in their type (masked columns +0.0); dtable: float32
     heads, buckets, summed over the batch and the rows."""
-    import torch
-
-    args = _bias_args(p, bucket_starts, cols, scale, row_offset, window, sinks)
-    _same("dp", dp, p.dtype, p.device)
+    args, heads, buckets, _keep = _bias_args(p, bucket_starts, cols, scale, row_offset, window, sinks)
+    device = p.device
+    _same("dp", dp, p.dtype, device)
     if dp.shape != p.shape or not dp.is_contiguous():
         raise ValueError(f"dp must be contiguous, of shape {tuple(p.shape)}")
     L = lib()
-    with _On(p.device, stream) as s:
+    with _on(device, stream):
         ds = _like("out", out, p)
-        dtable = torch.empty(args.heads, args.buckets, dtype=torch.float32, device=p.device)
-        need = L.cs_bias_softmax_backward_workspace(ctypes.byref(args))
+        dtable = torch.empty((heads, buckets), dtype=torch.float32, device=device)
+        need = L.cs_bias_softmax_backward_workspace(args)
         check(min(need, 0), "cs_bias_softmax_backward_workspace")
-        work = torch.empty(need, dtype=torch.uint8, device=p.device)
-        check(L.cs_bias_softmax_backward(ctypes.byref(args), p.data_ptr(), dp.data_ptr(), ds.data_ptr(),
-                                         dtable.data_ptr(), work.data_ptr(), need, s), "cs_bias_softmax_backward")
+        work = torch.empty(need, dtype=torch.uint8, device=device)
+        check(L.cs_bias_softmax_backward(args, p.data_ptr(), dp.data_ptr(), ds.data_ptr(), dtable.data_ptr(),
+                                         work.data_ptr(), need, _current(device)), "cs_bias_softmax_backward")
     return ds, dtable
 
 
 # ---------------------------------------------------------------- attention
 
-def _tensor(name: str, t, shape, like) -> _Tensor:
-    if t.dtype != like.dtype or t.device != like.device:
-        raise TypeError(f"{name} must be {like.dtype} on {like.device}, not {t.dtype} on {t.device}")
+def _tensor(name: str, t, shape, dtype, device) -> tuple:
+    """data, batch_stride, token_stride, head_stride."""
+    if t.dtype != dtype or t.device != device:
+        raise TypeError(f"{name} must be {dtype} on {device}, not {t.dtype} on {t.device}")
     if t.shape != shape:
         raise ValueError(f"{name} must be {list(shape)}, not {list(t.shape)}")
     b, n, h, d = t.stride()
     if d != 1 and shape[3] > 1:
         raise ValueError(f"{name}: the last dimension must be contiguous")
-    return _Tensor(t.data_ptr(), b, n, h)
+    return t.data_ptr(), b, n, h
 
 
-def _lens(name: str, t, batch: int, device):
-    import torch
-
+def _lens(name: str, t, batch: int, device) -> int:
     if t is None:
-        return None
+        return 0
     _same(name, t, torch.int32, device)
     if t.shape != (batch,) or not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous, [{batch}]")
     return t.data_ptr()
 
 
-def _attention_args(q, k, v, scale, window, sinks, q_lens, kv_lens) -> _AttentionArgs:
+def _attention_head(q, k, v, scale, window, sinks, q_lens, kv_lens) -> tuple:
+    """The fields of cs_attention_args up to v."""
     kind = _sixteen_bit("q", q)
-    if q.dim() != 4 or k.dim() != 4:
+    shape, dtype, device = q.shape, q.dtype, q.device
+    if len(shape) != 4 or k.dim() != 4:
         raise ValueError("q, k and v are batch, tokens, heads, head_dim")
-    batch, q_len, heads, dim = q.shape
-    kv_len, kv_heads = k.shape[1], k.shape[2]
+    batch, q_len, heads, dim = shape
+    _, kv_len, kv_heads, _ = k.shape
     kv_shape = (batch, kv_len, kv_heads, dim)
-    return _AttentionArgs(kind, batch, heads, kv_heads, dim, q_len, kv_len, _int("window", window),
-                          _int("sinks", sinks), 1.0 / math.sqrt(max(1, dim)) if scale is None else scale,
-                          _lens("q_lens", q_lens, batch, q.device), _lens("kv_lens", kv_lens, batch, q.device),
-                          _tensor("q", q, q.shape, q), _tensor("k", k, kv_shape, q), _tensor("v", v, kv_shape, q))
+    if max(batch, q_len, heads, dim, kv_len, kv_heads) > _I32_MAX:
+        raise ValueError(f"sizes of q {list(shape)} and k {list(k.shape)} do not fit 32 bits")
+    return (kind, batch, heads, kv_heads, dim, q_len, kv_len, _int("window", window), _int("sinks", sinks),
+            max(1, dim) ** -0.5 if scale is None else scale,
+            _lens("q_lens", q_lens, batch, device), _lens("kv_lens", kv_lens, batch, device),
+            *_tensor("q", q, shape, dtype, device), *_tensor("k", k, kv_shape, dtype, device),
+            *_tensor("v", v, kv_shape, dtype, device))
 
 
 def attention(q, k, v, *, scale: float | None = None, window: int = 0, sinks: int = 0, q_lens=None, kv_lens=None,
@@ -234,56 +246,47 @@ def attention(q, k, v, *, scale: float | None = None, window: int = 0, sinks: in
     are its last tokens, so q_len 1 with kv_lens reads a cache. Rows behind a
     sequence's queries come back zero. Returns out, or (out, lse) with the float32
     log-sum-exp [batch, heads, q_len] that attention_backward takes."""
-    import torch
-
-    args = _attention_args(q, k, v, scale, window, sinks, q_lens, kv_lens)
+    head = _attention_head(q, k, v, scale, window, sinks, q_lens, kv_lens)
+    shape, dtype, device = q.shape, q.dtype, q.device
     L = lib()
-    with _On(q.device, stream) as s:
+    with _on(device, stream):
         if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        args.o = _tensor("out", out, q.shape, q)
-        lse = None
-        if return_lse:
-            lse = torch.empty(args.batch, args.heads, args.q_len, dtype=torch.float32, device=q.device)
-            args.lse = lse.data_ptr()
-        ref = ctypes.byref(args)
-        need = L.cs_attention_workspace(ref)
+            out = torch.empty(shape, dtype=dtype, device=device)
+        lse = torch.empty((shape[0], shape[2], shape[1]), dtype=torch.float32, device=device) if return_lse else None
+        args = _PACK_ATTENTION(*head, *_tensor("out", out, shape, dtype, device), lse.data_ptr() if return_lse else 0)
+        need = L.cs_attention_workspace(args)
         check(min(need, 0), "cs_attention_workspace")
-        work = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-        check(L.cs_attention(ref, work.data_ptr() if need else None, need, s), "cs_attention")
+        work = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+        check(L.cs_attention(args, work.data_ptr() if need else None, need, _current(device)), "cs_attention")
     return (out, lse) if return_lse else out
 
 
 def attention_backward(dout, q, k, v, out, lse, *, scale: float | None = None, window: int = 0, sinks: int = 0,
                        q_lens=None, kv_lens=None, stream=None):
     """(dq, dk, dv) from dout, the gradient of attention's out, with the out and lse of the same arguments."""
-    import torch
-
-    args = _attention_args(q, k, v, scale, window, sinks, q_lens, kv_lens)
-    args.o = _tensor("out", out, q.shape, q)
-    _same("lse", lse, torch.float32, q.device)
-    if lse.shape != (args.batch, args.heads, args.q_len) or not lse.is_contiguous():
-        raise ValueError(f"lse must be contiguous, [{args.batch}, {args.heads}, {args.q_len}]")
-    args.lse = lse.data_ptr()
+    head = _attention_head(q, k, v, scale, window, sinks, q_lens, kv_lens)
+    shape, dtype, device = q.shape, q.dtype, q.device
+    _same("lse", lse, torch.float32, device)
+    if lse.shape != (shape[0], shape[2], shape[1]) or not lse.is_contiguous():
+        raise ValueError(f"lse must be contiguous, {[shape[0], shape[2], shape[1]]}")
+    args = _PACK_ATTENTION(*head, *_tensor("out", out, shape, dtype, device), lse.data_ptr())
+    d_o = _tensor("dout", dout, shape, dtype, device)
     L = lib()
-    with _On(q.device, stream) as s:
-        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
-        grads = _AttentionGrads(_tensor("dout", dout, q.shape, q), _tensor("dq", dq, q.shape, q),
-                                _tensor("dk", dk, k.shape, q), _tensor("dv", dv, v.shape, q))
-        ref = ctypes.byref(args)
-        need = L.cs_attention_backward_workspace(ref)
+    with _on(device, stream):
+        dq, dk, dv = (torch.empty(t.shape, dtype=dtype, device=device) for t in (q, k, v))
+        grads = _PACK_GRADS(*d_o, dq.data_ptr(), *dq.stride()[:3], dk.data_ptr(), *dk.stride()[:3],
+                            dv.data_ptr(), *dv.stride()[:3])
+        need = L.cs_attention_backward_workspace(args)
         check(min(need, 0), "cs_attention_backward_workspace")
-        work = torch.empty(need, dtype=torch.uint8, device=q.device)
-        check(L.cs_attention_backward(ref, ctypes.byref(grads), work.data_ptr(), need, s), "cs_attention_backward")
+        work = torch.empty(need, dtype=torch.uint8, device=device)
+        check(L.cs_attention_backward(args, grads, work.data_ptr(), need, _current(device)), "cs_attention_backward")
     return dq, dk, dv
 
 
 def attention_status(stream=None, device=None) -> tuple[int, int]:
     """(error code, bits) of the attention kernels' status word on a device, which it clears; waits for the stream."""
-    import torch
-
     device = torch.device("cuda", torch.cuda.current_device() if device is None else torch.device(device).index or 0)
     bits = ctypes.c_uint32()
-    with _On(device, stream) as s:
-        rc = lib().cs_attention_status(ctypes.byref(bits), s)
+    with _on(device, stream):
+        rc = lib().cs_attention_status(ctypes.byref(bits), _current(device))
     return rc, bits.value

@@ -395,7 +395,8 @@ int launch_backward(const cs_attention_args* a, const cs_attention_grads* g, con
   cudaError_t e = cudaSuccess;
   if (half) e = cudaMemsetAsync(norms, 0, (size_t)s.norms_bytes, static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return fail_cuda(e, "attention backward, norms");
-  const unsigned rows = (unsigned)(((s.q_pad >> p.pack_log2) + 15) / 16 + (half ? (a->kv_len + 15) / 16 : 0));
+  const unsigned rows = (unsigned)(((s.q_pad >> p.pack_log2) + cs::kRowsPerCta - 1) / cs::kRowsPerCta +
+                                   (half ? (a->kv_len + cs::kRowsPerCta - 1) / cs::kRowsPerCta : 0));
   e = cs_host::launch(half ? &cs::attention_rows_kernel<cs::F16> : &cs::attention_rows_kernel<cs::BF16>,
                       dim3(rows, (unsigned)std::min(a->batch * a->heads, 65535)), 256, 0, stream, r);
   if (e != cudaSuccess) return fail_cuda(e, "attention backward, rows");

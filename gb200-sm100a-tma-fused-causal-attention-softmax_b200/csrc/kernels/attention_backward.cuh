@@ -57,59 +57,86 @@ struct RowsParams {
   int32_t q_pad;
 };
 
-__device__ __forceinline__ void raise_max(uint32_t* at, float v) {
-  const float m = redux_max(v);  // NaN counts as nothing
-  if ((threadIdx.x & 31) == 0 && m > 0.f) atomicMax(at, __float_as_uint(m));
+constexpr int kRowsPerCta = 64;
+
+// The largest of a CTA's row norms, to the kv head's.
+__device__ __forceinline__ void raise_max(uint32_t* at, float v, float* words) {
+  v = redux_max(v);  // NaN counts as nothing
+  if ((threadIdx.x & 31) == 0) words[threadIdx.x >> 5] = v;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < 8; ++w) v = fmaxf(v, words[w]);
+    if (v > 0.f) atomicMax(at, __float_as_uint(v));
+  }
+  __syncthreads();
 }
 
-// 16 lanes a row. grid.x covers a head's tokens up to the end of its last tile,
-// then (fp16) the keys of a kv head; grid.y = batch * heads.
+// 16 lanes a row, four rows at a time. grid.x covers a head's tokens up to the end
+// of its last tile, then (fp16) the keys of a kv head; grid.y = batch * heads.
 template <typename T>
 __global__ void __launch_bounds__(256) attention_rows_kernel(const __grid_constant__ RowsParams rp) {
+  __shared__ float words[8];
   const AttentionParams& p = rp.a;
   pdl_wait();
-  const int lane = threadIdx.x & 15, d = lane * 8, per_cta = 16;
-  const int tokens = rp.q_pad >> p.pack_log2, q_ctas = (tokens + per_cta - 1) / per_cta;
+  const int lane = threadIdx.x & 15, d = lane * 8;
+  const bool has = d < p.head_dim;
+  const int tokens = rp.q_pad >> p.pack_log2, q_ctas = (tokens + kRowsPerCta - 1) / kRowsPerCta;
+  const uint4 none = make_uint4(0, 0, 0, 0);
   for (int bh = blockIdx.y; bh < p.batch * p.heads; bh += gridDim.y) {
     const int b = bh / p.heads, h = bh - b * p.heads, hk = h / p.group;
     const Lengths len(p, b);
-    float a[8], g[8];
+    uint4 ra[4], rg[4];
+    float a[8], g[8], most = 0.f;
     if ((int)blockIdx.x < q_ctas) {
-      const int i = blockIdx.x * per_cta + threadIdx.x / 16;
-      const bool in = i < len.q && len.position(i) >= 0;
-      float dot = 0.f, norm = 0.f;
-      if (in && d < p.head_dim) {
-        unpack8<T>(*reinterpret_cast<const uint4*>(p.o.at(b, i, h) + d), a);
-        unpack8<T>(*reinterpret_cast<const uint4*>(p.d_o.at(b, i, h) + d), g);
+      const int i0 = blockIdx.x * kRowsPerCta + threadIdx.x / 16;
+      bool in[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int i = i0 + r * 16;
+        in[r] = i < len.q && len.position(i) >= 0;
+        ra[r] = in[r] && has ? load16(p.o.at(b, i, h) + d) : none;
+        rg[r] = in[r] && has ? load16(p.d_o.at(b, i, h) + d) : none;
+      }
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int i = i0 + r * 16;
+        unpack8<T>(ra[r], a);
+        unpack8<T>(rg[r], g);
+        float dot = 0.f, norm = 0.f;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           dot = __fmaf_rn(a[e], g[e], dot);
-          norm = __fmaf_rn(g[e], g[e], norm);
+          if (T::kIsHalf) norm = __fmaf_rn(g[e], g[e], norm);
         }
-      }
 #pragma unroll
-      for (int x = 8; x > 0; x >>= 1) {
-        dot += __shfl_xor_sync(0xffffffffu, dot, x);
-        norm += __shfl_xor_sync(0xffffffffu, norm, x);
+        for (int x = 8; x > 0; x >>= 1) {
+          dot += __shfl_xor_sync(0xffffffffu, dot, x);
+          if (T::kIsHalf) norm += __shfl_xor_sync(0xffffffffu, norm, x);
+        }
+        if (lane == 0 && i < tokens) {
+          const int64_t row = (int64_t)(bh >> p.pack_log2) * rp.q_pad + (i << p.pack_log2) + (h & ((1 << p.pack_log2) - 1));
+          const float lse = in[r] ? p.lse[(int64_t)bh * p.q_len + i] : -INFINITY;
+          rp.lse2[row] = lse == -INFINITY ? -INFINITY : -lse * kLog2e;
+          rp.delta[row] = in[r] ? -dot : 0.f;
+        }
+        most = fmaxf(most, norm);
       }
-      if (lane == 0 && i < tokens) {
-        const int64_t row = (int64_t)(bh >> p.pack_log2) * rp.q_pad + (i << p.pack_log2) + (h & ((1 << p.pack_log2) - 1));
-        const float lse = in ? p.lse[(int64_t)bh * p.q_len + i] : -INFINITY;
-        rp.lse2[row] = lse == -INFINITY ? -INFINITY : -lse * kLog2e;
-        rp.delta[row] = in ? -dot : 0.f;
-      }
-      if (T::kIsHalf) raise_max(rp.norms + b * p.kv_heads + hk, norm);
+      if (T::kIsHalf) raise_max(rp.norms + b * p.kv_heads + hk, most, words);
     } else if (T::kIsHalf && h % p.group == 0) {
-      const int k = (blockIdx.x - q_ctas) * per_cta + threadIdx.x / 16;
-      float norm = 0.f;
-      if (k < len.kv && d < p.head_dim && sees(sequence_keys(p, len), k)) {
-        unpack8<T>(*reinterpret_cast<const uint4*>(p.v.at(b, k, hk) + d), a);
+      const int k0 = ((int)blockIdx.x - q_ctas) * kRowsPerCta + threadIdx.x / 16;
+      const Visible seen = sequence_keys(p, len);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int k = k0 + r * 16;
+        unpack8<T>(has && sees(seen, k) ? load16(p.v.at(b, k, hk) + d) : none, a);
+        float norm = 0.f;
 #pragma unroll
         for (int e = 0; e < 8; ++e) norm = __fmaf_rn(a[e], a[e], norm);
-      }
 #pragma unroll
-      for (int x = 8; x > 0; x >>= 1) norm += __shfl_xor_sync(0xffffffffu, norm, x);
-      raise_max(rp.norms + p.batch * p.kv_heads + b * p.kv_heads + hk, norm);
+        for (int x = 8; x > 0; x >>= 1) norm += __shfl_xor_sync(0xffffffffu, norm, x);
+        most = fmaxf(most, norm);
+      }
+      raise_max(rp.norms + p.batch * p.kv_heads + b * p.kv_heads + hk, most, words);
     }
   }
   pdl_trigger();

@@ -66,6 +66,15 @@ __device__ __forceinline__ F2 f2_fma(F2 a, F2 b, F2 c) {
   return r;
 }
 
+// 16 bytes that are read once.
+__device__ __forceinline__ uint4 load16(const uint16_t* p) {
+  uint4 r;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
+               : "l"(p));
+  return r;
+}
+
 // The 8 elements of a 16-byte vector, and back.
 template <typename T>
 __device__ __forceinline__ void unpack8(const uint4& r, float* f) {
