@@ -367,19 +367,19 @@ GradShape grad_shape(const cs_attention_args* a, int sms) {
   s.sink_shares = (int)((all + s.share - 1) / s.share);
   s.dkv_ctas = heads * ((int64_t)s.sink_tiles * s.sink_shares + (int64_t)(s.k_tiles - s.sink_tiles) * s.window_shares);
   s.rows_bytes = (int64_t)a->batch * (a->heads >> pack) * s.q_pad * 4;
-  s.norms_bytes = a->type == CS_TYPE_F16 ? (2 * heads * 4 + 15) / 16 * 16 : 0;
+  s.norms_bytes = (a->type == CS_TYPE_F16 ? (2 * heads * 4 + 15) / 16 * 16 : 0) + 16;  // and dQ's counter
   if (s.window_shares > 1 || (s.sink_tiles && s.sink_shares > 1)) s.partial_bytes = s.dkv_ctas * 2 * cs::kTile * s.dim * 4;
   return s;
 }
 
 int check_shape(const cs_attention_args* a, const GradShape& s) {
-  if (s.q_pad > kI32Max || s.dkv_ctas > kI32Max || (int64_t)a->batch * a->heads * s.q_tiles > kI32Max)
+  if (s.q_pad > kI32Max || s.dkv_ctas > kI32Max || (int64_t)a->batch * a->heads * s.q_tiles > kI32Max - 65536)
     return fail(CS_ERR_WRONG_LENGTH, "backward of q_len %d, kv_len %d: too many tiles", a->q_len, a->kv_len);
   return CS_OK;
 }
 
 int launch_backward(const cs_attention_args* a, const cs_attention_grads* g, const cs::AttentionParams& p, const GradShape& s,
-                    void* workspace, void* stream) {
+                    int sms, void* workspace, void* stream) {
   char* at = static_cast<char*>(workspace);
   float* lse2 = reinterpret_cast<float*>(at);
   float* delta = reinterpret_cast<float*>(at + s.rows_bytes);
@@ -391,9 +391,10 @@ int launch_backward(const cs_attention_args* a, const cs_attention_grads* g, con
   r.lse2 = lse2;
   r.delta = delta;
   r.norms = reinterpret_cast<uint32_t*>(norms);
+  r.next = reinterpret_cast<int32_t*>(at + 2 * s.rows_bytes + s.norms_bytes - 16);
   r.q_pad = (int32_t)s.q_pad;
   cudaError_t e = cudaSuccess;
-  if (half) e = cudaMemsetAsync(norms, 0, (size_t)s.norms_bytes, static_cast<cudaStream_t>(stream));
+  if (half) e = cudaMemsetAsync(norms, 0, (size_t)(s.norms_bytes - 16), static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return fail_cuda(e, "attention backward, norms");
   const unsigned rows = (unsigned)(((s.q_pad >> p.pack_log2) + cs::kRowsPerCta - 1) / cs::kRowsPerCta +
                                    (half ? (a->kv_len + cs::kRowsPerCta - 1) / cs::kRowsPerCta : 0));
@@ -406,6 +407,7 @@ int launch_backward(const cs_attention_args* a, const cs_attention_grads* g, con
   k.lse2 = lse2;
   k.delta = delta;
   k.norms = norms;
+  k.next = r.next;
   k.partial = reinterpret_cast<float*>(at + 2 * s.rows_bytes + s.norms_bytes);
   k.q_pad = (int32_t)s.q_pad;
   k.share = s.share;
@@ -427,8 +429,9 @@ int launch_backward(const cs_attention_args* a, const cs_attention_grads* g, con
   q.tiles = s.q_tiles;
   rc = make_map(&q.out0, a, g->dq, a->q_len, a->heads, p.pack_log2);
   if (rc) return rc;
-  e = cs_host::launch(dq_kernel(a->type, s.dim), dim3((unsigned)(a->batch * (a->heads >> p.pack_log2) * s.q_tiles)), cs::kGradThreads,
-                      (size_t)dq_smem(s.dim), stream, q);
+  q.units = (int)((int64_t)a->batch * (a->heads >> p.pack_log2) * s.q_tiles);
+  e = cs_host::launch(dq_kernel(a->type, s.dim), dim3((unsigned)std::min(q.units, sms)), cs::kGradThreads, (size_t)dq_smem(s.dim),
+                      stream, q);
   if (e != cudaSuccess) return fail_cuda(e, "attention backward, queries");
   if (s.partial_bytes) {
     const int64_t tiles = (int64_t)a->batch * a->kv_heads * (s.window_shares > 1 ? s.k_tiles : s.sink_tiles);
@@ -499,7 +502,7 @@ int cs_attention_backward(const cs_attention_args* args, const cs_attention_grad
   p.dq = strided(grads->dq);
   p.dk = strided(grads->dk);
   p.dv = strided(grads->dv);
-  return launch_backward(args, grads, p, s, workspace, stream);
+  return launch_backward(args, grads, p, s, d.sms, workspace, stream);
 }
 
 int cs_attention_status(uint32_t* status, void* stream) {

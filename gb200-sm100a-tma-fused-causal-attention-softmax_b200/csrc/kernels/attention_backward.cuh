@@ -42,7 +42,9 @@ struct GradParams {
   const float* norms;  // fp16: [2, batch * kv_heads], largest |d_o| and |v| of a row
   float* partial;      // dK, dV parts of key tiles cut into several CTAs' shares
   int32_t q_pad;
-  int32_t tiles;       // query (or key) tiles
+  int32_t tiles;       // query (or key) tiles of a pack of heads (a kv head)
+  int32_t units;       // dQ: query tiles in all
+  int32_t* next;       // the next one to take; the rows kernel sets it to 0
   int32_t share;       // units of one CTA (dK, dV)
   int32_t window_shares, sink_tiles, sink_shares;  // CTAs per key tile; those of the first sink_tiles ones
 };
@@ -54,6 +56,7 @@ struct RowsParams {
   float* lse2;
   float* delta;
   uint32_t* norms;  // as integers: the bits of non-negative floats order like them
+  int32_t* next;    // dQ's counter of query tiles
   int32_t q_pad;
 };
 
@@ -78,6 +81,7 @@ __global__ void __launch_bounds__(256) attention_rows_kernel(const __grid_consta
   __shared__ float words[8];
   const AttentionParams& p = rp.a;
   pdl_wait();
+  if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *rp.next = 0;
   const int lane = threadIdx.x & 15, d = lane * 8;
   const bool has = d < p.head_dim;
   const int tokens = rp.q_pad >> p.pack_log2, q_ctas = (tokens + kRowsPerCta - 1) / kRowsPerCta;
@@ -196,18 +200,26 @@ constexpr int kGradThreads = 384;  // registers: 384 x 168 = 256 x 192 + 128 x 1
 // ---- dQ
 
 struct QueryBarriers {
-  uint64_t q_full, s_full[2], dp_full, ds_full, done, k_full[3], k_empty[3], v_full, v_empty;
+  uint64_t q_full, q_empty, s_full[2], dp_full, ds_full, done, dq_free, k_full[3], k_empty[3], v_full, v_empty;
+  uint64_t unit_full[2], unit_empty[2];
+  int32_t unit[2];    // query tiles taken; gp.units or more: no more
   uint32_t tmem, gone;
+  uint32_t given_up;  // by a warpgroup's warp
 };
 
 template <int DP>
 struct QuerySmem {
   static constexpr int kTileBytes = kTile * DP * 2;
   static constexpr int kKeys = 3;  // key tiles: held until dQ has used them
-  static constexpr int kBytes = (2 + kKeys + 1) * kTileBytes + 256;
+  static constexpr int kBytes = (2 + kKeys + 1 + 1) * kTileBytes + 256;  // Q, d_o, keys, values, the output's staging
 };
 
-// Products in this order (S in two buffers):
+// Persistent: a CTA takes the next query tile, longest first, from a counter (the
+// result does not depend on who takes which); that tile's loads and first products
+// run while this one's last gradients are made and brought out. The CTAs start as
+// the dK/dV kernel's last ones leave, so equal shares fixed in advance would end
+// unevenly: causal 4096 queries 299 us a step with them, 288 with one CTA a tile.
+// Products of a tile, S in two buffers:
 //   S(0) dP(0) S(1) | dQ(0) dP(1) S(2) | dQ(1) dP(2) S(3) | ...
 // While the warpgroups turn S(j + 1) into P(j + 1), the tensor core has dQ(j) and
 // dP(j + 1); while they make dS(j + 1), S(j + 2).
@@ -221,7 +233,8 @@ __global__ void __launch_bounds__(kGradThreads, 1) attention_dq_kernel(const __g
   uint8_t* do_tile = q_tile + kTileBytes;
   uint8_t* k_tiles = do_tile + kTileBytes;
   uint8_t* v_tile = k_tiles + kKeys * kTileBytes;
-  QueryBarriers& bars = *reinterpret_cast<QueryBarriers*>(v_tile + kTileBytes);
+  uint8_t* out_tile = v_tile + kTileBytes;
+  QueryBarriers& bars = *reinterpret_cast<QueryBarriers*>(out_tile + kTileBytes);
   const AttentionParams& p = gp.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (smem_addr(aligned_smem) & 1023) {  // the swizzle needs it
@@ -230,18 +243,25 @@ __global__ void __launch_bounds__(kGradThreads, 1) attention_dq_kernel(const __g
   }
   if (warp == 8 && lane == 0) {
     mbar_init(&bars.q_full, 1);
+    mbar_init(&bars.q_empty, 1);
     mbar_init(&bars.s_full[0], 1);
     mbar_init(&bars.s_full[1], 1);
     mbar_init(&bars.dp_full, 1);
     mbar_init(&bars.ds_full, 8);
     mbar_init(&bars.done, 1);
+    mbar_init(&bars.dq_free, 8);
     for (int i = 0; i < kKeys; ++i) {
       mbar_init(&bars.k_full[i], 1);
       mbar_init(&bars.k_empty[i], 1);
     }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bars.unit_full[i], 1);
+      mbar_init(&bars.unit_empty[i], 9);
+    }
     mbar_init(&bars.v_full, 1);
     mbar_init(&bars.v_empty, 1);
     bars.gone = 0;
+    bars.given_up = 0;
     fence_barrier_init();
     prefetch_map(&gp.q);
     prefetch_map(&gp.d_o);
@@ -255,150 +275,213 @@ __global__ void __launch_bounds__(kGradThreads, 1) attention_dq_kernel(const __g
   const uint32_t tmem = bars.tmem, dp_tmem = tmem + 256, dq_tmem = tmem + 384;
   // Only the rows kernel's results are needed, and it was done before the dK/dV
   // kernel let this one start; the wait for that one is at the end.
-
-  const int unit = p.by_heads.div(blockIdx.x), bk = blockIdx.x - unit * p.by_heads.by, b = p.by_kv_heads.div(bk), hk = bk - b * p.kv_heads;
-  const QueryTile tile(p, hk, unit, gp.tiles);
-  const Lengths len(p, b);
-  const TileKeys keys(p, len, tile.first);
-  const TileList list(keys);
   const Waiter wait{&bars.gone, p.status, kWaitNs};
+  struct Unit {
+    int bk, b, hk;
+    QueryTile tile;
+    Lengths len;
+    TileKeys keys;
+    TileList list;
+    __device__ __forceinline__ Unit(const GradParams& gp, int index)
+        : bk(index - gp.a.by_heads.div(index) * (int)gp.a.by_heads.by), b(gp.a.by_kv_heads.div(bk)), hk(bk - b * gp.a.kv_heads),
+          tile(gp.a, hk, gp.a.by_heads.div(index), gp.tiles), len(gp.a, b), keys(gp.a, len, tile.first), list(keys) {}
+  };
+
+  // The tile of a round, for a converged warp; gp.units if the wait was given up.
+  auto next_unit = [&](int round) {
+    const int slot = round & 1;
+    int index = gp.units;
+    if (wait(&bars.unit_full[slot], (round >> 1) & 1)) index = *(volatile int32_t*)&bars.unit[slot];
+    index = __shfl_sync(0xffffffffu, index, 0);
+    if (lane == 0) mbar_arrive(&bars.unit_empty[slot]);
+    return index;
+  };
 
   if (warp >= 8) {
     registers_down<120>();
     if (warp == 8) {
-      if (lane == 0 && list.n > 0) {
-        mbar_arrive_expect_tx(&bars.q_full, 2 * kTileBytes);
-#pragma unroll
-        for (int box = 0; box < DP / 64; ++box) {
-          tma_load(q_tile + box * kBox, &gp.q, box * 64, tile.head, tile.first, b, &bars.q_full);
-          tma_load(do_tile + box * kBox, &gp.d_o, box * 64, tile.head, tile.first, b, &bars.q_full);
-        }
+      if (lane == 0) {
         RingPos ring;
-        auto load_key = [&](int j) {
-          if (!wait(&bars.k_empty[ring.s], ring.ph ^ 1)) return false;
-          mbar_arrive_expect_tx(&bars.k_full[ring.s], kTileBytes);
-#pragma unroll
-          for (int box = 0; box < DP / 64; ++box)
-            tma_load(k_tiles + ring.s * kTileBytes + box * kBox, &gp.k, box * 64, hk, list.key(j), b, &bars.k_full[ring.s]);
-          ring.next(kKeys);
-          return true;
-        };
-        // The order in which the products need them: K(0) V(0) K(1) | V(1) K(2) | ...
-        bool ok = load_key(0);
-        for (int j = 0; j < list.n && ok; ++j) {
-          ok = wait(&bars.v_empty, (j & 1) ^ 1);
+        uint32_t tiles = 0, used = 0;  // key tiles and query tiles so far
+        bool ok = true;
+        for (int round = 0; ok; ++round) {
+          const int slot = round & 1;
+          if (!wait(&bars.unit_empty[slot], ((round >> 1) & 1) ^ 1)) break;
+          const int index = atomicAdd(gp.next, 1);
+          *(volatile int32_t*)&bars.unit[slot] = index;
+          mbar_arrive(&bars.unit_full[slot]);
+          if (index >= gp.units) break;
+          const Unit u(gp, index);
+          if (u.list.n == 0) continue;
+          ok = wait(&bars.q_empty, (used & 1) ^ 1);
+          ++used;
           if (!ok) break;
-          mbar_arrive_expect_tx(&bars.v_full, kTileBytes);
+          mbar_arrive_expect_tx(&bars.q_full, 2 * kTileBytes);
 #pragma unroll
-          for (int box = 0; box < DP / 64; ++box)
-            tma_load(v_tile + box * kBox, &gp.v, box * 64, hk, list.key(j), b, &bars.v_full);
-          if (j + 1 < list.n) ok = load_key(j + 1);
+          for (int box = 0; box < DP / 64; ++box) {
+            tma_load(q_tile + box * kBox, &gp.q, box * 64, u.tile.head, u.tile.first, u.b, &bars.q_full);
+            tma_load(do_tile + box * kBox, &gp.d_o, box * 64, u.tile.head, u.tile.first, u.b, &bars.q_full);
+          }
+          auto load_key = [&](int j) {
+            if (!wait(&bars.k_empty[ring.s], ring.ph ^ 1)) return false;
+            mbar_arrive_expect_tx(&bars.k_full[ring.s], kTileBytes);
+#pragma unroll
+            for (int box = 0; box < DP / 64; ++box)
+              tma_load(k_tiles + ring.s * kTileBytes + box * kBox, &gp.k, box * 64, u.hk, u.list.key(j), u.b, &bars.k_full[ring.s]);
+            ring.next(kKeys);
+            return true;
+          };
+          // The order in which the products need them: K(0) V(0) K(1) | V(1) K(2) | ...
+          ok = load_key(0);
+          for (int j = 0; j < u.list.n && ok; ++j, ++tiles) {
+            ok = wait(&bars.v_empty, (tiles & 1) ^ 1);
+            if (!ok) break;
+            mbar_arrive_expect_tx(&bars.v_full, kTileBytes);
+#pragma unroll
+            for (int box = 0; box < DP / 64; ++box)
+              tma_load(v_tile + box * kBox, &gp.v, box * 64, u.hk, u.list.key(j), u.b, &bars.v_full);
+            if (j + 1 < u.list.n) ok = load_key(j + 1);
+          }
         }
       }
       __syncwarp();
-    } else if (warp == 9 && list.n > 0) {
-      const Visible seen = sequence_keys(p, len);
+    } else if (warp == 9) {
       const uint32_t one = elect_one();
       auto warp_wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)) != 0; };
-      RingPos ring, used;  // key tiles: of S; of dQ
-      auto scores = [&](int j) {  // S(j)
-        uint8_t* k_tile = k_tiles + ring.s * kTileBytes;
-        if (!warp_wait(&bars.k_full[ring.s], ring.ph)) return false;
-        clear_unseen<DP>(seen, k_tile, list.key(j), lane);
-        mma_rows<T, DP, kTile>(one, tmem + (j & 1) * 128, q_tile, kBox, k_tile, kBox);
-        mma_commit(one, &bars.s_full[j & 1]);
-        ring.next(kKeys);
-        return true;
-      };
-      auto products = [&](int j) {  // dP(j)
-        if (!warp_wait(&bars.v_full, j & 1)) return false;
-        mma_rows<T, DP, kTile>(one, dp_tmem, do_tile, kBox, v_tile, kBox);
-        mma_commit(one, &bars.dp_full);
-        mma_commit(one, &bars.v_empty);
-        return true;
-      };
-      bool ok = warp_wait(&bars.q_full, 0) && scores(0) && products(0);
-      if (ok && list.n > 1) ok = scores(1);
-      for (int j = 0; j < list.n && ok; ++j) {
-        if (!warp_wait(&bars.ds_full, j & 1)) break;
+      RingPos ring, spent;         // key tiles: of S; of dQ
+      uint32_t tiles = 0, used = 0;  // key tiles and query tiles so far
+      bool ok = true;
+      for (int round = 0; ok; ++round) {
+        const int index = next_unit(round);
+        if (index >= gp.units) break;
+        const Unit u(gp, index);
+        const int n = u.list.n;
+        if (n == 0) continue;
+        const Visible seen = sequence_keys(p, u.len);
+        auto scores = [&](int j) {  // S(j)
+          uint8_t* k_tile = k_tiles + ring.s * kTileBytes;
+          if (!warp_wait(&bars.k_full[ring.s], ring.ph)) return false;
+          clear_unseen<DP>(seen, k_tile, u.list.key(j), lane);
+          const uint32_t buffer = (tiles + j) & 1;
+          mma_rows<T, DP, kTile>(one, tmem + buffer * 128, q_tile, kBox, k_tile, kBox);
+          mma_commit(one, &bars.s_full[buffer]);
+          ring.next(kKeys);
+          return true;
+        };
+        auto products = [&](int j) {  // dP(j), the last one to read Q and d_o if j is
+          if (!warp_wait(&bars.v_full, (tiles + j) & 1)) return false;
+          mma_rows<T, DP, kTile>(one, dp_tmem, do_tile, kBox, v_tile, kBox);
+          mma_commit(one, &bars.dp_full);
+          mma_commit(one, &bars.v_empty);
+          if (j == n - 1) mma_commit(one, &bars.q_empty);
+          return true;
+        };
+        ok = warp_wait(&bars.q_full, used & 1) && scores(0) && products(0);
+        if (ok && n > 1) ok = scores(1);
+        if (ok && used > 0) ok = warp_wait(&bars.dq_free, (used & 1) ^ 1);  // the tile before is brought out
         tc_fence_after();
-        mma_columns<T, DP, kTile, 64>(one, dq_tmem, dp_tmem, k_tiles + used.s * kTileBytes, kBox, j > 0);
-        if (j + 1 < list.n) {
-          ok = products(j + 1);
-          mma_commit(one, &bars.k_empty[used.s]);
-          if (ok && j + 2 < list.n) ok = scores(j + 2);
-        } else {
-          mma_commit(one, &bars.done);
+        for (int j = 0; j < n && ok; ++j) {
+          ok = warp_wait(&bars.ds_full, (tiles + j) & 1);
+          if (!ok) break;
+          tc_fence_after();
+          mma_columns<T, DP, kTile, 64>(one, dq_tmem, dp_tmem, k_tiles + spent.s * kTileBytes, kBox, j > 0);
+          mma_commit(one, &bars.k_empty[spent.s]);
+          spent.next(kKeys);
+          if (j + 1 < n) {
+            ok = products(j + 1);
+            if (ok && j + 2 < n) ok = scores(j + 2);
+          } else {
+            mma_commit(one, &bars.done);
+          }
         }
-        used.next(kKeys);
+        tiles += n;
+        ++used;
       }
     }
   } else {
     registers_up<192>();
-    const int group = warp >> 2, in_tile = threadIdx.x & 127, i = tile.token(in_tile);  // this thread's query
+    const int group = warp >> 2, in_tile = threadIdx.x & 127;  // this thread's row
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, columns = group * 64;  // and its warpgroup's columns
-    const Visible see = visible_keys(i < len.q ? len.position(i) : -1, len.kv, p.window, p.sinks);
     const float sl = fmaxf(p.scale * kLog2e, 1.1754944e-38f);
-    const int64_t row = (int64_t)((b * p.heads + tile.head) >> p.pack_log2) * gp.q_pad + (tile.first << p.pack_log2) + in_tile;
-    const float c = ds_factor<T>(gp, bk);
-    const F2 minus_lse = f2(gp.lse2[row], gp.lse2[row]), minus_delta = f2(gp.delta[row], gp.delta[row]);
+    uint32_t tiles = 0, used = 0;
     bool ok = true;
-    for (int j = 0; j < list.n; ++j) {
-      const int k0 = list.key(j) + columns;
-      const bool every = keys.every(list.key(j));
-      const uint32_t bits0 = every ? 0u : visible_bits32(see, k0), bits1 = every ? 0u : visible_bits32(see, k0 + 32);
-      ok = __all_sync(0xffffffffu, wait(&bars.s_full[j & 1], (j >> 1) & 1));
-      if (!ok) break;
-      tc_fence_after();
-      float pr[64];
-      {
-        uint32_t s[64];
-        const uint32_t s_at = tmem + lanes + (j & 1) * 128 + columns;
-        tmem_load32(s_at, s);
-        tmem_load32(s_at + 32, s + 32);
-        tmem_wait_loads();
-        scores_to_p(s, every, bits0, bits1, sl, [&](int) { return minus_lse; }, pr);
-      }
-      ok = __all_sync(0xffffffffu, wait(&bars.dp_full, j & 1));
-      if (!ok) break;
-      tc_fence_after();
-      const uint32_t dp_at = dp_tmem + lanes + columns;
-      uint32_t dp[64], ds[32];
-      tmem_load32(dp_at, dp);
-      tmem_load32(dp_at + 32, dp + 32);
-      tmem_wait_loads();
-      p_to_ds<T>(pr, dp, every, bits0, c, [&](int) { return minus_delta; }, ds);
-      p_to_ds<T>(pr + 32, dp + 32, every, bits1, c, [&](int) { return minus_delta; }, ds + 16);
-      tmem_store32(dp_at, ds);  // over this warpgroup's own columns
-      tmem_wait_stores();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bars.ds_full);
-    }
-    if (ok && list.n > 0) ok = __all_sync(0xffffffffu, wait(&bars.done, 0));
-    if (ok) {
-      // Each warpgroup brings out half of the dims.
-      tc_fence_after();
-      const bool some = list.n > 0 && see.hi > 0;
-#pragma unroll 1
-      for (int cc = group * (DP / 2); cc < (group + 1) * (DP / 2); cc += 32) {
-        uint32_t o[32];
-        if (list.n > 0) {
-          tmem_load32(dq_tmem + lanes + cc, o);
+    for (int round = 0; ok; ++round) {
+      const int index = next_unit(round);
+      if (index >= gp.units) break;
+      const Unit u(gp, index);
+      const int i = u.tile.token(in_tile);
+      const Visible see = visible_keys(i < u.len.q ? u.len.position(i) : -1, u.len.kv, p.window, p.sinks);
+      const int64_t row = (int64_t)((u.b * p.heads + u.tile.head) >> p.pack_log2) * gp.q_pad + (u.tile.first << p.pack_log2) + in_tile;
+      const float c = ds_factor<T>(gp, u.bk);
+      const F2 minus_lse = f2(gp.lse2[row], gp.lse2[row]), minus_delta = f2(gp.delta[row], gp.delta[row]);
+      for (int j = 0; j < u.list.n; ++j, ++tiles) {
+        const int k0 = u.list.key(j) + columns;
+        const bool every = u.keys.every(u.list.key(j));
+        const uint32_t bits0 = every ? 0u : visible_bits32(see, k0), bits1 = every ? 0u : visible_bits32(see, k0 + 32);
+        ok = __all_sync(0xffffffffu, wait(&bars.s_full[tiles & 1], (tiles >> 1) & 1));
+        if (!ok) break;
+        tc_fence_after();
+        float pr[64];
+        {
+          uint32_t s[64];
+          const uint32_t s_at = tmem + lanes + (tiles & 1) * 128 + columns;
+          tmem_load32(s_at, s);
+          tmem_load32(s_at + 32, s + 32);
           tmem_wait_loads();
+          scores_to_p(s, every, bits0, bits1, sl, [&](int) { return minus_lse; }, pr);
         }
-        stage32<T>(q_tile, in_tile, cc, o, p.scale / c, some);
+        ok = __all_sync(0xffffffffu, wait(&bars.dp_full, tiles & 1));
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t dp_at = dp_tmem + lanes + columns;
+        uint32_t dp[64], ds[32];
+        tmem_load32(dp_at, dp);
+        tmem_load32(dp_at + 32, dp + 32);
+        tmem_wait_loads();
+        p_to_ds<T>(pr, dp, every, bits0, c, [&](int) { return minus_delta; }, ds);
+        p_to_ds<T>(pr + 32, dp + 32, every, bits1, c, [&](int) { return minus_delta; }, ds + 16);
+        tmem_store32(dp_at, ds);  // over this warpgroup's own columns
+        tmem_wait_stores();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars.ds_full);
       }
-      fence_proxy_async_smem();
-    }
-    asm volatile("bar.sync 1, 256;" ::: "memory");
-    if (threadIdx.x == 0 && !*(volatile uint32_t*)&bars.gone) {
+      if (ok && u.list.n > 0) {
+        ok = __all_sync(0xffffffffu, wait(&bars.done, used & 1));
+        ++used;
+      }
+      // Bring the tile out, each warpgroup half of the dims. All warps go through
+      // both barriers, also those that gave up waiting.
+      if (threadIdx.x == 0) bulk_wait_read_all();  // the staging tile is free again
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      if (ok) {
+        tc_fence_after();
+        const bool some = u.list.n > 0 && see.hi > 0;
+#pragma unroll 1
+        for (int cc = group * (DP / 2); cc < (group + 1) * (DP / 2); cc += 32) {
+          uint32_t o[32];
+          if (u.list.n > 0) {
+            tmem_load32(dq_tmem + lanes + cc, o);
+            tmem_wait_loads();
+          }
+          stage32<T>(out_tile, in_tile, cc, o, p.scale / c, some);
+        }
+        tc_fence_before();
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0 && u.list.n > 0) mbar_arrive(&bars.dq_free);
+      }
+      if (!ok && lane == 0) *(volatile uint32_t*)&bars.given_up = 1;
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      ok = !*(volatile uint32_t*)&bars.given_up;
+      if (threadIdx.x == 0 && ok) {
 #pragma unroll
-      for (int box = 0; box < DP / 64; ++box)
-        if (box * 64 < p.head_dim) tma_store(&gp.out0, q_tile + box * kBox, box * 64, tile.head, tile.first, b);
-      bulk_commit();
-      bulk_wait_all();
+        for (int box = 0; box < DP / 64; ++box)
+          if (box * 64 < p.head_dim) tma_store(&gp.out0, out_tile + box * kBox, box * 64, u.tile.head, u.tile.first, u.b);
+        bulk_commit();
+      }
     }
+    if (threadIdx.x == 0) bulk_wait_all();
   }
   pdl_wait();
   finish_tmem(bars.gone, warp == 9, tmem, kColumns);
