@@ -435,7 +435,7 @@ int launch_backward(const cs_attention_args* a, const cs_attention_grads* g, con
   if (e != cudaSuccess) return fail_cuda(e, "attention backward, queries");
   if (s.partial_bytes) {
     const int64_t tiles = (int64_t)a->batch * a->kv_heads * (s.window_shares > 1 ? s.k_tiles : s.sink_tiles);
-    e = cs_host::launch(dkv_join_kernel(a->type, s.dim), dim3((unsigned)tiles, 4), 256, 0, stream, k);
+    e = cs_host::launch(dkv_join_kernel(a->type, s.dim), dim3((unsigned)tiles, 16), 256, 0, stream, k);
   }
   return e == cudaSuccess ? CS_OK : fail_cuda(e, "attention backward, joining the shares");
 }

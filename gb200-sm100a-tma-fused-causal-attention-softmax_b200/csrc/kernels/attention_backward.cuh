@@ -6,9 +6,10 @@
 //
 // Three kernels: the rows' delta; dK and dV with a tile of 128 keys per CTA
 // (every sum over queries and over the heads of a group stays in one CTA's
-// TMEM); dQ with a tile of 128 queries per CTA. Both recompute P and dP, seven
-// products instead of five, so that no sum crosses CTAs: no atomics, the same
-// bits every time, and no fp32 copy of dQ in memory.
+// TMEM, or goes to memory as parts that a fourth kernel adds in order); dQ with
+// a tile of 128 queries at a time. Both recompute P and dP, seven products
+// instead of five, so that no sum goes through atomics: the same bits every
+// time, and no fp32 copy of dQ in memory.
 //
 // Tiles of 128 x 128, one CTA an SM: two softmax warpgroups that take 64 columns
 // of each tile, a warp of TMA loads, a warp of products. S and dP are
@@ -24,7 +25,9 @@
 // keep their bits and none overflows. bf16 needs neither.
 //
 // Bound: at dim 128 a tile costs 4 x 512 tensor-core cycles in dK/dV, 3 x 512 in
-// dQ, and 1024 cycles of the exponential unit in each.
+// dQ, and 1024 cycles of the exponential unit in each. Measured (B200, ncu; 2 x
+// 4096 queries, 16 heads over 4, window 1024, dim 128, bf16): rows 16 us, dK/dV
+// 144 us (tensor pipe active 62%), dQ 111 us (52%).
 #pragma once
 
 #include "attention_tiles.cuh"
@@ -89,17 +92,24 @@ __global__ void __launch_bounds__(256) attention_rows_kernel(const __grid_consta
   for (int bh = blockIdx.y; bh < p.batch * p.heads; bh += gridDim.y) {
     const int b = bh / p.heads, h = bh - b * p.heads, hk = h / p.group;
     const Lengths len(p, b);
+    const int pos0 = len.position(0);
     uint4 ra[4], rg[4];
     float a[8], g[8], most = 0.f;
     if ((int)blockIdx.x < q_ctas) {
       const int i0 = blockIdx.x * kRowsPerCta + threadIdx.x / 16;
+      const uint16_t* po = p.o.at(b, i0, h) + d;
+      const uint16_t* pg = p.d_o.at(b, i0, h) + d;
+      const float* plse = p.lse + (int64_t)bh * p.q_len + i0;
+      const int64_t row0 = (int64_t)(bh >> p.pack_log2) * rp.q_pad + (h & ((1 << p.pack_log2) - 1));
       bool in[4];
+      float lse[4];
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int i = i0 + r * 16;
-        in[r] = i < len.q && len.position(i) >= 0;
-        ra[r] = in[r] && has ? load16(p.o.at(b, i, h) + d) : none;
-        rg[r] = in[r] && has ? load16(p.d_o.at(b, i, h) + d) : none;
+        in[r] = i < len.q && pos0 + i >= 0;
+        ra[r] = in[r] && has ? load16(po + r * 16 * p.o.token) : none;
+        rg[r] = in[r] && has ? load16(pg + r * 16 * p.d_o.token) : none;
+        lse[r] = in[r] && lane == 0 ? plse[r * 16] : -INFINITY;
       }
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
@@ -118,9 +128,8 @@ __global__ void __launch_bounds__(256) attention_rows_kernel(const __grid_consta
           if (T::kIsHalf) norm += __shfl_xor_sync(0xffffffffu, norm, x);
         }
         if (lane == 0 && i < tokens) {
-          const int64_t row = (int64_t)(bh >> p.pack_log2) * rp.q_pad + (i << p.pack_log2) + (h & ((1 << p.pack_log2) - 1));
-          const float lse = in[r] ? p.lse[(int64_t)bh * p.q_len + i] : -INFINITY;
-          rp.lse2[row] = lse == -INFINITY ? -INFINITY : -lse * kLog2e;
+          const int64_t row = row0 + (i << p.pack_log2);
+          rp.lse2[row] = lse[r] == -INFINITY ? -INFINITY : -lse[r] * kLog2e;
           rp.delta[row] = in[r] ? -dot : 0.f;
         }
         most = fmaxf(most, norm);
@@ -239,6 +248,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) attention_dq_kernel(const __g
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (smem_addr(aligned_smem) & 1023) {  // the swizzle needs it
     if (threadIdx.x == 0) atomicOr(p.status, kStatusTimeout);
+    pdl_wait();
     return;
   }
   if (warp == 8 && lane == 0) {
@@ -547,7 +557,8 @@ __device__ __forceinline__ void queries_of(const AttentionParams& p, const Lengt
 // While the warpgroups turn S(u + 1) into P(u + 1) (kept in registers) the tensor
 // core has dV(u), dP(u + 1) and dK(u); while they make dS(u + 1), S(u + 2).
 // Measured in cycles a tile: P over S, so that S(u + 1) waits for dV(u), 3400; P
-// and dS over dP, so that dP(u + 1) waits for dK(u), 3290; this one TODO.
+// and dS over dP, so that dP(u + 1) waits for dK(u), 3290; this one 2950, most of them
+// the warpgroups' (P 1300, dS 1200), the tensor core's four products 2160.
 template <typename T, int DP>
 __global__ void __launch_bounds__(kGradThreads, 1) attention_dkv_kernel(const __grid_constant__ GradParams gp) {
   using Smem = KeySmem<DP>;
