@@ -103,10 +103,11 @@ TileKernel tile_kernel(int type, int dim) {
   return dim == 64 ? &cs::attention_tiles_kernel<cs::BF16, 64> : &cs::attention_tiles_kernel<cs::BF16, 128>;
 }
 
+template <int kGroups>
 TileKernel tile_join_kernel(int type, int dim) {
   if (type == CS_TYPE_F16)
-    return dim == 64 ? &cs::attention_tiles_join_kernel<cs::F16, 64> : &cs::attention_tiles_join_kernel<cs::F16, 128>;
-  return dim == 64 ? &cs::attention_tiles_join_kernel<cs::BF16, 64> : &cs::attention_tiles_join_kernel<cs::BF16, 128>;
+    return dim == 64 ? &cs::attention_tiles_join_kernel<cs::F16, 64, kGroups> : &cs::attention_tiles_join_kernel<cs::F16, 128, kGroups>;
+  return dim == 64 ? &cs::attention_tiles_join_kernel<cs::BF16, 64, kGroups> : &cs::attention_tiles_join_kernel<cs::BF16, 128, kGroups>;
 }
 
 int tile_smem(int dim) { return dim == 64 ? cs::TileSmem<64>::kBytes : cs::TileSmem<128>::kBytes; }
@@ -214,32 +215,47 @@ int check_workspace(const void* workspace, size_t bytes, int64_t need) {
 
 // Few queries: the kernel for single tokens. Its launch shape.
 struct TokenShape {
-  int rows, dim, blocks, splits;  // rows: 8 or 16 of a block; blocks: per kv head
+  int rows, dim, splits;  // rows: 8 or 16
   int64_t ctas;
   int64_t part_bytes, stats_bytes;
 };
 
-constexpr int kTokenRows = 16;         // most rows of a kv head, (query, head) pairs, that take it
 constexpr int64_t kTokenKeys = 128;    // of a CTA, at least: 2 steps a warp
 constexpr int kTokenResident[2][2] = {{4, 3}, {3, 2}};  // CTAs an SM: dim 64, 128; 8, 16 rows
 
-bool few_queries(const cs_attention_args* a) { return (int64_t)a->q_len * (a->heads / a->kv_heads) <= kTokenRows; }
+// Which calls those are, by the rows of a kv head, (query, head) pairs, and by the
+// kv heads. Up to 8 rows: all. Up to 16, whose accumulators leave the kernel two
+// CTAs an SM: while the kv heads are fewer than the SMs, so that their keys are
+// split (4 x 2 queries over 16384 keys, 32 heads over 4, dim 128: 29.1 us, tiles
+// 36.4; 64 x 2 over 4096: 102.9, tiles 88.1). More rows would read the keys more
+// than once (8 x 8 over 1024: 13.0, tiles 9.4).
+bool few_queries(const cs_attention_args* a, int sms) {
+  const int64_t rows = (int64_t)a->q_len * (a->heads / a->kv_heads);
+  return rows <= 8 || (rows <= 16 && (int64_t)a->batch * a->kv_heads < sms);
+}
 
 TokenShape token_shape(const cs_attention_args* a, int sms) {
   TokenShape s{};
   const int64_t rows = (int64_t)a->q_len * (a->heads / a->kv_heads);
   s.rows = rows <= 8 ? 8 : 16;
   s.dim = a->head_dim <= 64 ? 64 : 128;
-  s.blocks = (int)((rows + s.rows - 1) / s.rows);
-  const int64_t base = (int64_t)a->batch * a->kv_heads * s.blocks;
+  const int64_t base = (int64_t)a->batch * a->kv_heads;
   int64_t keys = a->kv_len;
   if (a->window) keys = std::min<int64_t>(keys, (int64_t)a->window + a->q_len + a->sinks + 32);
-  // Four rounds of resident CTAs or more for an even end, else one.
+  // Rounds of resident CTAs times a CTA's time, in keys: a CTA starts and ends in
+  // the time of about 150. Splits that fill whole rounds are the candidates.
+  // (64 tokens of 32 heads over 4, 4096 keys: 5 splits 89.5 us, 7 97.3, 2 114; 16
+  // tokens, 8 kv heads: 3 splits 46.2, 4 60.4, 14 55.8.)
   const int64_t wave = (int64_t)sms * kTokenResident[s.dim == 128][s.rows == 16];
-  const int64_t most = std::min<int64_t>(keys / kTokenKeys, cs::kMaxSplits);
-  int64_t splits = (4 * wave + base - 1) / base;
-  if (splits > most) splits = std::min(most, wave / base);
-  s.splits = (int)std::max<int64_t>(1, splits);
+  const int64_t most = std::max<int64_t>(1, std::min<int64_t>(keys / kTokenKeys, cs::kMaxSplits));
+  int64_t splits = 1, best = INT64_MAX;
+  const int64_t rounds = (base + wave - 1) / wave;
+  for (int64_t w = rounds; w < rounds + 8; ++w) {
+    const int64_t n = std::min(most, std::max<int64_t>(1, w * wave / base));
+    const int64_t cost = (base * n + wave - 1) / wave * (keys / n + 150);
+    if (cost < best) best = cost, splits = n;
+  }
+  s.splits = (int)splits;
   s.ctas = base * s.splits;
   if (s.splits > 1) {
     s.part_bytes = s.ctas * s.rows * s.dim * 4;
@@ -262,8 +278,7 @@ int launch_tokens(const cs_attention_args* a, const cs::AttentionParams& p, cons
   t.part_o = static_cast<float*>(workspace);
   t.part_stats = reinterpret_cast<float*>(static_cast<char*>(workspace) + s.part_bytes);
   t.splits = s.splits;
-  t.blocks = s.blocks;
-  t.block_rows = s.rows;
+  t.rows = s.rows;
   t.dim_pad = s.dim;
   if (s.ctas * s.rows > kI32Max) return fail(CS_ERR_WRONG_LENGTH, "%lld CTAs", (long long)s.ctas);
   const bool half = a->type == CS_TYPE_F16;
@@ -279,15 +294,17 @@ int launch_tokens(const cs_attention_args* a, const cs::AttentionParams& p, cons
   return e == cudaSuccess ? CS_OK : fail_cuda(e, "attention, joining the splits");
 }
 
-// Query tiles and, where they are too few for two CTAs an SM, the CTAs that share
-// one's keys: at least kTileKeys key tiles each, and only from four times as many
-// on (joining takes about 3 us, a key tile 1.5).
+// Query tiles and, where they are too few for the SMs, the CTAs that share one's
+// keys. Below 16 key tiles one CTA an SM and none split below 5: a CTA takes
+// about 2 us a key tile and joining 3 (64 queries over 1100 keys, 8 heads of one
+// kv head: 9 CTAs a tile 13.0 us, 1 22.1; 4096 queries, 4 heads, window 1024, two
+// CTAs an SM: 23.1, one 19.6). From 16 on two an SM with at least 4 key tiles
+// each (1 x 2000, 4 heads: 16.6 us, one an SM 21.0; 8 x 17 queries over 4096: 18.3
+// us, with 3 key tiles 24.9).
 struct TileShape {
   int dim, q_tiles, splits;
   int64_t ctas, part_bytes, stats_bytes;
 };
-
-constexpr int64_t kTileKeys = 4;
 
 TileShape tile_shape(const cs_attention_args* a, int sms) {
   TileShape s{};
@@ -298,7 +315,8 @@ TileShape tile_shape(const cs_attention_args* a, int sms) {
   int64_t keys = ((int64_t)a->kv_len + cs::kTile - 1) / cs::kTile;
   if (a->window)
     keys = std::min(keys, ((int64_t)a->window + tokens + cs::kTile - 1) / cs::kTile + ((int64_t)a->sinks + cs::kTile - 1) / cs::kTile);
-  s.splits = keys < 4 * kTileKeys ? 1 : (int)std::max<int64_t>(1, std::min(2 * (int64_t)sms / base, keys / kTileKeys));
+  const bool few = keys < 16;
+  s.splits = keys < 5 ? 1 : (int)std::max<int64_t>(1, std::min((few ? 1 : 2) * (int64_t)sms / base, few ? keys : keys / 4));
   s.ctas = base * s.splits;
   if (s.splits > 1) {
     s.part_bytes = s.ctas * cs::kTile * s.dim * 4;
@@ -324,8 +342,13 @@ int launch_tiles(const cs_attention_args* a, const cs::AttentionParams& p, const
                                   stream, t);
   if (e != cudaSuccess) return fail_cuda(e, "attention, tiles");
   if (s.splits == 1) return CS_OK;
-  e = cs_host::launch(tile_join_kernel(a->type, s.dim), dim3((unsigned)(s.ctas / s.splits), (unsigned)s.dim / 8), 256, 0,
-                      stream, t);
+  const unsigned tiles = (unsigned)(s.ctas / s.splits), dims = (unsigned)s.dim;
+  if (s.splits > 64)
+    e = cs_host::launch(tile_join_kernel<16>(a->type, s.dim), dim3(tiles, 2 * dims), 256, 0, stream, t);
+  else if (s.splits > 8)
+    e = cs_host::launch(tile_join_kernel<4>(a->type, s.dim), dim3(tiles, dims / 2), 256, 0, stream, t);
+  else
+    e = cs_host::launch(tile_join_kernel<1>(a->type, s.dim), dim3(tiles, dims / 8), 256, 0, stream, t);
   return e == cudaSuccess ? CS_OK : fail_cuda(e, "attention, joining the splits");
 }
 
@@ -449,7 +472,7 @@ int64_t cs_attention_workspace(const cs_attention_args* args) {
   cs_host::Device d;
   if (!rc) rc = cs_host::current_device(&d);
   if (rc) return rc;
-  if (few_queries(args)) {
+  if (few_queries(args, d.sms)) {
     const TokenShape s = token_shape(args, d.sms);
     return s.part_bytes + s.stats_bytes;
   }
@@ -464,7 +487,7 @@ int cs_attention(const cs_attention_args* args, void* workspace, size_t workspac
   cs_host::Device d;
   rc = params_of(args, &p, &d);
   if (rc) return rc;
-  if (few_queries(args)) {
+  if (few_queries(args, d.sms)) {
     const TokenShape s = token_shape(args, d.sms);
     rc = check_workspace(workspace, workspace_bytes, s.part_bytes + s.stats_bytes);
     return rc ? rc : launch_tokens(args, p, s, workspace, stream);

@@ -371,7 +371,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) attention_dq_kernel(const __g
         auto scores = [&](int j) {  // S(j)
           uint8_t* k_tile = k_tiles + ring.s * kTileBytes;
           if (!warp_wait(&bars.k_full[ring.s], ring.ph)) return false;
-          clear_unseen<DP>(seen, k_tile, u.list.key(j), lane);
+          clear_unseen<DP>(seen, k_tile, u.list.key(j), p.kv_len, lane);
           const uint32_t buffer = (tiles + j) & 1;
           mma_rows<T, DP, kTile>(one, tmem + buffer * 128, q_tile, kBox, k_tile, kBox);
           mma_commit(one, &bars.s_full[buffer]);
@@ -677,11 +677,9 @@ __global__ void __launch_bounds__(kGradThreads, 1) attention_dkv_kernel(const __
         auto clean = [&](uint8_t* tile, int& sub) {
           const int i0 = units.q_first + sub * units.step;
           if (++sub == units.per_pack) sub = 0;
-          if (i0 < q_lo || i0 + units.step > len.q)
-            clear_rows<DP>(tile, lane, [&](int r) {
-              const int i = i0 + (r >> p.pack_log2);
-              return i >= q_lo && i < len.q;
-            });
+          const int first = column_of(q_lo, i0, p.pack_log2), end = column_of(len.q, i0, p.pack_log2);
+          if (first > 0 || (end < kTile && len.q < p.q_len))  // (the copy wrote zeros behind q_len)
+            clear_rows<DP>(tile, lane, [&](int r) { return r >= first && r < end; });
         };
         auto scores = [&](int u) {  // S(u)
           uint8_t* q_tile = q_tiles + q_next.s * kTileBytes;

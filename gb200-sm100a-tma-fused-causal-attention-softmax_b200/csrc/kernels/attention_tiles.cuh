@@ -108,15 +108,15 @@ __device__ __forceinline__ uint32_t visible_bits32(const Visible& v, int k0) {
 }
 
 // Zero the rows of a staged tile for which keep(row) is false: they may hold
-// NaN, and 0 times NaN is NaN. One warp.
+// NaN, and 0 times NaN is NaN. One warp, 4 rows at a time.
 template <int DP, typename Keep>
 __device__ __forceinline__ void clear_rows(uint8_t* tile, int lane, Keep keep) {
+  tile += lane * 16;
 #pragma unroll 1
-  for (int r = 0; r < kTile; ++r) {
+  for (int r = lane >> 3; r < kTile; r += 4, tile += 512) {
     if (keep(r)) continue;
 #pragma unroll
-    for (int box = 0; box < DP / 64; ++box)
-      if (lane < 8) *reinterpret_cast<uint4*>(tile + box * (kTile * 128) + r * 128 + lane * 16) = make_uint4(0, 0, 0, 0);
+    for (int box = 0; box < DP / 64; ++box) *reinterpret_cast<uint4*>(tile + box * (kTile * 128)) = make_uint4(0, 0, 0, 0);
   }
   fence_proxy_async_smem();
   __syncwarp();
@@ -124,8 +124,9 @@ __device__ __forceinline__ void clear_rows(uint8_t* tile, int lane, Keep keep) {
 
 // Keys (or values) k0.. of which no query of the sequence sees some.
 template <int DP>
-__device__ __forceinline__ void clear_unseen(const Visible& seen, uint8_t* tile, int k0, int lane) {
-  if (k0 + kTile <= seen.s_end || (k0 >= seen.lo && k0 + kTile <= seen.hi)) return;
+__device__ __forceinline__ void clear_unseen(const Visible& seen, uint8_t* tile, int k0, int kv_len, int lane) {
+  const int end = min(k0 + kTile, kv_len);  // the copy wrote zeros from here on
+  if (end <= seen.s_end || (k0 >= seen.lo && end <= seen.hi)) return;
   clear_rows<DP>(tile, lane, [&](int r) { return sees(seen, k0 + r); });
 }
 
@@ -288,7 +289,7 @@ __global__ void __launch_bounds__(kTileThreads, 2) attention_tiles_kernel(const 
         const int v_slot = ring.s;
         if (j > 0) {
           if (!warp_wait(&bars.kv_full[v_slot], ring.ph)) break;
-          clear_unseen<DP>(seen, stages + v_slot * kTileBytes, list.key(j0 + j - 1), lane);
+          clear_unseen<DP>(seen, stages + v_slot * kTileBytes, list.key(j0 + j - 1), p.kv_len, lane);
           ring.next(kStages);
         }
         if (j < n && !warp_wait(&bars.kv_full[ring.s], ring.ph)) break;
@@ -408,28 +409,34 @@ __global__ void __launch_bounds__(kTileThreads, 2) attention_tiles_kernel(const 
   finish_tmem(bars.gone, warp == 5, tmem, kColumns);
 }
 
-// Joins the CTAs of a query tile: grid.x tiles as in the kernel above, grid.y 8
-// dims each, a thread 4 dims of a row.
-template <typename T, int DP>
+// Joins the CTAs of a query tile. kGroups threads take the CTAs of a row in
+// turn, 4 dims each; grid.x tiles as in the kernel above, grid.y the rest of the
+// rows and dims. (8 queries of 8 heads over 65536 keys, 128 CTAs a tile: 52.6 us with
+// one thread a row, 27.9 with 4, 21.0 with 16; 128 over 16384, 32 CTAs: 24.8, 19.0,
+// 24.2; 288 over 16384, 16 CTAs: 28.3, 28.1, 38.8.)
+template <typename T, int DP, int kGroups>
 __global__ void __launch_bounds__(256) attention_tiles_join_kernel(const __grid_constant__ TileParams tp) {
   constexpr float kShift = T::kIsHalf ? 7.f : 0.f;
+  constexpr int kRows = kGroups == 1 ? kTile : 256 / kGroups, kQuads = 256 / kRows / kGroups;
+  __shared__ float sm[kGroups == 1 ? 1 : kGroups][kRows][6];
   const AttentionParams& p = tp.a;
   const int unit = p.by_heads.div(blockIdx.x), bk = blockIdx.x - unit * p.by_heads.by, b = p.by_kv_heads.div(bk), hk = bk - b * p.kv_heads;
-  const int row = threadIdx.x & 127, quad = blockIdx.y * 2 + (threadIdx.x >> 7);
+  const int in_cta = threadIdx.x % kRows, group = threadIdx.x / kRows % kGroups;
+  const int row = blockIdx.y % (kTile / kRows) * kRows + in_cta;
+  const int quad = blockIdx.y / (kTile / kRows) * kQuads + threadIdx.x / (kRows * kGroups);
   const QueryTile tile(p, hk, unit, tp.q_tiles);
   const int i = tile.token(row), h = tile.head_of(row);
   pdl_wait();
-  if (i >= p.q_len) return;
   const int64_t first = (int64_t)unit * tp.splits * p.by_heads.by + bk;  // CTA of split 0; the next is by_heads.by further
   const float2* stats = reinterpret_cast<const float2*>(tp.part_stats) + first * kTile + row;
   const float4* part = reinterpret_cast<const float4*>(tp.part_o) + first * (kTile * DP / 4) + quad * kTile + row;
   const int64_t step = (int64_t)p.by_heads.by * kTile;
   float top = -INFINITY, sum = 0.f;
 #pragma unroll 4
-  for (int s = 0; s < tp.splits; ++s) top = fmaxf(top, stats[s * step].x);
+  for (int s = group; s < tp.splits; s += kGroups) top = fmaxf(top, stats[s * step].x);
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-  for (int s = 0; s < tp.splits; ++s) {
+  for (int s = group; s < tp.splits; s += kGroups) {
     const float2 st = stats[s * step];
     const float4 v = part[s * step * (DP / 4)];
     if (st.x == -INFINITY) continue;  // saw no key
@@ -440,6 +447,33 @@ __global__ void __launch_bounds__(256) attention_tiles_join_kernel(const __grid_
     o.z = __fmaf_rn(f, v.z, o.z);
     o.w = __fmaf_rn(f, v.w, o.w);
   }
+  if (kGroups > 1) {
+    float* mine = sm[group][in_cta];
+    mine[0] = top;
+    mine[1] = sum;
+    mine[2] = o.x;
+    mine[3] = o.y;
+    mine[4] = o.z;
+    mine[5] = o.w;
+    __syncthreads();
+    if (group) return;
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) top = fmaxf(top, sm[g][in_cta][0]);
+    sum = 0.f;
+    o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) {
+      const float* other = sm[g][in_cta];
+      if (other[0] == -INFINITY) continue;
+      const float f = ex2(other[0] - top);
+      sum = __fmaf_rn(f, other[1], sum);
+      o.x = __fmaf_rn(f, other[2], o.x);
+      o.y = __fmaf_rn(f, other[3], o.y);
+      o.z = __fmaf_rn(f, other[4], o.z);
+      o.w = __fmaf_rn(f, other[5], o.w);
+    }
+  }
+  if (i >= p.q_len) return;
   const float inv = sum == 0.f ? 0.f : rcp_rn(sum);
   if (quad * 4 < p.head_dim)
     *reinterpret_cast<uint2*>(p.o.at(b, i, h) + quad * 4) = make_uint2(T::pack(o.x * inv, o.y * inv), T::pack(o.z * inv, o.w * inv));

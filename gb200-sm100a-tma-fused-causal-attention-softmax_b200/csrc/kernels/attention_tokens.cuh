@@ -1,10 +1,9 @@
 // Attention of few queries over many keys: single tokens reading a cache.
 //
-// The query rows that share a kv head, (query, head) pairs, form blocks of
-// 8 NT rows; a CTA reads a share ("split") of the block's visible keys and its
-// warps take 16 keys in turn, each with its own running maximum, sum and
+// The query rows that share a kv head, (query, head) pairs, are at most 8 NT;
+// a CTA reads a share ("split") of their visible keys and its warps take 16 keys in turn, each with its own running maximum, sum and
 // output; warps are joined in shared memory, splits by a second kernel.
-// Bound: HBM, each visible key and value read once per row block.
+// Bound: HBM, each visible key and value read once.
 //
 // Products run on mma m16n8k16 with keys (then dims) as the 16 rows and the
 // query rows as the 8 columns: 8 rows fill it, so one token of a group of up to
@@ -31,11 +30,10 @@ constexpr float kMaxLag = 8.f;  // in units of log2
 
 struct TokenParams {
   AttentionParams a;
-  float* part_o;      // [block, split, 8 NT, DP]
-  float* part_stats;  // [block, split, 8 NT, 2]: maximum (log2 units), sum
+  float* part_o;      // [kv head, split, 8 NT, DP]
+  float* part_stats;  // [kv head, split, 8 NT, 2]: maximum (log2 units), sum
   int32_t splits;
-  int32_t blocks;     // row blocks per kv head
-  int32_t block_rows; // 8 NT
+  int32_t rows;       // 8 NT
   int32_t dim_pad;    // DP
 };
 
@@ -59,16 +57,15 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t v) {
   return r;
 }
 
-// The steps of 16 keys that hold a row block's visible keys, numbered densely.
+// The steps of 16 keys that hold the visible keys, numbered densely.
 struct KeySteps {
-  Visible u;  // union over the block's rows
+  Visible u;  // union over the rows
   int32_t n_sink, w_beg, n;
-  __device__ __forceinline__ KeySteps(const AttentionParams& p, const Lengths& len, int i0, int i1) {
+  __device__ __forceinline__ KeySteps(const AttentionParams& p, const Lengths& len) {
     u.s_end = u.lo = u.hi = 0;
-    i1 = min(i1, len.q - 1);
-    if (i0 <= i1) {
-      const Visible first = visible_keys(len.position(i0), len.kv, p.window, p.sinks);
-      u = visible_keys(len.position(i1), len.kv, p.window, p.sinks);
+    if (len.q > 0) {
+      const Visible first = visible_keys(len.position(0), len.kv, p.window, p.sinks);
+      u = visible_keys(len.position(len.q - 1), len.kv, p.window, p.sinks);
       u.lo = min(u.lo, first.lo);
       u.s_end = min(u.s_end, u.lo);
     }
@@ -88,14 +85,12 @@ __global__ void __launch_bounds__(kTokenWarps * 32, NT == 1 ? 3 : 2) attention_t
   __shared__ float sm_m[kTokenWarps][kRows], sm_l[kTokenWarps][kRows];
   const AttentionParams& p = tp.a;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-  const int block = blockIdx.x / tp.splits, split = blockIdx.x - block * tp.splits;
-  const int bk = block / tp.blocks, rb = block - bk * tp.blocks;
+  const int bk = blockIdx.x / tp.splits, split = blockIdx.x - bk * tp.splits;
   const int b = bk / p.kv_heads, hk = bk - b * p.kv_heads;
-  const int rows = p.q_len * p.group, row0 = rb * kRows;
+  const int rows = p.q_len * p.group;
   pdl_wait();
   const Lengths len(p, b);
-  const int last = min(row0 + kRows, rows) - 1;
-  const KeySteps steps(p, len, row0 / p.group, last / p.group);
+  const KeySteps steps(p, len);
   const int begin = (int)((int64_t)steps.n * split / tp.splits), end = (int)((int64_t)steps.n * (split + 1) / tp.splits);
   const float sl = p.scale * kLog2e;
 
@@ -105,14 +100,14 @@ __global__ void __launch_bounds__(kTokenWarps * 32, NT == 1 ? 3 : 2) attention_t
   Visible see[NT][2];
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
-    const int r = row0 + n * 8 + g, i = r / p.group;
+    const int r = n * 8 + g, i = r / p.group;
     const uint16_t* src = p.q.at(b, i, hk * p.group + r - i * p.group);
 #pragma unroll
     for (int c = 0; c < KC; ++c)
       q[n][c] = r < rows && i < len.q && c * 32 + t * 8 < p.head_dim ? load16(src + c * 32 + t * 8) : make_uint4(0, 0, 0, 0);
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      const int col = row0 + n * 8 + 2 * t + e, ci = col / p.group;
+      const int col = n * 8 + 2 * t + e, ci = col / p.group;
       see[n][e] = visible_keys(col < rows && ci < len.q ? len.position(ci) : -1, len.kv, p.window, p.sinks);
     }
   }
@@ -244,7 +239,7 @@ __global__ void __launch_bounds__(kTokenWarps * 32, NT == 1 ? 3 : 2) attention_t
     }
   __syncthreads();
   constexpr int kLanes = DP / 4;  // 4 dims a thread
-  for (int r = threadIdx.x / kLanes; r < kRows && row0 + r < rows; r += kTokenWarps * 32 / kLanes) {
+  for (int r = threadIdx.x / kLanes; r < rows; r += kTokenWarps * 32 / kLanes) {
     const int d = (threadIdx.x % kLanes) * 4;
     float top = -INFINITY;
 #pragma unroll
@@ -267,7 +262,7 @@ __global__ void __launch_bounds__(kTokenWarps * 32, NT == 1 ? 3 : 2) attention_t
       // -infinity: no key seen; a NaN among the scores goes on in the sum.
       if (d == 0) *reinterpret_cast<float2*>(tp.part_stats + at * 2) = make_float2(top == -INFINITY && sum != 0.f ? 0.f : top, sum);
     } else {
-      const int i = (row0 + r) / p.group, h = hk * p.group + (row0 + r) - i * p.group;
+      const int i = r / p.group, h = hk * p.group + r - i * p.group;
       const float inv = sum == 0.f ? 0.f : rcp_rn(sum);
       if (d < p.head_dim)
         *reinterpret_cast<uint2*>(p.o.at(b, i, h) + d) = make_uint2(T::pack(v.x * inv, v.y * inv), T::pack(v.z * inv, v.w * inv));
@@ -289,15 +284,14 @@ __global__ void __launch_bounds__(kWarps * 32) attention_join_kernel(const __gri
   __shared__ float weight[kMaxSplits], sm_v[kWarps][128 + 4], words[kWarps];
   const AttentionParams& p = tp.a;
   const int rows = p.q_len * p.group, bk = blockIdx.x / rows, row = blockIdx.x - bk * rows;
-  const int rb = row / tp.block_rows, r = row - rb * tp.block_rows, block = bk * tp.blocks + rb;
   const int b = bk / p.kv_heads, hk = bk - b * p.kv_heads;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, d = lane * 4;
-  const int64_t first = (int64_t)block * tp.splits * tp.block_rows + r;  // of the splits' rows
+  const int64_t first = (int64_t)bk * tp.splits * tp.rows + row;  // of the splits' rows
   pdl_wait();
   // The maximum, the weights, the sum.
   float top = -INFINITY;
   for (int s = threadIdx.x; s < tp.splits; s += kJoinThreads) {
-    weight[s] = tp.part_stats[(first + (int64_t)s * tp.block_rows) * 2];
+    weight[s] = tp.part_stats[(first + (int64_t)s * tp.rows) * 2];
     top = fmaxf(top, weight[s]);
   }
   top = redux_max(top);
@@ -310,7 +304,7 @@ __global__ void __launch_bounds__(kWarps * 32) attention_join_kernel(const __gri
   for (int s = threadIdx.x; s < tp.splits; s += kJoinThreads) {
     const float f = weight[s] == -INFINITY ? 0.f : ex2(weight[s] - top);
     weight[s] = f;
-    if (f != 0.f) sum = __fmaf_rn(f, tp.part_stats[(first + (int64_t)s * tp.block_rows) * 2 + 1], sum);
+    if (f != 0.f) sum = __fmaf_rn(f, tp.part_stats[(first + (int64_t)s * tp.rows) * 2 + 1], sum);
   }
   sum = warp_sum(sum);
   if (lane == 0) words[warp] = sum;
@@ -322,7 +316,7 @@ __global__ void __launch_bounds__(kWarps * 32) attention_join_kernel(const __gri
   if (d < tp.dim_pad) {
 #pragma unroll 8
     for (int s = warp; s < tp.splits; s += kWarps) {
-      const float4 x = *reinterpret_cast<const float4*>(tp.part_o + (first + (int64_t)s * tp.block_rows) * tp.dim_pad + d);
+      const float4 x = *reinterpret_cast<const float4*>(tp.part_o + (first + (int64_t)s * tp.rows) * tp.dim_pad + d);
       const float f = weight[s];
       if (f != 0.f) {  // a split without keys holds nothing
         v.x = __fmaf_rn(f, x.x, v.x);
