@@ -58,7 +58,17 @@ int check_args(const cs_attention_args* a) {
   if (!rc) rc = check_tensor("k", a->k, a->batch, a->kv_len, a->kv_heads, a->head_dim);
   if (!rc) rc = check_tensor("v", a->v, a->batch, a->kv_len, a->kv_heads, a->head_dim);
   if (!rc) rc = check_tensor("o", a->o, a->batch, a->q_len, a->heads, a->head_dim);
-  return rc;
+  if (rc) return rc;
+  for (const void* word : {(const void*)a->q_lens, (const void*)a->kv_lens, (const void*)a->lse})
+    if (reinterpret_cast<uintptr_t>(word) & 3) return fail(CS_ERR_ALIGNMENT, "q_lens, kv_lens and lse must be 4-byte aligned");
+  return CS_OK;
+}
+
+// Outputs overlap neither inputs nor each other; what is plainly wrong is refused.
+int check_outputs(const cs_attention_args* a) {
+  for (const void* in : {a->q.data, a->k.data, a->v.data})
+    if (in == a->o.data) return fail(CS_ERR_ARG, "the output is an input");
+  return CS_OK;
 }
 
 int check_grads(const cs_attention_args* a, const cs_attention_grads* g) {
@@ -69,6 +79,15 @@ int check_grads(const cs_attention_args* a, const cs_attention_grads* g) {
   if (!rc) rc = check_tensor("dk", g->dk, a->batch, a->kv_len, a->kv_heads, a->head_dim);
   if (!rc) rc = check_tensor("dv", g->dv, a->batch, a->kv_len, a->kv_heads, a->head_dim);
   return rc;
+}
+
+int check_grad_outputs(const cs_attention_args* a, const cs_attention_grads* g) {
+  const void* outs[] = {g->dq.data, g->dk.data, g->dv.data};
+  for (const void* in : {a->q.data, a->k.data, a->v.data, a->o.data, g->d_o.data})
+    for (const void* out : outs)
+      if (in == out) return fail(CS_ERR_ARG, "a gradient's tensor is an input");
+  if (outs[0] == outs[1] || outs[0] == outs[2] || outs[1] == outs[2]) return fail(CS_ERR_ARG, "two gradients share a tensor");
+  return CS_OK;
 }
 
 cs::Strided strided(const cs_tensor& t) {
@@ -482,6 +501,7 @@ int64_t cs_attention_workspace(const cs_attention_args* args) {
 
 int cs_attention(const cs_attention_args* args, void* workspace, size_t workspace_bytes, void* stream) {
   int rc = check_args(args);
+  if (!rc) rc = check_outputs(args);
   if (rc) return rc;
   cs::AttentionParams p{};
   cs_host::Device d;
@@ -512,6 +532,7 @@ int cs_attention_backward(const cs_attention_args* args, const cs_attention_grad
   int rc = check_args(args);
   if (!rc) rc = check_grads(args, grads);
   if (!rc) rc = check_workspace(workspace, workspace_bytes, 16);
+  if (!rc) rc = check_grad_outputs(args, grads);
   if (rc) return rc;
   cs::AttentionParams p{};
   cs_host::Device d;

@@ -105,13 +105,35 @@ int64_t max_vectors(const cs_bias_args* a) {
   return n;
 }
 
-// CTAs of a matrix: enough that the launch holds about four rounds of resident
-// CTAs (rows differ in length), no more than its rows fill.
-int ctas_per_matrix(const cs_bias_args* a, int sms, int groups) {
-  const int64_t matrices = (int64_t)a->batch * a->heads;
-  const int64_t want = ((int64_t)sms * 8 * 4 + matrices - 1) / matrices;
-  const int64_t most = ((int64_t)a->rows + groups - 1) / groups;
-  return (int)std::max<int64_t>(1, std::min(want, most));
+// CTAs of a matrix. The launch takes rounds of resident CTAs, and a CTA the time
+// of its groups' rows and of its start and end, `ends` in quarters of a row (the
+// backward adds up its groups' arrays by distance). Numbers that fill whole rounds are
+// the candidates, and within 5% the one with more rounds, whose CTAs end more
+// evenly. Against four rounds always: backward 1024 x 512^2 287 us, 391; 128 x
+// 1024^2 159, 205; 16 x 2048^2 66, 133; 24 x 257^2 13, 20; forward 16 x 2048^2 47, 55.
+int ctas_per_matrix(const cs_bias_args* a, int64_t resident, int groups, int ends) {
+  const int64_t matrices = (int64_t)a->batch * a->heads, most = ((int64_t)a->rows + groups - 1) / groups;
+  const int64_t rounds = (matrices + resident - 1) / resident;
+  int64_t turns = most, best = INT64_MAX;  // rows of a group
+  for (int64_t w = rounds; w < rounds + 8; ++w) {
+    const int64_t n = std::min(most, std::max<int64_t>(1, w * resident / matrices)), t = (most + n - 1) / n;
+    const int64_t cost = (matrices * n + resident - 1) / resident * (4 * t + ends);
+    if (best == INT64_MAX || 20 * cost <= 21 * best) turns = t;
+    best = std::min(best, cost);
+  }
+  return (int)((most + turns - 1) / turns);
+}
+
+using Kernel = void (*)(cs::BiasParams);
+
+Kernel forward_kernel(int type, bool staged) {
+  return type == CS_TYPE_F16 ? (staged ? &cs::bias_softmax_kernel<cs::F16, true> : &cs::bias_softmax_kernel<cs::F16, false>)
+                             : (staged ? &cs::bias_softmax_kernel<cs::BF16, true> : &cs::bias_softmax_kernel<cs::BF16, false>);
+}
+
+Kernel backward_kernel(int type, bool staged) {
+  return type == CS_TYPE_F16 ? (staged ? &cs::bias_backward_kernel<cs::F16, true> : &cs::bias_backward_kernel<cs::F16, false>)
+                             : (staged ? &cs::bias_backward_kernel<cs::BF16, true> : &cs::bias_backward_kernel<cs::BF16, false>);
 }
 
 // Few lanes a row keep the work that each row costs a warp (its geometry, the
@@ -126,8 +148,9 @@ int ctas_per_matrix(const cs_bias_args* a, int sms, int groups) {
 constexpr int64_t kTargetSmem = 72 * 1024;
 
 // matrices: 1 (scores) or 2 (probabilities and their gradient); words: fp32
-// words a CTA needs besides, per group and once.
-Shape shape_of(const cs_bias_args* a, const cs_host::Device& d, int matrices, int64_t group_words, int64_t words) {
+// words a CTA needs besides, per group and once; kernels: the staged one and the other.
+int shape_of(const cs_bias_args* a, const cs_host::Device& d, int matrices, int64_t group_words, int64_t words, Kernel staged,
+             Kernel direct, Shape* shape) {
   const int64_t nv = max_vectors(a);
   auto bytes = [&](int lanes) {
     const int64_t block = std::max(cs::kBiasThreads, lanes), groups = block / lanes;
@@ -143,28 +166,14 @@ Shape shape_of(const cs_bias_args* a, const cs_host::Device& d, int matrices, in
     s.smem -= (size_t)(s.block / s.lanes * nv * 32 * matrices);
     s.slots = 0;
   }
-  s.ctas = ctas_per_matrix(a, d.sms, s.block / s.lanes);
-  return s;
-}
-
-Shape forward_shape(const cs_bias_args* a, const cs_host::Device& d) {
-  return shape_of(a, d, 1, 0, cs::bias_slots(a->bucket_starts[a->buckets - 1]));
-}
-
-Shape backward_shape(const cs_bias_args* a, const cs_host::Device& d) {
-  return shape_of(a, d, 2, cs::bias_slots(a->bucket_starts[a->buckets - 1]), 0);
-}
-
-using Kernel = void (*)(cs::BiasParams);
-
-Kernel forward_kernel(int type, bool staged) {
-  return type == CS_TYPE_F16 ? (staged ? &cs::bias_softmax_kernel<cs::F16, true> : &cs::bias_softmax_kernel<cs::F16, false>)
-                             : (staged ? &cs::bias_softmax_kernel<cs::BF16, true> : &cs::bias_softmax_kernel<cs::BF16, false>);
-}
-
-Kernel backward_kernel(int type, bool staged) {
-  return type == CS_TYPE_F16 ? (staged ? &cs::bias_backward_kernel<cs::F16, true> : &cs::bias_backward_kernel<cs::F16, false>)
-                             : (staged ? &cs::bias_backward_kernel<cs::BF16, true> : &cs::bias_backward_kernel<cs::BF16, false>);
+  int per_sm = 0;
+  const cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(
+      &per_sm, reinterpret_cast<const void*>(s.slots ? staged : direct), s.block, s.smem);
+  if (e != cudaSuccess) return fail_cuda(e, "bias kernels");
+  const int groups = s.block / s.lanes;
+  s.ctas = ctas_per_matrix(a, (int64_t)d.sms * std::max(1, per_sm), groups, matrices == 1 ? 6 : 3 * groups);
+  *shape = s;
+  return CS_OK;
 }
 
 // Shared-memory limits of the kernels, once per device.
@@ -180,6 +189,11 @@ int set_up(const cs_host::Device& d) {
       if (e == cudaSuccess)
         e = cudaFuncSetAttribute(reinterpret_cast<const void*>(backward_kernel(type, staged)),
                                  cudaFuncAttributeMaxDynamicSharedMemorySize, d.max_smem);
+      // Rows bypass L1: all of it for the buffers.
+      for (Kernel k : {forward_kernel(type, staged), backward_kernel(type, staged)})
+        if (e == cudaSuccess)
+          e = cudaFuncSetAttribute(reinterpret_cast<const void*>(k), cudaFuncAttributePreferredSharedMemoryCarveout,
+                                   cudaSharedmemCarveoutMaxShared);
       if (e != cudaSuccess) return fail_cuda(e, "bias kernels");
     }
   cudaFuncAttributes fa{};
@@ -187,6 +201,16 @@ int set_up(const cs_host::Device& d) {
   if (e != cudaSuccess) return fail_cuda(e, "bias kernels");
   done[d.id] = true;
   return CS_OK;
+}
+
+int forward_shape(const cs_bias_args* a, const cs_host::Device& d, Shape* s) {
+  return shape_of(a, d, 1, 0, cs::bias_slots(a->bucket_starts[a->buckets - 1]), forward_kernel(a->type, true),
+                  forward_kernel(a->type, false), s);
+}
+
+int backward_shape(const cs_bias_args* a, const cs_host::Device& d, Shape* s) {
+  return shape_of(a, d, 2, cs::bias_slots(a->bucket_starts[a->buckets - 1]), 0, backward_kernel(a->type, true),
+                  backward_kernel(a->type, false), s);
 }
 
 cs::BiasParams params_of(const cs_bias_args* a, const Shape& s) {
@@ -243,13 +267,14 @@ int cs_bias_softmax(const cs_bias_args* args, const void* x, const float* table,
   if (!rc) rc = check_matrices(args, x, x, p);
   if (rc) return rc;
   if (!table) return fail(CS_ERR_NULL, "table is null");
+  if (reinterpret_cast<uintptr_t>(table) & 3) return fail(CS_ERR_ALIGNMENT, "table must be 4-byte aligned");
   cs_host::Device d;
   rc = cs_host::current_device(&d);
   if (!rc) rc = set_up(d);
-  if (rc) return rc;
-  const Shape s = forward_shape(args, d);
+  Shape s{};
   int64_t grid = 0;
-  rc = grid_of(args, s, &grid);
+  if (!rc) rc = forward_shape(args, d, &s);
+  if (!rc) rc = grid_of(args, s, &grid);
   if (rc) return rc;
   cs::BiasParams k = params_of(args, s);
   k.x = static_cast<const uint16_t*>(x);
@@ -263,8 +288,10 @@ int64_t cs_bias_softmax_backward_workspace(const cs_bias_args* args) {
   int rc = check_args(args);
   cs_host::Device d;
   if (!rc) rc = cs_host::current_device(&d);
+  Shape s{};
+  if (!rc) rc = set_up(d);
+  if (!rc) rc = backward_shape(args, d, &s);
   if (rc) return rc;
-  const Shape s = backward_shape(args, d);
   return (int64_t)args->batch * args->heads * s.ctas * args->buckets * 4;
 }
 
@@ -274,14 +301,15 @@ int cs_bias_softmax_backward(const cs_bias_args* args, const void* p, const void
   if (!rc) rc = check_matrices(args, p, dp, ds);
   if (rc) return rc;
   if (!dtable || !workspace) return fail(CS_ERR_NULL, "dtable or workspace is null");
-  if (!aligned16(workspace)) return fail(CS_ERR_ALIGNMENT, "workspace must be 16-byte aligned");
+  if (!aligned16(workspace) || (reinterpret_cast<uintptr_t>(dtable) & 3))
+    return fail(CS_ERR_ALIGNMENT, "workspace must be 16-byte aligned, dtable 4-byte");
   cs_host::Device d;
   rc = cs_host::current_device(&d);
   if (!rc) rc = set_up(d);
-  if (rc) return rc;
-  const Shape s = backward_shape(args, d);
+  Shape s{};
   int64_t grid = 0;
-  rc = grid_of(args, s, &grid);
+  if (!rc) rc = backward_shape(args, d, &s);
+  if (!rc) rc = grid_of(args, s, &grid);
   if (rc) return rc;
   const int64_t need = grid * args->buckets * 4;
   if ((int64_t)workspace_bytes < need)
@@ -300,6 +328,7 @@ int cs_bias_softmax_backward(const cs_bias_args* args, const void* p, const void
   r.heads = args->heads;
   r.ctas = s.ctas;
   r.buckets = args->buckets;
+  r.by_ctas = cs::Divider::of((uint32_t)s.ctas);
   e = cs_host::launch(&cs::bias_table_kernel, dim3((unsigned)args->heads, (unsigned)((args->buckets + 31) / 32)), 1024, 0,
                       stream, r);
   return e == cudaSuccess ? CS_OK : fail_cuda(e, "bias table gradient");

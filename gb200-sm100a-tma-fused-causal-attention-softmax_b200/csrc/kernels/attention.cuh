@@ -2,26 +2,13 @@
 #pragma once
 
 #include "common.cuh"
+#include "divider.cuh"
 #include "positions.cuh"
 #include "types.cuh"
 
 namespace cs {
 
 constexpr uint64_t kWaitNs = 2000000000ull;  // bound on a device-side wait: 2 s of GPU time
-
-// Division by a number the host knows, for 0 <= n < 2^31: a CTA of a few tiles
-// would spend a tenth of its time on the compiler's division routine.
-struct Divider {
-  uint32_t by, mul, shift;
-  static Divider of(uint32_t d) {  // 1 <= d < 2^31
-    Divider r{d, 0, 31};
-    while ((1ull << (r.shift - 31)) < d) ++r.shift;
-    r.mul = (uint32_t)(((1ull << r.shift) + d - 1) / d);
-    return r;
-  }
-  __device__ __forceinline__ int div(int n) const { return (int)((uint64_t)(uint32_t)n * mul >> shift); }
-  __device__ __forceinline__ int mod(int n) const { return n - div(n) * (int)by; }
-};
 
 struct Strided {  // [batch, token, head, dim], element strides, dim contiguous
   uint16_t* data;

@@ -29,6 +29,7 @@
 #pragma once
 
 #include "common.cuh"
+#include "divider.cuh"
 #include "positions.cuh"
 #include "types.cuh"
 
@@ -212,12 +213,13 @@ __global__ void __launch_bounds__(kBiasMaxThreads) bias_softmax_kernel(const __g
   const float* table = p.table + (matrix % p.heads) * p.buckets;
   const int64_t base = matrix * p.rows * (int64_t)p.pitch;
   const int step = p.ctas * groups;
-  int row = p.rows - 1 - (cta * groups + group.id);  // the longest rows first
+  int i = cta * groups + group.id;
+  auto nth = [&](int i) { return min(max(p.rows - 1 - i, 0), p.rows - 1); };  // the longest rows first
 
   pdl_wait();
   auto source = [&](int r) { return reinterpret_cast<const uint4*>(p.x + base + (int64_t)r * p.pitch); };
   if (kStaged) {
-    if (row >= 0) fetch_row(RowWalk(p, row), source(row), buffers, gt, gn);
+    if (i < p.rows) fetch_row(RowWalk(p, nth(i)), source(nth(i)), buffers, gt, gn);
     cp_async_commit();
   }
   for (int d = threadIdx.x - 8; d < p.near + 8; d += blockDim.x)
@@ -226,15 +228,16 @@ __global__ void __launch_bounds__(kBiasMaxThreads) bias_softmax_kernel(const __g
   const float far = tab[bias_slot(p.near)], sl = p.scale * kLog2e;
   const F2 far2 = f2(far, far), sl2 = f2(sl, sl);
 
-  RowWalk w(p, max(row, 0));
-  for (int turn = 0; row >= 0; row -= step, turn ^= 1) {
+  RowWalk w(p, nth(i));
+  for (int turn = 0; i < p.rows; i += step, turn ^= 1) {
+    const int row = nth(i), after = nth(i + step);
     uint4* out = reinterpret_cast<uint4*>(p.out + base + (int64_t)row * p.pitch);
     const uint4* in = source(row);
     const uint4* staged = buffers + turn * p.slots;
-    const RowWalk next(p, max(row - step, 0));
+    const RowWalk next(p, after);
     if (kStaged) {
       group.sync();  // the row before, in the other buffer, is done with
-      if (row >= step) fetch_row(next, source(row - step), buffers + (turn ^ 1) * p.slots, gt, gn);
+      if (i + step < p.rows) fetch_row(next, source(after), buffers + (turn ^ 1) * p.slots, gt, gn);
       cp_async_commit();
       zero_masked(p, w, out, gt, gn);
       cp_async_wait<1>();
@@ -337,7 +340,8 @@ __global__ void __launch_bounds__(kBiasMaxThreads) bias_backward_kernel(const __
   const int cta = blockIdx.x - (int)(matrix * p.ctas);
   const int64_t base = matrix * p.rows * (int64_t)p.pitch;
   const int step = p.ctas * groups;
-  int row = p.rows - 1 - (cta * groups + group.id);
+  int i = cta * groups + group.id;
+  auto nth = [rows = p.rows](int i) { return max(rows - 1 - i, 0); };  // the longest rows first
   for (int d = gt; d < slots; d += gn) acc[d] = 0.f;
 
   pdl_wait();
@@ -347,22 +351,23 @@ __global__ void __launch_bounds__(kBiasMaxThreads) bias_backward_kernel(const __
     fetch_row(w, source(p.dp, r), to + p.slots, gt, gn);
   };
   if (kStaged) {
-    if (row >= 0) fetch(RowWalk(p, row), row, buffers);
+    if (i < p.rows) fetch(RowWalk(p, nth(i)), nth(i), buffers);
     cp_async_commit();
   }
   group.sync();
   float far = 0.f;
 
-  RowWalk w(p, max(row, 0));
-  for (int turn = 0; row >= 0; row -= step, turn ^= 1) {
+  RowWalk w(p, nth(i));
+  for (int turn = 0; i < p.rows; i += step, turn ^= 1) {
+    const int row = nth(i), after = nth(i + step);
     uint4* out = reinterpret_cast<uint4*>(p.out + base + (int64_t)row * p.pitch);
     const uint4* in = source(p.x, row);
     const uint4* in2 = source(p.dp, row);
     const uint4* staged = buffers + turn * 2 * p.slots;
-    const RowWalk next(p, max(row - step, 0));
+    const RowWalk next(p, after);
     group.sync();  // the row before is done with: its buffer, and its additions to acc
     if (kStaged) {
-      if (row >= step) fetch(next, row - step, buffers + (turn ^ 1) * 2 * p.slots);
+      if (i + step < p.rows) fetch(next, after, buffers + (turn ^ 1) * 2 * p.slots);
       cp_async_commit();
       zero_masked(p, w, out, gt, gn);
       cp_async_wait<1>();
@@ -479,6 +484,7 @@ struct BiasReduceParams {
   const float* partial;
   float* dtable;
   int32_t batch, heads, ctas, buckets;
+  Divider by_ctas;
 };
 
 // dtable[h, j]: grid.x heads, grid.y tiles of 32 buckets. Lanes are buckets, so
@@ -491,10 +497,12 @@ __global__ void __launch_bounds__(1024) bias_table_kernel(const __grid_constant_
   const int b = blockIdx.y * 32 + lane;
   double s = 0.0;
   if (b < p.buckets) {
-    for (int64_t k = 0; k < p.batch; ++k) {
-      const float* part = p.partial + (k * p.heads + h) * p.ctas * (int64_t)p.buckets + b;
-#pragma unroll 4
-      for (int c = warp; c < p.ctas; c += 32) s += (double)part[(int64_t)c * p.buckets];
+    // CTAs of the head's matrices, one after the other.
+    const int n = p.batch * p.ctas;
+#pragma unroll 8
+    for (int c = warp; c < n; c += 32) {
+      const int k = p.by_ctas.div(c);
+      s += (double)p.partial[(((int64_t)k * p.heads + h) * p.ctas + (c - k * p.ctas)) * p.buckets + b];
     }
   }
   sums[warp][lane] = s;
@@ -503,7 +511,7 @@ __global__ void __launch_bounds__(1024) bias_table_kernel(const __grid_constant_
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
   const int bucket = blockIdx.y * 32 + warp;
-  if (lane == 0 && bucket < p.buckets) p.dtable[h * p.buckets + bucket] = (float)t;
+  if (lane == 0 && bucket < p.buckets) p.dtable[(int64_t)h * p.buckets + bucket] = (float)t;
 }
 
 }  // namespace cs

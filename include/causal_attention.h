@@ -15,7 +15,8 @@
  * of zeros, a log-sum-exp of -infinity and gradients of zero.
  *
  * Conventions as in causal_softmax.h: device pointers of the current device,
- * 16-byte aligned; `stream` is a cudaStream_t as void*; functions return 0 or
+ * 16-byte aligned (fp32 and int32 arrays: 4-byte); outputs overlap neither
+ * inputs nor each other; `stream` is a cudaStream_t as void*; functions return 0 or
  * a CS_ERR_* code (text in cs_last_error_detail), launch asynchronously,
  * allocate nothing, and keep nothing between calls; workspaces are the
  * caller's, need no initialisation, and may be reused once the call's work on
@@ -116,7 +117,8 @@ typedef struct cs_attention_args {
  * rows that see no key; keys and values behind its length, and those that no
  * query sees, may hold anything. (A NaN or infinity in a value that some query
  * of the sequence sees may also reach other queries of that sequence that do
- * not see it.) One call serves prompts, chunks of prompts over a cache
+ * not see it.) A row whose visible scores are all -infinity is like one that
+ * sees no key; one with a NaN or +infinity among them is NaN. One call serves prompts, chunks of prompts over a cache
  * (q_len < kv_len) and single tokens (q_len 1). `workspace`: at least
  * cs_attention_workspace bytes (0 for most shapes). */
 int64_t cs_attention_workspace(const cs_attention_args *args);
@@ -126,6 +128,8 @@ int cs_attention(const cs_attention_args *args, void *workspace, size_t workspac
  * wrote for the same arguments. Rows of dq behind a sequence's queries, and
  * rows of dk and dv behind its keys, are written zero; what d_o holds there is
  * not used. Gradients of a kv head are summed over its query heads in binary32.
+ * A NaN or infinity in a row of q, d_o or o, or in a key or value that is seen,
+ * may reach all gradients of its sequence.
  * `workspace`: at least cs_attention_backward_workspace bytes. */
 typedef struct cs_attention_grads {
     cs_tensor d_o, dq, dk, dv;

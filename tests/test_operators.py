@@ -58,6 +58,15 @@ def test_positions_by_brute_force(tmp_path):
     assert out.returncode == 0 and out.stdout.startswith("ok"), out.stdout + out.stderr
 
 
+def test_division_by_brute_force(tmp_path):
+    exe = str(tmp_path / "divider_check")
+    subprocess.run(["g++", "-O2", "-std=c++17", "-fsanitize=undefined", "-fno-sanitize-recover", "-I",
+                    os.path.join(cs.PKG_DIR, "csrc"), "-o", exe, os.path.join(ROOT, "tests", "divider_check.cpp")],
+                   check=True)
+    out = subprocess.run([exe], capture_output=True, text=True)
+    assert out.returncode == 0 and out.stdout.startswith("ok"), out.stdout + out.stderr
+
+
 def bias_args(starts=(0, 1, 2, 3), **kw):
     array = (ctypes.c_int32 * max(1, len(starts)))(*starts)
     f = dict(type=0, batch=1, heads=2, rows=8, cols=8, pitch=8, row_offset=0, window=0, sinks=0, buckets=len(starts),
@@ -155,3 +164,26 @@ def test_attention_backward_refusals():
     assert call(work=None) == "NULL" and call(work=FAKE + 4) == "ALIGNMENT" and call(size=3) == "WRONG_LENGTH"
     assert cs.ERR[L.cs_attention_backward(ctypes.byref(good), None, FAKE, 1 << 30, None)] == "NULL"
     assert cs.ERR[L.cs_attention_status(None, None)] == "NULL"
+
+
+def test_refusals_of_overlaps_and_misaligned_words():
+    L = cs.lib()
+
+    def forward(**kw):
+        return cs.ERR[L.cs_attention(ctypes.byref(attention_args(**kw)), FAKE, 1 << 30, None)]
+
+    def backward(lse=FAKE, **kw):
+        g = dict(d_o=t(), dq=t(2 * FAKE), dk=t(3 * FAKE, token=128), dv=t(4 * FAKE, token=128))
+        g.update(kw)
+        return cs.ERR[L.cs_attention_backward(ctypes.byref(attention_args(lse=lse)), ctypes.byref(ops._AttentionGrads(**g)),
+                                              FAKE, 1 << 30, None)]
+
+    assert forward(o=t()) == "ARG"
+    for words in (dict(lse=FAKE + 2), dict(q_lens=FAKE + 1), dict(kv_lens=FAKE + 2)):
+        assert forward(o=t(2 * FAKE), **words) == "ALIGNMENT"
+    assert backward(dq=t()) == "ARG" and backward(dk=t(2 * FAKE, token=128)) == "ARG"
+    assert backward(dv=t(3 * FAKE, token=128)) == "ARG" and backward(lse=FAKE + 2) == "ALIGNMENT"
+    a = bias_args()
+    assert cs.ERR[L.cs_bias_softmax(ctypes.byref(a), FAKE, FAKE + 2, 2 * FAKE, None)] == "ALIGNMENT"
+    assert cs.ERR[L.cs_bias_softmax_backward(ctypes.byref(a), FAKE, 2 * FAKE, 3 * FAKE, FAKE + 2, FAKE, 1 << 20,
+                                             None)] == "ALIGNMENT"

@@ -253,6 +253,34 @@ def test_ragged_batch_with_garbage_behind_the_sequences(q_len, kv_len, q_lens, k
             assert (t[b, rows:] == 0).all(), f"{n}: rows outside the sequences are zero"
 
 
+SPLIT = [
+    # calls whose keys several CTAs share, or whose few rows are tiles; kv_lens
+    (1, 24, 700, 2, 1, 128, 0, 0, (650,)),               # a CTA per key tile
+    (1, 40, 1100, 4, 2, 64, 900, 130, (1100,)),
+    (2, 30, 6000, 3, 1, 80, 0, 0, (6000, 40)),           # most CTAs of a tile see no key
+    (1, 20, 40000, 1, 1, 64, 0, 0, (39000,)),            # more than 64 CTAs a tile
+    (1, 500, 2500, 2, 2, 128, 2100, 3, (2400,)),
+    (75, 3, 200, 8, 2, 64, 0, 0, tuple(range(1, 151, 2))),  # 12 rows of 150 kv heads
+    (3, 2, 5000, 16, 2, 128, 4000, 9, (5000, 130, 1)),   # 16 rows, split
+]
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("case", SPLIT)
+def test_split_keys(case, dtype):
+    *case, kv_lens = case
+    q, k, v, how = attention_inputs(case, dtype)
+    how["kv_lens"] = torch.tensor(kv_lens, dtype=torch.int32, device="cuda")
+    for b, n in enumerate(kv_lens):
+        k[b, n:], v[b, n:] = math.inf, math.nan
+    got, lse = cs.attention(q, k, v, return_lse=True, **how)
+    status_ok()
+    want, bound, wl, bl = ref.attention(q, k, v, **how)
+    within(got, want, bound, "out")
+    within(lse, wl, bl, "lse")
+    assert torch.equal(cs.attention(q, k, v, **how), got)
+
+
 @pytest.mark.parametrize("q_len,kv_len", [(1, 200), (190, 200)])
 def test_strides(q_len, kv_len):
     """Heads before tokens, tokens apart, and one tensor that holds q, k and v."""
