@@ -184,7 +184,7 @@ def bias_softmax_backward(p, dp, bucket_starts, *, cols: int, scale: float, row_
     L = lib()
     with _on(device, stream):
         ds = _like("out", out, p)
-        dtable = torch.empty((heads, buckets), dtype=torch.float32, device=device)
+        dtable = torch.empty(heads, buckets, dtype=torch.float32, device=device)
         need = L.cs_bias_softmax_backward_workspace(args)
         check(min(need, 0), "cs_bias_softmax_backward_workspace")
         work = torch.empty(need, dtype=torch.uint8, device=device)
@@ -205,6 +205,11 @@ def _tensor(name: str, t, shape, dtype, device) -> tuple:
     if d != 1 and shape[3] > 1:
         raise ValueError(f"{name}: the last dimension must be contiguous")
     return t.data_ptr(), b, n, h
+
+
+def _fresh(t):
+    """A contiguous tensor like t. (empty_like takes 1.3 us, empty with a shape and a device 3.3.)"""
+    return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=t.device)
 
 
 def _lens(name: str, t, batch: int, device) -> int:
@@ -251,7 +256,7 @@ def attention(q, k, v, *, scale: float | None = None, window: int = 0, sinks: in
     L = lib()
     with _on(device, stream):
         if out is None:
-            out = torch.empty(shape, dtype=dtype, device=device)
+            out = _fresh(q)
         lse = torch.empty((shape[0], shape[2], shape[1]), dtype=torch.float32, device=device) if return_lse else None
         args = _PACK_ATTENTION(*head, *_tensor("out", out, shape, dtype, device), lse.data_ptr() if return_lse else 0)
         need = L.cs_attention_workspace(args)
@@ -273,7 +278,7 @@ def attention_backward(dout, q, k, v, out, lse, *, scale: float | None = None, w
     d_o = _tensor("dout", dout, shape, dtype, device)
     L = lib()
     with _on(device, stream):
-        dq, dk, dv = (torch.empty(t.shape, dtype=dtype, device=device) for t in (q, k, v))
+        dq, dk, dv = _fresh(q), _fresh(k), _fresh(v)
         grads = _PACK_GRADS(*d_o, dq.data_ptr(), *dq.stride()[:3], dk.data_ptr(), *dk.stride()[:3],
                             dv.data_ptr(), *dv.stride()[:3])
         need = L.cs_attention_backward_workspace(args)
