@@ -91,9 +91,9 @@ int check_matrices(const cs_bias_args* a, const void* x, const void* y, const vo
 
 // Launch shape: a row takes `lanes` lanes; a CTA works on block / lanes rows at
 // a time, and each matrix has `ctas` CTAs. slots: vectors of a staged
-// row's buffer, 0 where rows stay in global memory.
+// row's buffer; buffers: of a group; both 0 where rows stay in global memory.
 struct Shape {
-  int lanes, block, ctas, slots;
+  int lanes, block, ctas, slots, buffers;
   size_t smem;
 };
 
@@ -126,20 +126,27 @@ int ctas_per_matrix(const cs_bias_args* a, int64_t resident, int groups, int end
 
 using Kernel = void (*)(cs::BiasParams);
 
-Kernel forward_kernel(int type, bool staged) {
-  return type == CS_TYPE_F16 ? (staged ? &cs::bias_softmax_kernel<cs::F16, true> : &cs::bias_softmax_kernel<cs::F16, false>)
-                             : (staged ? &cs::bias_softmax_kernel<cs::BF16, true> : &cs::bias_softmax_kernel<cs::BF16, false>);
+template <typename T>
+Kernel forward_kernel_of(int buffers) {
+  return buffers == 2 ? &cs::bias_softmax_kernel<T, 2> : buffers == 1 ? &cs::bias_softmax_kernel<T, 1> : &cs::bias_softmax_kernel<T, 0>;
 }
 
-Kernel backward_kernel(int type, bool staged) {
-  return type == CS_TYPE_F16 ? (staged ? &cs::bias_backward_kernel<cs::F16, true> : &cs::bias_backward_kernel<cs::F16, false>)
-                             : (staged ? &cs::bias_backward_kernel<cs::BF16, true> : &cs::bias_backward_kernel<cs::BF16, false>);
+template <typename T>
+Kernel backward_kernel_of(int buffers) {
+  return buffers == 2 ? &cs::bias_backward_kernel<T, 2>
+                      : buffers == 1 ? &cs::bias_backward_kernel<T, 1> : &cs::bias_backward_kernel<T, 0>;
+}
+
+// matrices: 1, forward; 2, backward.
+Kernel kernel_of(int type, int matrices, int buffers) {
+  if (matrices == 1) return type == CS_TYPE_F16 ? forward_kernel_of<cs::F16>(buffers) : forward_kernel_of<cs::BF16>(buffers);
+  return type == CS_TYPE_F16 ? backward_kernel_of<cs::F16>(buffers) : backward_kernel_of<cs::BF16>(buffers);
 }
 
 // Few lanes a row keep the work that each row costs a warp (its geometry, the
 // reductions, the vectors near the diagonal) shared among several rows, and
-// shared memory for two rows a group limits how few: a CTA takes up to
-// kTargetSmem, three CTAs an SM. Measured on B200 in us, lanes 8 / 16 / 32 / 64
+// shared memory for the groups' rows limits how few: a CTA takes up to
+// kTargetSmem, three CTAs an SM. Measured on B200 in us, two buffers a group, lanes 8 / 16 / 32 / 64
 // (/ 128): forward 64 x 16 matrices of 512^2 223 / 267 / 457 / 859, 16 x 16 of
 // 1024^2 197 / 187 / 287 / 513, 8 x 16 of 2048^2 626 / 318 / 363 / 589,
 // 64 x 4096^2 1096 / 1046 / 609 / 742, 16 x 8192^2 - / 1043 / 1059 / 635 / 722;
@@ -147,28 +154,36 @@ Kernel backward_kernel(int type, bool staged) {
 // (each group has its array by distance), 32 x 4096^2 856 / 640 / 854 / 451 / 544.
 constexpr int64_t kTargetSmem = 72 * 1024;
 
+// Longer rows (in vectors) have one buffer a group instead of two, so half the lanes
+// a row; loads are then covered by the other groups alone. One / two buffers, us:
+// forward 1024 x 512^2 242 / 218, 256 x 1024^2 212 / 183, 128 x 2048^2 319 / 317,
+// 64 x 4096^2 578 / 607, 16 x 8192^2 570 / 631; backward 345 / 286, 354 / 317,
+// 424 / 430, 719 / 823, 712 / 778.
+constexpr int64_t kOneBuffer = 256;
+
 // matrices: 1 (scores) or 2 (probabilities and their gradient); words: fp32
-// words a CTA needs besides, per group and once; kernels: the staged one and the other.
-int shape_of(const cs_bias_args* a, const cs_host::Device& d, int matrices, int64_t group_words, int64_t words, Kernel staged,
-             Kernel direct, Shape* shape) {
+// words a CTA needs besides, per group and once.
+int shape_of(const cs_bias_args* a, const cs_host::Device& d, int matrices, int64_t group_words, int64_t words, Shape* shape) {
   const int64_t nv = max_vectors(a);
+  Shape s{};
+  s.buffers = nv > kOneBuffer ? 1 : 2;
+  const int64_t row_bytes = nv * 16 * matrices * s.buffers;
   auto bytes = [&](int lanes) {
     const int64_t block = std::max(cs::kBiasThreads, lanes), groups = block / lanes;
-    return groups * (nv * 32 * matrices + group_words * 4) + (words + block / 32 * 2) * 4;
+    return groups * (row_bytes + group_words * 4) + (words + block / 32 * 2) * 4;
   };
-  Shape s{};
   s.lanes = (nv <= 64 ? 8 : 16) * matrices;
   while (s.lanes < cs::kBiasMaxThreads && bytes(s.lanes) > kTargetSmem) s.lanes *= 2;
   s.block = std::max(cs::kBiasThreads, s.lanes);
   s.slots = (int)nv;
   s.smem = (size_t)bytes(s.lanes);
   if ((int64_t)s.smem > d.max_smem) {
-    s.smem -= (size_t)(s.block / s.lanes * nv * 32 * matrices);
-    s.slots = 0;
+    s.smem -= (size_t)(s.block / s.lanes * row_bytes);
+    s.slots = s.buffers = 0;
   }
   int per_sm = 0;
   const cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(
-      &per_sm, reinterpret_cast<const void*>(s.slots ? staged : direct), s.block, s.smem);
+      &per_sm, reinterpret_cast<const void*>(kernel_of(a->type, matrices, s.buffers)), s.block, s.smem);
   if (e != cudaSuccess) return fail_cuda(e, "bias kernels");
   const int groups = s.block / s.lanes;
   s.ctas = ctas_per_matrix(a, (int64_t)d.sms * std::max(1, per_sm), groups, matrices == 1 ? 6 : 3 * groups);
@@ -183,19 +198,14 @@ int set_up(const cs_host::Device& d) {
   std::lock_guard<std::mutex> lock(mu);
   if (done[d.id]) return CS_OK;
   for (int type : {CS_TYPE_F16, CS_TYPE_BF16})
-    for (bool staged : {true, false}) {
-      cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(forward_kernel(type, staged)),
-                                           cudaFuncAttributeMaxDynamicSharedMemorySize, d.max_smem);
-      if (e == cudaSuccess)
-        e = cudaFuncSetAttribute(reinterpret_cast<const void*>(backward_kernel(type, staged)),
-                                 cudaFuncAttributeMaxDynamicSharedMemorySize, d.max_smem);
-      // Rows bypass L1: all of it for the buffers.
-      for (Kernel k : {forward_kernel(type, staged), backward_kernel(type, staged)})
-        if (e == cudaSuccess)
-          e = cudaFuncSetAttribute(reinterpret_cast<const void*>(k), cudaFuncAttributePreferredSharedMemoryCarveout,
-                                   cudaSharedmemCarveoutMaxShared);
-      if (e != cudaSuccess) return fail_cuda(e, "bias kernels");
-    }
+    for (int matrices : {1, 2})
+      for (int buffers : {0, 1, 2}) {
+        const void* k = reinterpret_cast<const void*>(kernel_of(type, matrices, buffers));
+        cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, d.max_smem);
+        if (e == cudaSuccess && buffers)  // rows bypass L1: all of it for the buffers
+          e = cudaFuncSetAttribute(k, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+        if (e != cudaSuccess) return fail_cuda(e, "bias kernels");
+      }
   cudaFuncAttributes fa{};
   const cudaError_t e = cudaFuncGetAttributes(&fa, reinterpret_cast<const void*>(&cs::bias_table_kernel));
   if (e != cudaSuccess) return fail_cuda(e, "bias kernels");
@@ -204,13 +214,11 @@ int set_up(const cs_host::Device& d) {
 }
 
 int forward_shape(const cs_bias_args* a, const cs_host::Device& d, Shape* s) {
-  return shape_of(a, d, 1, 0, cs::bias_slots(a->bucket_starts[a->buckets - 1]), forward_kernel(a->type, true),
-                  forward_kernel(a->type, false), s);
+  return shape_of(a, d, 1, 0, cs::bias_slots(a->bucket_starts[a->buckets - 1]), s);
 }
 
 int backward_shape(const cs_bias_args* a, const cs_host::Device& d, Shape* s) {
-  return shape_of(a, d, 2, cs::bias_slots(a->bucket_starts[a->buckets - 1]), 0, backward_kernel(a->type, true),
-                  backward_kernel(a->type, false), s);
+  return shape_of(a, d, 2, cs::bias_slots(a->bucket_starts[a->buckets - 1]), 0, s);
 }
 
 cs::BiasParams params_of(const cs_bias_args* a, const Shape& s) {
@@ -280,7 +288,7 @@ int cs_bias_softmax(const cs_bias_args* args, const void* x, const float* table,
   k.x = static_cast<const uint16_t*>(x);
   k.out = static_cast<uint16_t*>(p);
   k.table = table;
-  const cudaError_t e = cs_host::launch(forward_kernel(args->type, s.slots > 0), dim3((unsigned)grid), s.block, s.smem, stream, k);
+  const cudaError_t e = cs_host::launch(kernel_of(args->type, 1, s.buffers), dim3((unsigned)grid), s.block, s.smem, stream, k);
   return e == cudaSuccess ? CS_OK : fail_cuda(e, "biased softmax");
 }
 
@@ -319,7 +327,7 @@ int cs_bias_softmax_backward(const cs_bias_args* args, const void* p, const void
   k.dp = static_cast<const uint16_t*>(dp);
   k.out = static_cast<uint16_t*>(ds);
   k.partial = static_cast<float*>(workspace);
-  cudaError_t e = cs_host::launch(backward_kernel(args->type, s.slots > 0), dim3((unsigned)grid), s.block, s.smem, stream, k);
+  cudaError_t e = cs_host::launch(kernel_of(args->type, 2, s.buffers), dim3((unsigned)grid), s.block, s.smem, stream, k);
   if (e != cudaSuccess) return fail_cuda(e, "biased softmax backward");
   cs::BiasReduceParams r{};
   r.partial = k.partial;

@@ -2,9 +2,9 @@
 //
 // A group of 8 to 256 lanes works on one row at a time. The row's visible 16-byte
 // vectors are copied to shared memory (cp.async) while the group works on the
-// row before, and the passes (maximum, sum, result; backward: the row's sum of
-// p dp, result) read them there, so HBM sees each score once. Rows too long for
-// the group's two buffers are read from global memory in each pass.
+// row before (long rows: once it is done with it), and the passes (maximum, sum,
+// result; backward: the row's sum of p dp, result) read them there, so HBM sees
+// each score once. Rows too long for that are read from global memory in each pass.
 // Bound: HBM (2 bytes in per visible score, 2 out per column; the backward
 // reads two matrices).
 //
@@ -197,14 +197,15 @@ __device__ __forceinline__ float sum8(const float* z) {
   return ((z[0] + z[1]) + (z[2] + z[3])) + ((z[4] + z[5]) + (z[6] + z[7]));
 }
 
-// kStaged: rows go through shared memory (p.slots vectors a buffer, two buffers a group).
-template <typename T, bool kStaged>
+// kBuffers: of a group in shared memory, p.slots vectors each; 0: rows stay in global memory.
+template <typename T, int kBuffers>
 __global__ void __launch_bounds__(kBiasMaxThreads) bias_softmax_kernel(const __grid_constant__ BiasParams p) {
+  constexpr bool kStaged = kBuffers > 0;
   extern __shared__ __align__(16) uint4 smem[];
   const Group group(p.lanes);
   const int gn = p.lanes, groups = blockDim.x / gn, gt = group.rank;
-  uint4* buffers = smem + group.id * 2 * p.slots;
-  float* tab = reinterpret_cast<float*>(smem + groups * 2 * p.slots);  // bias by distance, [0, near]
+  uint4* buffers = smem + group.id * kBuffers * p.slots;
+  float* tab = reinterpret_cast<float*>(smem + groups * kBuffers * p.slots);  // bias by distance, [0, near]
   float* words = tab + bias_slots(p.near);  // two per warp, for groups of several warps
   float* words_max = words + (threadIdx.x / 32 - gt / 32) * 2;
   float* words_sum = words_max + (gn >> 5);
@@ -233,17 +234,17 @@ __global__ void __launch_bounds__(kBiasMaxThreads) bias_softmax_kernel(const __g
     const int row = nth(i), after = nth(i + step);
     uint4* out = reinterpret_cast<uint4*>(p.out + base + (int64_t)row * p.pitch);
     const uint4* in = source(row);
-    const uint4* staged = buffers + turn * p.slots;
+    const uint4* staged = buffers + (kBuffers == 2 ? turn * p.slots : 0);
     const RowWalk next(p, after);
-    if (kStaged) {
+    if (kBuffers == 2) {
       group.sync();  // the row before, in the other buffer, is done with
       if (i + step < p.rows) fetch_row(next, source(after), buffers + (turn ^ 1) * p.slots, gt, gn);
       cp_async_commit();
-      zero_masked(p, w, out, gt, gn);
-      cp_async_wait<1>();
+    }
+    zero_masked(p, w, out, gt, gn);
+    if (kStaged) {
+      cp_async_wait<kBuffers == 2 ? 1 : 0>();
       group.sync();
-    } else {
-      zero_masked(p, w, out, gt, gn);
     }
     auto vec = [&](int j) { return kStaged ? staged[j] : in[vector_at(w.m, j)]; };
     // A lane's first vector that is not plain, mostly its only one, stays in registers.
@@ -320,19 +321,25 @@ __global__ void __launch_bounds__(kBiasMaxThreads) bias_softmax_kernel(const __g
       }
       __stcs(plain_out + j, pack8<T>(z));
     }
+    if (kBuffers == 1) {
+      group.sync();
+      if (i + step < p.rows) fetch_row(next, source(after), buffers, gt, gn);
+      cp_async_commit();
+    }
     w = next;
   }
   pdl_trigger();
 }
 
-template <typename T, bool kStaged>
+template <typename T, int kBuffers>
 __global__ void __launch_bounds__(kBiasMaxThreads) bias_backward_kernel(const __grid_constant__ BiasParams p) {
+  constexpr bool kStaged = kBuffers > 0;
   extern __shared__ __align__(16) uint4 smem[];
   const Group group(p.lanes);
   const int gn = p.lanes, groups = blockDim.x / gn, gt = group.rank, lane = threadIdx.x & 31;
   const int slots = bias_slots(p.near);
-  uint4* buffers = smem + group.id * 4 * p.slots;  // two rows of p, two of dp
-  float* sums = reinterpret_cast<float*>(smem + groups * 4 * p.slots);
+  uint4* buffers = smem + group.id * 2 * kBuffers * p.slots;  // a row of p and one of dp each
+  float* sums = reinterpret_cast<float*>(smem + groups * 2 * kBuffers * p.slots);
   float* acc = sums + group.id * slots;  // sums by distance, [0, near)
   float* words = sums + groups * slots + (threadIdx.x / 32 - gt / 32);  // one per warp
   float* far_sums = sums + groups * slots + blockDim.x / 32;  // one per warp
@@ -363,17 +370,17 @@ __global__ void __launch_bounds__(kBiasMaxThreads) bias_backward_kernel(const __
     uint4* out = reinterpret_cast<uint4*>(p.out + base + (int64_t)row * p.pitch);
     const uint4* in = source(p.x, row);
     const uint4* in2 = source(p.dp, row);
-    const uint4* staged = buffers + turn * 2 * p.slots;
+    const uint4* staged = buffers + (kBuffers == 2 ? turn * 2 * p.slots : 0);
     const RowWalk next(p, after);
-    group.sync();  // the row before is done with: its buffer, and its additions to acc
-    if (kStaged) {
+    if (kBuffers != 1) group.sync();  // the row before is done with: its buffer, and its additions to acc
+    if (kBuffers == 2) {
       if (i + step < p.rows) fetch(next, after, buffers + (turn ^ 1) * 2 * p.slots);
       cp_async_commit();
-      zero_masked(p, w, out, gt, gn);
-      cp_async_wait<1>();
+    }
+    zero_masked(p, w, out, gt, gn);
+    if (kStaged) {
+      cp_async_wait<kBuffers == 2 ? 1 : 0>();
       group.sync();
-    } else {
-      zero_masked(p, w, out, gt, gn);
     }
     auto vec = [&](int j) { return kStaged ? staged[j] : in[vector_at(w.m, j)]; };
     auto vec2 = [&](int j) { return kStaged ? staged[p.slots + j] : in2[vector_at(w.m, j)]; };
@@ -459,6 +466,11 @@ __global__ void __launch_bounds__(kBiasMaxThreads) bias_backward_kernel(const __
     }
     const float2 far3 = f2_out(far2);
     far += far3.x + far3.y;
+    if (kBuffers == 1) {
+      group.sync();
+      if (i + step < p.rows) fetch(next, after, buffers);
+      cp_async_commit();
+    }
     w = next;
   }
   far = warp_sum(far);

@@ -95,6 +95,21 @@ def test_bias_softmax_backward(case, dtype):
     assert torch.equal(again[0], ds) and torch.equal(again[1], dtable), "the same inputs give the same bits"
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("case", [
+    (8, 16, 300, 300, 0, 0, 0, 32, 128),
+    (4, 8, 400, 2500, 2100, 0, 0, 32, 128),
+    (4, 8, 400, 2500, 2300, 700, 9, 64, 512),  # the last rows are beyond the columns
+    (450, 1, 2, 120000, 119998, 0, 0, 32, 128),  # rows that stay in global memory
+])
+def test_bias_several_rows_a_group(case, dtype):
+    """Matrices enough that a group of lanes works on several rows, one after the other."""
+    test_bias_softmax(case, dtype)
+    torch.cuda.empty_cache()
+    test_bias_softmax_backward(case, dtype)
+    torch.cuda.empty_cache()
+
+
 def test_bias_infinities_in_seen_places():
     x, table, starts, how = bias_inputs((1, 1, 40, 40, 0, 0, 0, 32, 128), F16)
     x[0, 0, 3, :] = -math.inf       # a row of -infinity only: zeros
