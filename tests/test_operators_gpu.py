@@ -110,6 +110,21 @@ def test_bias_several_rows_a_group(case, dtype):
     torch.cuda.empty_cache()
 
 
+def test_bias_of_more_than_2_to_the_31_elements():
+    """The last matrix of a batch as if it were alone, bit for bit."""
+    x, dp = (torch.empty(130, 1, 4096, 4096, dtype=F16, device="cuda").normal_(generator=torch.Generator("cuda").manual_seed(n))
+             for n in (1, 2))
+    starts, table = cs.bias_buckets(32, 128), randn(1, 32, dtype=torch.float32, seed=3)
+    how = dict(cols=4096, scale=0.3, window=900, sinks=3)
+    p = cs.bias_softmax(x, table, starts, **how)
+    alone = cs.bias_softmax(x[-1:], table, starts, **how)
+    assert torch.equal(p[-1:], alone) and float(alone.sum()) > 4000
+    ds = cs.bias_softmax_backward(p, dp, starts, **how)[0]
+    assert torch.equal(ds[-1:], cs.bias_softmax_backward(alone, dp[-1:], starts, **how)[0])
+    del x, dp, p, ds
+    torch.cuda.empty_cache()
+
+
 def test_bias_infinities_in_seen_places():
     x, table, starts, how = bias_inputs((1, 1, 40, 40, 0, 0, 0, 32, 128), F16)
     x[0, 0, 3, :] = -math.inf       # a row of -infinity only: zeros
@@ -409,6 +424,58 @@ def test_a_chain_on_another_stream_and_in_a_graph():
         assert all(torch.equal(a, b) for a, b in zip(r, fresh))
     assert not torch.equal(fresh[0], eager[0])
     status_ok()
+
+
+def test_calls_at_once_on_two_streams():
+    """Each call has its workspace: calls that overlap do not meet."""
+    cases = [((2, 300, 300, 8, 2, 64, 90, 2), 11), ((1, 40, 1100, 4, 2, 128, 0, 0), 12)]
+    streams = [torch.cuda.Stream() for _ in cases]
+    inputs, alone, together = [], [], [[], []]
+
+    def step(q, k, v, dout, how):
+        out, lse = cs.attention(q, k, v, return_lse=True, **how)
+        return [out, lse, *cs.attention_backward(dout, q, k, v, out, lse, **how)]
+
+    for case, seed in cases:
+        q, k, v, how = attention_inputs(case, BF16, seed=seed)
+        inputs.append((q, k, v, randn(*q.shape, dtype=BF16, seed=seed + 5), how))
+        alone.append(step(*inputs[-1]))
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for n, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                together[n].append(step(*inputs[n]))
+    torch.cuda.synchronize()
+    status_ok()
+    for want, runs in zip(alone, together):
+        assert all(torch.equal(a, b) for got in runs for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("q_len", [1, 40])
+def test_a_cache_of_more_than_2_to_the_31_elements(q_len):
+    n, heads, kv_heads, dim, sinks, window, tail = 2**21 + 300, 8, 8, 128, 4, 100, 300
+    q = randn(1, q_len, heads, dim, dtype=BF16, seed=1)
+    k, v = (torch.full((1, n, kv_heads, dim), math.nan, dtype=BF16, device="cuda") for _ in range(2))
+    small = []
+    for t, seed in ((k, 2), (v, 3)):  # only what some query sees, or next to it
+        part = randn(1, sinks + tail, kv_heads, dim, dtype=BF16, seed=seed)
+        t[:, :sinks], t[:, -tail:] = part[:, :sinks], part[:, sinks:]
+        small.append(part)
+    how = dict(scale=dim ** -0.5, window=window, sinks=sinks)
+    out, lse = cs.attention(q, k, v, return_lse=True, **how)
+    want, bound, wl, bl = ref.attention(q, *small, **how)
+    within(out, want, bound, "out")
+    within(lse, wl, bl, "lse")
+    dout = randn(*q.shape, dtype=BF16, seed=4)
+    grads = cs.attention_backward(dout, q, k, v, out, lse, **how)
+    status_ok()
+    want = ref.attention_backward(dout, q, *small, **how)
+    within(grads[0], *want["dq"], "dq")
+    for name, t in (("dk", grads[1]), ("dv", grads[2])):
+        within(torch.cat([t[:, :sinks], t[:, -tail:]], 1), *want[name], name)
+        assert not t[:, sinks:-tail].any(), "keys that no query sees have no gradient"
+    del k, v, t, grads
+    torch.cuda.empty_cache()
 
 
 def test_python_refusals():
