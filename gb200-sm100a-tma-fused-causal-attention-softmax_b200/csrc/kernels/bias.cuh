@@ -476,18 +476,28 @@ __global__ void __launch_bounds__(kBiasMaxThreads) bias_backward_kernel(const __
   far = warp_sum(far);
   if (lane == 0) far_sums[threadIdx.x >> 5] = far;
   __syncthreads();
+  // The groups' arrays into the first, then 8 lanes a bucket. (A warp a bucket, over all
+  // groups' arrays: 72 x 72^2 26.4 us, this 7.8; 132 x 1085^2 208, 176.)
+  for (int d = threadIdx.x; d < slots; d += blockDim.x) {
+    float s = sums[d];
+#pragma unroll 8
+    for (int k = 1; k < groups; ++k) s += sums[k * slots + d];
+    sums[d] = s;
+  }
+  __syncthreads();
   float* partial = p.partial + (int64_t)blockIdx.x * p.buckets;
-  for (int b = threadIdx.x >> 5; b < p.buckets; b += blockDim.x / 32) {
+  const int part = threadIdx.x & 7;
+  for (int b0 = 0; b0 < p.buckets; b0 += blockDim.x / 8) {
+    const int b = b0 + (threadIdx.x >> 3);
     float s = 0.f;
     if (b == p.buckets - 1) {
-      for (int k = lane; k < groups * 8; k += 32) s += sums[(k >> 3) * slots + bias_slot(p.near + (k & 7))];
-      if (lane < (int)(blockDim.x / 32)) s += far_sums[lane];
-    } else {
-      for (int k = 0; k < groups; ++k)
-        for (int d = p.starts[b] + lane; d < p.starts[b + 1]; d += 32) s += sums[k * slots + bias_slot(d)];
+      s = sums[bias_slot(p.near + part)] + (part < (int)(blockDim.x / 32) ? far_sums[part] : 0.f);
+    } else if (b < p.buckets) {
+      for (int d = p.starts[b] + part; d < p.starts[b + 1]; d += 8) s += sums[bias_slot(d)];
     }
-    s = warp_sum(s);
-    if (lane == 0) partial[b] = s;
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    if (part == 0 && b < p.buckets) partial[b] = s;
   }
   pdl_trigger();
 }
