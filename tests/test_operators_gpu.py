@@ -101,6 +101,8 @@ def test_bias_softmax_backward(case, dtype):
     (4, 8, 400, 2500, 2100, 0, 0, 32, 128),
     (4, 8, 400, 2500, 2300, 700, 9, 64, 512),  # the last rows are beyond the columns
     (450, 1, 2, 120000, 119998, 0, 0, 32, 128),  # rows that stay in global memory
+    (40, 16, 120, 120, 0, 0, 0, 32, 128),  # short rows, and many
+    (40, 16, 120, 700, 590, 60, 4, 16, 64),
 ])
 def test_bias_several_rows_a_group(case, dtype):
     """Matrices enough that a group of lanes works on several rows, one after the other."""
