@@ -109,8 +109,8 @@ int64_t max_vectors(const cs_bias_args* a) {
 // of its groups' rows and of its start and end, `ends` in quarters of a row (the
 // backward adds up its groups' arrays by distance). Numbers that fill whole rounds are
 // the candidates, and within 5% the one with more rounds, whose CTAs end more
-// evenly. Against four rounds always: backward 1024 x 512^2 287 us, 391; 128 x
-// 1024^2 159, 205; 16 x 2048^2 66, 133; 24 x 257^2 13, 20; forward 16 x 2048^2 47, 55.
+// evenly. Against four rounds always: backward 128 x 1024^2 146 us, 152; 16 x 2048^2
+// 57, 77; 24 x 257^2 8.8, 11.1; forward 16 x 2048^2 46, 55.
 int ctas_per_matrix(const cs_bias_args* a, int64_t resident, int groups, int ends) {
   const int64_t matrices = (int64_t)a->batch * a->heads, most = ((int64_t)a->rows + groups - 1) / groups;
   const int64_t rounds = (matrices + resident - 1) / resident;
@@ -146,19 +146,24 @@ Kernel kernel_of(int type, int matrices, int buffers) {
 // Few lanes a row keep the work that each row costs a warp (its geometry, the
 // reductions, the vectors near the diagonal) shared among several rows, and
 // shared memory for the groups' rows limits how few: a CTA takes up to
-// kTargetSmem, three CTAs an SM. Measured on B200 in us, two buffers a group, lanes 8 / 16 / 32 / 64
-// (/ 128): forward 64 x 16 matrices of 512^2 223 / 267 / 457 / 859, 16 x 16 of
-// 1024^2 197 / 187 / 287 / 513, 8 x 16 of 2048^2 626 / 318 / 363 / 589,
-// 64 x 4096^2 1096 / 1046 / 609 / 742, 16 x 8192^2 - / 1043 / 1059 / 635 / 722;
-// backward 512^2 x 512 367 / 250 / 312 / 464, 128 x 1024^2 766 / 231 / 205 / 279
-// (each group has its array by distance), 32 x 4096^2 856 / 640 / 854 / 451 / 544.
-constexpr int64_t kTargetSmem = 72 * 1024;
+// kTargetSmem, three CTAs an SM. Measured on B200 in us, lanes 8 / 16 / 32 / 64:
+// forward 1024 x 512^2 218 / 264 / 453 / 848, 1024 x 700^2 339 / 405 / 672 / -,
+// 256 x 1024^2 185 / 183 / 282 / 507, 128 x 2048^2 578 / 317 / 362 / 586, 64 x
+// 4096^2 991 / 578 / 605 / 854, 16 x 8192^2 1335 / 922 / 571 / 627; backward 1024 x
+// 512^2 251 / 268 / 461 / 792, 1024 x 700^2 470 / 394 / 671 / -, 128 x 1024^2 180 /
+// 113 / 146 / 239, 128 x 2048^2 649 / 561 / 405 / 530, 64 x 4096^2 1465 / 1007 / 696 /
+// 806, 16 x 8192^2 1512 / 1324 / 991 / 703 (each group has its array by distance).
+// 4 lanes where rows are short and many: 4 / 8 lanes forward 1024 x 128^2 29 / 35, 24 x
+// 257^2 7.7 / 5.8; backward 1024 x 128^2 30 / 36, 1024 x 257^2 117 / 87. (Windows, lanes
+// 4 / 8 / 16, forward: 144 x 759 x 2841, 615 keys seen, 183 / 162 / 150; 48 x 2000^2,
+// 128 seen, 102 / 86 / 83.)
+constexpr int64_t kTargetSmem = 74 * 1024;
 
 // Longer rows (in vectors) have one buffer a group instead of two, so half the lanes
 // a row; loads are then covered by the other groups alone. One / two buffers, us:
-// forward 1024 x 512^2 242 / 218, 256 x 1024^2 212 / 183, 128 x 2048^2 319 / 317,
-// 64 x 4096^2 578 / 607, 16 x 8192^2 570 / 631; backward 345 / 286, 354 / 317,
-// 424 / 430, 719 / 823, 712 / 778.
+// forward 1024 x 512^2 242 / 218, 256 x 1024^2 211 / 183, 128 x 2048^2 322 / 319,
+// 64 x 4096^2 581 / 607, 16 x 8192^2 570 / 631; backward 331 / 268, 128 x 1024^2 165 /
+// 146, 64 x 2048^2 213 / 210, 697 / 800, 702 / 762.
 constexpr int64_t kOneBuffer = 256;
 
 // matrices: 1 (scores) or 2 (probabilities and their gradient); words: fp32
@@ -172,7 +177,9 @@ int shape_of(const cs_bias_args* a, const cs_host::Device& d, int matrices, int6
     const int64_t block = std::max(cs::kBiasThreads, lanes), groups = block / lanes;
     return groups * (row_bytes + group_words * 4) + (words + block / 32 * 2) * 4;
   };
-  s.lanes = (nv <= 64 ? 8 : 16) * matrices;
+  const bool many = (int64_t)a->batch * a->heads * a->rows >= (int64_t)d.sms * 512;
+  const int64_t work = nv + (a->pitch / 8 - nv) / 4;  // vectors that get zeros alone are less work
+  s.lanes = work * matrices <= 32 && many ? 4 : work <= (matrices == 1 ? 96 : 64) ? 8 : 16;
   while (s.lanes < cs::kBiasMaxThreads && bytes(s.lanes) > kTargetSmem) s.lanes *= 2;
   s.block = std::max(cs::kBiasThreads, s.lanes);
   s.slots = (int)nv;

@@ -1,6 +1,6 @@
 // Causal softmax with a learned relative-position bias, and its gradient.
 //
-// A group of 8 to 256 lanes works on one row at a time. The row's visible 16-byte
+// A group of 4 to 256 lanes works on one row at a time. The row's visible 16-byte
 // vectors are copied to shared memory (cp.async) while the group works on the
 // row before (long rows: once it is done with it), and the passes (maximum, sum,
 // result; backward: the row's sum of p dp, result) read them there, so HBM sees
@@ -47,7 +47,7 @@ struct BiasParams {
   float* partial;       // backward: [matrix, CTA, buckets]
   int32_t heads, rows, cols, pitch, row_offset, window, sinks;
   int32_t ctas;         // per matrix
-  int32_t lanes;        // of a group: a power of two, 8 to 256
+  int32_t lanes;        // of a group: a power of two, 4 to 256
   int32_t slots;        // vectors of one shared-memory row buffer (0: rows stay in global memory)
   int32_t buckets, near;  // near: first distance of the last bucket
   float scale;
