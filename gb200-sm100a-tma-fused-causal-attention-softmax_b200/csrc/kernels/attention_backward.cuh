@@ -844,6 +844,7 @@ __global__ void __launch_bounds__(256) attention_dkv_join_kernel(const __grid_co
   for (int x = blockIdx.y * blockDim.x + threadIdx.x; x < 2 * kTile * DP / 4; x += gridDim.y * blockDim.x) {
     const int which = x / (kTile * DP / 4), at = x - which * (kTile * DP / 4), d = at / kTile * 4, row = at % kTile;
     float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
     for (int s = 0; s < shares; ++s) {
       const int64_t cta = (int64_t)(first + s) * heads + bk;
       const float4 v = reinterpret_cast<const float4*>(gp.partial)[(cta * 2 + which) * (kTile * DP / 4) + at];
