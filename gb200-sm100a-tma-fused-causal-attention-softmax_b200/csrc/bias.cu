@@ -145,33 +145,43 @@ Kernel kernel_of(int type, int matrices, int buffers) {
 
 // Few lanes a row keep the work that each row costs a warp (its geometry, the
 // reductions, the vectors near the diagonal) shared among several rows, and
-// shared memory for the groups' rows limits how few: a CTA takes up to
-// kTargetSmem, three CTAs an SM. Measured on B200 in us, lanes 8 / 16 / 32 / 64:
-// forward 1024 x 512^2 218 / 264 / 453 / 848, 1024 x 700^2 339 / 405 / 672 / -,
-// 256 x 1024^2 185 / 183 / 282 / 507, 128 x 2048^2 578 / 317 / 362 / 586, 64 x
-// 4096^2 991 / 578 / 605 / 854, 16 x 8192^2 1335 / 922 / 571 / 627; backward 1024 x
-// 512^2 251 / 268 / 461 / 792, 1024 x 700^2 470 / 394 / 671 / -, 128 x 1024^2 180 /
-// 113 / 146 / 239, 128 x 2048^2 649 / 561 / 405 / 530, 64 x 4096^2 1465 / 1007 / 696 /
-// 806, 16 x 8192^2 1512 / 1324 / 991 / 703 (each group has its array by distance).
-// 4 lanes where rows are short and many: 4 / 8 lanes forward 1024 x 128^2 29 / 35, 24 x
-// 257^2 7.7 / 5.8; backward 1024 x 128^2 30 / 36, 1024 x 257^2 117 / 87. (Windows, lanes
-// 4 / 8 / 16, forward: 144 x 759 x 2841, 615 keys seen, 183 / 162 / 150; 48 x 2000^2,
-// 128 seen, 102 / 86 / 83.)
-constexpr int64_t kTargetSmem = 74 * 1024;
+// shared memory for the groups' rows limits how few. Measured on B200 in us, lanes
+// 4 / 8 / 16 / 32 / 64: forward 1024 x 128^2 28 / 32 / 43 / 74, 24 x 257^2 7.7 / 5.7 / 6.0 /
+// 8.0, 1024 x 512^2 242 / 186 / 222 / 379, 128 x 1024^2 203 / 104 / 86 / 127, 64 x 2048^2
+// - / - / 158 / 184 / 275, 64 x 4096^2 - / - / 566 / 536 / 697, 8 x 8192^2 - / - / 454 / 289 /
+// 289; backward 1024 x 128^2 30 / 35 / 49 / 86, 24 x 257^2 9.3 / 7.9 / 8.7 / 11, 1024 x
+// 512^2 416 / 252 / 239 / 418, 128 x 1024^2 186 / 182 / 113 / 139, 64 x 2048^2 - / - / 199 /
+// 197 / 291, 64 x 4096^2 - / - / 1010 / 700 / 743, 8 x 8192^2 - / - / 685 / 503 / 362 (each
+// group has its array by distance). 4 lanes only where rows are short and many.
+// (Windows, lanes 4 / 8 / 16, forward: 144 x 759 x 2841, 615 keys seen, 183 / 162 / 150;
+// 48 x 2000^2, 128 seen, 102 / 86 / 83.)
+int least_lanes(int matrices, int64_t work, bool many) {
+  if (work * matrices <= 32 && many) return 4;
+  return work <= (matrices == 1 ? 96 : 64) ? 8 : 16;
+}
 
-// Longer rows (in vectors) have one buffer a group instead of two, so half the lanes
-// a row; loads are then covered by the other groups alone. One / two buffers, us:
-// forward 1024 x 512^2 242 / 218, 256 x 1024^2 211 / 183, 128 x 2048^2 322 / 319,
-// 64 x 4096^2 581 / 607, 16 x 8192^2 570 / 631; backward 331 / 268, 128 x 1024^2 165 /
-// 146, 64 x 2048^2 213 / 210, 697 / 800, 702 / 762.
-constexpr int64_t kOneBuffer = 256;
+// Long rows (in vectors) have one buffer a group instead of two and fewer lanes a
+// row; loads are then covered by the other groups alone. One / two buffers, us:
+// forward 128 x 1300^2 141 / 128, 64 x 2048^2 158 / 162, 32 x 3300^2 197 / 199, 32 x
+// 4096^2 279 / 309; backward 256 x 700^2 124 / 118, 128 x 1100^2 128 / 127, 96 x 1500^2
+// 164 / 179, 64 x 2048^2 197 / 210, 32 x 4096^2 356 / 409.
+int buffers_of(int matrices, int64_t vectors) { return vectors > (matrices == 1 ? 192 : 96) ? 1 : 2; }
+
+// Shared memory of a CTA at most, else more lanes a row (fewer groups): 74 KB
+// leaves three CTAs an SM, 56 four, 46 five. 32 x 4096^2 forward, one buffer: 46 KB 279 us,
+// 74 KB 293; 32 x 4096^2 backward, one buffer: 74 KB 356, 56 KB 381; 96 x 1500^2
+// forward, two buffers: 74 KB 130, 46 KB 160; 256 x 400^2 backward, two: 56 KB 53, 74 KB 61.
+int64_t most_smem(int matrices, int buffers) {
+  if (matrices == 1) return (buffers == 1 ? 46 : 74) * 1024;
+  return (buffers == 1 ? 74 : 56) * 1024;
+}
 
 // matrices: 1 (scores) or 2 (probabilities and their gradient); words: fp32
 // words a CTA needs besides, per group and once.
 int shape_of(const cs_bias_args* a, const cs_host::Device& d, int matrices, int64_t group_words, int64_t words, Shape* shape) {
   const int64_t nv = max_vectors(a);
   Shape s{};
-  s.buffers = nv > kOneBuffer ? 1 : 2;
+  s.buffers = buffers_of(matrices, nv);
   const int64_t row_bytes = nv * 16 * matrices * s.buffers;
   auto bytes = [&](int lanes) {
     const int64_t block = std::max(cs::kBiasThreads, lanes), groups = block / lanes;
@@ -179,8 +189,8 @@ int shape_of(const cs_bias_args* a, const cs_host::Device& d, int matrices, int6
   };
   const bool many = (int64_t)a->batch * a->heads * a->rows >= (int64_t)d.sms * 512;
   const int64_t work = nv + (a->pitch / 8 - nv) / 4;  // vectors that get zeros alone are less work
-  s.lanes = work * matrices <= 32 && many ? 4 : work <= (matrices == 1 ? 96 : 64) ? 8 : 16;
-  while (s.lanes < cs::kBiasMaxThreads && bytes(s.lanes) > kTargetSmem) s.lanes *= 2;
+  s.lanes = least_lanes(matrices, work, many);
+  while (s.lanes < cs::kBiasMaxThreads && bytes(s.lanes) > most_smem(matrices, s.buffers)) s.lanes *= 2;
   s.block = std::max(cs::kBiasThreads, s.lanes);
   s.slots = (int)nv;
   s.smem = (size_t)bytes(s.lanes);

@@ -81,8 +81,11 @@ struct Group {
     mask = n >= 32 ? 0xffffffffu : ((1u << n) - 1u) << (threadIdx.x & 31 & ~(n - 1));
   }
   __device__ __forceinline__ void sync() const {
+    // Barriers by number: with a number in a register the kernel would get all 16 of
+    // them, and the SM's 64 would hold it to four CTAs.
     if (lanes <= 32) __syncwarp(mask);
-    else asm volatile("bar.sync %0, %1;" ::"r"(1 + id), "r"(lanes) : "memory");
+    else if (id == 0) asm volatile("bar.sync 1, %0;" ::"r"(lanes) : "memory");
+    else asm volatile("bar.sync 2, %0;" ::"r"(lanes) : "memory");
   }
   __device__ __forceinline__ float max(float v, float* words) const {
     float m;
