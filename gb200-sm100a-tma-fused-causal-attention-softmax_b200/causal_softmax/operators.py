@@ -55,6 +55,16 @@ _PACK_GRADS = struct.Struct("@" + "P3q" * 4).pack
 
 _TYPES = {torch.float16: 0, torch.bfloat16: 1}
 
+_library = None
+
+
+def _lib():
+    """The library, without the loader's lock once it is there."""
+    global _library
+    if _library is None:
+        _library = lib()
+    return _library
+
 
 class _On:
     """A launch stream other than the current one of the current device, made current
@@ -165,7 +175,7 @@ def bias_softmax(x, table, bucket_starts, *, cols: int, scale: float, row_offset
         raise ValueError(f"table must be contiguous, [{heads}, {buckets}]")
     with _on(device, stream):
         out = _like("out", out, x)
-        check(lib().cs_bias_softmax(args, x.data_ptr(), table.data_ptr(), out.data_ptr(), _current(device)),
+        check(_lib().cs_bias_softmax(args, x.data_ptr(), table.data_ptr(), out.data_ptr(), _current(device)),
               "cs_bias_softmax")
     return out
 
@@ -181,7 +191,7 @@ def bias_softmax_backward(p, dp, bucket_starts, *, cols: int, scale: float, row_
     _same("dp", dp, p.dtype, device)
     if dp.shape != p.shape or not dp.is_contiguous():
         raise ValueError(f"dp must be contiguous, of shape {tuple(p.shape)}")
-    L = lib()
+    L = _lib()
     with _on(device, stream):
         ds = _like("out", out, p)
         dtable = torch.empty(heads, buckets, dtype=torch.float32, device=device)
@@ -197,7 +207,7 @@ def bias_softmax_backward(p, dp, bucket_starts, *, cols: int, scale: float, row_
 
 def _tensor(name: str, t, shape, dtype, device) -> tuple:
     """data, batch_stride, token_stride, head_stride."""
-    if t.dtype != dtype or t.device != device:
+    if t.dtype is not dtype or t.get_device() != device.index:
         raise TypeError(f"{name} must be {dtype} on {device}, not {t.dtype} on {t.device}")
     if t.shape != shape:
         raise ValueError(f"{name} must be {list(shape)}, not {list(t.shape)}")
@@ -253,7 +263,7 @@ def attention(q, k, v, *, scale: float | None = None, window: int = 0, sinks: in
     log-sum-exp [batch, heads, q_len] that attention_backward takes."""
     head = _attention_head(q, k, v, scale, window, sinks, q_lens, kv_lens)
     shape, dtype, device = q.shape, q.dtype, q.device
-    L = lib()
+    L = _lib()
     with _on(device, stream):
         if out is None:
             out = _fresh(q)
@@ -276,7 +286,7 @@ def attention_backward(dout, q, k, v, out, lse, *, scale: float | None = None, w
         raise ValueError(f"lse must be contiguous, {[shape[0], shape[2], shape[1]]}")
     args = _PACK_ATTENTION(*head, *_tensor("out", out, shape, dtype, device), lse.data_ptr())
     d_o = _tensor("dout", dout, shape, dtype, device)
-    L = lib()
+    L = _lib()
     with _on(device, stream):
         dq, dk, dv = _fresh(q), _fresh(k), _fresh(v)
         grads = _PACK_GRADS(*d_o, dq.data_ptr(), *dq.stride()[:3], dk.data_ptr(), *dk.stride()[:3],
