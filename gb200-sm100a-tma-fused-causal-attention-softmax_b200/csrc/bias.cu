@@ -109,7 +109,7 @@ int64_t max_vectors(const cs_bias_args* a) {
 // of its groups' rows and of its start and end, `ends` in quarters of a row (the
 // backward adds up its groups' arrays by distance). Numbers that fill whole rounds are
 // the candidates, and within 5% the one with more rounds, whose CTAs end more
-// evenly. Against four rounds always: backward 128 x 1024^2 146 us, 152; 16 x 2048^2
+// evenly. Against four rounds always, at the same lanes: backward 128 x 1024^2 146 us, 152; 16 x 2048^2
 // 57, 77; 24 x 257^2 8.8, 11.1; forward 16 x 2048^2 46, 55.
 int ctas_per_matrix(const cs_bias_args* a, int64_t resident, int groups, int ends) {
   const int64_t matrices = (int64_t)a->batch * a->heads, most = ((int64_t)a->rows + groups - 1) / groups;
