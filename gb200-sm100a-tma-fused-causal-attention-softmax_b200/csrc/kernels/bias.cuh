@@ -218,14 +218,12 @@ __global__ void __launch_bounds__(kBiasMaxThreads) bias_softmax_kernel(const __g
   const int cta = blockIdx.x - (int)(matrix * p.ctas);
   const float* table = p.table + (matrix % p.heads) * p.buckets;
   const int64_t base = matrix * p.rows * (int64_t)p.pitch;
-  const int step = p.ctas * groups;
-  int i = cta * groups + group.id;
-  auto nth = [&](int i) { return min(max(p.rows - 1 - i, 0), p.rows - 1); };  // the longest rows first
+  RowTurns turns(p.rows, cta * groups + group.id, p.ctas * groups);
 
   pdl_wait();
   auto source = [&](int r) { return reinterpret_cast<const uint4*>(p.x + base + (int64_t)r * p.pitch); };
   if (kStaged) {
-    if (i < p.rows) fetch_row(RowWalk(p, nth(i)), source(nth(i)), buffers, gt, gn);
+    if (turns.inside()) fetch_row(RowWalk(p, turns.row()), source(turns.row()), buffers, gt, gn);
     cp_async_commit();
   }
   for (int d = threadIdx.x - 8; d < p.near + 8; d += blockDim.x)
@@ -234,16 +232,16 @@ __global__ void __launch_bounds__(kBiasMaxThreads) bias_softmax_kernel(const __g
   const float far = tab[bias_slot(p.near)], sl = p.scale * kLog2e;
   const F2 far2 = f2(far, far), sl2 = f2(sl, sl);
 
-  RowWalk w(p, nth(i));
-  for (int turn = 0; i < p.rows; i += step, turn ^= 1) {
-    const int row = nth(i), after = nth(i + step);
+  RowWalk w(p, turns.row());
+  for (int turn = 0; turns.inside(); turns.next(), turn ^= 1) {
+    const int row = turns.row(), after = turns.next_row();
     uint4* out = reinterpret_cast<uint4*>(p.out + base + (int64_t)row * p.pitch);
     const uint4* in = source(row);
     const uint4* staged = buffers + (kBuffers == 2 ? turn * p.slots : 0);
     const RowWalk next(p, after);
     if (kBuffers == 2) {
       group.sync();  // the row before, in the other buffer, is done with
-      if (i + step < p.rows) fetch_row(next, source(after), buffers + (turn ^ 1) * p.slots, gt, gn);
+      if (!turns.last()) fetch_row(next, source(after), buffers + (turn ^ 1) * p.slots, gt, gn);
       cp_async_commit();
     }
     zero_masked(p, w, out, gt, gn);
@@ -328,7 +326,7 @@ __global__ void __launch_bounds__(kBiasMaxThreads) bias_softmax_kernel(const __g
     }
     if (kBuffers == 1) {
       group.sync();
-      if (i + step < p.rows) fetch_row(next, source(after), buffers, gt, gn);
+      if (!turns.last()) fetch_row(next, source(after), buffers, gt, gn);
       cp_async_commit();
     }
     w = next;
@@ -351,9 +349,7 @@ __global__ void __launch_bounds__(kBiasMaxThreads) bias_backward_kernel(const __
   const int64_t matrix = blockIdx.x / p.ctas;
   const int cta = blockIdx.x - (int)(matrix * p.ctas);
   const int64_t base = matrix * p.rows * (int64_t)p.pitch;
-  const int step = p.ctas * groups;
-  int i = cta * groups + group.id;
-  auto nth = [rows = p.rows](int i) { return max(rows - 1 - i, 0); };  // the longest rows first
+  RowTurns turns(p.rows, cta * groups + group.id, p.ctas * groups);
   for (int d = gt; d < slots; d += gn) acc[d] = 0.f;
 
   pdl_wait();
@@ -363,15 +359,15 @@ __global__ void __launch_bounds__(kBiasMaxThreads) bias_backward_kernel(const __
     fetch_row(w, source(p.dp, r), to + p.slots, gt, gn);
   };
   if (kStaged) {
-    if (i < p.rows) fetch(RowWalk(p, nth(i)), nth(i), buffers);
+    if (turns.inside()) fetch(RowWalk(p, turns.row()), turns.row(), buffers);
     cp_async_commit();
   }
   group.sync();
   float far = 0.f;
 
-  RowWalk w(p, nth(i));
-  for (int turn = 0; i < p.rows; i += step, turn ^= 1) {
-    const int row = nth(i), after = nth(i + step);
+  RowWalk w(p, turns.row());
+  for (int turn = 0; turns.inside(); turns.next(), turn ^= 1) {
+    const int row = turns.row(), after = turns.next_row();
     uint4* out = reinterpret_cast<uint4*>(p.out + base + (int64_t)row * p.pitch);
     const uint4* in = source(p.x, row);
     const uint4* in2 = source(p.dp, row);
@@ -379,7 +375,7 @@ __global__ void __launch_bounds__(kBiasMaxThreads) bias_backward_kernel(const __
     const RowWalk next(p, after);
     if (kBuffers != 1) group.sync();  // the row before is done with: its buffer, and its additions to acc
     if (kBuffers == 2) {
-      if (i + step < p.rows) fetch(next, after, buffers + (turn ^ 1) * 2 * p.slots);
+      if (!turns.last()) fetch(next, after, buffers + (turn ^ 1) * 2 * p.slots);
       cp_async_commit();
     }
     zero_masked(p, w, out, gt, gn);
@@ -473,7 +469,7 @@ __global__ void __launch_bounds__(kBiasMaxThreads) bias_backward_kernel(const __
     far += far3.x + far3.y;
     if (kBuffers == 1) {
       group.sync();
-      if (i + step < p.rows) fetch(next, after, buffers);
+      if (!turns.last()) fetch(next, after, buffers);
       cp_async_commit();
     }
     w = next;
