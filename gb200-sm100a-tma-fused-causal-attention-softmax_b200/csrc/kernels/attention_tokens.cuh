@@ -81,7 +81,7 @@ template <typename T, int DP, int NT>
 __global__ void __launch_bounds__(kTokenWarps * 32, NT == 1 ? 3 : 2) attention_tokens_kernel(const __grid_constant__ TokenParams tp) {
   constexpr int KC = DP / 32, VC = DP / 64, MT = DP / 16, kRows = 8 * NT;
   constexpr float kShift = T::kIsHalf ? 7.f : 0.f;
-  __shared__ float sm_o[kTokenWarps][kRows][DP + 4];
+  __shared__ __align__(16) float sm_o[kTokenWarps][kRows][DP + 4];
   __shared__ float sm_m[kTokenWarps][kRows], sm_l[kTokenWarps][kRows];
   const AttentionParams& p = tp.a;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
@@ -281,7 +281,8 @@ template <typename T, int kWarps>
 __global__ void __launch_bounds__(kWarps * 32) attention_join_kernel(const __grid_constant__ TokenParams tp) {
   constexpr float kShift = T::kIsHalf ? 7.f : 0.f;
   constexpr int kJoinThreads = kWarps * 32;
-  __shared__ float weight[kMaxSplits], sm_v[kWarps][128 + 4], words[kWarps];
+  __shared__ __align__(16) float sm_v[kWarps][128 + 4];
+  __shared__ float weight[kMaxSplits], words[kWarps];
   const AttentionParams& p = tp.a;
   const int rows = p.q_len * p.group, bk = blockIdx.x / rows, row = blockIdx.x - bk * rows;
   const int b = bk / p.kv_heads, hk = bk - b * p.kv_heads;

@@ -1,5 +1,7 @@
 """Host side of the operators beside the softmax at the edges of what they accept."""
+import glob
 import os
+import re
 import subprocess
 
 import causal_softmax as cs
@@ -15,3 +17,22 @@ def test_rows_of_a_group_up_to_the_largest_matrix(tmp_path):
                    check=True)
     out = subprocess.run([exe], capture_output=True, text=True)
     assert out.returncode == 0 and out.stdout.startswith("ok"), out.stdout + out.stderr
+
+
+VECTORS = r"reinterpret_cast<(?:const )?(?:float2|float4|uint2|uint4|double2)\*>\(&?(\w+)\["
+
+
+def test_shared_arrays_read_as_vectors_are_declared_aligned():
+    """A neighbour's size would otherwise decide whether a vector access of a float array is aligned."""
+    found = 0
+    for path in sorted(glob.glob(os.path.join(cs.PKG_DIR, "csrc", "kernels", "*.cuh"))):
+        with open(path, encoding="utf-8") as fh:
+            text = fh.read()
+        shared = {}
+        for declaration in re.findall(r"__shared__([^;]*);", text):
+            for name in re.findall(r"(\w+)\s*\[", re.sub(r"\[[^\]]*\]", "[", declaration)):
+                shared[name] = "__align__(16)" in declaration
+        for name in set(re.findall(VECTORS, text)) & set(shared):
+            assert shared[name], f"{os.path.basename(path)}: {name}"
+            found += 1
+    assert found >= 2
