@@ -234,7 +234,7 @@ __global__ void __launch_bounds__(kBiasMaxThreads) bias_softmax_kernel(const __g
 
   RowWalk w(p, turns.row());
   for (int turn = 0; turns.inside(); turns.next(), turn ^= 1) {
-    const int row = turns.row(), after = turns.next_row();
+    const int row = turns.at, after = turns.next_row();
     uint4* out = reinterpret_cast<uint4*>(p.out + base + (int64_t)row * p.pitch);
     const uint4* in = source(row);
     const uint4* staged = buffers + (kBuffers == 2 ? turn * p.slots : 0);
@@ -367,7 +367,7 @@ __global__ void __launch_bounds__(kBiasMaxThreads) bias_backward_kernel(const __
 
   RowWalk w(p, turns.row());
   for (int turn = 0; turns.inside(); turns.next(), turn ^= 1) {
-    const int row = turns.row(), after = turns.next_row();
+    const int row = turns.at, after = turns.next_row();
     uint4* out = reinterpret_cast<uint4*>(p.out + base + (int64_t)row * p.pitch);
     const uint4* in = source(p.x, row);
     const uint4* in2 = source(p.dp, row);
