@@ -185,7 +185,7 @@ int shape_of(const cs_bias_args* a, const cs_host::Device& d, int matrices, int6
   const int64_t row_bytes = nv * 16 * matrices * s.buffers;
   auto bytes = [&](int lanes) {
     const int64_t block = std::max(cs::kBiasThreads, lanes), groups = block / lanes;
-    return groups * (row_bytes + group_words * 4) + (words + block / 32 * 2) * 4;
+    return groups * (row_bytes + group_words * 4) + (words + block / 32 * (matrices == 1 ? 4 : 2)) * 4;
   };
   const bool many = (int64_t)a->batch * a->heads * a->rows >= (int64_t)d.sms * 512;
   const int64_t work = nv + (a->pitch / 8 - nv) / 4;  // vectors that get zeros alone are less work

@@ -24,6 +24,12 @@
 // the subtraction into the multiply-add would leave the rounding error of the
 // maximum, which a large scale blows up.
 //
+// A row whose maximum is kNarrow or more in magnitude, or a head whose table holds
+// a number that large, leaves these fp32 exponents: their rounding would be a
+// hundredth of a unit and more, and a finite score next to the type's ends (its
+// lowest value as a mask) times log2 e is infinite. wide_row works such rows out in
+// binary64, relative to the row's largest score. fp16 scores at a scale of up to 1 never are.
+//
 // Table gradient: a row holds each distance once, so a group adds its row's dz
 // into its own array by distance without conflicts, row after row: no atomics,
 // and the sums come in a fixed order. Distances in the last bucket go to a
@@ -40,6 +46,7 @@ namespace cs {
 constexpr int kMaxBuckets = 128;
 constexpr int kBiasThreads = 128;     // CTA size while a row takes at most 4 warps
 constexpr int kBiasMaxThreads = 256;  // rows of 8 warps
+constexpr float kNarrow = 131072.f;   // 2^17, in units of log2
 
 struct BiasParams {
   const uint16_t* x;    // scores; backward: probabilities
@@ -98,6 +105,25 @@ struct Group {
       for (int k = 0; k < lanes >> 5; ++k) m = fmaxf(m, words[k]);
     }
     return m;
+  }
+  // The same for binary64 and any operation; words: two per warp. Its own barriers
+  // keep the words from other uses, before and after.
+  template <typename Op>
+  __device__ __forceinline__ double join(double v, float* words, Op op) const {
+    for (int o = (lanes < 32 ? lanes : 32) >> 1; o > 0; o >>= 1) v = op(v, __shfl_xor_sync(mask, v, o));
+    if (lanes > 32) {
+      sync();
+      if ((rank & 31) == 0) {
+        words[rank >> 4] = __int_as_float(__double2hiint(v));
+        words[(rank >> 4) + 1] = __int_as_float(__double2loint(v));
+      }
+      sync();
+      v = __hiloint2double(__float_as_int(words[0]), __float_as_int(words[1]));
+      for (int k = 1; k < lanes >> 5; ++k)
+        v = op(v, __hiloint2double(__float_as_int(words[2 * k]), __float_as_int(words[2 * k + 1])));
+      sync();
+    }
+    return v;
   }
   __device__ __forceinline__ float sum(float v, float* words) const {
     for (int o = (lanes < 32 ? lanes : 32) >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(mask, v, o);
@@ -202,6 +228,72 @@ __device__ __forceinline__ float sum8(const float* z) {
   return ((z[0] + z[1]) + (z[2] + z[3])) + ((z[4] + z[5]) + (z[6] + z[7]));
 }
 
+// A row in binary64: scale (x - top) + bias, top the largest score seen, so that
+// neither overflows and the bias counts beside scores of any size. A lane takes one
+// column at a time. table: the head's.
+template <typename T>
+__device__ __forceinline__ void wide_row(const BiasParams& p, const RowWalk& w, const Group& group, const uint16_t* from,
+                                         const float* table, float* words, uint16_t* out) {
+  constexpr double kInfinity = INFINITY, kLog2 = 1.4426950408889634;
+  auto larger = [](double a, double b) { return fmax(a, b); };
+  // f(column, score, whether it is seen) of this lane's columns among the visible vectors.
+  auto each = [&](auto f) {
+#pragma unroll 1
+    for (uint32_t i = group.rank; i < (uint32_t)w.m.n * 8u; i += group.lanes) {
+      const int at = vector_at(w.m, i >> 3) * 8, e = i & 7;
+      f(at + e, T::unpack(from[at + e]).x, ((visible_bits(w.v, at) >> e) & 1) != 0);
+    }
+  };
+  double top = -kInfinity;
+  each([&](int, float x, bool seen) {
+    if (seen) top = fmax(top, x == x ? (double)x : kInfinity);  // a NaN: on to the sum
+  });
+  top = group.join(top, words, larger);
+  const bool none = top == -kInfinity;  // all of them -infinity: zeros
+  if (top == kInfinity) top = 0.0;
+  auto score = [&](int c, float x) {
+    return (double)p.scale * ((double)x - top) + (double)table[bucket_of(p, w.pos - c)];
+  };
+  double m = -kInfinity, s = 0.0;
+  if (!none) {
+    each([&](int c, float x, bool seen) {
+      if (seen) m = fmax(m, score(c, x));
+    });
+    m = group.join(m, words, larger);
+    if (m == -kInfinity) m = 0.0;  // every exponential is 0
+    each([&](int c, float x, bool seen) {
+      if (seen) s += ex2((float)((score(c, x) - m) * kLog2));
+    });
+    s = group.join(s, words, [](double a, double b) { return a + b; });
+  }
+  const float inv = s == 0.0 ? 0.f : rcp_rn((float)s);  // a NaN stays one
+  each([&](int c, float x, bool seen) {
+    out[c] = seen && !none ? (uint16_t)T::pack(ex2((float)((score(c, x) - m) * kLog2)) * inv, 0.f) : (uint16_t)0;
+  });
+}
+
+// A warp's wide rows once more: the marked ones, or all of them. (Kept apart from the
+// main loop, which pays for a register more or a call in it with every row: rows of
+// 512 columns bf16 188 us, 195 to 219.)
+template <typename T>
+__device__ __forceinline__ void wide_rows(const BiasParams& p, float* words, bool all) {
+  const Group group(p.lanes);
+  const int groups = blockDim.x / p.lanes;
+  const int64_t matrix = blockIdx.x / p.ctas;
+  const int cta = blockIdx.x - (int)(matrix * p.ctas);
+  words += (threadIdx.x / 32 - group.rank / 32) * 2;
+  group.sync();  // the other warps' marks
+  for (RowTurns turns(p.rows, cta * groups + group.id, p.ctas * groups); turns.inside(); turns.next()) {
+    const RowWalk w(p, turns.at);
+    if (w.m.n == 0) continue;
+    const int64_t row = (matrix * p.rows + turns.at) * p.pitch;
+    uint16_t* out = p.out + row;
+    const float mark = T::unpack(out[w.v.s_end > 0 ? 0 : w.v.lo]).x;
+    group.sync();  // all have read it
+    if (all || mark != mark) wide_row<T>(p, w, group, p.x + row, p.table + (matrix % p.heads) * p.buckets, words, out);
+  }
+}
+
 // kBuffers: of a group in shared memory, p.slots vectors each; 0: rows stay in global memory.
 template <typename T, int kBuffers>
 __global__ void __launch_bounds__(kBiasMaxThreads) bias_softmax_kernel(const __grid_constant__ BiasParams p) {
@@ -212,6 +304,8 @@ __global__ void __launch_bounds__(kBiasMaxThreads) bias_softmax_kernel(const __g
   uint4* buffers = smem + group.id * kBuffers * p.slots;
   float* tab = reinterpret_cast<float*>(smem + groups * kBuffers * p.slots);  // bias by distance, [0, near]
   float* words = tab + bias_slots(p.near);  // two per warp, for groups of several warps
+  // Whether this warp met wide rows; whether all rows are.
+  int* wide = reinterpret_cast<int*>(words + (blockDim.x / 32 + threadIdx.x / 32) * 2);
   float* words_max = words + (threadIdx.x / 32 - gt / 32) * 2;
   float* words_sum = words_max + (gn >> 5);
   const int64_t matrix = blockIdx.x / p.ctas;
@@ -226,9 +320,14 @@ __global__ void __launch_bounds__(kBiasMaxThreads) bias_softmax_kernel(const __g
     if (turns.inside()) fetch_row(RowWalk(p, turns.row()), source(turns.row()), buffers, gt, gn);
     cp_async_commit();
   }
-  for (int d = threadIdx.x - 8; d < p.near + 8; d += blockDim.x)
-    tab[bias_slot(d)] = table[bucket_of(p, max(d, 0))] * kLog2e;
-  __syncthreads();
+  bool large = false;
+  for (int d = threadIdx.x - 8; d < p.near + 8; d += blockDim.x) {
+    const float v = table[bucket_of(p, max(d, 0))], t = v * kLog2e;
+    large |= fabsf(t) >= kNarrow && fabsf(v) < INFINITY;
+    tab[bias_slot(d)] = t;
+  }
+  wide[0] = 0;
+  wide[1] = __syncthreads_or(large);
   const float far = tab[bias_slot(p.near)], sl = p.scale * kLog2e;
   const F2 far2 = f2(far, far), sl2 = f2(sl, sl);
 
@@ -272,7 +371,7 @@ __global__ void __launch_bounds__(kBiasMaxThreads) bias_softmax_kernel(const __g
       const float2 t = T::unpack(most);
       m = fmaxf(m, __fmaf_rn(fmaxf(t.x, t.y), sl, far));
     }
-    m = fmaxf(group.max(m, words_max), -3.0e38f);  // a row of -infinity only: every exponential is 0
+    m = group.max(m, words_max);
     const F2 minus_m = f2(-m, -m);
 
     float s = 0.f;
@@ -297,7 +396,12 @@ __global__ void __launch_bounds__(kBiasMaxThreads) bias_softmax_kernel(const __g
     }
     const float2 s4 = f2_out(f2_add(s2, s3));
     s = group.sum(s + (s4.x + s4.y), words_sum);
-    const float inv = s == 0.f ? 0.f : rcp_rn(s);  // a NaN stays one
+    // s >= 1, or a NaN. A wide row is marked: NaN in all visible columns.
+    float inv = rcp_rn(s);
+    if (!(fabsf(m) < kNarrow)) {
+      inv = NAN;
+      wide[0] = 1;
+    }
     const F2 inv2 = f2(inv, inv);
 
     if (gt < others) {
@@ -331,6 +435,8 @@ __global__ void __launch_bounds__(kBiasMaxThreads) bias_softmax_kernel(const __g
     }
     w = next;
   }
+  __syncwarp();
+  if (wide[0] || wide[1]) wide_rows<T>(p, words, wide[1] != 0);
   pdl_trigger();
 }
 

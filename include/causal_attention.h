@@ -69,8 +69,11 @@ typedef struct cs_bias_args {
 
 /* p = softmax over the visible keys of scale * x + table[head, bucket(position
  * - key)]; every other column of the row, padding included, +0.0. The table
- * is fp32, [heads, buckets]. Arithmetic is binary32. x and p must not
- * overlap. A row whose visible scores are all -infinity is all zeros. */
+ * is fp32, [heads, buckets]. Arithmetic is binary32, and binary64 relative to
+ * the row's largest score where biased scores reach 90000 in magnitude, so that
+ * finite ones stay finite up to the ends of their types (a mask of the lowest
+ * value). x and p must not overlap. A row whose visible scores are all -infinity is
+ * all zeros; one with a NaN or +infinity among them is NaN. */
 int cs_bias_softmax(const cs_bias_args *args, const void *x, const float *table, void *p, void *stream);
 
 /* From probabilities p and their gradient dp: dz = p (dp - sum p dp) over the

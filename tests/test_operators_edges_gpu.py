@@ -1,0 +1,103 @@
+"""GPU tests of the operators beside the softmax at the edges of what they accept:
+scores at the ends of the type's range, NaN and infinities in seen places, rows of
+very different sizes."""
+import math
+
+import pytest
+import torch
+
+import attention_ref as ref
+import causal_softmax as cs
+from test_operators_gpu import BF16, F16, randn, status_ok, within
+
+pytestmark = pytest.mark.gpu
+
+
+# ---------------------------------------------------------------- biased softmax
+
+def shifted_bias_softmax(x, table, starts, *, cols, scale, row_offset=0, window=0, sinks=0):
+    """The definition in 64 bits with each row's scores relative to its largest one (the softmax
+    does not change), so that scores at the ends of the range keep their bias; and the bound of
+    a result rounded once from exponentials of relative error 2^-16 (an argument above -128 in
+    units of log2 rounded to 24 bits)."""
+    pos = torch.arange(x.shape[2], device=x.device) + row_offset
+    keep = ref.mask(pos, cols, window, sinks)
+    s = torch.where(keep, x[..., :cols].double(), -math.inf)
+    top = s.amax(-1, keepdim=True)
+    s = s - torch.where(top.isinf(), 0.0, top)
+    z = torch.where(keep, scale * s + table.double()[:, ref.buckets(pos, cols, starts)], -math.inf)
+    p = torch.zeros(x.shape, dtype=torch.float64, device=x.device)
+    p[..., :cols] = ref.softmax_rows(z)[0]
+    return p, p * (ref.half_step(x.dtype) + 2 ** -15) + ref.tiny(x.dtype) + ref.FLUSHED
+
+
+EXTREME = [
+    # batch, heads, rows, cols, row_offset, window, sinks: rows of one lane's vectors to several warps' and unstaged ones
+    (1, 2, 24, 24, 0, 0, 0),
+    (40, 16, 120, 120, 0, 0, 0),
+    (2, 2, 24, 700, 600, 200, 3),
+    (1, 2, 24, 2500, 2476, 0, 0),
+    (1, 1, 24, 9001, 8977, 0, 0),
+    (1, 1, 24, 34000, 33976, 0, 0),
+    (1, 1, 24, 70001, 69977, 0, 0),
+]
+
+
+@pytest.mark.parametrize("case", EXTREME)
+@pytest.mark.parametrize("scale", [1.0, 0.125, 1e30])
+def test_bias_scores_at_the_ends_of_the_range(case, scale):
+    """Only infinite scores count as infinite: finite ones whose multiple of log2 e is not finite stay what they are."""
+    batch, heads, rows, cols, row_offset, window, sinks = case
+    starts = cs.bias_buckets(16, 64)
+    how = dict(cols=cols, scale=scale, row_offset=row_offset, window=window, sinks=sinks)
+    x = randn(batch, heads, rows, cs.padded_pitch(cols), dtype=BF16, seed=1)
+    table = randn(heads, 16, dtype=torch.float32, seed=2)
+    low, high = torch.finfo(BF16).min, torch.finfo(BF16).max
+    x[:, :, 3] = low                       # masked by the lowest value everywhere: the softmax of the bias
+    x[:, :, 4] = high
+    x[:, :, 5, ::2], x[:, :, 5, 1::2] = low, high
+    x[:, :, 6, ::3] = high                 # some at the top, others ordinary
+    x[:, :, 7] = low
+    x[:, :, 7, 2::5] = -3.1e38             # the lowest and a little above it
+    x[:, :, 8] = 3.1e38
+    x[:, :, 8, 1::4] = 2.9e38
+    x[:, :, 9] = -math.inf                 # nothing but -infinity: zeros
+    x[:, :, 10] = -math.inf
+    x[:, :, 10, 3::2] = low                # the lowest value and -infinity
+    x[:, :, 11] = -2.5e38
+    x[:, :, 12] = 1e10
+    x[:, :, 12, ::2] = 1.0078125e10
+    got = cs.bias_softmax(x, table, starts, **how)
+    want, bound = shifted_bias_softmax(x, table, starts, **how)
+    within(got[:, :, 3:13], want[:, :, 3:13], bound[:, :, 3:13], "p")
+    assert not got[:, :, 9].any()
+    assert (got[:, :, 3:9].double().sum(-1) > 0.9).all()
+    plain, plain_bound = ref.bias_softmax(x[:, :, :3], table, starts, **how)  # the rows beside them
+    if scale <= 1:
+        within(got[:, :, :3], plain, plain_bound, "ordinary rows")
+    x[:, :, 3:9, 0] = math.nan             # the first sinks, or the first key where there is no window
+    x[:, :, 10, 0] = math.inf
+    got = cs.bias_softmax(x, table, starts, **how)
+    seen = ref.mask(torch.arange(rows, device="cuda") + row_offset, cols, window, sinks)
+    for row in (*range(3, 9), 10):
+        if seen[row, 0]:
+            assert torch.isnan(got[:, :, row, :cols][..., seen[row]]).all(), row
+        assert not got[:, :, row, :cols][..., ~seen[row]].any()
+
+
+def test_bias_tables_at_the_ends_of_the_range():
+    starts, x = (0, 1, 2, 3, 11), randn(2, 3, 40, 40, dtype=BF16, seed=1)
+    f = torch.finfo(torch.float32)
+    for values in ((f.min, f.min, 0.0, 1.0, -1.0), (f.max, 0.0, f.max, 1.0, f.min), (-math.inf, f.min, -3e38, f.min, f.min),
+                   (-math.inf, -math.inf, 0.5, -math.inf, -math.inf), (f.min, f.min, f.min, f.min, f.min)):
+        table = torch.tensor([values] * 3, device="cuda")
+        table[1] = randn(5, dtype=torch.float32, seed=3)  # a head with an ordinary one
+        how = dict(cols=40, scale=0.125)
+        want, bound = shifted_bias_softmax(x, table, starts, **how)
+        # In 64 bits scores vanish beside a bias of 3e38, as they do here.
+        within(cs.bias_softmax(x, table, starts, **how), want, bound + want * 2 ** -15, str(values))
+    table = torch.tensor([[f.max, f.max]], device="cuda")  # cancels against the scores
+    x = torch.full((1, 1, 4, 8), -3.3e38, dtype=BF16, device="cuda")
+    x[..., 0] = 0.0
+    got = cs.bias_softmax(x, table, (0, 2), cols=4, scale=1.0)[0, 0, :, :4]
+    assert torch.equal(got, torch.eye(4, dtype=BF16, device="cuda")[[0, 0, 0, 0]])
