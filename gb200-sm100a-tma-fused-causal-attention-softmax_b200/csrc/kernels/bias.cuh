@@ -24,11 +24,11 @@
 // the subtraction into the multiply-add would leave the rounding error of the
 // maximum, which a large scale blows up.
 //
-// A row whose maximum is kNarrow or more in magnitude, or a head whose table holds
-// a number that large, leaves these fp32 exponents: their rounding would be a
-// hundredth of a unit and more, and a finite score next to the type's ends (its
-// lowest value as a mask) times log2 e is infinite. wide_row works such rows out in
-// binary64, relative to the row's largest score. fp16 scores at a scale of up to 1 never are.
+// A row whose maximum is kNarrow or more in magnitude leaves these fp32 exponents:
+// their rounding would be a hundredth of a unit and more, and a finite score next to
+// the type's ends (its lowest value as a mask) times log2 e is infinite. wide_row works
+// such rows out in binary64, relative to the row's largest score; by their scores, fp16
+// rows at a scale of up to 1 never are.
 //
 // Table gradient: a row holds each distance once, so a group adds its row's dz
 // into its own array by distance without conflicts, row after row: no atomics,
@@ -244,31 +244,42 @@ __device__ __forceinline__ void wide_row(const BiasParams& p, const RowWalk& w, 
       f(at + e, T::unpack(from[at + e]).x, ((visible_bits(w.v, at) >> e) & 1) != 0);
     }
   };
-  double top = -kInfinity;
-  each([&](int, float x, bool seen) {
-    if (seen) top = fmax(top, x == x ? (double)x : kInfinity);  // a NaN: on to the sum
-  });
-  top = group.join(top, words, larger);
-  const bool none = top == -kInfinity;  // all of them -infinity: zeros
+  // The largest score; +infinity if one is a NaN: on to the sum.
+  float most = -INFINITY;
+  for (int j = group.rank; j < w.m.n; j += group.lanes) {
+    const int at = vector_at(w.m, j) * 8;
+    float x[8];
+    unpack8<T>(*reinterpret_cast<const uint4*>(from + at), x);
+    const uint32_t bits = visible_bits(w.v, at);
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if ((bits >> e) & 1) most = fmaxf(most, x[e] == x[e] ? x[e] : INFINITY);
+  }
+  double top = group.join(most, words, larger);
+  if (top == -kInfinity) {  // all of them -infinity
+    for (int j = group.rank; j < w.m.n; j += group.lanes)
+      *reinterpret_cast<uint4*>(out + vector_at(w.m, j) * 8) = make_uint4(0, 0, 0, 0);
+    return;
+  }
   if (top == kInfinity) top = 0.0;
+  const double last = table[p.buckets - 1];
   auto score = [&](int c, float x) {
-    return (double)p.scale * ((double)x - top) + (double)table[bucket_of(p, w.pos - c)];
+    const int d = w.pos - c;
+    return (double)p.scale * ((double)x - top) + (d >= p.near ? last : (double)table[bucket_of(p, d)]);
   };
   double m = -kInfinity, s = 0.0;
-  if (!none) {
-    each([&](int c, float x, bool seen) {
-      if (seen) m = fmax(m, score(c, x));
-    });
-    m = group.join(m, words, larger);
-    if (m == -kInfinity) m = 0.0;  // every exponential is 0
-    each([&](int c, float x, bool seen) {
-      if (seen) s += ex2((float)((score(c, x) - m) * kLog2));
-    });
-    s = group.join(s, words, [](double a, double b) { return a + b; });
-  }
+  each([&](int c, float x, bool seen) {
+    if (seen) m = fmax(m, score(c, x));
+  });
+  m = group.join(m, words, larger);
+  if (m == -kInfinity) m = 0.0;  // by the bias: every exponential is 0
+  each([&](int c, float x, bool seen) {
+    if (seen) s += ex2((float)((score(c, x) - m) * kLog2));
+  });
+  s = group.join(s, words, [](double a, double b) { return a + b; });
   const float inv = s == 0.0 ? 0.f : rcp_rn((float)s);  // a NaN stays one
   each([&](int c, float x, bool seen) {
-    out[c] = seen && !none ? (uint16_t)T::pack(ex2((float)((score(c, x) - m) * kLog2)) * inv, 0.f) : (uint16_t)0;
+    out[c] = seen ? (uint16_t)T::pack(ex2((float)((score(c, x) - m) * kLog2)) * inv, 0.f) : (uint16_t)0;
   });
 }
 
@@ -323,8 +334,8 @@ __global__ void __launch_bounds__(kBiasMaxThreads) bias_softmax_kernel(const __g
   bool large = false;
   for (int d = threadIdx.x - 8; d < p.near + 8; d += blockDim.x) {
     const float v = table[bucket_of(p, max(d, 0))], t = v * kLog2e;
-    large |= fabsf(t) >= kNarrow && fabsf(v) < INFINITY;
-    tab[bias_slot(d)] = t;
+    large |= t >= 0x1p126f;  // a score's sum with it may not fit
+    tab[bias_slot(d)] = t < -0x1p127f ? -0x1p127f : t;  // a mask; rows of nothing else are wide
   }
   wide[0] = 0;
   wide[1] = __syncthreads_or(large);
@@ -371,7 +382,7 @@ __global__ void __launch_bounds__(kBiasMaxThreads) bias_softmax_kernel(const __g
       const float2 t = T::unpack(most);
       m = fmaxf(m, __fmaf_rn(fmaxf(t.x, t.y), sl, far));
     }
-    m = group.max(m, words_max);
+    m = fmaxf(group.max(m, words_max), -3.0e38f);  // a row of -infinity only: every exponential is 0
     const F2 minus_m = f2(-m, -m);
 
     float s = 0.f;
@@ -396,11 +407,12 @@ __global__ void __launch_bounds__(kBiasMaxThreads) bias_softmax_kernel(const __g
     }
     const float2 s4 = f2_out(f2_add(s2, s3));
     s = group.sum(s + (s4.x + s4.y), words_sum);
-    // s >= 1, or a NaN. A wide row is marked: NaN in all visible columns.
-    float inv = rcp_rn(s);
+    float inv = rcp_rn(s);  // s >= 1, or a NaN
     if (!(fabsf(m) < kNarrow)) {
-      inv = NAN;
-      wide[0] = 1;
+      // Nothing but -infinity: so were the scores, if their multiples are finite. Else a
+      // wide row, marked by NaN in all visible columns.
+      inv = s == 0.f && (T::kIsHalf || p.scale < 0.5f) ? 0.f : NAN;
+      if (inv != 0.f) wide[0] = 1;
     }
     const F2 inv2 = f2(inv, inv);
 
