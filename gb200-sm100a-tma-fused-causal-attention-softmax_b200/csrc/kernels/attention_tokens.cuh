@@ -303,9 +303,10 @@ __global__ void __launch_bounds__(kWarps * 32) attention_join_kernel(const __gri
   __syncthreads();
   float sum = 0.f;
   for (int s = threadIdx.x; s < tp.splits; s += kJoinThreads) {
-    const float f = weight[s] == -INFINITY ? 0.f : ex2(weight[s] - top);
+    const bool none = weight[s] == -INFINITY;
+    const float f = none ? 0.f : ex2(weight[s] - top);
     weight[s] = f;
-    if (f != 0.f) sum = __fmaf_rn(f, tp.part_stats[(first + (int64_t)s * tp.rows) * 2 + 1], sum);
+    if (!none) sum = __fmaf_rn(f, tp.part_stats[(first + (int64_t)s * tp.rows) * 2 + 1], sum);  // a NaN goes on at any weight
   }
   sum = warp_sum(sum);
   if (lane == 0) words[warp] = sum;
@@ -319,7 +320,7 @@ __global__ void __launch_bounds__(kWarps * 32) attention_join_kernel(const __gri
     for (int s = warp; s < tp.splits; s += kWarps) {
       const float4 x = *reinterpret_cast<const float4*>(tp.part_o + (first + (int64_t)s * tp.rows) * tp.dim_pad + d);
       const float f = weight[s];
-      if (f != 0.f) {  // a split without keys holds nothing
+      if (f != 0.f) {  // a split without keys may hold anything
         v.x = __fmaf_rn(f, x.x, v.x);
         v.y = __fmaf_rn(f, x.y, v.y);
         v.z = __fmaf_rn(f, x.z, v.z);

@@ -101,3 +101,64 @@ def test_bias_tables_at_the_ends_of_the_range():
     x[..., 0] = 0.0
     got = cs.bias_softmax(x, table, (0, 2), cols=4, scale=1.0)[0, 0, :, :4]
     assert torch.equal(got, torch.eye(4, dtype=BF16, device="cuda")[[0, 0, 0, 0]])
+
+
+# ---------------------------------------------------------------- attention
+
+def one_key(value, dim, dtype):
+    """A key whose product with a query of ones is value."""
+    k = torch.zeros(dim, dtype=dtype, device="cuda")
+    k[0] = value
+    return k
+
+
+UNUSUAL = [
+    # batch, q_len, kv_len, heads, kv_heads: one token in one split and in several; few and many rows of tiles, split and whole
+    (128, 1, 96, 4, 4),
+    (300, 1, 300, 8, 8),
+    (1, 1, 4000, 8, 1),
+    (1, 1, 30000, 16, 1),
+    (1, 2, 4000, 8, 1),
+    (1, 40, 4000, 2, 1),
+    (1, 200, 460, 2, 2),
+    (1, 130, 20000, 1, 1),
+]
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("case", UNUSUAL)
+@pytest.mark.parametrize("near", [True, False])
+def test_nan_and_infinite_scores_at_seen_keys(case, dtype, near):
+    """The largest score stands in the last key, an unusual one in the first keys (far from it in other splits or
+    tiles) or next to it; scores differ by more than an exponential's range."""
+    batch, q_len, kv_len, heads, kv_heads = case
+    dim = 64
+    q = torch.zeros(batch, q_len, heads, dim, dtype=dtype, device="cuda")
+    q[..., 0] = 1.0
+    v = randn(batch, kv_len, kv_heads, dim, dtype=dtype, seed=1)
+    where = kv_len - q_len if near else 3  # every query sees it
+
+    def call(value, last=300.0, rest=0.0):
+        k = torch.zeros(batch, kv_len, kv_heads, dim, dtype=dtype, device="cuda")
+        k[..., 0] = rest
+        k[:, kv_len - q_len - 1] = one_key(last, dim, dtype)
+        k[:, where] = one_key(value, dim, dtype)
+        out, lse = cs.attention(q, k, v, scale=1.0, return_lse=True)
+        status_ok()
+        return k, out, lse
+
+    for value in (math.nan, math.inf):
+        _, out, lse = call(value)
+        assert torch.isnan(out).all() and torch.isnan(lse).all(), value
+    _, out, lse = call(-math.inf)
+    k = call(-30000.0)[0]  # the same probability 0 in 64 bits, and a finite bound
+    k0 = k.clone()
+    k0[k0 == -30000.0] = 0.0
+    want, _, wl, _ = ref.attention(q, k, v, scale=1.0)
+    _, bound, _, bl = ref.attention(q, k0, v, scale=1.0)  # bounds of the scores that count
+    within(out, want, bound, "out")
+    within(lse, wl, bl, "lse")
+    _, out, lse = call(-math.inf, -math.inf, -math.inf)  # nothing but -infinity
+    assert not out.any() and torch.isneginf(lse).all()
+    _, out, lse = call(math.nan, -math.inf, -math.inf)
+    assert torch.isnan(out).all() and torch.isnan(lse).all()
