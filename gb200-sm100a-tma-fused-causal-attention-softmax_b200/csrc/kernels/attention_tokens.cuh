@@ -264,6 +264,7 @@ __global__ void __launch_bounds__(kTokenWarps * 32, NT == 1 ? 3 : 2) attention_t
     } else {
       const int i = r / p.group, h = hk * p.group + r - i * p.group;
       const float inv = sum == 0.f ? 0.f : rcp_rn(sum);
+      if (sum == 0.f) v = make_float4(0.f, 0.f, 0.f, 0.f);  // 0 times another row's NaN among the values
       if (d < p.head_dim)
         *reinterpret_cast<uint2*>(p.o.at(b, i, h) + d) = make_uint2(T::pack(v.x * inv, v.y * inv), T::pack(v.z * inv, v.w * inv));
       if (d == 0 && p.lse)

@@ -162,3 +162,26 @@ def test_nan_and_infinite_scores_at_seen_keys(case, dtype, near):
     assert not out.any() and torch.isneginf(lse).all()
     _, out, lse = call(math.nan, -math.inf, -math.inf)
     assert torch.isnan(out).all() and torch.isnan(lse).all()
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("value", [math.nan, math.inf])
+@pytest.mark.parametrize("q_len,kv_len,heads,kv_heads", [
+    (1, 100, 4, 4), (3, 100, 8, 4), (2, 200, 8, 1), (3, 5000, 8, 4), (2, 5000, 8, 1), (40, 100, 8, 4), (40, 5000, 2, 2),
+])
+def test_rows_that_see_nothing_are_zero_beside_values_that_are_no_numbers(q_len, kv_len, heads, kv_heads, value, dtype):
+    """Padded rows and queries before the first key, in batches whose other rows meet a NaN or an infinity."""
+    q, k, v = (randn(3, n, h, 64, dtype=dtype, seed=i) for i, (n, h) in
+               enumerate(((q_len, heads), (kv_len, kv_heads), (kv_len, kv_heads))))
+    v[:, 0] = value
+    q_lens = torch.tensor([max(0, q_len - 1), q_len, q_len], dtype=torch.int32, device="cuda")
+    kv_lens = torch.tensor([kv_len, kv_len, max(0, q_len - 1)], dtype=torch.int32, device="cuda")
+    out, lse = cs.attention(q, k, v, q_lens=q_lens, kv_lens=kv_lens, return_lse=True)
+    status_ok()
+    sees = torch.ones(3, q_len, dtype=torch.bool, device="cuda")
+    sees[0, q_len - 1] = False  # behind the sequence's queries
+    sees[2, 0] = False          # at position -1
+    assert not out[~sees].any(), "rows that see nothing are zero"
+    assert torch.isneginf(lse.transpose(1, 2)[~sees]).all() and not torch.isneginf(lse.transpose(1, 2)[sees]).any()
+    assert not torch.isfinite(out[sees]).any(), "every other query sees key 0"
+    assert torch.isfinite(lse.transpose(1, 2)[sees]).all()
