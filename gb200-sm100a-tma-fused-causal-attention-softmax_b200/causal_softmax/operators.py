@@ -101,7 +101,10 @@ def _current(device) -> int:
 def _int(name: str, v) -> int:
     if not -_I32_MAX <= v <= _I32_MAX:
         raise ValueError(f"{name} {v} does not fit 32 bits")
-    return int(v)
+    n = int(v)
+    if n != v:
+        raise ValueError(f"{name} {v} is not a whole number")
+    return n
 
 
 def _same(name: str, t, dtype, device) -> None:

@@ -4,7 +4,10 @@ import os
 import re
 import subprocess
 
+import pytest
+
 import causal_softmax as cs
+from causal_softmax import operators as ops
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
@@ -36,3 +39,10 @@ def test_shared_arrays_read_as_vectors_are_declared_aligned():
             assert shared[name], f"{os.path.basename(path)}: {name}"
             found += 1
     assert found >= 2
+
+
+def test_whole_numbers_are_not_cut_down_to_whole_ones():
+    for v in (3.5, -0.25, 2.0 ** 31, float("nan"), float("inf"), 2 ** 31):
+        with pytest.raises(ValueError):
+            ops._int("window", v)
+    assert [ops._int("window", v) for v in (3, 3.0, -5, 2 ** 31 - 1, True)] == [3, 3, -5, 2 ** 31 - 1, 1]
