@@ -132,7 +132,7 @@ def bias_buckets(buckets: int, max_distance: int) -> tuple[int, ...]:
 
 @functools.lru_cache(maxsize=64)
 def _starts_array(starts: tuple):
-    return (ctypes.c_int32 * max(1, len(starts)))(*starts)
+    return (ctypes.c_int32 * max(1, len(starts)))(*(_int("bucket start", s) for s in starts))
 
 
 def _bias_args(x, starts, cols, scale, row_offset, window, sinks):

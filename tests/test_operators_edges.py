@@ -46,3 +46,10 @@ def test_whole_numbers_are_not_cut_down_to_whole_ones():
         with pytest.raises(ValueError):
             ops._int("window", v)
     assert [ops._int("window", v) for v in (3, 3.0, -5, 2 ** 31 - 1, True)] == [3, 3, -5, 2 ** 31 - 1, 1]
+
+
+def test_bucket_starts_are_not_taken_modulo_2_to_the_32():
+    assert list(ops._starts_array((0, 1, 8192))) == [0, 1, 8192]
+    for starts in ((0, 1, 2 ** 32 + 2), (2 ** 32, 1), (0, -2 ** 32 + 5), (0, 1.5)):
+        with pytest.raises((TypeError, ValueError)):
+            ops._starts_array(starts)
