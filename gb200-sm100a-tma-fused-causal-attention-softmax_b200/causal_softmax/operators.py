@@ -23,6 +23,7 @@ import torch
 from . import check, lib
 
 _I32_MAX = 2**31 - 1
+_MAX_BUCKETS = 128  # CS_MAX_BUCKETS
 
 
 class _BiasArgs(ctypes.Structure):
@@ -124,10 +125,10 @@ def _sixteen_bit(name: str, t) -> int:
 def bias_buckets(buckets: int, max_distance: int) -> tuple[int, ...]:
     """First distance of each bucket: half of them hold one distance each, the
     rest grow by an even ratio up to max_distance; the last holds all beyond."""
-    starts = (ctypes.c_int32 * max(1, buckets))()
-    check(lib().cs_bias_buckets(_int("buckets", buckets), _int("max_distance", max_distance), starts),
-          "cs_bias_buckets")
-    return tuple(starts)
+    n = _int("buckets", buckets)
+    starts = (ctypes.c_int32 * _MAX_BUCKETS)()
+    check(lib().cs_bias_buckets(n, _int("max_distance", max_distance), starts), "cs_bias_buckets")
+    return tuple(starts[:n])
 
 
 @functools.lru_cache(maxsize=64)

@@ -2,6 +2,7 @@
 import glob
 import os
 import re
+import resource
 import subprocess
 
 import pytest
@@ -53,3 +54,13 @@ def test_bucket_starts_are_not_taken_modulo_2_to_the_32():
     for starts in ((0, 1, 2 ** 32 + 2), (2 ** 32, 1), (0, -2 ** 32 + 5), (0, 1.5)):
         with pytest.raises((TypeError, ValueError)):
             ops._starts_array(starts)
+
+
+def test_bucket_counts_that_are_refused_cost_no_memory():
+    before = resource.getrusage(resource.RUSAGE_SELF).ru_maxrss
+    for buckets in (2 ** 28, 2 ** 31 - 1):
+        with pytest.raises(cs.CausalSoftmaxError):
+            cs.bias_buckets(buckets, 8000)
+    with pytest.raises(ValueError):
+        cs.bias_buckets(2 ** 40, 8000)
+    assert resource.getrusage(resource.RUSAGE_SELF).ru_maxrss - before < 1 << 18  # KB
