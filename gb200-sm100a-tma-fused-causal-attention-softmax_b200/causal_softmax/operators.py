@@ -304,7 +304,8 @@ def attention_backward(dout, q, k, v, out, lse, *, scale: float | None = None, w
 
 def attention_status(stream=None, device=None) -> tuple[int, int]:
     """(error code, bits) of the attention kernels' status word on a device, which it clears; waits for the stream."""
-    device = torch.device("cuda", torch.cuda.current_device() if device is None else torch.device(device).index or 0)
+    index = None if device is None else torch.device(device).index
+    device = torch.device("cuda", torch.cuda.current_device() if index is None else index)
     bits = ctypes.c_uint32()
     with _on(device, stream):
         rc = lib().cs_attention_status(ctypes.byref(bits), _current(device))

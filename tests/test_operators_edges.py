@@ -1,4 +1,5 @@
 """Host side of the operators beside the softmax at the edges of what they accept."""
+import contextlib
 import glob
 import os
 import re
@@ -64,3 +65,19 @@ def test_bucket_counts_that_are_refused_cost_no_memory():
     with pytest.raises(ValueError):
         cs.bias_buckets(2 ** 40, 8000)
     assert resource.getrusage(resource.RUSAGE_SELF).ru_maxrss - before < 1 << 18  # KB
+
+
+@pytest.mark.parametrize("device,want", [(None, 1), ("cuda", 1), ("cuda:0", 0), (0, 0), (2, 2)])
+def test_status_of_the_current_device_unless_one_is_named(monkeypatch, device, want):
+    seen = []
+
+    class Library:
+        def cs_attention_status(self, bits, stream):
+            return 0
+
+    monkeypatch.setattr(ops.torch.cuda, "current_device", lambda: 1)
+    monkeypatch.setattr(ops, "lib", Library)
+    monkeypatch.setattr(ops, "_on", lambda d, stream: seen.append(d) or contextlib.nullcontext())
+    monkeypatch.setattr(ops, "_current", lambda d: 0)
+    assert ops.attention_status(device=device) == (0, 0)
+    assert [d.index for d in seen] == [want]
