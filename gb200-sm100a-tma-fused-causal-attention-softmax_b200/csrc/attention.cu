@@ -377,8 +377,12 @@ struct GradShape {
   int64_t q_pad;  // rows of a pack of heads
   int share, window_shares, sink_tiles, sink_shares;
   int64_t dkv_ctas;
-  int64_t rows_bytes, norms_bytes, partial_bytes;  // two arrays of rows
-  int64_t bytes() const { return 2 * rows_bytes + norms_bytes + partial_bytes; }
+  int query_blocks, key_blocks;  // fp16: of 64, whose largest norms are kept
+  // An array of rows (lse2, delta; fp16: |d_o|), those norms and dQ's counter.
+  int64_t rows_bytes, query_bytes, key_bytes, partial_bytes;
+  int64_t counter_at() const { return (query_bytes ? 3 : 2) * rows_bytes + query_bytes + key_bytes; }
+  int64_t partial_at() const { return counter_at() + 16; }
+  int64_t bytes() const { return partial_at() + partial_bytes; }
 };
 
 // A key tile's work is its units, the query tiles that see it. Tiles are cut into shares
@@ -415,7 +419,12 @@ GradShape grad_shape(const cs_attention_args* a, int sms) {
   s.sink_shares = (int)((all + s.share - 1) / s.share);
   s.dkv_ctas = heads * ((int64_t)s.sink_tiles * s.sink_shares + (int64_t)(s.k_tiles - s.sink_tiles) * s.window_shares);
   s.rows_bytes = (int64_t)a->batch * (a->heads >> pack) * s.q_pad * 4;
-  s.norms_bytes = (a->type == CS_TYPE_F16 ? (2 * heads * 4 + 15) / 16 * 16 : 0) + 16;  // and dQ's counter
+  if (a->type == CS_TYPE_F16) {
+    s.query_blocks = (int)((s.q_pad >> pack) + cs::kRowsPerCta - 1) / cs::kRowsPerCta;
+    s.key_blocks = 2 * s.k_tiles;
+    s.query_bytes = ((int64_t)a->batch * a->heads * s.query_blocks * 8 + 15) / 16 * 16;
+    s.key_bytes = (heads * s.key_blocks * 4 + 15) / 16 * 16;
+  }
   if (s.window_shares > 1 || (s.sink_tiles && s.sink_shares > 1)) s.partial_bytes = s.dkv_ctas * 2 * cs::kTile * s.dim * 4;
   return s;
 }
@@ -431,22 +440,24 @@ int launch_backward(const cs_attention_args* a, const cs_attention_grads* g, con
   char* at = static_cast<char*>(workspace);
   float* lse2 = reinterpret_cast<float*>(at);
   float* delta = reinterpret_cast<float*>(at + s.rows_bytes);
-  float* norms = reinterpret_cast<float*>(at + 2 * s.rows_bytes);
+  float* grad_norms = reinterpret_cast<float*>(at + 2 * s.rows_bytes);
+  float2* grad_tops = reinterpret_cast<float2*>(at + 3 * s.rows_bytes);
+  float* value_tops = reinterpret_cast<float*>(at + 3 * s.rows_bytes + s.query_bytes);
   const bool half = a->type == CS_TYPE_F16;
 
   cs::RowsParams r{};
   r.a = p;
   r.lse2 = lse2;
   r.delta = delta;
-  r.norms = reinterpret_cast<uint32_t*>(norms);
-  r.next = reinterpret_cast<int32_t*>(at + 2 * s.rows_bytes + s.norms_bytes - 16);
+  r.grad_norms = grad_norms;
+  r.grad_tops = grad_tops;
+  r.value_tops = value_tops;
+  r.next = reinterpret_cast<int32_t*>(at + s.counter_at());
   r.q_pad = (int32_t)s.q_pad;
-  cudaError_t e = cudaSuccess;
-  if (half) e = cudaMemsetAsync(norms, 0, (size_t)(s.norms_bytes - 16), static_cast<cudaStream_t>(stream));
-  if (e != cudaSuccess) return fail_cuda(e, "attention backward, norms");
-  const unsigned rows = (unsigned)(((s.q_pad >> p.pack_log2) + cs::kRowsPerCta - 1) / cs::kRowsPerCta +
-                                   (half ? (a->kv_len + cs::kRowsPerCta - 1) / cs::kRowsPerCta : 0));
-  e = cs_host::launch(half ? &cs::attention_rows_kernel<cs::F16> : &cs::attention_rows_kernel<cs::BF16>,
+  r.query_blocks = s.query_blocks;
+  r.key_blocks = s.key_blocks;
+  const unsigned rows = (unsigned)(((s.q_pad >> p.pack_log2) + cs::kRowsPerCta - 1) / cs::kRowsPerCta + s.key_blocks);
+  cudaError_t e = cs_host::launch(half ? &cs::attention_rows_kernel<cs::F16> : &cs::attention_rows_kernel<cs::BF16>,
                       dim3(rows, (unsigned)std::min(a->batch * a->heads, 65535)), 256, 0, stream, r);
   if (e != cudaSuccess) return fail_cuda(e, "attention backward, rows");
 
@@ -454,9 +465,13 @@ int launch_backward(const cs_attention_args* a, const cs_attention_grads* g, con
   k.a = p;
   k.lse2 = lse2;
   k.delta = delta;
-  k.norms = norms;
+  k.grad_norms = grad_norms;
+  k.grad_tops = grad_tops;
+  k.value_tops = value_tops;
+  k.query_blocks = s.query_blocks;
+  k.key_blocks = s.key_blocks;
   k.next = r.next;
-  k.partial = reinterpret_cast<float*>(at + 2 * s.rows_bytes + s.norms_bytes);
+  k.partial = reinterpret_cast<float*>(at + s.partial_at());
   k.q_pad = (int32_t)s.q_pad;
   k.share = s.share;
   k.window_shares = s.window_shares;

@@ -20,9 +20,11 @@
 // both operands in shared memory takes as long as one of 128.)
 //
 // 16 bits: P and dS are rounded for the tensor core. In fp16 P is taken times
-// 2^15 and dS times a power of two, from the largest norms of d_o and v rows of
-// the kv head, that brings the largest possible |dS| to 2^15: small gradients
-// keep their bits and none overflows. bf16 needs neither.
+// 2^15 and dS times a power of two that brings the largest possible |dS| of one sum,
+// at most |d_o| |v| + |delta|, to 2^15: none overflows and small gradients keep their
+// bits, also beside large ones of other sums. dQ's sums are rows, each with its own
+// |d_o| and delta and the values of the key tiles that its tile sees; dK's are those of a
+// tile of keys and all queries that see it. bf16 needs neither.
 //
 // Bound: at dim 128 a tile costs 4 x 512 tensor-core cycles in dK/dV, 3 x 512 in
 // dQ, and 1024 cycles of the exponential unit in each. Measured (B200, ncu; 2 x
@@ -42,7 +44,12 @@ struct GradParams {
   AttentionParams a;
   const float* lse2;   // [pack of heads, q_pad rows]: minus lse in units of log2; -infinity for rows without keys
   const float* delta;  // the same: minus the sum of d_o * o
-  const float* norms;  // fp16: [2, batch * kv_heads], largest |d_o| and |v| of a row
+  // fp16: |d_o| as lse2; [batch * heads, query_blocks], the largest |d_o| and |delta| of 64
+  // queries; [batch * kv_heads, key_blocks], the largest |v| of 64 keys.
+  const float* grad_norms;
+  const float2* grad_tops;
+  const float* value_tops;
+  int32_t query_blocks, key_blocks;  // key_blocks: two a key tile
   float* partial;      // dK, dV parts of key tiles cut into several CTAs' shares
   int32_t q_pad;
   int32_t tiles;       // query (or key) tiles of a pack of heads (a kv head)
@@ -58,27 +65,28 @@ struct RowsParams {
   AttentionParams a;
   float* lse2;
   float* delta;
-  uint32_t* norms;  // as integers: the bits of non-negative floats order like them
-  int32_t* next;    // dQ's counter of query tiles
-  int32_t q_pad;
+  float* grad_norms;
+  float2* grad_tops;
+  float* value_tops;
+  int32_t* next;  // dQ's counter of query tiles
+  int32_t q_pad, query_blocks, key_blocks;
 };
 
-constexpr int kRowsPerCta = 64;
+constexpr int kRowsPerCta = 64;  // half a key tile
 
-// The largest of a CTA's row norms, to the kv head's.
-__device__ __forceinline__ void raise_max(uint32_t* at, float v, float* words) {
-  v = redux_max(v);  // NaN counts as nothing
+// The largest v of a CTA, NaN counting as nothing; words: one a warp. For thread 0.
+__device__ __forceinline__ float cta_max(float v, float* words) {
+  v = redux_max(v);
+  __syncthreads();  // the words' last readers
   if ((threadIdx.x & 31) == 0) words[threadIdx.x >> 5] = v;
   __syncthreads();
-  if (threadIdx.x == 0) {
+  if (threadIdx.x == 0)
     for (int w = 1; w < 8; ++w) v = fmaxf(v, words[w]);
-    if (v > 0.f) atomicMax(at, __float_as_uint(v));
-  }
-  __syncthreads();
+  return v;
 }
 
 // 16 lanes a row, four rows at a time. grid.x covers a head's tokens up to the end
-// of its last tile, then (fp16) the keys of a kv head; grid.y = batch * heads.
+// of its last tile, then (fp16) the key blocks of a kv head; grid.y = batch * heads.
 template <typename T>
 __global__ void __launch_bounds__(256) attention_rows_kernel(const __grid_constant__ RowsParams rp) {
   __shared__ float words[8];
@@ -94,7 +102,7 @@ __global__ void __launch_bounds__(256) attention_rows_kernel(const __grid_consta
     const Lengths len(p, b);
     const int pos0 = len.position(0);
     uint4 ra[4], rg[4];
-    float a[8], g[8], most = 0.f;
+    float a[8], g[8], most = 0.f, most_delta = 0.f;
     if ((int)blockIdx.x < q_ctas) {
       const int i0 = blockIdx.x * kRowsPerCta + threadIdx.x / 16;
       const uint16_t* po = p.o.at(b, i0, h) + d;
@@ -131,12 +139,20 @@ __global__ void __launch_bounds__(256) attention_rows_kernel(const __grid_consta
           const int64_t row = row0 + (i << p.pack_log2);
           rp.lse2[row] = lse[r] == -INFINITY ? -INFINITY : -lse[r] * kLog2e;
           rp.delta[row] = in[r] ? -dot : 0.f;
+          if (T::kIsHalf) rp.grad_norms[row] = sqrtf(norm);
         }
-        most = fmaxf(most, norm);
+        if (T::kIsHalf) {
+          most = fmaxf(most, norm);
+          most_delta = fmaxf(most_delta, fabsf(dot));
+        }
       }
-      if (T::kIsHalf) raise_max(rp.norms + b * p.kv_heads + hk, most, words);
+      if (T::kIsHalf) {
+        most = cta_max(most, words);
+        most_delta = cta_max(most_delta, words);
+        if (threadIdx.x == 0) rp.grad_tops[(int64_t)bh * rp.query_blocks + blockIdx.x] = make_float2(sqrtf(most), most_delta);
+      }
     } else if (T::kIsHalf && h % p.group == 0) {
-      const int k0 = ((int)blockIdx.x - q_ctas) * kRowsPerCta + threadIdx.x / 16;
+      const int block = (int)blockIdx.x - q_ctas, k0 = block * kRowsPerCta + threadIdx.x / 16;
       const Visible seen = sequence_keys(p, len);
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
@@ -149,20 +165,17 @@ __global__ void __launch_bounds__(256) attention_rows_kernel(const __grid_consta
         for (int x = 8; x > 0; x >>= 1) norm += __shfl_xor_sync(0xffffffffu, norm, x);
         most = fmaxf(most, norm);
       }
-      raise_max(rp.norms + p.batch * p.kv_heads + b * p.kv_heads + hk, most, words);
+      most = cta_max(most, words);
+      if (threadIdx.x == 0) rp.value_tops[(int64_t)(b * p.kv_heads + hk) * rp.key_blocks + block] = sqrtf(most);
     }
   }
   pdl_trigger();
 }
 
-// Factor of dS: 1, or in fp16 the power of two that brings the bound
-// |dP - delta| <= 2 |d_o| |v| to at most 2^15.
-template <typename T>
-__device__ __forceinline__ float ds_factor(const GradParams& g, int bk) {
-  if (!T::kIsHalf) return 1.f;
-  const float top = 2.f * sqrtf(g.norms[bk]) * sqrtf(g.norms[g.a.batch * g.a.kv_heads + bk]);
-  if (!(top > 1e-30f && top < 1e30f)) return 1.f;
-  const int up = (int)((__float_as_uint(top) >> 23) & 0xff) - 126;  // top <= 2^up
+// Factor of dS in fp16: the power of two that brings a bound of |dP - delta| to at most 2^15.
+__device__ __forceinline__ float ds_factor(float bound) {
+  if (!(bound > 1e-30f && bound < 1e30f)) return 1.f;
+  const int up = (int)((__float_as_uint(bound) >> 23) & 0xff) - 126;  // bound <= 2^up
   return __uint_as_float((uint32_t)(127 + 15 - up) << 23);
 }
 
@@ -422,7 +435,14 @@ __global__ void __launch_bounds__(kGradThreads, 1) attention_dq_kernel(const __g
       const int i = u.tile.token(in_tile);
       const Visible see = visible_keys(i < u.len.q ? u.len.position(i) : -1, u.len.kv, p.window, p.sinks);
       const int64_t row = (int64_t)((u.b * p.heads + u.tile.head) >> p.pack_log2) * gp.q_pad + (u.tile.first << p.pack_log2) + in_tile;
-      const float c = ds_factor<T>(gp, u.bk);
+      // fp16: the numbers that c is made of, on their way until the first dS.
+      const float* tops = gp.value_tops + (int64_t)u.bk * gp.key_blocks;
+      auto top = [&](int x) { return x < 2 * u.list.n ? tops[u.list.key(x >> 1) / kRowsPerCta + (x & 1)] : 0.f; };
+      float c = 1.f, values = 0.f, grad = 0.f;
+      if (T::kIsHalf) {
+        values = top(lane);
+        grad = gp.grad_norms[row];
+      }
       const F2 minus_lse = f2(gp.lse2[row], gp.lse2[row]), minus_delta = f2(gp.delta[row], gp.delta[row]);
       for (int j = 0; j < u.list.n; ++j, ++tiles) {
         const int k0 = u.list.key(j) + columns;
@@ -439,6 +459,10 @@ __global__ void __launch_bounds__(kGradThreads, 1) attention_dq_kernel(const __g
           tmem_load32(s_at + 32, s + 32);
           tmem_wait_loads();
           scores_to_p(s, every, bits0, bits1, sl, [&](int) { return minus_lse; }, pr);
+        }
+        if (T::kIsHalf && j == 0) {
+          for (int x = lane + 32; x < 2 * u.list.n; x += 32) values = fmaxf(values, top(x));
+          c = ds_factor(__fmaf_rn(grad, redux_max(values), fabsf(f2_out(minus_delta).x)));
         }
         ok = __all_sync(0xffffffffu, wait(&bars.dp_full, tiles & 1));
         if (!ok) break;
@@ -502,7 +526,9 @@ __global__ void __launch_bounds__(kGradThreads, 1) attention_dq_kernel(const __g
 struct KeyBarriers {
   uint64_t kv_full, s_full[2], s_free, dp_full, ds_full, done, q_full[3], q_empty[3], o_full[2], o_empty[2];
   uint32_t tmem, gone;
+  float factor;  // of dS, fp16
 };
+static_assert(sizeof(KeyBarriers) <= 256 && sizeof(QueryBarriers) <= 256, "the shared memory behind the tiles");
 
 template <int DP>
 struct KeySmem {
@@ -719,6 +745,23 @@ __global__ void __launch_bounds__(kGradThreads, 1) attention_dkv_kernel(const __
           o_used.next(kGrads);
           q_used.next(kQueries);
         }
+      } else if (T::kIsHalf && warp == 10 && n > 0) {
+        // The factor of dS, from all queries that see the tile.
+        const float* norms = gp.value_tops + (int64_t)bk * gp.key_blocks + tile * 2;
+        const float v = fmaxf(norms[0], norms[1]);
+        const int first = units.q_first / kRowsPerCta;
+        const int blocks = (units.q_first + units.per_pack * units.step - 1) / kRowsPerCta - first + 1;
+        const float2* tops = gp.grad_tops + (int64_t)(b * p.heads + hk * p.group) * gp.query_blocks + first;
+        float most = 0.f;
+#pragma unroll 4
+        for (int x = lane; x < blocks * p.group; x += 32) {
+          const int h = x / blocks;
+          const float2 top = tops[(int64_t)h * gp.query_blocks + (x - h * blocks)];
+          most = fmaxf(most, __fmaf_rn(top.x, v, top.y));
+        }
+        most = redux_max(most);
+        if (lane == 0) bars.factor = ds_factor(most);
+        asm volatile("bar.arrive 3, 288;" ::: "memory");
       }
     } else {
       registers_up<224>();
@@ -726,7 +769,12 @@ __global__ void __launch_bounds__(kGradThreads, 1) attention_dkv_kernel(const __
       const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
       const int columns = group * 64;  // this warpgroup's queries of a tile
       const float sl = fmaxf(p.scale * kLog2e, 1.1754944e-38f);
-      const float c = ds_factor<T>(gp, bk), k1 = T::kIsHalf ? c * (1.f / kHalfTop) : 1.f;
+      float c = 1.f;
+      if (T::kIsHalf && n > 0) {
+        asm volatile("bar.sync 3, 288;" ::: "memory");
+        c = bars.factor;
+      }
+      const float k1 = T::kIsHalf ? c * (1.f / kHalfTop) : 1.f;
       int q_lo, q_hi;
       queries_of(p, len, k0 + row, q_lo, q_hi);
       bool ok = true;

@@ -185,3 +185,67 @@ def test_rows_that_see_nothing_are_zero_beside_values_that_are_no_numbers(q_len,
     assert torch.isneginf(lse.transpose(1, 2)[~sees]).all() and not torch.isneginf(lse.transpose(1, 2)[sees]).any()
     assert not torch.isfinite(out[sees]).any(), "every other query sees key 0"
     assert torch.isfinite(lse.transpose(1, 2)[sees]).all()
+
+
+def gradients_by_row(dout, q, k, v, *, scale, window):
+    """ref.attention_backward for one sequence, with fp16's held ds off by what its own factor leaves: of each row for
+    dq, of each tile of 128 keys for dk (2^-25 / 2^14 of the largest |dP| + |delta| there; tiles are taken 256 wider)."""
+    n, heads, dim = q.shape[1:]
+    group, u = heads // k.shape[2], ref.half_step(q.dtype)
+    result = {m: tuple(torch.zeros(t.shape[1:], dtype=torch.float64, device="cuda") for _ in range(2))
+              for m, t in (("dq", q), ("dk", k), ("dv", v))}
+    pos = torch.arange(n, device="cuda")
+    keep, wide = ref.mask(pos, n, window, 0), window + 256 if window else n
+    near = (pos[None, :] <= pos[:, None] + 256) & (pos[:, None] - pos[None, :] <= wide + 256)  # [query, key]
+    small = 2.0 ** -39 if q.dtype == F16 else 0.0
+    for h in range(heads):
+        hk = h // group
+        Q, G, K, V = (t[0, :, i].double() for t, i in ((q, h), (dout, h), (k, hk), (v, hk)))
+        p, _ = ref.softmax_rows(torch.where(keep, Q @ K.T * scale, -math.inf))
+        e = float((Q.abs() @ K.abs().T).max()) * scale * (dim + 8) * 2 ** -24 + 2 ** -20
+        O, dp = p @ V, G @ V.T
+        delta = (G * O).sum(-1, keepdim=True)
+        ds = p * (dp - delta)
+        off = (u + 4 * e) * ds.abs() + p * (u * (G * O).abs().sum(-1, keepdim=True) +
+                                            (4 * e + (dim + 8) * 2 ** -24) * (G.abs() @ V.abs().T))
+        off = off + keep * ref.FLUSHED * (dp.abs() + delta.abs())
+        rows = torch.where(near, V.norm(dim=-1)[None, :], 0.0).amax(1, keepdim=True) * G.norm(dim=-1, keepdim=True) + delta.abs()
+        group_rows = torch.stack([(dout[0, :, i].double().norm(dim=-1)) for i in range(hk * group, hk * group + group)]).amax(0)
+        both = group_rows[:, None] * torch.where(near, V.norm(dim=-1)[None, :], 0.0).amax(1, keepdim=True) * 2
+        keys = torch.where(near, both, 0.0).amax(0, keepdim=True)
+        result["dq"][0][:, h] = scale * ds @ K
+        result["dq"][1][:, h] = scale * (off + keep * small * rows) @ K.abs()
+        result["dk"][0][:, hk] += scale * ds.T @ Q
+        result["dk"][1][:, hk] += scale * (off + keep * small * keys).T @ Q.abs()
+        small_p = 2.0 ** -40 if q.dtype == F16 else 0.0
+        result["dv"][0][:, hk] += p.T @ G
+        result["dv"][1][:, hk] += (u + 4 * e) * (p.T @ G.abs()) + (ref.FLUSHED + small_p) * G.abs().sum(0)
+    return {m: (t[None], (bound + u * t.abs() + 2 * ref.tiny(q.dtype))[None]) for m, (t, bound) in result.items()}
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(2, 2, 64), (4, 1, 64), (6, 2, 128)])
+@pytest.mark.parametrize("window,large", [(0, "dout"), (300, "dout"), (300, "v"), (0, "one row")])
+def test_gradients_of_rows_of_very_different_sizes(window, large, heads, kv_heads, dim, dtype):
+    """Small rows of d_o keep their bits beside rows 2^19 times larger, and where the large values are out of sight."""
+    n = 2048
+    q, dout = (randn(1, n, heads, dim, dtype=dtype, seed=i) for i in (1, 2))
+    k, v = (randn(1, n, kv_heads, dim, dtype=dtype, seed=i) for i in (3, 4))
+    if large == "v":
+        v[:, :200] *= 2.0 ** 9
+        dout[:, 700:] *= 2.0 ** -8
+    elif large == "one row":
+        dout *= 2.0 ** -8
+        dout[:, 1100] *= 2.0 ** 19
+    else:
+        dout[:, 128:] *= 2.0 ** -8
+        dout[:, :128] *= 2.0 ** 11
+    how = dict(scale=dim ** -0.5, window=window)
+    out, lse = cs.attention(q, k, v, return_lse=True, **how)
+    got = cs.attention_backward(dout, q, k, v, out, lse, **how)
+    status_ok()
+    want = gradients_by_row(dout, q, k, v, **how)
+    for name, t in zip(("dq", "dk", "dv"), got):
+        within(t, *want[name], name)
+    again = cs.attention_backward(dout, q, k, v, out, lse, **how)
+    assert all(torch.equal(a, b) for a, b in zip(got, again))
