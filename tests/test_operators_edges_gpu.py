@@ -249,3 +249,26 @@ def test_gradients_of_rows_of_very_different_sizes(window, large, heads, kv_head
         within(t, *want[name], name)
     again = cs.attention_backward(dout, q, k, v, out, lse, **how)
     assert all(torch.equal(a, b) for a, b in zip(got, again))
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("case", [
+    # batch, q_len, kv_len, heads, kv_heads, dim, window, sinks: one split and several, 8 and 16 rows, both dims
+    (150, 1, 200, 4, 4, 64, 0, 0),
+    (2, 1, 3000, 8, 2, 128, 0, 0),
+    (1, 2, 4000, 16, 2, 64, 3000, 4),
+    (2, 4, 900, 12, 3, 80, 0, 0),
+    (1, 1, 40000, 16, 1, 128, 0, 0),
+])
+def test_single_tokens_round_nothing_but_the_result(case, dtype):
+    """Probabilities meet the values in two 16-bit parts: what the second one rounds is the half step squared."""
+    batch, q_len, kv_len, heads, kv_heads, dim, window, sinks = case
+    q = randn(batch, q_len, heads, dim, dtype=dtype, seed=1)
+    k, v = (randn(batch, kv_len, kv_heads, dim, dtype=dtype, seed=i) for i in (2, 3))
+    how = dict(scale=dim ** -0.5, window=window, sinks=sinks)
+    out = cs.attention(q, k, v, **how)
+    status_ok()
+    want, bound, _, _ = ref.attention(q, k, v, **how)
+    magnitude, u = ref.attention(q, k, v.abs(), **how)[0], ref.half_step(dtype)
+    # ref's bound has u (p |v|) for a probability rounded once; here it is u^2.
+    within(out, want, bound - (u - u * u) * magnitude, "out")
