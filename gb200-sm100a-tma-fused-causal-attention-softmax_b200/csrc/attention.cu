@@ -564,7 +564,6 @@ int cs_attention_backward(const cs_attention_args* args, const cs_attention_grad
   if (!rc) rc = check_workspace(workspace, workspace_bytes, s.bytes());
   if (rc) return rc;
   p.d_o = strided(grads->d_o);
-  p.dq = strided(grads->dq);
   p.dk = strided(grads->dk);
   p.dv = strided(grads->dv);
   return launch_backward(args, grads, p, s, d.sms, workspace, stream);

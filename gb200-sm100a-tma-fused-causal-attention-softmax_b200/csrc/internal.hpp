@@ -20,7 +20,6 @@ struct Device {
 // Properties of the calling thread's current device; CS_ERR_DEVICE unless it is sm_10x.
 int current_device(Device* out);
 
-constexpr uint64_t kWaitTimeoutNs = 2000000000ull;  // 2 s of GPU time per device-side wait
 constexpr int kMaxDeviceIds = 64;
 
 // Launch with programmatic stream serialisation: the kernel's CTAs may start

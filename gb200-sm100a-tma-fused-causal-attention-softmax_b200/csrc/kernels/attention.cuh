@@ -20,7 +20,7 @@ struct Strided {  // [batch, token, head, dim], element strides, dim contiguous
 
 struct AttentionParams {
   Strided q, k, v, o;       // o: output; backward: the forward's output
-  Strided d_o, dq, dk, dv;  // backward
+  Strided d_o, dk, dv;      // backward (dq is written through its map)
   float* lse;               // [batch, heads, q_len]
   const int32_t* q_lens;
   const int32_t* kv_lens;
