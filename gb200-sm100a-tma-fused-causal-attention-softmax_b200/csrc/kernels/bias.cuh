@@ -295,9 +295,9 @@ __device__ __forceinline__ void wide_rows(const BiasParams& p, float* words, boo
   words += (threadIdx.x / 32 - group.rank / 32) * 2;
   group.sync();  // the other warps' marks
   for (RowTurns turns(p.rows, cta * groups + group.id, p.ctas * groups); turns.inside(); turns.next()) {
-    const RowWalk w(p, turns.at);
+    const RowWalk w(p, turns.here());
     if (w.m.n == 0) continue;
-    const int64_t row = (matrix * p.rows + turns.at) * p.pitch;
+    const int64_t row = (matrix * p.rows + turns.here()) * p.pitch;
     uint16_t* out = p.out + row;
     const float mark = T::unpack(out[w.v.s_end > 0 ? 0 : w.v.lo]).x;
     group.sync();  // all have read it
@@ -344,7 +344,7 @@ __global__ void __launch_bounds__(kBiasMaxThreads) bias_softmax_kernel(const __g
 
   RowWalk w(p, turns.row());
   for (int turn = 0; turns.inside(); turns.next(), turn ^= 1) {
-    const int row = turns.at, after = turns.next_row();
+    const int row = turns.here(), after = turns.next_row();
     uint4* out = reinterpret_cast<uint4*>(p.out + base + (int64_t)row * p.pitch);
     const uint4* in = source(row);
     const uint4* staged = buffers + (kBuffers == 2 ? turn * p.slots : 0);
@@ -485,7 +485,7 @@ __global__ void __launch_bounds__(kBiasMaxThreads) bias_backward_kernel(const __
 
   RowWalk w(p, turns.row());
   for (int turn = 0; turns.inside(); turns.next(), turn ^= 1) {
-    const int row = turns.at, after = turns.next_row();
+    const int row = turns.here(), after = turns.next_row();
     uint4* out = reinterpret_cast<uint4*>(p.out + base + (int64_t)row * p.pitch);
     const uint4* in = source(p.x, row);
     const uint4* in2 = source(p.dp, row);

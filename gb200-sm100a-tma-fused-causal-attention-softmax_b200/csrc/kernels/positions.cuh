@@ -75,16 +75,18 @@ CS_HD uint32_t visible_bits(const Visible& v, int32_t c0) {
 CS_HD int32_t vector_at(const VisibleVectors& m, int32_t j) { return j < m.n_sink ? j : j - m.n_sink + m.w_beg; }
 
 // The rows that one of a matrix's groups of lanes takes in turn, the last (longest)
-// ones first: rows - 1 - first, then `step` less each time. Counted down, so that no sum
-// passes 2^31 - 1 where rows is close to it. 0 <= first, step < 2^31.
+// ones first: row rows - 1 - i for i = first, first + step, ... In unsigned
+// arithmetic: i + step passes 2^31 - 1 where rows is close to it. 0 <= first, step <
+// 2^31. (Counted down in signed numbers: backward 32 x 4096^2 377 us, this 371.)
 struct RowTurns {
-  int32_t at, step;
-  CS_HD RowTurns(int32_t rows, int32_t first, int32_t step) : at(rows - 1 - first), step(step) {}
-  CS_HD bool inside() const { return at >= 0; }
-  CS_HD bool last() const { return at < step; }
-  CS_HD int32_t row() const { return at > 0 ? at : 0; }  // outside: row 0, read ahead and not used
-  CS_HD int32_t next_row() const { return at > step ? at - step : 0; }
-  CS_HD void next() { at -= step; }
+  uint32_t i, step, rows;
+  CS_HD RowTurns(int32_t rows, int32_t first, int32_t step) : i((uint32_t)first), step((uint32_t)step), rows((uint32_t)rows) {}
+  CS_HD bool inside() const { return i < rows; }
+  CS_HD bool last() const { return i + step >= rows; }
+  CS_HD int32_t here() const { return (int32_t)(rows - 1 - i); }  // inside only
+  CS_HD int32_t row() const { return i < rows ? here() : 0; }     // 0: read ahead, not used
+  CS_HD int32_t next_row() const { return i + step < rows ? (int32_t)(rows - 1 - i - step) : 0; }
+  CS_HD void next() { i += step; }
 };
 
 }  // namespace cs

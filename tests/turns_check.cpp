@@ -15,7 +15,7 @@ int main() {
         int64_t i = first;
         for (; t.inside(); t.next(), i += step, ++checked) {
           const int64_t row = rows - 1 - i, next = row - step;
-          if (row < 0 || t.row() != row || t.last() != (next < 0) || t.next_row() != (next < 0 ? 0 : next))
+          if (row < 0 || t.row() != row || t.here() != row || t.last() != (next < 0) || t.next_row() != (next < 0 ? 0 : next))
             return std::printf("rows %d step %d first %d turn %lld\n", rows, step, first, (long long)i), 1;
         }
         if (i < rows) return std::printf("rows %d step %d first %d ends early\n", rows, step, first), 1;
