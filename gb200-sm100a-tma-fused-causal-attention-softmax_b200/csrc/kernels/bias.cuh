@@ -411,7 +411,7 @@ __global__ void __launch_bounds__(kBiasMaxThreads) bias_softmax_kernel(const __g
     if (!(fabsf(m) < kNarrow)) {
       // Nothing but -infinity: so were the scores, if their multiples are finite. Else a
       // wide row, marked by NaN in all visible columns.
-      inv = s == 0.f && (T::kIsHalf || p.scale < 0.5f) ? 0.f : NAN;
+      inv = s == 0.f && (T::kIsHalf || p.scale <= 0.25f) ? 0.f : NAN;
       if (inv != 0.f) wide[0] = 1;
     }
     const F2 inv2 = f2(inv, inv);

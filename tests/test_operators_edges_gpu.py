@@ -272,3 +272,13 @@ def test_single_tokens_round_nothing_but_the_result(case, dtype):
     magnitude, u = ref.attention(q, k, v.abs(), **how)[0], ref.half_step(dtype)
     # ref's bound has u (p |v|) for a probability rounded once; here it is u^2.
     within(out, want, bound - (u - u * u) * magnitude, "out")
+
+
+@pytest.mark.parametrize("scale", [0.1, 0.25, 0.26, 0.49, 1.0])
+def test_bias_of_lowest_scores_beside_a_lowest_table(scale):
+    """Neither is -infinity, nor is their sum in binary64: every visible key has the same share."""
+    for bias in (-2e38, torch.finfo(torch.float32).min):
+        x = torch.full((1, 1, 24, 24), torch.finfo(BF16).min, dtype=BF16, device="cuda")
+        got = cs.bias_softmax(x, torch.full((1, 2), bias, device="cuda"), (0, 5), cols=24, scale=scale)[0, 0]
+        want = torch.tril(torch.ones(24, 24, device="cuda")) / torch.arange(1, 25, device="cuda")[:, None]
+        assert torch.equal(got, want.to(BF16)), bias
