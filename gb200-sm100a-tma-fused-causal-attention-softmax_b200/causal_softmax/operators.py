@@ -10,6 +10,10 @@ the outputs' use after it, is the caller's, as with any torch stream.
 
 A query at position p sees the keys k <= p with p - k < window (window 0: all
 of them) or k < sinks.
+
+No call records an autograd graph: what comes back does not require a gradient,
+whatever the inputs do. Training calls the *_backward function itself, or from the
+backward of a torch.autograd.Function.
 """
 from __future__ import annotations
 
@@ -171,7 +175,8 @@ def bias_softmax(x, table, bucket_starts, *, cols: int, scale: float, row_offset
     x: float16 or bfloat16 [batch,] heads, rows, pitch (pitch % 8 == 0); row i is
     position row_offset + i. table: float32 heads, buckets. bucket_starts: the
     buckets' first distances (bias_buckets, or any ascending ones from 0).
-    Every other column of the result, padding included, is +0.0."""
+    Every other column of the result, padding included, is +0.0. Autograd stops
+    here; bias_softmax_backward has the gradients."""
     args, heads, buckets, _keep = _bias_args(x, bucket_starts, cols, scale, row_offset, window, sinks)
     device = x.device
     _same("table", table, torch.float32, device)
@@ -264,7 +269,8 @@ def attention(q, k, v, *, scale: float | None = None, window: int = 0, sinks: in
     device, the sequences' lengths (the tensors' by default); a sequence's queries
     are its last tokens, so q_len 1 with kv_lens reads a cache. Rows behind a
     sequence's queries come back zero. Returns out, or (out, lse) with the float32
-    log-sum-exp [batch, heads, q_len] that attention_backward takes."""
+    log-sum-exp [batch, heads, q_len] that attention_backward takes. Autograd stops
+    here; attention_backward has the gradients."""
     head = _attention_head(q, k, v, scale, window, sinks, q_lens, kv_lens)
     shape, dtype, device = q.shape, q.dtype, q.device
     L = _lib()

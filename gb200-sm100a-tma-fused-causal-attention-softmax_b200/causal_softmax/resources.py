@@ -40,7 +40,7 @@ BUDGETS = [
     (r"online_kernel<[12]>", 64, 0, "launch bounds of 1024 threads (the long-row shape)"),
     (r"cluster_kernel", 64, 0, "shared-memory passes with 17 warps per CTA; nothing to keep in registers"),
     (r"attention_dkv_kernelINS_.*", 168, 64,
-     "one word of a warpgroup's loop bookkeeping (4 bytes stored, read back 9 times); the launch "
+     "one word of a warpgroup's loop bookkeeping (4 bytes stored, read back 8 to 10 times); the launch "
      "value of 168 registers grows to 224 for the warpgroups at run time"),
     (r"rowres_kernel<8, 256, 1, [01]>", 168, 0, "V = 8 at up to 8 warps; tuning request only"),
     (r"rowres_kernel<0, 1024, 1, [01]>", 64, 0, "shared-memory passes, 32 warps in one CTA"),

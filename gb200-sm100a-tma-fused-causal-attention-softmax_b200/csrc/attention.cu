@@ -245,8 +245,10 @@ constexpr int kTokenResident[2][2] = {{4, 3}, {3, 2}};  // CTAs an SM: dim 64, 1
 // Which calls those are, by the rows of a kv head, (query, head) pairs, and by the
 // kv heads. Up to 8 rows: all. Up to 16, whose accumulators leave the kernel two
 // CTAs an SM: while the kv heads are fewer than the SMs, so that their keys are
-// split (4 x 2 queries over 16384 keys, 32 heads over 4, dim 128: 29.1 us, tiles
-// 36.4; 64 x 2 over 4096: 102.9, tiles 88.1). More rows would read the keys more
+// split (4 x 2 queries over 16384 keys, 32 heads over 4, dim 128: 34.4 us, tiles
+// 39.0; 64 x 2 over 4096: 108.7, tiles 91.8). Groups that are no power of two, whose
+// tiles read the keys more than once, would gain by it there too: 64 x 1 of 48 heads
+// over 4, 4096 keys: 108, by the rule's tiles 262. More rows would read the keys more
 // than once (8 x 8 over 1024: 13.0, tiles 9.4).
 bool few_queries(const cs_attention_args* a, int sms) {
   const int64_t rows = (int64_t)a->q_len * (a->heads / a->kv_heads);
@@ -391,8 +393,8 @@ struct GradShape {
 // dK and dV in fp32, written and read once more. So: about two shares an SM of at least
 // 16 units, fewer units only if those would not be two an SM, and no cut of a
 // window's tiles as long as that makes them at most twice as long. (Training step,
-// at least 16 units / this: 4 x 236 tokens, 8 heads over 1: 47.6 / 33.3 us; 5 x 149, 16
-// over 2: 36.9 / 29.2. With one share an SM 2048 tokens, 8 heads over 1, took 80.3 us,
+// at least 16 units / this: 4 x 236 tokens, 8 heads over 1: 47.1 / 31.3 us; 5 x 149, 16
+// over 2: 36.9 / 29.9. With one share an SM 2048 tokens, 8 heads over 1, took 80.3 us,
 // this 68.3.)
 GradShape grad_shape(const cs_attention_args* a, int sms) {
   GradShape s{};

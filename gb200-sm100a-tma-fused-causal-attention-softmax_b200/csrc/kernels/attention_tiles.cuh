@@ -21,7 +21,9 @@
 // also covers. Measured against one CTA an SM with two query tiles that share
 // each key tile (half the L2 traffic): 16384 queries x 16 heads, window 4096,
 // dim 128: 468 us against 509; dim 64: 425 against 459; 512 over 8192: 112
-// against 147. (A query in two threads, 64 keys of a tile each: 440, 374 and 104
+// against 147. Both sides then issued products under a branch on the lane, which cost
+// the one warp with two tiles' products more; with a converged warp (442 us for the
+// first case in a short replay) the second form has not been measured. (A query in two threads, 64 keys of a tile each: 440, 374 and 104
 // against 435, 362 and 105 of one thread. At dim 128 the power limit holds the
 // clock down: 1.62 GHz under this kernel alone, 1.95 at dim 64.)
 //

@@ -6,9 +6,10 @@
 // result; backward: the row's sum of p dp, result) read them there, so HBM sees
 // each score once. Rows too long for that are read from global memory in each pass.
 // Bound: HBM (2 bytes in per visible score, 2 out per column; the backward
-// reads two matrices). B200: forward 64 x 4096^2 535 us, 0.92 of the copy rate;
-// backward 32 x 4096^2 369 us, 0.89, 512 x 4096^2 5.5 ms, 0.95; rows of 512 columns, bound
-// by their instructions, 0.66 and 0.69.
+// reads two matrices). B200, through the entry points in a stream, after a rest / in a
+// second of calls, whose power holds the clock down: forward 64 x 4096^2 538 / 558 us,
+// 0.92 / 0.88 of the copy rate; backward 32 x 4096^2 377 / 378 us, 0.87, 512 x 4096^2 5.7
+// / 5.9 ms, 0.93 / 0.89; rows of 512 columns, bound by their instructions, 0.65 and 0.69.
 //
 // Bias: a distance d = position - key lies in the last bucket from its start
 // on; the other distances (at most CS_MAX_BUCKET_START) are looked up in a

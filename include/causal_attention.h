@@ -114,15 +114,19 @@ typedef struct cs_attention_args {
     float *lse;                   /* [batch, heads, q_len] natural log-sum-exp; may be NULL in cs_attention */
 } cs_attention_args;
 
-/* o = softmax(scale q k^T) v. The queries of a sequence are its last ones:
+/* o = softmax(scale q k^T) v. Scores are binary32 in units of log2: one of 2.3e38
+ * and more in magnitude counts as infinite. The queries of a sequence are its last ones:
  * query i is at position kv_lens[b] - q_lens[b] + i. Lengths are clipped to
  * [0, q_len] and [0, kv_len]. Rows behind a sequence's queries are written as
  * rows that see no key; keys and values behind its length, and those that no
  * query sees, may hold anything. (A NaN or infinity in a value that some query
  * of the sequence sees may also reach other queries of that sequence that do
  * not see it.) A row whose visible scores are all -infinity is like one that
- * sees no key; one with a NaN or +infinity among them is NaN. One call serves prompts, chunks of prompts over a cache
- * (q_len < kv_len) and single tokens (q_len 1). `workspace`: at least
+ * sees no key; one with a NaN or +infinity among them is NaN. One call serves
+ * prompts, chunks of prompts over a cache (q_len < kv_len) and single tokens
+ * (q_len 1). Probabilities are rounded to 16 bits before they meet the values, but
+ * for few queries (up to 8, in some shapes 16, of a kv head's heads together),
+ * where nothing is rounded but the result. `workspace`: at least
  * cs_attention_workspace bytes (0 for most shapes). */
 int64_t cs_attention_workspace(const cs_attention_args *args);
 int cs_attention(const cs_attention_args *args, void *workspace, size_t workspace_bytes, void *stream);
@@ -131,6 +135,9 @@ int cs_attention(const cs_attention_args *args, void *workspace, size_t workspac
  * wrote for the same arguments. Rows of dq behind a sequence's queries, and
  * rows of dk and dv behind its keys, are written zero; what d_o holds there is
  * not used. Gradients of a kv head are summed over its query heads in binary32.
+ * P and the gradient of the scores are rounded to 16 bits on the way. In fp16 the
+ * latter is scaled to the largest that a row of dq, or the queries that see a tile of
+ * 128 keys, can reach: smaller ones beside it are kept down to 2^-39 of that.
  * A NaN or infinity in a row of q, d_o or o, or in a key or value that is seen,
  * may reach all gradients of its sequence.
  * `workspace`: at least cs_attention_backward_workspace bytes. */
