@@ -282,3 +282,47 @@ def test_bias_of_lowest_scores_beside_a_lowest_table(scale):
         got = cs.bias_softmax(x, torch.full((1, 2), bias, device="cuda"), (0, 5), cols=24, scale=scale)[0, 0]
         want = torch.tril(torch.ones(24, 24, device="cuda")) / torch.arange(1, 25, device="cuda")[:, None]
         assert torch.equal(got, want.to(BF16)), bias
+
+
+def test_fp16_gradients_and_wide_rows_in_graphs_and_on_two_streams():
+    """Captured twice and replayed on new inputs, some rows of them wide, then eagerly on two streams at once."""
+    x, table = randn(2, 4, 100, 104, dtype=BF16, seed=1), randn(4, 32, dtype=torch.float32, seed=2)
+    starts, how = cs.bias_buckets(32, 128), dict(cols=100, scale=1.0, window=40, sinks=2)
+    q, dout = (randn(2, 300, 6, 80, dtype=F16, seed=i) for i in (3, 4))
+    k, v = (randn(2, 300, 2, 80, dtype=F16, seed=i) for i in (5, 6))
+
+    def chain():
+        p = cs.bias_softmax(x, table, starts, **how)
+        out, lse = cs.attention(q, k, v, window=90, sinks=3, return_lse=True)
+        return [p, out, lse, *cs.attention_backward(dout, q, k, v, out, lse, window=90, sinks=3)]
+
+    chain()
+    torch.cuda.synchronize()
+    graphs, results = [], []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            results.append(chain())
+        graphs.append(g)
+    for seed in (10, 20):
+        for t in (x, q, k, v, dout):
+            t.copy_(randn(*t.shape, dtype=t.dtype, seed=seed))
+            seed += 1
+        x[:, :, seed % 7::7] = torch.finfo(BF16).min
+        dout[:, ::3] *= 2.0 ** 10
+        for g in graphs:
+            g.replay()
+        torch.cuda.synchronize()
+        fresh = chain()
+        for r in results:
+            assert all(torch.equal(a, b) for a, b in zip(r, fresh))
+        assert (fresh[0].float().sum(-1) > 0.9).all()
+    streams, runs = [torch.cuda.Stream() for _ in range(2)], []
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for s in streams:
+            with torch.cuda.stream(s):
+                runs.append(chain())
+    torch.cuda.synchronize()
+    status_ok()
+    assert all(torch.equal(a, b) for r in runs for a, b in zip(r, fresh))
