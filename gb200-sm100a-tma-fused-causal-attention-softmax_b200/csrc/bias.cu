@@ -168,8 +168,8 @@ int least_lanes(int matrices, int64_t work, bool many) {
 int buffers_of(int matrices, int64_t vectors) { return vectors > (matrices == 1 ? 192 : 96) ? 1 : 2; }
 
 // Shared memory of a CTA at most, else more lanes a row (fewer groups): 74 KB
-// leaves three CTAs an SM, 56 and 46 four (five would need 44). 32 x 4096^2 forward, one buffer: 46 KB 279 us,
-// 74 KB 293; 32 x 4096^2 backward, one buffer: 74 KB 356, 56 KB 381; 96 x 1500^2
+// leaves three CTAs an SM, 56 and 46 four (five would need 44). 32 x 4096^2 forward, one
+// buffer: 46 KB 279 us, 74 KB 293; 32 x 4096^2 backward, one buffer: 74 KB 356, 56 KB 381; 96 x 1500^2
 // forward, two buffers: 74 KB 130, 46 KB 160; 256 x 400^2 backward, two: 56 KB 53, 74 KB 61.
 int64_t most_smem(int matrices, int buffers) {
   if (matrices == 1) return (buffers == 1 ? 46 : 74) * 1024;

@@ -29,7 +29,7 @@
 // Bound: at dim 128 a tile costs 4 x 512 tensor-core cycles in dK/dV, 3 x 512 in
 // dQ, and 1024 cycles of the exponential unit in each. Measured (B200, ncu; 2 x
 // 4096 queries, 16 heads over 4, window 1024, dim 128, bf16): rows 17 us, dK/dV
-// 148 us at 1.65 GHz (tensor pipe active 62%), dQ 112 us at 1.67 GHz (52%).
+// 148 us at 1.65 GHz (tensor pipe active 62%), dQ 113 us at 1.66 GHz (52%).
 #pragma once
 
 #include "attention_tiles.cuh"

@@ -22,10 +22,11 @@
 // each key tile (half the L2 traffic): 16384 queries x 16 heads, window 4096,
 // dim 128: 468 us against 509; dim 64: 425 against 459; 512 over 8192: 112
 // against 147. Both sides then issued products under a branch on the lane, which cost
-// the one warp with two tiles' products more; with a converged warp (442 us for the
-// first case in a short replay) the second form has not been measured. (A query in two threads, 64 keys of a tile each: 440, 374 and 104
-// against 435, 362 and 105 of one thread. At dim 128 the power limit holds the
-// clock down: 1.62 GHz under this kernel alone, 1.95 at dim 64.)
+// the one warp with two tiles' products more; with a converged warp (451 us for the
+// first case in a short replay) the second form has not been measured. (A query in
+// two threads, 64 keys of a tile each: 440, 374 and 104 against 435, 362 and 105 of
+// one thread. At dim 128 the power limit holds the clock down: 1.62 GHz in a second
+// of these calls, 1.95 at dim 64.)
 //
 // Running maximum: it moves only when a row passes it by more than 2^8, so the
 // output in TMEM is rescaled rarely (all sums are relative to the same
